@@ -18,6 +18,9 @@ LIB_PATH = os.path.join(PKG_DIR, LIB_NAME)
 SOURCES = [
     "fi_context.cpp",
     "fi_attention.hip",
+    "fi_attention_fp4.hip",
+    "fi_kv_fp4.hip",
+    "fi_qkv_norm.hip",
     "fi_prefill.hip",
     "fi_ops.hip",
     "fi_gemm.hip",

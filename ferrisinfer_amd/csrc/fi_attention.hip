@@ -10,7 +10,10 @@
 #include <type_traits>
 
 #include "fi_common.h"
+#include "fi_decode.h"
 #include "fi_device.h"
+#include "fi_fp4.h"
+#include "fi_fp4_ops.h"
 
 // Split-KV partials of fi_attn_decode_paged_noalloc: a fixed array of this library, one copy
 // per device (each GPU holds it from the load of this code object until the process ends).
@@ -22,26 +25,10 @@ static __device__ __align__(256) unsigned char scratch[FI_DECODE_NOALLOC_SCRATCH
 
 namespace {
 
-// Tunables (compile-time).  The wave chunk fixes the reduction order for a given context
-// length and model shape, so it is a constant of the library, not of a launch.
-#ifndef FI_DECODE_WIDE_WAVE_TOKENS
-#define FI_DECODE_WIDE_WAVE_TOKENS 128  // context tokens per wave when Hkv * D >= 512
-#endif
-#ifndef FI_DECODE_NARROW_WAVE_TOKENS
-#define FI_DECODE_NARROW_WAVE_TOKENS 64  // narrow KV rows (few, small heads): more workgroups
-#endif
+// Tunable (compile-time).
 #ifndef FI_DECODE_INFLIGHT_BYTES
 #define FI_DECODE_INFLIGHT_BYTES 16384  // f32 K or V bytes each wave keeps in flight (bf16: half)
 #endif
-
-constexpr int kWaves = 4;
-constexpr int kThreads = 64 * kWaves;
-constexpr int kMaxParts = 256;  // merge weights live in LDS
-
-// Tokens per wave for a model shape (never a batch property: outputs stay batch-invariant).
-constexpr int wave_tokens_for(int hkv, int d) {
-  return hkv * d >= 512 ? FI_DECODE_WIDE_WAVE_TOKENS : FI_DECODE_NARROW_WAVE_TOKENS;
-}
 
 constexpr int clamp_int(int v, int lo, int hi) { return v < lo ? lo : (v > hi ? hi : v); }
 
@@ -76,157 +63,6 @@ struct KvIO<uint16_t> {
     }
   }
 };
-
-struct DecodeArgs {
-  const float* q;
-  const void* k_cache;
-  const void* v_cache;
-  const int* block_tables;
-  const int* context_lens;
-  float* part_acc;  // [num_seqs * Hq * parts_per_seq, D]
-  float* part_ml;   // [num_seqs * Hq * parts_per_seq, 2]
-  // Merge in the partition kernel: one arrival counter per (sequence, kv head), zero between
-  // launches (the last arriver resets it).  Null: decode_merge_kernel merges.
-  unsigned* counters;
-  // Fused q|k|v consumer (decode ticks, one new token per sequence), when qkv_parts is set:
-  // every workgroup forms its group's query rows from the q|k|v projection's split-K partials
-  // (+ bias, RoPE) instead of reading q, and the last partition's workgroup of each
-  // (sequence, kv head) first writes the new token's K/V row into the pool at slots[seq].
-  const float* qkv_parts;  // [qkv_splits][num_seqs][Hq D + 2 Hkv D]
-  int qkv_splits;
-  const float* bias_q;
-  const float* bias_k;
-  const float* bias_v;
-  const int* positions;  // [num_seqs] RoPE positions
-  const float* cos_t;    // [max_positions][rotary_dims / 2]
-  const float* sin_t;
-  int rotary_dims;
-  int max_positions;
-  const int64_t* slots;  // [num_seqs] pool slots of the new tokens
-  float* out;
-  uint32_t* faults;
-  int num_seqs;
-  int max_blocks;
-  int parts_per_seq;
-  int hq;
-  int hkv;
-  int group;       // query heads per kv head
-  int heads_per;   // of them, the heads of one workgroup (gridDim.y workgroups share the group)
-  int block_size;
-  int num_blocks;
-  float scale;
-};
-
-// The query heads of one workgroup: `pair` numbers (sequence, kv head), `share` the part of its
-// group (gridDim.y shares, so that a pair's workgroups lie gridDim.x apart: where that is a
-// multiple of 8 they run on one XCD and its L2 serves the second read of their K/V).
-struct HeadUnit {
-  int seq, kvh;
-  int first;     // first query head of the share, within the sequence
-  int heads;     // <= 0: the group has no heads left for this share
-  size_t head0;  // first query head of the share over the batch
-};
-
-template <bool SHARES>
-__device__ __forceinline__ HeadUnit head_unit(const DecodeArgs& a, int pair) {
-  HeadUnit u;
-  u.seq = pair / a.hkv;
-  u.kvh = pair - u.seq * a.hkv;
-  u.first = u.kvh * a.group;
-  u.heads = a.group;
-  if constexpr (SHARES) {
-    const int skip = static_cast<int>(blockIdx.y) * a.heads_per;
-    u.first += skip;
-    u.heads = min(a.heads_per, a.group - skip);
-  }
-  u.head0 = (size_t)u.seq * a.hq + u.first;
-  return u;
-}
-
-// Orders this wave's LDS stores before its later LDS loads by other lanes (a compiler
-// barrier only: a wave's LDS operations execute in order).
-__device__ __forceinline__ void wave_lds_sync() { __builtin_amdgcn_fence(__ATOMIC_SEQ_CST, "wavefront"); }
-
-// Keeps the instruction scheduler from moving code across this point, so loads issued
-// before it stay ahead of the arithmetic after it (the ring's depth is what stays in flight).
-__device__ __forceinline__ void sched_fence() { __builtin_amdgcn_sched_barrier(0); }
-
-// A partial of another workgroup: a plain load after a kernel boundary, a device-coherent
-// load (past the XCDs' private L2s) inside the partition kernel.
-template <bool COHERENT>
-__device__ __forceinline__ float load_partial(float* p) {
-  if constexpr (COHERENT) return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-  return *p;
-}
-
-// Combines the partitions of one (sequence, kv_head) group: M = max m_p,
-// L = sum l_p e^(m_p-M), out = sum acc_p e^(m_p-M) / L per query head.  The first
-// partitions' partials are fetched before the weights are known so the loads overlap.  The
-// same arithmetic, in the same order, runs in decode_merge_kernel and in the partition
-// kernel's last-arriving workgroup, so both give identical outputs.
-template <int D, int MAXG, bool COHERENT>
-__device__ __forceinline__ void merge_unit(const DecodeArgs& a, size_t head0, int group, int nparts,
-                                           float (*s_w)[kMaxParts], float* s_inv) {
-  constexpr int kPrefetch = 8;
-  constexpr int kPerThread = (MAXG * D + kThreads - 1) / kThreads;
-  const int tid = threadIdx.x;
-  const int w = tid >> 6;
-  const int lane = tid & 63;
-  const int P = a.parts_per_seq;
-
-  float pre[kPerThread][kPrefetch];
-#pragma unroll
-  for (int k = 0; k < kPerThread; ++k) {
-    const int i = tid + k * kThreads;
-    const int g = i / D, d = i % D;
-#pragma unroll
-    for (int p = 0; p < kPrefetch; ++p)
-      pre[k][p] = (g < group && p < nparts) ? load_partial<COHERENT>(&a.part_acc[((head0 + g) * P + p) * D + d]) : 0.0f;
-  }
-  for (int g = w; g < group; g += 4) {
-    // each lane's (max, sum) pairs are read once and kept for the weights
-    constexpr int kPartsPerLane = kMaxParts / 64;
-    float* ml = a.part_ml + (head0 + g) * P * 2;
-    float2 mlv[kPartsPerLane];
-    float m = -INFINITY;
-#pragma unroll
-    for (int j = 0; j < kPartsPerLane; ++j) {
-      const int p = lane + 64 * j;
-      if constexpr (COHERENT)
-        mlv[j] = p < nparts ? make_float2(load_partial<true>(&ml[2 * p]), load_partial<true>(&ml[2 * p + 1]))
-                            : make_float2(-INFINITY, 0.0f);
-      else
-        mlv[j] = p < nparts ? reinterpret_cast<const float2*>(ml)[p] : make_float2(-INFINITY, 0.0f);
-      m = fmaxf(m, mlv[j].x);
-    }
-    m = fi::wave_max(m);
-    float l = 0.0f;
-#pragma unroll
-    for (int j = 0; j < kPartsPerLane; ++j) {
-      const int p = lane + 64 * j;
-      if (p < nparts) {
-        const float wgt = __expf(mlv[j].x - m);
-        s_w[g][p] = wgt;
-        l += mlv[j].y * wgt;
-      }
-    }
-    l = fi::wave_sum(l);
-    if (lane == 0) s_inv[g] = 1.0f / l;
-  }
-  __syncthreads();
-#pragma unroll
-  for (int k = 0; k < kPerThread; ++k) {
-    const int i = tid + k * kThreads;
-    const int g = i / D, d = i % D;
-    if (g >= group) continue;
-    float acc = 0.0f;
-#pragma unroll
-    for (int p = 0; p < kPrefetch; ++p) acc += pre[k][p] * (p < nparts ? s_w[g][p] : 0.0f);
-    for (int p = kPrefetch; p < nparts; ++p)
-      acc += load_partial<COHERENT>(&a.part_acc[((head0 + g) * P + p) * D + d]) * s_w[g][p];
-    a.out[(head0 + g) * D + d] = acc * s_inv[g];
-  }
-}
 
 // The fused q|k|v consumer's share of one workgroup: the group's query rows into s_q and,
 // with `append`, the new token's K and V rows of kv head kvh into the pool.  The arithmetic
@@ -577,74 +413,7 @@ __global__ __launch_bounds__(kThreads) void decode_partition_kernel(DecodeArgs a
   }
   __syncthreads();
 
-  // ---- combine the waves (in wave order) ----
-  const int nw = (n_part + kWaveTokens - 1) / kWaveTokens;
-  for (int i = tid; i < group * D; i += kThreads) {
-    const int g = i / D, d = i - (i / D) * D;
-    float mx = s_ml[0][g][0];
-    for (int v = 1; v < nw; ++v) mx = fmaxf(mx, s_ml[v][g][0]);
-    float l = 0.0f, sum = 0.0f;
-    for (int v = 0; v < nw; ++v) {
-      const float wgt = __expf(s_ml[v][g][0] - mx);
-      l += s_ml[v][g][1] * wgt;
-      sum += s_acc[v][g][d] * wgt;
-    }
-    if (nparts == 1) {
-      a.out[(head0 + g) * D + d] = sum * (1.0f / l);
-    } else if (a.counters) {  // read by another workgroup of this launch: device-coherent stores
-      const size_t slot = (head0 + g) * a.parts_per_seq + part;
-      __hip_atomic_store(&a.part_acc[slot * D + d], sum, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-      if (d == 0) {
-        __hip_atomic_store(&a.part_ml[slot * 2], mx, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-        __hip_atomic_store(&a.part_ml[slot * 2 + 1], l, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-      }
-    } else {
-      const size_t slot = (head0 + g) * a.parts_per_seq + part;
-      a.part_acc[slot * D + d] = sum;
-      if (d == 0) {
-        a.part_ml[slot * 2] = mx;
-        a.part_ml[slot * 2 + 1] = l;
-      }
-    }
-  }
-  if (nparts <= 1 || a.counters == nullptr) return;  // workgroup-uniform
-
-  // ---- the last of the group's partitions to finish merges them ----
-  // Each thread waits until its coherent stores have completed, so when the counter shows
-  // every partition arrived, every partial is readable at the coherence point.  No cache-wide
-  // fence is used (a device-scope fence writes back the whole L2 of the XCD).  The last
-  // arriver resets the counter for the next launch or graph replay.
-  __shared__ float s_w[G][kMaxParts];
-  __shared__ float s_inv[G];
-  __shared__ int s_last;
-  __builtin_amdgcn_s_waitcnt(0);
-  __syncthreads();
-  if (tid == 0) {
-    const int unit = (SHARES ? blockIdx.y * pairs : 0) + pair;
-    const unsigned arrived =
-        __hip_atomic_fetch_add(&a.counters[unit], 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) + 1u;
-    s_last = arrived == static_cast<unsigned>(nparts);
-    if (s_last) __hip_atomic_store(&a.counters[unit], 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-  }
-  __syncthreads();
-  if (!s_last) return;
-  merge_unit<D, G, true>(a, head0, group, nparts, s_w, s_inv);
-}
-
-// The separate merge launch (used where the partition kernel does not merge): one workgroup
-// per (sequence, kv_head) group; sequences with a single partition were finished by the
-// partition kernel, and the launch boundary orders the partials' stores before these loads.
-template <int D, int MAXG, int WT>
-__global__ __launch_bounds__(kThreads) void decode_merge_kernel(DecodeArgs a) {
-  constexpr int kPartTokens = kWaves * WT;
-  __shared__ float s_w[MAXG][kMaxParts];
-  __shared__ float s_inv[MAXG];
-  const HeadUnit u = head_unit<true>(a, blockIdx.x);
-  if (u.heads <= 0) return;
-  const int ctx = min(a.context_lens[u.seq], a.parts_per_seq * kPartTokens);  // clamped as in the partitions
-  const int nparts = (ctx + kPartTokens - 1) / kPartTokens;
-  if (nparts <= 1) return;
-  merge_unit<D, MAXG, false>(a, u.head0, u.heads, nparts, s_w, s_inv);
+  combine_waves<D, G, WT, SHARES>(a, hu, pairs, pair, part, nparts, n_part, s_ml, s_acc);
 }
 
 // One workgroup per token: copies the token's [Hkv, D] K and V rows into their pool slot.
@@ -898,6 +667,22 @@ int32_t fi_buf_zero(fi_context* ctx, void* d_ptr, size_t bytes) {
   return zero_async(ctx, d_ptr, bytes);
 }
 
+int32_t fi_kv_pool_bytes(int32_t kv_dtype, int32_t num_blocks, int32_t block_size, int32_t num_kv_heads,
+                         int32_t head_dim, size_t* bytes) {
+  FI_REQUIRE(num_blocks > 0 && block_size > 0 && num_kv_heads > 0 && head_dim > 0, FI_ERR_INVALID_CONFIG,
+             "fi_kv_pool_bytes: pool dimensions must be greater than zero");
+  FI_REQUIRE(kv_dtype == FI_DTYPE_F32 || kv_dtype == FI_DTYPE_BF16 || kv_dtype == FI_DTYPE_MXFP4, FI_ERR_INVALID_TYPE,
+             "fi_kv_pool_bytes: KV dtype must be f32, bf16 or mxfp4");
+  FI_REQUIRE(bytes != nullptr, FI_ERR_INVALID_CONFIG, "fi_kv_pool_bytes: null pointer");
+  if (kv_dtype == FI_DTYPE_MXFP4) {
+    FI_TRY(fi::check_fp4_pool("fi_kv_pool_bytes", nullptr, nullptr, head_dim));
+    *bytes = fi::fp4_pool_bytes(num_blocks, num_kv_heads, block_size, head_dim);
+  } else {
+    *bytes = static_cast<size_t>(num_blocks) * num_kv_heads * block_size * head_dim * (kv_dtype == FI_DTYPE_F32 ? 4 : 2);
+  }
+  return FI_OK;
+}
+
 int32_t fi_kv_append(fi_context* ctx, const float* d_key, const float* d_value,
                      const int64_t* d_slot_mapping, int32_t num_tokens, void* d_k_cache,
                      void* d_v_cache, int32_t kv_dtype, int32_t num_blocks, int32_t block_size,
@@ -906,11 +691,15 @@ int32_t fi_kv_append(fi_context* ctx, const float* d_key, const float* d_value,
   FI_REQUIRE(num_tokens >= 0, FI_ERR_INVALID_SHAPE, "fi_kv_append: negative token count");
   FI_REQUIRE(num_blocks > 0 && block_size > 0 && num_kv_heads > 0 && head_dim > 0,
              FI_ERR_INVALID_CONFIG, "fi_kv_append: pool dimensions must be greater than zero");
-  FI_REQUIRE(kv_dtype == FI_DTYPE_F32 || kv_dtype == FI_DTYPE_BF16, FI_ERR_INVALID_TYPE,
-             "fi_kv_append: KV dtype must be f32 or bf16");
+  FI_REQUIRE(kv_dtype == FI_DTYPE_F32 || kv_dtype == FI_DTYPE_BF16 || kv_dtype == FI_DTYPE_MXFP4, FI_ERR_INVALID_TYPE,
+             "fi_kv_append: KV dtype must be f32, bf16 or mxfp4");
+  if (kv_dtype == FI_DTYPE_MXFP4) FI_TRY(fi::check_fp4_pool("fi_kv_append", d_k_cache, d_v_cache, head_dim));
   if (num_tokens == 0) return FI_OK;
   FI_REQUIRE(d_key && d_value && d_slot_mapping && d_k_cache && d_v_cache, FI_ERR_INVALID_CONFIG,
              "fi_kv_append: null pointer");
+  if (kv_dtype == FI_DTYPE_MXFP4)
+    return fi::kv_append_fp4(ctx, d_key, d_value, d_slot_mapping, num_tokens, d_k_cache, d_v_cache, num_blocks,
+                             block_size, num_kv_heads, head_dim);
   const int64_t pool_slots = static_cast<int64_t>(num_blocks) * block_size;
   const bool vec = head_dim % 4 == 0 && reinterpret_cast<uintptr_t>(d_key) % 16 == 0 &&
                    reinterpret_cast<uintptr_t>(d_value) % 16 == 0;
@@ -948,11 +737,18 @@ int32_t fi_kv_copy_blocks(fi_context* ctx, void* d_k_cache, void* d_v_cache, int
                           int32_t block_size, int32_t num_kv_heads, int32_t head_dim) {
   FI_TRY(fi::enter(ctx));
   FI_REQUIRE(num_pairs >= 0, FI_ERR_INVALID_SHAPE, "fi_kv_copy_blocks: negative pair count");
-  FI_REQUIRE(kv_dtype == FI_DTYPE_F32 || kv_dtype == FI_DTYPE_BF16, FI_ERR_INVALID_TYPE,
-             "fi_kv_copy_blocks: KV dtype must be f32 or bf16");
+  FI_REQUIRE(kv_dtype == FI_DTYPE_F32 || kv_dtype == FI_DTYPE_BF16 || kv_dtype == FI_DTYPE_MXFP4, FI_ERR_INVALID_TYPE,
+             "fi_kv_copy_blocks: KV dtype must be f32, bf16 or mxfp4");
   FI_REQUIRE(num_blocks > 0 && block_size > 0 && num_kv_heads > 0 && head_dim > 0,
              FI_ERR_INVALID_CONFIG, "fi_kv_copy_blocks: pool dimensions must be greater than zero");
+  if (kv_dtype == FI_DTYPE_MXFP4) FI_TRY(fi::check_fp4_pool("fi_kv_copy_blocks", d_k_cache, d_v_cache, head_dim));
   if (num_pairs == 0) return FI_OK;
+  if (kv_dtype == FI_DTYPE_MXFP4) {
+    FI_REQUIRE(d_k_cache && d_v_cache && d_src_blocks && d_dst_blocks && d_token_counts, FI_ERR_INVALID_CONFIG,
+               "fi_kv_copy_blocks: null pointer");
+    return fi::kv_copy_blocks_fp4(ctx, d_k_cache, d_v_cache, d_src_blocks, d_dst_blocks, d_token_counts, num_pairs,
+                                  num_blocks, block_size, num_kv_heads, head_dim);
+  }
   dim3 grid(static_cast<unsigned>(num_pairs) * num_kv_heads);
   if (kv_dtype == FI_DTYPE_F32) {
     hipLaunchKernelGGL(kv_copy_blocks_kernel<float>, grid, dim3(256), 0, ctx->stream,
@@ -975,11 +771,12 @@ int32_t fi_kv_gather(fi_context* ctx, const void* d_k_cache, const void* d_v_cac
                      float* d_k_out, float* d_v_out) {
   FI_TRY(fi::enter(ctx));
   FI_REQUIRE(length >= 0 && num_table_blocks >= 0, FI_ERR_INVALID_SHAPE, "fi_kv_gather: negative sizes");
-  FI_REQUIRE(kv_dtype == FI_DTYPE_F32 || kv_dtype == FI_DTYPE_BF16, FI_ERR_INVALID_TYPE,
-             "fi_kv_gather: KV dtype must be f32 or bf16");
+  FI_REQUIRE(kv_dtype == FI_DTYPE_F32 || kv_dtype == FI_DTYPE_BF16 || kv_dtype == FI_DTYPE_MXFP4, FI_ERR_INVALID_TYPE,
+             "fi_kv_gather: KV dtype must be f32, bf16 or mxfp4");
   FI_REQUIRE(num_blocks > 0 && block_size > 0 && num_kv_heads > 0 && head_dim > 0, FI_ERR_INVALID_CONFIG,
              "fi_kv_gather: pool dimensions must be greater than zero");
   FI_REQUIRE(head_dim % 4 == 0, FI_ERR_UNSUPPORTED, "fi_kv_gather: head_dim must be a multiple of 4");
+  if (kv_dtype == FI_DTYPE_MXFP4) FI_TRY(fi::check_fp4_pool("fi_kv_gather", d_k_cache, d_v_cache, head_dim));
   // paged_kv.rs:303-308: a prefix longer than the sequence's pages
   FI_REQUIRE(static_cast<int64_t>(length) <= static_cast<int64_t>(num_table_blocks) * block_size, FI_ERR_RUNTIME,
              "fi_kv_gather: KV cache block table ran out of committed pages");
@@ -989,6 +786,9 @@ int32_t fi_kv_gather(fi_context* ctx, const void* d_k_cache, const void* d_v_cac
   FI_REQUIRE(((reinterpret_cast<uintptr_t>(d_k_cache) | reinterpret_cast<uintptr_t>(d_v_cache) |
                reinterpret_cast<uintptr_t>(d_k_out) | reinterpret_cast<uintptr_t>(d_v_out)) & 15) == 0,
              FI_ERR_INVALID_LAYOUT, "fi_kv_gather: pools and outputs must be 16-byte aligned (vector accesses)");
+  if (kv_dtype == FI_DTYPE_MXFP4)
+    return fi::kv_gather_fp4(ctx, d_k_cache, d_v_cache, d_block_table, length, num_blocks, block_size, num_kv_heads,
+                             head_dim, d_k_out, d_v_out);
   const int64_t quads = static_cast<int64_t>(length) * num_kv_heads * (head_dim / 4);
   const unsigned grid = static_cast<unsigned>(std::min<int64_t>((quads + 255) / 256, 4096));
   if (kv_dtype == FI_DTYPE_F32) {
@@ -1041,6 +841,10 @@ int head_split(int64_t whole, int group, int parts, bool bf16, int64_t cus) {
   return whole <= limit ? 2 : 1;
 }
 
+// Over a 4-bit pool a workgroup's arithmetic goes by tiles of four heads: groups of more are cut in
+// two where that leaves every workgroup a CU.
+int head_split_fp4(int64_t whole, int group, int64_t cus) { return group > 4 && 2 * whole <= cus ? 2 : 1; }
+
 // Shared by both decode entry points: validation, launch shape and launches.  With
 // `noalloc` the partials go to the library's fixed scratch array instead of the context
 // workspace (nothing is allocated).
@@ -1071,8 +875,8 @@ int32_t decode_paged(fi_context* ctx, const float* d_q, const void* d_k_cache, c
              FI_ERR_INVALID_SHAPE, "number of query heads must be divisible by number of KV heads");
   FI_REQUIRE(block_size > 0 && num_blocks > 0 && max_blocks_per_seq > 0, FI_ERR_INVALID_CONFIG,
              "fi_attn_decode_paged: pool dimensions must be greater than zero");
-  FI_REQUIRE(kv_dtype == FI_DTYPE_F32 || kv_dtype == FI_DTYPE_BF16, FI_ERR_INVALID_TYPE,
-             "fi_attn_decode_paged: KV dtype must be f32 or bf16");
+  FI_REQUIRE(kv_dtype == FI_DTYPE_F32 || kv_dtype == FI_DTYPE_BF16 || kv_dtype == FI_DTYPE_MXFP4, FI_ERR_INVALID_TYPE,
+             "fi_attn_decode_paged: KV dtype must be f32, bf16 or mxfp4");
   FI_REQUIRE(static_cast<int64_t>(max_context_len) <= static_cast<int64_t>(max_blocks_per_seq) * block_size,
              FI_ERR_INVALID_SHAPE, "fi_attn_decode_paged: max_context_len exceeds the block-table width");
   FI_REQUIRE(head_dim == 32 || head_dim == 64 || head_dim == 128, FI_ERR_UNSUPPORTED,
@@ -1092,6 +896,13 @@ int32_t decode_paged(fi_context* ctx, const float* d_q, const void* d_k_cache, c
   if (num_seqs == 0) return FI_OK;
   FI_REQUIRE((d_q || qkv) && d_k_cache && d_v_cache && d_block_tables && d_context_lens && d_out,
              FI_ERR_INVALID_CONFIG, "fi_attn_decode_paged: null pointer");
+  if (kv_dtype == FI_DTYPE_MXFP4) {
+    FI_TRY(fi::check_fp4_pool("fi_attn_decode_paged", d_k_cache, d_v_cache, head_dim));
+    FI_REQUIRE((reinterpret_cast<uintptr_t>(d_q) & 15) == 0, FI_ERR_INVALID_LAYOUT,
+               "fi_attn_decode_paged: q must be 16-byte aligned (vector accesses)");
+    FI_REQUIRE(num_q_heads / num_kv_heads <= 8, FI_ERR_UNSUPPORTED,
+               "decode attention supports at most 8 query heads per KV head");
+  }
   if (qkv) {
     auto aligned16 = [](const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; };
     FI_REQUIRE(qkv->parts && qkv->positions && qkv->slots, FI_ERR_INVALID_CONFIG,
@@ -1154,7 +965,8 @@ int32_t decode_paged(fi_context* ctx, const float* d_q, const void* d_k_cache, c
   }
   const int64_t cus = ctx->compute_units > 0 ? ctx->compute_units : 256;
   const int64_t whole = static_cast<int64_t>(num_seqs) * num_kv_heads * parts;  // workgroups with whole groups
-  const int shares = head_split(whole, args.group, parts, kv_dtype == FI_DTYPE_BF16, cus);
+  const int shares = kv_dtype == FI_DTYPE_MXFP4 ? head_split_fp4(whole, args.group, cus)
+                                               : head_split(whole, args.group, parts, kv_dtype == FI_DTYPE_BF16, cus);
   args.heads_per = (args.group + shares - 1) / shares;
   const dim3 grid(static_cast<unsigned>(whole), static_cast<unsigned>(shares));
   // Small launches (at most six workgroups a CU, e.g. a decode tick of a small model) merge
@@ -1165,6 +977,7 @@ int32_t decode_paged(fi_context* ctx, const float* d_q, const void* d_k_cache, c
   if (parts > 1 && !noalloc && ctx->d_merge_counters != nullptr &&
       static_cast<int64_t>(num_seqs) * num_kv_heads * shares <= FI_MERGE_COUNTERS && whole <= 6 * cus)
     args.counters = ctx->d_merge_counters;
+  if (kv_dtype == FI_DTYPE_MXFP4) return fi::decode_fp4(ctx, args, head_dim, grid, wt);
   switch (head_dim) {
     case 32:
       return launch_decode_dtype<32>(ctx, kv_dtype, args, grid, wt);
@@ -1204,11 +1017,12 @@ int32_t fi_attn_decode_paged_qkv(fi_context* ctx, const float* d_qkv_parts, int3
   // Large launches (more than six workgroups a CU) run the consumer and the attention as two
   // launches: every workgroup of the fused kernel forms its query rows again (one more
   // dependent load round each), which costs more there than the consumer launch (C5's
-  // 256-sequence decode, 32768 workgroups: 27.4 against 24.7 ms a tick).
+  // 256-sequence decode, 32768 workgroups: 27.4 against 24.7 ms a tick).  4-bit pools always do: a
+  // group's scale needs 32 elements of the row at once.
   const int part_tokens = kWaves * wave_tokens_for(num_kv_heads, head_dim);
   const int64_t parts = max_context_len == 0 ? 1 : (max_context_len + part_tokens - 1) / part_tokens;
   const int64_t cus = ctx->compute_units > 0 ? ctx->compute_units : 256;
-  if (static_cast<int64_t>(num_seqs) * num_kv_heads * parts > 6 * cus) {
+  if (kv_dtype == FI_DTYPE_MXFP4 || static_cast<int64_t>(num_seqs) * num_kv_heads * parts > 6 * cus) {
     FI_REQUIRE(d_q_out != nullptr, FI_ERR_INVALID_CONFIG, "fi_attn_decode_paged_qkv: null q_out");
     FI_TRY(fi_qkv_rope_append(ctx, d_qkv_parts, splits, d_bias_q, d_bias_k, d_bias_v, d_positions, d_cos, d_sin,
                               rotary_dims, max_positions, d_slot_mapping, d_k_cache, d_v_cache, kv_dtype, num_blocks,

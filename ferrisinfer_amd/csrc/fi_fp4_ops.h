@@ -1,0 +1,33 @@
+// Launches over 4-bit KV pools, called by the pool entry points once their arguments are checked.
+#pragma once
+
+#include "fi_common.h"
+
+namespace fi {
+
+struct DecodeArgs;
+
+// What every entry point requires of a 4-bit pool beyond a pool's own checks: head_dim 32, 64 or
+// 128 (whole groups, and the head dims of the attention kernels) and 16-byte aligned arrays.
+inline int32_t check_fp4_pool(const char* name, const void* k_cache, const void* v_cache, int32_t head_dim) {
+  FI_REQUIRE(head_dim == 32 || head_dim == 64 || head_dim == 128, FI_ERR_UNSUPPORTED,
+             std::string(name) + ": a 4-bit pool needs head_dim 32, 64 or 128");
+  FI_REQUIRE(((reinterpret_cast<uintptr_t>(k_cache) | reinterpret_cast<uintptr_t>(v_cache)) & 15) == 0,
+             FI_ERR_INVALID_LAYOUT, std::string(name) + ": a 4-bit pool must be 16-byte aligned (vector accesses)");
+  return FI_OK;
+}
+
+int32_t kv_append_fp4(fi_context* ctx, const float* key, const float* value, const int64_t* slots, int32_t num_tokens,
+                      void* k_cache, void* v_cache, int32_t num_blocks, int32_t block_size, int32_t hkv, int32_t d);
+
+int32_t kv_copy_blocks_fp4(fi_context* ctx, void* k_cache, void* v_cache, const int32_t* src, const int32_t* dst,
+                           const int32_t* counts, int32_t num_pairs, int32_t num_blocks, int32_t block_size,
+                           int32_t hkv, int32_t d);
+
+int32_t kv_gather_fp4(fi_context* ctx, const void* k_cache, const void* v_cache, const int32_t* table, int32_t length,
+                      int32_t num_blocks, int32_t block_size, int32_t hkv, int32_t d, float* k_out, float* v_out);
+
+// Decode attention: the partition launch and, where the launch does not merge by itself, the merge.
+int32_t decode_fp4(fi_context* ctx, const DecodeArgs& args, int32_t head_dim, dim3 grid, int wave_tokens);
+
+}  // namespace fi

@@ -27,6 +27,7 @@
 
 #include "fi_common.h"
 #include "fi_device.h"
+#include "fi_qkv_norm.h"
 
 extern "C" int32_t fi_weight_packed_floats(int32_t k, int32_t n, int32_t pack_width, size_t* floats);
 
@@ -1535,6 +1536,29 @@ int32_t fi_qkv_rope_append(fi_context* ctx, const float* d_parts, int32_t splits
                            int32_t max_positions, const int64_t* d_slot_mapping, void* d_k_cache, void* d_v_cache,
                            int32_t kv_dtype, int32_t num_blocks, int32_t block_size, int32_t num_tokens,
                            int32_t num_q_heads, int32_t num_kv_heads, int32_t head_dim, float* d_q_out) {
+  if (kv_dtype == FI_DTYPE_MXFP4) {
+    fi::QkvNormArgs a{};
+    a.parts = d_parts;
+    a.splits = splits;
+    a.bias_q = d_bias_q;
+    a.bias_k = d_bias_k;
+    a.bias_v = d_bias_v;
+    a.positions = d_positions;
+    a.num_axes = 1;
+    a.cos_t = d_cos;
+    a.sin_t = d_sin;
+    a.rotary_dims = rotary_dims;
+    a.max_positions = max_positions;
+    a.slots = d_slot_mapping;
+    a.k_cache = d_k_cache;
+    a.v_cache = d_v_cache;
+    a.block_size = block_size;
+    a.tokens = num_tokens;
+    a.hq = num_q_heads;
+    a.hkv = num_kv_heads;
+    a.q_out = d_q_out;
+    return fi::qkv_norm_rope_append(ctx, "fi_qkv_rope_append", a, head_dim, kv_dtype, num_blocks, nullptr);
+  }
   FI_TRY(fi::enter(ctx));
   FI_REQUIRE(num_tokens >= 0 && splits >= 1, FI_ERR_INVALID_SHAPE, "fi_qkv_rope_append: bad shape");
   FI_REQUIRE(num_q_heads > 0 && num_kv_heads > 0 && head_dim > 0 && num_q_heads % num_kv_heads == 0,
@@ -1543,7 +1567,7 @@ int32_t fi_qkv_rope_append(fi_context* ctx, const float* d_parts, int32_t splits
              "rope.rotary_dims must be even and at most the head dimension");
   FI_REQUIRE(num_blocks > 0 && block_size > 0, FI_ERR_INVALID_CONFIG, "fi_qkv_rope_append: pool dimensions must be positive");
   FI_REQUIRE(kv_dtype == FI_DTYPE_F32 || kv_dtype == FI_DTYPE_BF16, FI_ERR_INVALID_TYPE,
-             "fi_qkv_rope_append: KV dtype must be f32 or bf16");
+             "fi_qkv_rope_append: KV dtype must be f32, bf16 or mxfp4");
   if (num_tokens == 0) return FI_OK;
   FI_REQUIRE(d_parts && d_positions && d_slot_mapping && d_k_cache && d_v_cache && d_q_out, FI_ERR_INVALID_CONFIG,
              "fi_qkv_rope_append: null pointer");

@@ -22,6 +22,7 @@ ERROR_KINDS = ["Io", "Parse", "InvalidShape", "InvalidLayout", "InvalidType", "I
 DTYPE_F32 = 0
 DTYPE_BF16 = 1
 DTYPE_F16 = 2
+DTYPE_MXFP4 = 3  # KV pools only: 4-bit codes in groups of 32 with a power-of-two scale
 
 
 class FerrisError(RuntimeError):
@@ -65,6 +66,7 @@ _SIGNATURES = {
     "fi_event_wait": [_P],
     "fi_event_destroy": [_P],
     "fi_token_feed": [_P, _P, _I32, _P, _I32, _P],
+    "fi_kv_pool_bytes": [_I32, _I32, _I32, _I32, _I32, C.POINTER(_SZ)],
     "fi_kv_append": [_P, _P, _P, _P, _I32, _P, _P, _I32, _I32, _I32, _I32, _I32],
     "fi_kv_copy_blocks": [_P, _P, _P, _I32, _P, _P, _P, _I32, _I32, _I32, _I32, _I32],
     "fi_kv_gather": [_P, _P, _P, _I32, _P, _I32, _I32, _I32, _I32, _I32, _I32, _P, _P],
@@ -95,6 +97,8 @@ _SIGNATURES = {
     "fi_splitk_residual_rms_norm": [_P, _P, _I32, _P, _P, _P, _P, _P, _I32, _I32, _F32],
     "fi_qkv_rope_append": [_P, _P, _I32, _P, _P, _P, _P, _P, _P, _I32, _I32, _P, _P, _P, _I32, _I32,
                            _I32, _I32, _I32, _I32, _I32, _P],
+    "fi_qkv_norm_rope_append": [_P, _P, _I32, _P, _P, _P, _P, _P, _F32, _P, _I32, C.POINTER(_I32), _P, _P, _I32,
+                                _I32, _P, _P, _P, _I32, _I32, _I32, _I32, _I32, _I32, _I32, _P],
     "fi_weight_pack_columns": [_P, C.POINTER(_P), C.POINTER(_I32), _I32, _I32, _I32, _P],
     "fi_attn_prefill_paged_bf16": [_P, _P, _P, _P, _P, _I32, _P, _P, _I32, _I32, _I32, _I32, _I32, _I32,
                                    _I32, _F32, _P],
@@ -169,6 +173,14 @@ def ptr(t) -> int | None:
     if isinstance(t, int):
         return t
     return t.data_ptr()
+
+
+def kv_pool_bytes(kv_dtype, num_blocks, block_size, num_kv_heads, head_dim) -> int:
+    """Bytes of one K or V pool array of a layer."""
+    out = _SZ()
+    check(load().fi_kv_pool_bytes(int(kv_dtype), int(num_blocks), int(block_size), int(num_kv_heads),
+                                  int(head_dim), C.byref(out)))
+    return int(out.value)
 
 
 class Context:
@@ -539,3 +551,25 @@ class Context:
                                           int(block_size), int(positions.numel()),
                                           int(num_q_heads), int(num_kv_heads), int(head_dim),
                                           ptr(q_out)))
+
+    def qkv_norm_rope_append(self, parts, splits, biases, norms, eps, positions, pair_axes, cos_t, sin_t,
+                             rotary_dims, max_positions, slot_mapping, k_cache, v_cache, kv_dtype,
+                             num_blocks, block_size, num_q_heads, num_kv_heads, head_dim, q_out):
+        """qkv_rope_append with RMS norms of the query and key heads (norms: a pair of [D] weights,
+        either may be None, or None) and positions int32 [T] or [axes, T]; pair_axes names each
+        rotary pair's axis (a sequence of rotary_dims / 2 ints, or None with one axis)."""
+        bq, bk, bv = biases if biases is not None else (None, None, None)
+        nq, nk = norms if norms is not None else (None, None)
+        axes = 1 if positions.dim() == 1 else int(positions.shape[0])
+        if not positions.is_contiguous():
+            raise FerrisError(4, "qkv_norm_rope_append: positions must be contiguous")
+        if pair_axes is not None and len(pair_axes) != int(rotary_dims) // 2:
+            raise FerrisError(3, "qkv_norm_rope_append: pair_axes needs rotary_dims / 2 entries")
+        named = None if pair_axes is None else (_I32 * max(len(pair_axes), 1))(*[int(x) for x in pair_axes])
+        check(self.lib.fi_qkv_norm_rope_append(self.handle, ptr(parts), int(splits), ptr(bq), ptr(bk), ptr(bv),
+                                               ptr(nq), ptr(nk), float(eps), ptr(positions), axes, named,
+                                               ptr(cos_t), ptr(sin_t), int(rotary_dims), int(max_positions),
+                                               ptr(slot_mapping), ptr(k_cache), ptr(v_cache), int(kv_dtype),
+                                               int(num_blocks), int(block_size), int(positions.shape[-1]),
+                                               int(num_q_heads), int(num_kv_heads), int(head_dim),
+                                               ptr(q_out)))

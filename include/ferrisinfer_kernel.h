@@ -25,7 +25,7 @@
  *   activations are row-major f32: q [T, Hq, D], k/v [T, Hkv, D], hidden [T, H];
  *   weights are [in, out] row-major f32 (model/decoder.rs:76-104);
  *   the KV pool holds, per layer, K and V arrays [num_blocks, Hkv, block_size, D] in
- *   f32 or bf16; physical slot = block_id * block_size + offset
+ *   f32, bf16 or 4 bits (below); physical slot = block_id * block_size + offset
  *   (runtime/paged_kv.rs:605-606);
  *   block_tables is int32 [num_seqs, max_blocks_per_seq]; context_lens int32 [num_seqs];
  *   cu_seqlens int32 [num_seqs + 1]; slot_mapping int64 [T] (negative = skip).
@@ -53,9 +53,21 @@ enum {
   FI_ERR_RUNTIME = 9
 };
 
-/* Element dtypes: KV storage (core/dtype.rs:1-42 F32 / BF16) and, with F16, the safetensors
- * payloads fi_convert_to_f32 imports (io/safetensors.rs:11-16). */
-enum { FI_DTYPE_F32 = 0, FI_DTYPE_BF16 = 1, FI_DTYPE_F16 = 2 };
+/* Element dtypes: KV storage (core/dtype.rs:1-42 F32 / BF16; MXFP4 has no counterpart in the
+ * reference) and, with F16, the safetensors payloads fi_convert_to_f32 imports
+ * (io/safetensors.rs:11-16).
+ *
+ * FI_DTYPE_MXFP4, 4-bit KV storage: each group of 32 consecutive elements of a head's row holds 32
+ * e2m1 codes (bit 3 the sign, bits 0-2 the magnitude 0, 0.5, 1, 1.5, 2, 3, 4, 6) and one scale byte
+ * E; an element's value is magnitude * 2^(E - 127), exactly, and E = 255 makes the group NaN.  17
+ * bytes for 32 elements.  A pool array (K or V of one layer, fi_kv_pool_bytes bytes, 16-byte
+ * aligned) is the codes [num_blocks, Hkv, block_size, D / 2], element 2 i of a row in the low half
+ * of its byte i, followed by the scales [num_blocks, Hkv, block_size, D / 32].  Appending takes the
+ * smallest scale 2^(E - 127), E in [2, 252], with every magnitude of the group below 7 scales (off
+ * by at most half a step; larger ones are cut off at 6 * 2^125) and rounds to the nearest code, ties
+ * to the even one; a group that holds an infinity or a NaN gets E = 255.  head_dim must be 32, 64 or
+ * 128 (Unsupported otherwise). */
+enum { FI_DTYPE_F32 = 0, FI_DTYPE_BF16 = 1, FI_DTYPE_F16 = 2, FI_DTYPE_MXFP4 = 3 };
 
 typedef struct fi_context fi_context;
 
@@ -162,8 +174,14 @@ int32_t fi_token_feed(fi_context* ctx, const int32_t* d_prev_tokens, int32_t pre
 
 /* ---------------------------------------------------------------- KV pool ops */
 
+/* Bytes of one K or V pool array of a layer (num_blocks * Hkv * block_size rows of head_dim
+ * elements of kv_dtype).  Host arithmetic only; no counterpart in the reference. */
+int32_t fi_kv_pool_bytes(int32_t kv_dtype, int32_t num_blocks, int32_t block_size, int32_t num_kv_heads,
+                         int32_t head_dim, size_t* bytes);
+
 /* Scatters this step's K/V rows into the paged pool by slot_mapping, converting f32 to the
- * pool dtype (bf16: round-to-nearest-even).  Replaces KvCacheStorage::write_uncommitted_f32
+ * pool dtype (bf16: round-to-nearest-even; mxfp4: see FI_DTYPE_MXFP4).  A slot named by several
+ * rows of one call is left unspecified.  Replaces KvCacheStorage::write_uncommitted_f32
  * and write_sequence_uncommitted_f32 (runtime/kv_cache.rs:48-62; paged write path
  * runtime/paged_kv.rs:583-631, 679-767).  Rows whose slot is negative are skipped; a slot
  * beyond num_blocks * block_size is skipped and reported as Runtime by the next
@@ -183,7 +201,7 @@ int32_t fi_kv_copy_blocks(fi_context* ctx, void* d_k_cache, void* d_v_cache, int
                           int32_t block_size, int32_t num_kv_heads, int32_t head_dim);
 
 /* Gathers the first `length` token rows of one sequence's K and V from the paged pool of one
- * layer into contiguous f32 [length, Hkv, D] tensors (bf16 pools widen exactly, bits << 16).
+ * layer into contiguous f32 [length, Hkv, D] tensors (bf16 and mxfp4 pools widen exactly).
  * Replaces KvCacheStorage::read_prefix_f32 (runtime/kv_cache.rs:63) over paged storage:
  * PagedKvCacheStorage::read_prefix_f32 concatenating pages by block table
  * (runtime/paged_kv.rs:769-791, block_table at :260-314).  block_table holds the sequence's
@@ -211,7 +229,9 @@ int32_t fi_ctx_check_faults(fi_context* ctx);
  * cached_prefixed_causal_attention_f32 (runtime/reference.rs:497-508,
  * runtime/paged_kv.rs:769-791, kernel/cpu/attention.rs:332-518) and
  * decode_causal_attention_f32 (kernel/cpu/attention.rs:520-686).
- * q/out: f32 [num_seqs, Hq, D]; scale is 1/sqrt(D) in the reference (attention.rs:659).
+ * q/out: f32 [num_seqs, Hq, D]; scale is 1/sqrt(D) in the reference (attention.rs:659).  Scores,
+ * softmax and sums are f32 whatever the pool's dtype, and the pool's values enter them exactly;
+ * over an mxfp4 pool q must be 16-byte aligned (InvalidLayout otherwise).
  * max_context_len must bound every context_lens entry (it sizes the grid); an entry beyond
  * the partitions it sizes is clamped to them on device and reported as Runtime by
  * fi_ctx_check_faults. */
@@ -234,7 +254,7 @@ int32_t fi_attn_decode_paged(fi_context* ctx, const float* d_q, const void* d_k_
  * positions[b]); the workgroup holding a sequence's last partition appends the K/V row of its
  * kv head before reading the keys.  Launches of more than six workgroups a CU (large batches
  * of long contexts) run the two calls instead, with q_out [num_seqs, Hq, D] as the query
- * buffer between them; q_out is left unwritten otherwise.  Outputs and the pool contents
+ * buffer between them, and so do mxfp4 pools; q_out is left unwritten otherwise.  Outputs and the pool contents
  * equal those of the two calls bit for bit either way.  rotary_dims / 2 and head_dim - rotary_dims must be multiples of 4
  * (Unsupported otherwise); the partials, biases and RoPE tables 16-byte aligned.  A slot or a
  * position out of range is reported as by fi_qkv_rope_append. */
@@ -438,6 +458,29 @@ int32_t fi_qkv_rope_append(fi_context* ctx, const float* d_parts, int32_t splits
                            const int64_t* d_slot_mapping, void* d_k_cache, void* d_v_cache, int32_t kv_dtype,
                            int32_t num_blocks, int32_t block_size, int32_t num_tokens, int32_t num_q_heads,
                            int32_t num_kv_heads, int32_t head_dim, float* d_q_out);
+
+/* fi_qkv_rope_append for decoders that normalise their query and key heads, and for positions of
+ * several axes (time, height and width of images and video).  No counterpart in the reference,
+ * whose block has neither (runtime/reference.rs:163-300).  In this order:
+ *   x = sum of the splits + bias;
+ *   each query (key) head's row x becomes x / sqrt(mean(x^2) + eps) * d_q_norm (d_k_norm), a weight
+ *   [D] shared by the heads; a NULL weight leaves the heads as they are;
+ *   rotary pair i (elements i and i + rotary_dims / 2) turns by row positions[pair_axes[i]][t] of the
+ *   tables; d_positions is int32 [num_axes, T] and pair_axes a HOST array of rotary_dims / 2 entries in
+ *   [0, num_axes), read during the call (NULL with one axis);
+ *   q to d_q_out [T, Hq, D], k and v appended to the pool by slot_mapping (as fi_kv_append).
+ * With NULL weights and one axis the results equal fi_qkv_rope_append's bit for bit.  head_dim must be
+ * 32, 64 or 128 and rotary_dims / 2 a multiple of 4 (Unsupported otherwise); num_axes 1 to 4 and eps
+ * finite and not negative (InvalidConfig); every float array, q_out and the pools 16-byte aligned
+ * (InvalidLayout).  A slot or a position out of range is reported as by fi_qkv_rope_append.
+ * fi_qkv_rope_append over an mxfp4 pool has the same requirements. */
+int32_t fi_qkv_norm_rope_append(fi_context* ctx, const float* d_parts, int32_t splits, const float* d_bias_q,
+                                const float* d_bias_k, const float* d_bias_v, const float* d_q_norm,
+                                const float* d_k_norm, float eps, const int32_t* d_positions, int32_t num_axes,
+                                const int32_t* pair_axes, const float* d_cos, const float* d_sin, int32_t rotary_dims,
+                                int32_t max_positions, const int64_t* d_slot_mapping, void* d_k_cache, void* d_v_cache,
+                                int32_t kv_dtype, int32_t num_blocks, int32_t block_size, int32_t num_tokens,
+                                int32_t num_q_heads, int32_t num_kv_heads, int32_t head_dim, float* d_q_out);
 
 /* ---- Projections over bf16-stored weights (bf16 configurations) ----
  * The reference loads bf16 weights by exact widening (io/safetensors.rs:540-542) and runs the
