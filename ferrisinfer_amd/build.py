@@ -22,6 +22,7 @@ SOURCES = [
     "fi_kv_fp4.hip",
     "fi_qkv_norm.hip",
     "fi_prefill.hip",
+    "fi_prefill_fp4.hip",
     "fi_ops.hip",
     "fi_gemm.hip",
     "fi_gemm_packed.hip",

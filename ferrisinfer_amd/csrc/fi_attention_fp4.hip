@@ -28,31 +28,6 @@ namespace {
 typedef float v4f __attribute__((ext_vector_type(4)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 
-// kBytes of codes from p, in one load (16, 8, 4, 2 or 1 bytes).
-template <int kBytes>
-struct Codes {
-  uint32_t w[kBytes < 4 ? 1 : kBytes / 4];
-  __device__ __forceinline__ void load(const uint8_t* p) {
-    if constexpr (kBytes == 16) {
-      const uint4 v = *reinterpret_cast<const uint4*>(p);
-      w[0] = v.x;
-      w[1] = v.y;
-      w[2] = v.z;
-      w[3] = v.w;
-    } else if constexpr (kBytes == 8) {
-      const uint2 v = *reinterpret_cast<const uint2*>(p);
-      w[0] = v.x;
-      w[1] = v.y;
-    } else if constexpr (kBytes == 4) {
-      w[0] = *reinterpret_cast<const uint32_t*>(p);
-    } else if constexpr (kBytes == 2) {
-      w[0] = *reinterpret_cast<const uint16_t*>(p);
-    } else {
-      w[0] = *p;
-    }
-  }
-};
-
 // The sum over the four lanes of a quad, in every lane.
 __device__ __forceinline__ float quad_sum(float v) { return fi::group_sum<4>(v); }
 
@@ -170,7 +145,7 @@ __global__ __launch_bounds__(kThreads, 2) void decode_fp4_kernel(DecodeArgs a) {
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
         const size_t row = rows[min(32 * s + 16 * i + m, n - 1)];
-        Codes<KB> kc;
+        fi::Codes<KB> kc;
         kc.load(k_codes + row * (D / 2) + kb * KB);
         const float scale = fi::fp4_scale_f32(k_scales[row * GROUPS + kb * GROUPS / 4]);
         v4f acc[T];
@@ -228,7 +203,7 @@ __global__ __launch_bounds__(kThreads, 2) void decode_fp4_kernel(DecodeArgs a) {
 #pragma unroll
     for (int s = 0; s < STEPS; ++s) {
       if (32 * s >= n) break;  // wave-uniform: the step holds no key
-      Codes<VB> vc[8];
+      fi::Codes<VB> vc[8];
       float scale[8];
 #pragma unroll
       for (int e = 0; e < 8; ++e) {

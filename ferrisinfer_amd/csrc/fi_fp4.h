@@ -13,6 +13,8 @@
 // A group with an infinity or a NaN has E = 255 and codes 0, and reads as NaN throughout.
 #pragma once
 
+#include <type_traits>
+
 #include "fi_device.h"
 
 namespace fi {
@@ -87,6 +89,31 @@ __device__ __forceinline__ float4 bf16x4_to_f32(uint32_t lo, uint32_t hi) {
   return make_float4(bf16_bits_to_f32(lo & 0xffffu), bf16_bits_to_f32(lo >> 16), bf16_bits_to_f32(hi & 0xffffu),
                      bf16_bits_to_f32(hi >> 16));
 }
+
+// kBytes of codes from p, in one load (16, 8, 4, 2 or 1 bytes).
+template <int kBytes>
+struct Codes {
+  uint32_t w[kBytes < 4 ? 1 : kBytes / 4];
+  __device__ __forceinline__ void load(const uint8_t* p) {
+    if constexpr (kBytes == 16) {
+      const uint4 v = *reinterpret_cast<const uint4*>(p);
+      w[0] = v.x;
+      w[1] = v.y;
+      w[2] = v.z;
+      w[3] = v.w;
+    } else if constexpr (kBytes == 8) {
+      const uint2 v = *reinterpret_cast<const uint2*>(p);
+      w[0] = v.x;
+      w[1] = v.y;
+    } else if constexpr (kBytes == 4) {
+      w[0] = *reinterpret_cast<const uint32_t*>(p);
+    } else if constexpr (kBytes == 2) {
+      w[0] = *reinterpret_cast<const uint16_t*>(p);
+    } else {
+      w[0] = *p;
+    }
+  }
+};
 
 // Eight consecutive elements of a group held by four neighbouring lanes: their codes, with the
 // group's scale byte.

@@ -6,6 +6,7 @@
 namespace fi {
 
 struct DecodeArgs;
+struct PrefillArgs;
 
 // What every entry point requires of a 4-bit pool beyond a pool's own checks: head_dim 32, 64 or
 // 128 (whole groups, and the head dims of the attention kernels) and 16-byte aligned arrays.
@@ -29,5 +30,8 @@ int32_t kv_gather_fp4(fi_context* ctx, const void* k_cache, const void* v_cache,
 
 // Decode attention: the partition launch and, where the launch does not merge by itself, the merge.
 int32_t decode_fp4(fi_context* ctx, const DecodeArgs& args, int32_t head_dim, dim3 grid, int wave_tokens);
+
+// Prefill attention, its arguments checked as the other pools'.
+int32_t prefill_fp4(fi_context* ctx, const PrefillArgs& args, int32_t head_dim);
 
 }  // namespace fi

@@ -1,7 +1,8 @@
 // Varlen causal prefill attention over the paged KV pool, on MFMA.  f32 pools run
 // prefill_x3_kernel (f32 accuracy from three-piece bf16 products on v_mfma_f32_16x16x32_bf16,
 // at the end of this file); bf16 pools run prefill_kernel (K/V widened exactly, f32 MFMA,
-// v_mfma_f32_16x16x4_f32) or, through fi_attn_prefill_paged_bf16, prefill_bf16_kernel.
+// v_mfma_f32_16x16x4_f32) or, through fi_attn_prefill_paged_bf16, prefill_bf16_kernel; 4-bit pools
+// run prefill_fp4_kernel (fi_prefill_fp4.hip).
 // Replaces causal_self_attention_f32 / prefixed_causal_attention_f32 /
 // cached_prefixed_causal_attention_f32 (crates/ferrisinfer-kernel/src/cpu/attention.rs:222-518,
 // 688-962) plus the paged prefix gather that feeds them (runtime/paged_kv.rs:769-791,
@@ -28,109 +29,12 @@
 // and leave the device idle behind them.
 #include "fi_common.h"
 #include "fi_device.h"
+#include "fi_fp4_ops.h"
+#include "fi_prefill.h"
 
 namespace {
 
-typedef float v4f __attribute__((ext_vector_type(4)));
-
-constexpr int kThreads = 256;
-constexpr int kRows = 64;     // (head, token) rows per workgroup
 constexpr int kKeys = 32;     // keys per staged chunk
-
-struct PrefillArgs {
-  const float* q;            // [T, Hq, D]
-  const void* k_cache;       // [blocks, Hkv, bs, D]
-  const void* v_cache;
-  const int* cu_seqlens;     // [B+1]
-  const int* context_lens;   // [B]
-  const int* block_tables;   // [B, max_blocks]
-  float* out;                // [T, Hq, D]
-  uint32_t* faults;
-  int max_blocks;
-  int hq, hkv, group;
-  int block_size, num_blocks;
-  float scale;
-  int num_seqs;
-  int max_query_len;
-  const int* order;          // (sequence, query tile) pairs, largest first; null: tile_of's own order
-  int fold;                  // that order pairs long and short tiles (see prefill_plan_kernel)
-  // prefill_x3_kernel with key splits: each (tile, kv head) runs as kv_splits workgroups over
-  // consecutive ranges of its key chunks, writing partials (unnormalised O, reference point and
-  // row sum per row) that prefill_split_merge_kernel combines in split order
-  int kv_splits;
-  float* part;
-};
-
-// One workgroup sorts the (sequence, query tile) pairs by the number of kb-key chunks they
-// attend, largest first (counting sort over 1024 buckets; order within a bucket arbitrary,
-// which no result depends on; tiles past a sequence's end sort last).
-__global__ __launch_bounds__(1024) void prefill_plan_kernel(const int* __restrict__ cu, const int* __restrict__ ctxl,
-                                                            int num_seqs, int ntiles, int qt_rows, int kb, int fold,
-                                                            int* __restrict__ order, uint32_t* __restrict__ faults) {
-  __shared__ int hist[1024];
-  __shared__ int part[1024];
-  __shared__ int s_live;
-  const int tid = threadIdx.x;
-  const int total = num_seqs * ntiles;
-  hist[tid] = 0;
-  // a query length beyond the tiles that max_query_len sized: its tail rows get no workgroup
-  for (int s = tid; s < num_seqs; s += 1024) {
-    if (cu[s + 1] - cu[s] > ntiles * qt_rows) atomicOr(faults, FI_FAULT_QUERY_RANGE);
-  }
-  __syncthreads();
-  auto bucket = [&](int t) {  // 0 = past the sequence's end, else chunks + 1 (capped)
-    const int seq = t / ntiles, qt = t - (t / ntiles) * ntiles;
-    const int qs = cu[seq], qlen = cu[seq + 1] - qs;
-    const int q0 = qt * qt_rows;
-    if (q0 >= qlen) return 0;
-    const int kend = ctxl[seq] - qlen + min(qlen, q0 + qt_rows);
-    return min(max((kend + kb - 1) / kb, 0) + 1, 1023);
-  };
-  for (int t = tid; t < total; t += 1024) atomicAdd(&hist[1023 - bucket(t)], 1);
-  __syncthreads();
-  if (tid == 0) s_live = total - hist[1023];  // tiles with rows (bucket 0 sorts last)
-  const int v = hist[tid];  // exclusive scan of the bucket counts (Hillis-Steele)
-  part[tid] = v;
-  __syncthreads();
-  for (int off = 1; off < 1024; off <<= 1) {
-    const int x = tid >= off ? part[tid - off] : 0;
-    __syncthreads();
-    part[tid] += x;
-    __syncthreads();
-  }
-  hist[tid] = part[tid] - v;
-  __syncthreads();
-  // fold (a launch that fits the device in one round, two workgroups per CU): sorted position
-  // p of the n live tiles goes to rank p in the first half and to rank half + (n - 1 - p) in
-  // the second, so ranks r and r + half, which the dispatcher places on the same CU, pair a
-  // long tile with a short one
-  const int n = s_live, half = (n + 1) / 2;
-  for (int t = tid; t < total; t += 1024) {
-    const int p = atomicAdd(&hist[1023 - bucket(t)], 1);
-    order[fold && p < n && p >= half ? half + (n - 1 - p) : p] = t;
-  }
-}
-
-// The tile (seq * ntiles + query tile) of a rank.  Without a planned order: one sequence's tiles
-// from its last to its first, which is largest first, folded as the plan folds them; several
-// sequences' last tiles, then the ones before, and so on (launches of at most one workgroup a CU).
-__device__ __forceinline__ int tile_of(const PrefillArgs& a, int rank, int ntiles, int qt_tokens) {
-  if (a.order) return a.order[rank];
-  if (a.num_seqs > 1) {
-    const int t = rank / a.num_seqs;
-    return (rank - t * a.num_seqs) * ntiles + ntiles - 1 - t;
-  }
-  const int n = min(ntiles, (a.cu_seqlens[1] - a.cu_seqlens[0] + qt_tokens - 1) / qt_tokens);
-  if (rank >= n) return rank;  // past the sequence's end
-  const int half = (n + 1) / 2;
-  return a.fold && rank >= half ? rank - half : n - 1 - rank;
-}
-
-// What the plan reports, where there is none: a query length beyond the tiles that max_query_len
-// sized (its tail rows get no workgroup).
-__device__ __forceinline__ void check_query_length(const PrefillArgs& a, int qt, int qlen, int rows) {
-  if (!a.order && qt == 0 && qlen > rows && threadIdx.x == 0) atomicOr(a.faults, FI_FAULT_QUERY_RANGE);
-}
 
 // Four consecutive K/V elements of one row as raw registers, widened when staged.
 template <typename KVT>
@@ -393,55 +297,6 @@ __global__ __launch_bounds__(kThreads, 2) void prefill_kernel(PrefillArgs a) {
   }
 }
 
-// Sizes the grid (one workgroup per tile and kv head, and split) and sorts the tiles largest first
-// into the context workspace, one small launch before the attention kernel (4.7 us).  No plan
-// where the kernels know as good an order: a single sequence, and several whose workgroups
-// have a CU each (13 prompts of 20-70 tokens, 14/2 heads: 12.1 -> 8.2 us; a 2048-token chunk
-// after 2048, bf16: 130.6 -> 126.5 us; 700 tokens after 300, f32 pool: 71.5 -> 67.5 us).  At two to
-// four a CU the unplanned order cost more than the launch (3 sequences of 20-150 tokens after up
-// to 2000, 32/8 heads, f32 pool: 104 planned, 118 us without).
-#ifndef FI_PREFILL_FOLD
-#define FI_PREFILL_FOLD 1
-#endif
-
-int32_t plan_tiles(fi_context* ctx, PrefillArgs& args, int qt, int kb, const char* name, dim3* grid, int splits = 1,
-                   size_t part_floats = 0) {
-  const int ntiles = (args.max_query_len + qt - 1) / qt;
-  const long pairs = (long)ntiles * args.num_seqs;
-  const long wgs = pairs * args.hkv * splits;
-  FI_REQUIRE(wgs <= 0x7fffffffL, FI_ERR_INVALID_SHAPE, std::string(name) + ": grid too large");
-  const long cus = ctx->compute_units > 0 ? ctx->compute_units : 256;
-  const bool plan = args.num_seqs > 1 && wgs > cus;
-  // the tile order, then (split launches) each workgroup's partials
-  const size_t order_bytes = plan ? ((size_t)pairs * sizeof(int) + 255) & ~static_cast<size_t>(255) : 0;
-  const size_t part_bytes = splits > 1 ? (size_t)wgs * part_floats * sizeof(float) : 0;
-  if (order_bytes + part_bytes > 0) FI_TRY(fi::ensure_workspace(ctx, order_bytes + part_bytes));
-  args.kv_splits = splits;
-  args.part = splits > 1 ? reinterpret_cast<float*>(static_cast<char*>(ctx->workspace) + order_bytes) : nullptr;
-  // one round of workgroups (two per CU): pair long and short tiles on each CU
-  args.fold = FI_PREFILL_FOLD && splits == 1 && wgs <= 2 * cus;
-  args.order = nullptr;
-  if (plan) {
-    int* order = static_cast<int*>(ctx->workspace);
-    hipLaunchKernelGGL(prefill_plan_kernel, dim3(1), dim3(1024), 0, ctx->stream, args.cu_seqlens, args.context_lens,
-                       args.num_seqs, ntiles, qt, kb, args.fold, order, ctx->d_faults);
-    FI_CHECK_LAUNCH("prefill_plan_kernel");
-    args.order = order;
-  }
-  *grid = dim3(static_cast<unsigned>(wgs));
-  return FI_OK;
-}
-
-// Row groups per wave: two when the grid still gives every CU two workgroups (every K/V
-// fragment read from LDS then feeds two MFMAs), one for launches with few (sequence, tile,
-// kv head) triples, such as a prefill chunk over two kv heads.
-int row_groups(fi_context* ctx, const PrefillArgs& args, int g) {
-  const long cus = ctx->compute_units > 0 ? ctx->compute_units : 256;
-  const int qt2 = kRows * 2 / g;
-  const long tiles2 = (long)((args.max_query_len + qt2 - 1) / qt2) * args.num_seqs * args.hkv;
-  return tiles2 >= 2 * cus ? 2 : 1;
-}
-
 template <int D, typename KVT, int RG>
 int32_t launch_prefill_rg(fi_context* ctx, PrefillArgs& args, int g) {
   const int qt = kRows * RG / g;
@@ -478,15 +333,6 @@ int32_t launch_prefill(fi_context* ctx, const PrefillArgs& args_in) {
 // v_mfma_f32_16x16x32_bf16: K and V stay bf16 in LDS, row-major (V^T fragments come from
 // ds_read_b64_tr_b16), Q and the softmax probabilities are rounded to bf16 (nearest even);
 // scores, softmax and accumulation stay f32.  64-key chunks.
-typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
-typedef float f32x8 __attribute__((ext_vector_type(8)));
-typedef short v4s __attribute__((ext_vector_type(4)));
-typedef __attribute__((address_space(3))) v4s lds_v4s;
-
-// ds_read_b64_tr_b16 at an LDS address (8-byte aligned)
-__device__ __forceinline__ v4s lds_read_tr16(const uint16_t* p) {
-  return __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s*)(p));
-}
 #ifndef FI_PREFILL_BF16_WAVES
 #define FI_PREFILL_BF16_WAVES 2  // waves per SIMD the register budget must allow
 #endif
@@ -796,17 +642,6 @@ int32_t launch_prefill_bf16(fi_context* ctx, const PrefillArgs& args_in) {
 // rounding together), accumulated in f32 on v_mfma_f32_16x16x32_bf16: the f32 result at 2.7x
 // the f32 MFMA rate.  One LDS buffer (52 KB at D = 128, two workgroups per CU); the next chunk
 // is in registers while the current one is multiplied, two barriers per chunk.
-__device__ __forceinline__ void split3(const f32x8& x, bf16x8 (&p)[3]) {
-  uint4 h, m, l;
-  fi::split3_pk(x[0], x[1], h.x, m.x, l.x);
-  fi::split3_pk(x[2], x[3], h.y, m.y, l.y);
-  fi::split3_pk(x[4], x[5], h.z, m.z, l.z);
-  fi::split3_pk(x[6], x[7], h.w, m.w, l.w);
-  p[0] = __builtin_bit_cast(bf16x8, h);
-  p[1] = __builtin_bit_cast(bf16x8, m);
-  p[2] = __builtin_bit_cast(bf16x8, l);
-}
-
 // four f32 values -> their three bf16 pieces, each as 8 bytes
 __device__ __forceinline__ void split3_quad(const float4& v, uint2 (&p)[3]) {
   fi::split3_pk(v.x, v.y, p[0].x, p[1].x, p[2].x);
@@ -1133,71 +968,6 @@ __global__ __launch_bounds__(kThreads, 2) void prefill_x3_kernel(PrefillArgs a) 
   }
 }
 
-#ifndef FI_PREFILL_MAX_SPLITS
-#define FI_PREFILL_MAX_SPLITS 4  // key splits of a small f32-pool prefill launch, at most
-#endif
-
-// One workgroup per (tile, kv head) of a split launch: each row's output is the splits'
-// partials combined in split order, each rescaled from its own reference point to the largest
-// (a split with no key the row sees carries -inf and adds nothing; the split holding key 0
-// always sees one), then normalised by the combined row sum.
-template <int D, int RG>
-__global__ __launch_bounds__(kThreads) void prefill_split_merge_kernel(PrefillArgs a, int qt_tokens, int ntiles) {
-  constexpr int ROWS = kRows * RG, DQ = D / 4;
-  constexpr int ITER = ROWS * DQ / kThreads;  // (row, column quad) items a thread
-  constexpr int BATCH = ITER < 4 ? ITER : 4;  // items whose loads are issued together
-  constexpr int MAXS = FI_PREFILL_MAX_SPLITS;
-  static_assert(ROWS * DQ % kThreads == 0 && ITER % BATCH == 0, "items must split over the workgroup");
-  const int tile = blockIdx.x / a.hkv, kvh = blockIdx.x % a.hkv;
-  const int seq = tile / ntiles, q0 = (tile % ntiles) * qt_tokens;
-  const int qs = a.cu_seqlens[seq], qlen = a.cu_seqlens[seq + 1] - qs;
-  if (q0 >= qlen) return;
-  const int S = a.kv_splits;
-  const float* pml = a.part + (size_t)gridDim.x * S * ROWS * D;
-  const size_t unit0 = (size_t)tile * S * a.hkv + kvh;  // split sp: unit0 + sp * hkv
-  for (int it0 = 0; it0 < ITER; it0 += BATCH) {
-    // every split's (point, sum) and O quad of BATCH items are loaded before any is combined
-    // (splits past S read split 0 and are dropped)
-    float2 ml[BATCH][MAXS];
-    float4 ov[BATCH][MAXS];
-#pragma unroll
-    for (int b = 0; b < BATCH; ++b) {
-      const int idx = threadIdx.x + (it0 + b) * kThreads;
-      const int r = idx / DQ, dq = idx - (idx / DQ) * DQ;
-#pragma unroll
-      for (int sp = 0; sp < MAXS; ++sp) {
-        const size_t unit = unit0 + (size_t)(sp < S ? sp : 0) * a.hkv;
-        ml[b][sp] = *reinterpret_cast<const float2*>(pml + (unit * ROWS + r) * 2);
-        ov[b][sp] = *reinterpret_cast<const float4*>(a.part + (unit * ROWS + r) * D + 4 * dq);
-      }
-    }
-#pragma unroll
-    for (int b = 0; b < BATCH; ++b) {
-      const int idx = threadIdx.x + (it0 + b) * kThreads;
-      const int r = idx / DQ, dq = idx - (idx / DQ) * DQ;
-      const int h = r / qt_tokens, t = r - (r / qt_tokens) * qt_tokens;
-      if (h >= a.group || q0 + t >= qlen) continue;
-      float mx = -INFINITY;
-#pragma unroll
-      for (int sp = 0; sp < MAXS; ++sp)
-        if (sp < S) mx = fmaxf(mx, ml[b][sp].x);
-      float l = 0.0f;
-      float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll
-      for (int sp = 0; sp < MAXS; ++sp) {
-        if (sp >= S || ml[b][sp].x == -INFINITY) continue;
-        const float wgt = __builtin_amdgcn_exp2f(ml[b][sp].x - mx);
-        const float4 o = ov[b][sp];
-        l = l + wgt * ml[b][sp].y;
-        acc = make_float4(acc.x + wgt * o.x, acc.y + wgt * o.y, acc.z + wgt * o.z, acc.w + wgt * o.w);
-      }
-      const float inv = 1.0f / l;
-      *reinterpret_cast<float4*>(a.out + ((size_t)(qs + q0 + t) * a.hq + kvh * a.group + h) * D + 4 * dq) =
-          make_float4(acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv);
-    }
-  }
-}
-
 template <int D, int G, int RG, bool SPLIT>
 void launch_x3(fi_context* ctx, const PrefillArgs& args, dim3 grid) {
   hipLaunchKernelGGL((prefill_x3_kernel<D, G, RG, SPLIT>), grid, dim3(kThreads), 0, ctx->stream, args);
@@ -1282,8 +1052,8 @@ int32_t prefill_args(fi_context* ctx, const char* name, const float* d_q, const 
              "number of query heads must be divisible by number of KV heads");
   FI_REQUIRE(block_size > 0 && num_blocks > 0 && max_blocks_per_seq > 0, FI_ERR_INVALID_CONFIG,
              n + ": pool dimensions must be greater than zero");
-  FI_REQUIRE(kv_dtype == FI_DTYPE_F32 || kv_dtype == FI_DTYPE_BF16, FI_ERR_INVALID_TYPE,
-             n + ": KV dtype must be f32 or bf16");
+  FI_REQUIRE(kv_dtype == FI_DTYPE_F32 || kv_dtype == FI_DTYPE_BF16 || kv_dtype == FI_DTYPE_MXFP4, FI_ERR_INVALID_TYPE,
+             n + ": KV dtype must be f32, bf16 or mxfp4");
   FI_REQUIRE(head_dim == 32 || head_dim == 64 || head_dim == 128, FI_ERR_UNSUPPORTED,
              n + ": head_dim must be 32, 64 or 128");
   FI_REQUIRE(num_q_heads / num_kv_heads <= 8, FI_ERR_UNSUPPORTED, n + " supports at most 8 query heads per KV head");
@@ -1332,6 +1102,11 @@ int32_t fi_attn_prefill_paged(fi_context* ctx, const float* d_q, const void* d_k
                       max_blocks_per_seq, d_cu_seqlens, d_context_lens, num_seqs, max_query_len, num_q_heads,
                       num_kv_heads, head_dim, block_size, num_blocks, scale, d_out, &args, &empty));
   if (empty) return FI_OK;
+  if (kv_dtype == FI_DTYPE_MXFP4) {
+    FI_REQUIRE(scale > 0.0f && scale < INFINITY, FI_ERR_INVALID_CONFIG,
+               "fi_attn_prefill_paged: scale must be positive and finite");
+    return fi::prefill_fp4(ctx, args, head_dim);
+  }
   switch (head_dim) {
     case 32:
       return launch_prefill_dtype<32>(ctx, kv_dtype, args);

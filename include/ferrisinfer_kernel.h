@@ -293,7 +293,9 @@ int32_t fi_attn_decode_paged_noalloc(fi_context* ctx, const float* d_q, const vo
  * runtime/paged_kv.rs:769-791).  max_query_len must bound every qlen_b (it sizes the grid); a
  * longer qlen_b is reported as Runtime by fi_ctx_check_faults and its rows past the tiles that
  * max_query_len sized are left unwritten.  q, out and the pools must be 16-byte aligned
- * (InvalidLayout otherwise). */
+ * (InvalidLayout otherwise).  Every pool dtype is attended in f32 accuracy.  Over an mxfp4 pool a
+ * query row at a negative position (context_lens[b] below qlen_b) sees no key and gets zeros, and
+ * scale must be positive and finite (InvalidConfig otherwise). */
 int32_t fi_attn_prefill_paged(fi_context* ctx, const float* d_q, const void* d_k_cache,
                               const void* d_v_cache, int32_t kv_dtype,
                               const int32_t* d_block_tables, int32_t max_blocks_per_seq,
