@@ -21,21 +21,23 @@ __global__ __launch_bounds__(256) void kv_append_fp4_kernel(const float* __restr
                                                             uint8_t* __restrict__ k_cache,
                                                             uint8_t* __restrict__ v_cache, int64_t pool_slots,
                                                             int block_size, int hkv, int d, size_t code_bytes,
-                                                            int64_t total8, uint32_t* __restrict__ faults) {
-  const int64_t idx = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
+                                                            uint32_t total8, fi::FastDiv row8,
+                                                            uint32_t* __restrict__ faults) {
+  const uint32_t idx = blockIdx.x * blockDim.x + threadIdx.x;
   if (idx >= total8) return;
-  const int row8 = hkv * d / 8;
-  const int64_t t = idx / row8;
-  const int i = static_cast<int>(idx - t * row8) * 8;
+  const uint32_t t = row8.div(idx);
+  const int i = static_cast<int>(idx - t * row8.d) * 8;
   const int64_t slot = slots[t];
   if (slot < 0) return;
   if (slot >= pool_slots) {
     if (i == 0) atomicOr(faults, FI_FAULT_SLOT_RANGE);
     return;
   }
-  const int64_t blk = slot / block_size;
+  // slots past 32 bits take the long division
+  const int64_t blk = slot <= 0xffffffffLL ? static_cast<int64_t>(static_cast<uint32_t>(slot) / static_cast<uint32_t>(block_size))
+                                           : slot / block_size;
   const int off = static_cast<int>(slot - blk * block_size);
-  const int h = i / d, e = i - (i / d) * d;
+  const int h = i >> (31 - __clz(d)), e = i & (d - 1);  // d is 32, 64 or 128
   const size_t row = ((size_t)blk * hkv + h) * block_size + off;
   const size_t src = (size_t)t * hkv * d + i;
   auto load = [&](const float* p) {
@@ -83,20 +85,20 @@ __global__ __launch_bounds__(256) void kv_copy_blocks_fp4_kernel(uint8_t* __rest
 __global__ __launch_bounds__(256) void kv_gather_fp4_kernel(const uint8_t* __restrict__ k_cache,
                                                             const uint8_t* __restrict__ v_cache,
                                                             const int* __restrict__ table, int64_t total8,
-                                                            int num_blocks, int block_size, int hkv, int d,
+                                                            int num_blocks, fi::FastDiv bs, fi::FastDiv heads, int d,
                                                             size_t code_bytes, float* __restrict__ k_out,
                                                             float* __restrict__ v_out, uint32_t* __restrict__ faults) {
-  const int d8 = d / 8;
+  const int d8_shift = 28 - __clz(d);  // d / 8; d is 32, 64 or 128
   const int64_t stride = (int64_t)gridDim.x * blockDim.x;
   for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < total8; i += stride) {
-    const int e = static_cast<int>(i % d8) * 8;
-    const int64_t r = i / d8;
-    const int h = static_cast<int>(r % hkv);
-    const int t = static_cast<int>(r / hkv);
-    const int b = table[t / block_size];
+    const int e = (static_cast<int>(i) & ((1 << d8_shift) - 1)) * 8;
+    const uint32_t r = static_cast<uint32_t>(i >> d8_shift);
+    const uint32_t t = heads.div(r), h = r - t * heads.d;
+    const uint32_t lb = bs.div(t);
+    const int b = table[lb];
     const bool bad = b < 0 || b >= num_blocks;
     if (bad) atomicOr(faults, FI_FAULT_BLOCK_RANGE);
-    const size_t row = ((size_t)(bad ? 0 : b) * hkv + h) * block_size + t % block_size;
+    const size_t row = ((size_t)(bad ? 0 : b) * heads.d + h) * bs.d + (t - lb * bs.d);
     auto widen = [&](const uint8_t* cache, float* out) {
       const uint32_t codes = *reinterpret_cast<const uint32_t*>(cache + row * (d / 2) + e / 2);
       const uint32_t scale = cache[code_bytes + row * (d / fi::kFp4Group) + e / fi::kFp4Group];
@@ -119,15 +121,14 @@ int32_t kv_append_fp4(fi_context* ctx, const float* key, const float* value, con
                       void* k_cache, void* v_cache, int32_t num_blocks, int32_t block_size, int32_t hkv, int32_t d) {
   const int64_t pool_slots = static_cast<int64_t>(num_blocks) * block_size;
   const int64_t total8 = static_cast<int64_t>(num_tokens) * hkv * d / 8;
-  const int64_t blocks = (total8 + 255) / 256;
-  FI_REQUIRE(blocks <= 0x7fffffffLL, FI_ERR_INVALID_SHAPE, "fi_kv_append: too many tokens for one launch");
+  FI_REQUIRE(total8 < 0x7fffffffLL, FI_ERR_INVALID_SHAPE, "fi_kv_append: too many tokens for one launch");
   const bool vec = ((reinterpret_cast<uintptr_t>(key) | reinterpret_cast<uintptr_t>(value)) & 15) == 0;
-  const dim3 grid(static_cast<unsigned>(blocks));
+  const dim3 grid(static_cast<unsigned>((total8 + 255) / 256));
   const size_t code_bytes = fp4_code_bytes(num_blocks, hkv, block_size, d);
   auto launch = [&](auto kernel) {
     hipLaunchKernelGGL(kernel, grid, dim3(256), 0, ctx->stream, key, value, slots, static_cast<uint8_t*>(k_cache),
-                       static_cast<uint8_t*>(v_cache), pool_slots, block_size, hkv, d, code_bytes, total8,
-                       ctx->d_faults);
+                       static_cast<uint8_t*>(v_cache), pool_slots, block_size, hkv, d, code_bytes,
+                       static_cast<uint32_t>(total8), FastDiv(static_cast<uint32_t>(hkv * d / 8)), ctx->d_faults);
   };
   if (vec) {
     launch(kv_append_fp4_kernel<true>);
@@ -151,9 +152,11 @@ int32_t kv_copy_blocks_fp4(fi_context* ctx, void* k_cache, void* v_cache, const 
 int32_t kv_gather_fp4(fi_context* ctx, const void* k_cache, const void* v_cache, const int32_t* table, int32_t length,
                       int32_t num_blocks, int32_t block_size, int32_t hkv, int32_t d, float* k_out, float* v_out) {
   const int64_t total8 = static_cast<int64_t>(length) * hkv * (d / 8);
+  FI_REQUIRE(static_cast<int64_t>(length) * hkv < 0x7fffffffLL, FI_ERR_INVALID_SHAPE, "fi_kv_gather: too many rows for one launch");
   const unsigned grid = static_cast<unsigned>(std::min<int64_t>((total8 + 255) / 256, 4096));
   hipLaunchKernelGGL(kv_gather_fp4_kernel, dim3(grid), dim3(256), 0, ctx->stream, static_cast<const uint8_t*>(k_cache),
-                     static_cast<const uint8_t*>(v_cache), table, total8, num_blocks, block_size, hkv, d,
+                     static_cast<const uint8_t*>(v_cache), table, total8, num_blocks,
+                     FastDiv(static_cast<uint32_t>(block_size)), FastDiv(static_cast<uint32_t>(hkv)), d,
                      fp4_code_bytes(num_blocks, hkv, block_size, d), k_out, v_out, ctx->d_faults);
   FI_CHECK_LAUNCH("kv_gather_fp4_kernel");
   return FI_OK;

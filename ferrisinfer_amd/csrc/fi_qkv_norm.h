@@ -2,6 +2,7 @@
 #pragma once
 
 #include "fi_common.h"
+#include "fi_device.h"
 
 namespace fi {
 
@@ -16,7 +17,9 @@ struct QkvNormArgs {
   float eps;
   const int* positions;  // [num_axes][tokens]
   int num_axes;
-  uint32_t pair_axes[4];  // two bits a rotary pair: the axis whose position turns it
+  // two bits a rotary pair, sixteen pairs a word: the axis whose position turns it.  Four names, not an
+  // array: indexed by a lane it would be copied to scratch memory
+  uint32_t pair_axes0, pair_axes1, pair_axes2, pair_axes3;
   const float* cos_t;     // [max_positions][rotary_dims / 2]
   const float* sin_t;
   int rotary_dims;
@@ -28,6 +31,7 @@ struct QkvNormArgs {
   size_t code_bytes;  // 4-bit pools: where an array's scales begin
   int block_size;
   int tokens;
+  FastDiv chunks;  // workgroups a token
   int hq, hkv;
   float* q_out;
   uint32_t* faults;

@@ -31,104 +31,172 @@ __device__ __forceinline__ float row_sum(float v, int lane) {
   return v;
 }
 
-template <int D, typename Pool>
+// y cos + o sin of four elements, each product rounded before the add as in fi::rope4 (the first
+// half's minus sign is in sin: -(o sin) = o (-sin) exactly).
+__device__ __forceinline__ float4 turn(const float4& y, const float4& o, const float4& cs, const float4& sn) {
+#pragma clang fp contract(off)
+  return make_float4(y.x * cs.x + o.x * sn.x, y.y * cs.y + o.y * sn.y, y.z * cs.z + o.z * sn.z,
+                     y.w * cs.w + o.w * sn.w);
+}
+
+// The table row of a token's position on one axis.
+__device__ __forceinline__ size_t table_row(const fi::QkvNormArgs& a, int t, uint32_t axis, int half) {
+  int pos = a.positions[(size_t)axis * a.tokens + t];
+  if (pos < 0 || pos >= a.max_positions) {
+    atomicOr(a.faults, FI_FAULT_POSITION_RANGE);
+    pos = 0;
+  }
+  return (size_t)pos * half;
+}
+
+// One workgroup = ROWS * kThreads / LPR head rows of one token: the token's slot, block and positions are
+// uniform, and a thread's ROWS rows (the same elements of heads kThreads / LPR apart) share its
+// weights, cosines and sines.  Every load is issued before the first is waited for, but for the table
+// rows, which wait for the positions: the chain of dependent loads, not the arithmetic, bounds this.
+template <int D, typename Pool, int ROWS>
 __global__ __launch_bounds__(kThreads) void qkv_norm_rope_append_kernel(fi::QkvNormArgs a) {
-  constexpr int LPR = D / 4;  // lanes per head row
+  constexpr int LPR = D / 4;            // lanes per head row
+  constexpr int STEP = kThreads / LPR;  // heads between a thread's rows
   const int lane = threadIdx.x & 63;
   const int c = lane % LPR;  // this lane's elements are 4 c .. 4 c + 3
   const int heads = a.hq + 2 * a.hkv;
-  const int64_t row = ((int64_t)blockIdx.x * kThreads + threadIdx.x) / LPR;
-  if (row >= (int64_t)a.tokens * heads) return;  // whole rows leave
-  const int t = static_cast<int>(row / heads);
-  const int head = static_cast<int>(row - (int64_t)t * heads);
-  const bool is_q = head < a.hq, is_v = head >= a.hq + a.hkv;
-  const int local = is_q ? head : (is_v ? head - a.hq - a.hkv : head - a.hq);  // within its projection
-
+  const int t = static_cast<int>(a.chunks.div(blockIdx.x));
+  const int chunk = static_cast<int>(blockIdx.x - t * a.chunks.d);
+  const int head0 = chunk * (ROWS * STEP) + static_cast<int>(threadIdx.x) / LPR;
   const int64_t slot = a.slots[t];
-  const bool write_kv = slot >= 0 && slot < a.pool_slots;
-  if (head == 0 && c == 0 && slot >= a.pool_slots) atomicOr(a.faults, FI_FAULT_SLOT_RANGE);
-  if (!is_q && !write_kv) return;
-
-  const size_t plane = (size_t)a.tokens * heads * D;
-  const float* bias = is_q ? a.bias_q : (is_v ? a.bias_v : a.bias_k);
-  float4 x = fi::qkv_value4(a.parts + (size_t)t * heads * D, plane, a.splits, bias, local * D + 4 * c,
-                            head * D + 4 * c);
-  const float* weight = is_q ? a.q_norm : a.k_norm;
-  if (!is_v && weight) {
-    const float ms = row_sum<LPR>(x.x * x.x + x.y * x.y + x.z * x.z + x.w * x.w, lane) * (1.0f / D);
-    const float inv = 1.0f / sqrtf(ms + a.eps);
-    const float4 w = *reinterpret_cast<const float4*>(weight + 4 * c);
-    x = make_float4(x.x * inv * w.x, x.y * inv * w.y, x.z * inv * w.z, x.w * inv * w.w);
-  }
   const int half = a.rotary_dims / 2;
-  if (!is_v && half > 0) {
-    // the partner's elements: half / 4 lanes up for the first half of the rotary dims, down for the second
-    const bool rotary = 4 * c < 2 * half, low = 4 * c < half;
-    const int from = lane + (rotary ? (low ? half / 4 : -(half / 4)) : 0);
-    const float4 o = make_float4(__shfl(x.x, from, 64), __shfl(x.y, from, 64), __shfl(x.z, from, 64),
-                                 __shfl(x.w, from, 64));
-    if (rotary) {
-      const int pair = low ? 4 * c : 4 * c - half;
-      float4 cs, sn;
-      auto position = [&](int axis) {
-        int pos = a.positions[(size_t)axis * a.tokens + t];
-        if (pos < 0 || pos >= a.max_positions) {
-          atomicOr(a.faults, FI_FAULT_POSITION_RANGE);
-          pos = 0;
-        }
-        return (size_t)pos * half;
-      };
-      if (a.num_axes == 1) {
-        const size_t at = position(0) + pair;
-        cs = *reinterpret_cast<const float4*>(a.cos_t + at);
-        sn = *reinterpret_cast<const float4*>(a.sin_t + at);
-      } else {
-        // two bits a pair; four consecutive pairs lie in one word (pair is a multiple of 4)
-        const uint32_t axes = a.pair_axes[pair / 16] >> (2 * (pair % 16));
-        const size_t p0 = position(axes & 3) + pair, p1 = position((axes >> 2) & 3) + pair + 1,
-                     p2 = position((axes >> 4) & 3) + pair + 2, p3 = position((axes >> 6) & 3) + pair + 3;
-        cs = make_float4(a.cos_t[p0], a.cos_t[p1], a.cos_t[p2], a.cos_t[p3]);
-        sn = make_float4(a.sin_t[p0], a.sin_t[p1], a.sin_t[p2], a.sin_t[p3]);
+  const size_t plane = (size_t)a.tokens * heads * D;
+  const float* p0 = a.parts + (size_t)t * heads * D;
+
+  float4 x[ROWS];
+  if (a.splits == 1) {
+#pragma unroll
+    for (int i = 0; i < ROWS; ++i) {  // rows past the last head read head 0 and are dropped
+      const int head = head0 + i * STEP < heads ? head0 + i * STEP : 0;
+      x[i] = *reinterpret_cast<const float4*>(p0 + head * D + 4 * c);
+    }
+  }
+  // this lane's rotary pairs (of the first or the second half) and their cosines and sines
+  const bool rotary = 4 * c < 2 * half, low = 4 * c < half;
+  float4 cs = make_float4(1.f, 1.f, 1.f, 1.f), sn = make_float4(0.f, 0.f, 0.f, 0.f);
+  if (rotary && head0 < a.hq + a.hkv) {
+    const int pair = low ? 4 * c : 4 * c - half;
+    // two bits a pair; four consecutive pairs lie in one word (pair is a multiple of 4)
+    const uint32_t word = pair < 32 ? (pair < 16 ? a.pair_axes0 : a.pair_axes1) : (pair < 48 ? a.pair_axes2 : a.pair_axes3);
+    const uint32_t axes = (word >> (2 * (pair % 16))) & 0xffu;
+    const size_t r0 = table_row(a, t, axes & 3, half) + pair;
+    if (axes == (axes & 3) * 0x55u) {  // one axis turns the four pairs, as all but a few lanes find
+      cs = *reinterpret_cast<const float4*>(a.cos_t + r0);
+      sn = *reinterpret_cast<const float4*>(a.sin_t + r0);
+    } else {
+      const size_t r1 = table_row(a, t, (axes >> 2) & 3, half) + pair + 1, r2 = table_row(a, t, (axes >> 4) & 3, half) + pair + 2,
+                   r3 = table_row(a, t, axes >> 6, half) + pair + 3;
+      cs = make_float4(a.cos_t[r0], a.cos_t[r1], a.cos_t[r2], a.cos_t[r3]);
+      sn = make_float4(a.sin_t[r0], a.sin_t[r1], a.sin_t[r2], a.sin_t[r3]);
+    }
+    if (low) sn = make_float4(-sn.x, -sn.y, -sn.z, -sn.w);
+  }
+  // the pool row of the token's kv head 0; slots past 32 bits take the long division
+  const bool write_kv = slot >= 0 && slot < a.pool_slots;
+  if (chunk == 0 && threadIdx.x == 0 && slot >= a.pool_slots) atomicOr(a.faults, FI_FAULT_SLOT_RANGE);
+  const int64_t blk = !write_kv ? 0
+                      : slot <= 0xffffffffLL
+                          ? static_cast<int64_t>(static_cast<uint32_t>(slot) / static_cast<uint32_t>(a.block_size))
+                          : slot / a.block_size;
+  const size_t pool_row0 = (size_t)blk * a.hkv * a.block_size + (write_kv ? slot - blk * a.block_size : 0);
+
+#pragma unroll
+  for (int i = 0; i < ROWS; ++i) {
+    const int head = head0 + i * STEP;
+    if (head >= heads) return;  // whole rows leave
+    const bool is_q = head < a.hq, is_v = head >= a.hq + a.hkv;
+    const int local = is_q ? head : (is_v ? head - a.hq - a.hkv : head - a.hq);  // within its projection
+    const float* bias = is_q ? a.bias_q : (is_v ? a.bias_v : a.bias_k);
+    float4 y;
+    if (a.splits == 1) {
+      y = bias ? fi::add(x[i], *reinterpret_cast<const float4*>(bias + local * D + 4 * c)) : x[i];
+    } else {
+      y = fi::qkv_value4(p0, plane, a.splits, bias, local * D + 4 * c, head * D + 4 * c);
+    }
+    if (!is_v) {
+      const float* weight = is_q ? a.q_norm : a.k_norm;
+      if (weight) {
+        const float ms = row_sum<LPR>(y.x * y.x + y.y * y.y + y.z * y.z + y.w * y.w, lane) * (1.0f / D);
+        const float inv = 1.0f / sqrtf(ms + a.eps);
+        const float4 w = *reinterpret_cast<const float4*>(weight + 4 * c);
+        y = make_float4(y.x * inv * w.x, y.y * inv * w.y, y.z * inv * w.z, y.w * inv * w.w);
       }
-      float4 y0, y1;
-      fi::rope4(low ? x : o, low ? o : x, cs, sn, y0, y1);
-      x = low ? y0 : y1;
+      if (half > 0) {
+        // the partner's elements: half / 4 lanes up for the first half of the rotary dims, down for the second
+        const int from = lane + (rotary ? (low ? half / 4 : -(half / 4)) : 0);
+        const float4 o = make_float4(__shfl(y.x, from, 64), __shfl(y.y, from, 64), __shfl(y.z, from, 64),
+                                     __shfl(y.w, from, 64));
+        const float4 z = turn(y, o, cs, sn);
+        y = make_float4(rotary ? z.x : y.x, rotary ? z.y : y.y, rotary ? z.z : y.z, rotary ? z.w : y.w);
+      }
     }
-  }
-  if (is_q) {
-    *reinterpret_cast<float4*>(a.q_out + ((size_t)t * a.hq + local) * D + 4 * c) = x;
-    return;
-  }
-  const int64_t blk = slot / a.block_size;
-  const int off = static_cast<int>(slot - blk * a.block_size);
-  const size_t dst = ((size_t)blk * a.hkv + local) * a.block_size + off;  // pool row
-  void* cache = is_v ? a.v_cache : a.k_cache;
-  if constexpr (std::is_same_v<Pool, Fp4Pool>) {
-    uint8_t* pool = static_cast<uint8_t*>(cache);
-    // eight lanes hold a group
-    const uint32_t top = fi::group_max<8>(max(max(fi::magnitude_bits(x.x), fi::magnitude_bits(x.y)),
-                                              max(fi::magnitude_bits(x.z), fi::magnitude_bits(x.w))));
-    const uint32_t scale = fi::fp4_scale(top);
-    uint32_t codes = 0;
-    if (scale != 255u) {
-      codes = fi::fp4_pack2<0>(codes, x.x, x.y, fi::fp4_scale_f32(scale));
-      codes = fi::fp4_pack2<1>(codes, x.z, x.w, fi::fp4_scale_f32(scale));
+    if (is_q) {
+      *reinterpret_cast<float4*>(a.q_out + ((size_t)t * a.hq + local) * D + 4 * c) = y;
+      continue;
     }
-    *reinterpret_cast<uint16_t*>(pool + dst * (D / 2) + 2 * c) = static_cast<uint16_t>(codes);
-    if (c % 8 == 0) pool[a.code_bytes + dst * (D / fi::kFp4Group) + c / 8] = static_cast<uint8_t>(scale);
-  } else {
-    fi::put_kv4(static_cast<Pool*>(cache), dst * D + 4 * c, x);
+    if (!write_kv) continue;
+    const size_t dst = pool_row0 + (size_t)local * a.block_size;
+    void* cache = is_v ? a.v_cache : a.k_cache;
+    if constexpr (std::is_same_v<Pool, Fp4Pool>) {
+      uint8_t* pool = static_cast<uint8_t*>(cache);
+      // eight lanes hold a group
+      const uint32_t top = fi::group_max<8>(max(max(fi::magnitude_bits(y.x), fi::magnitude_bits(y.y)),
+                                                max(fi::magnitude_bits(y.z), fi::magnitude_bits(y.w))));
+      const uint32_t scale = fi::fp4_scale(top);
+      uint32_t codes = 0;
+      if (scale != 255u) {
+        codes = fi::fp4_pack2<0>(codes, y.x, y.y, fi::fp4_scale_f32(scale));
+        codes = fi::fp4_pack2<1>(codes, y.z, y.w, fi::fp4_scale_f32(scale));
+      }
+      *reinterpret_cast<uint16_t*>(pool + dst * (D / 2) + 2 * c) = static_cast<uint16_t>(codes);
+      if (c % 8 == 0) pool[a.code_bytes + dst * (D / fi::kFp4Group) + c / 8] = static_cast<uint8_t>(scale);
+    } else {
+      fi::put_kv4(static_cast<Pool*>(cache), dst * D + 4 * c, y);
+    }
   }
 }
 
-template <int D>
-void launch(fi_context* ctx, const fi::QkvNormArgs& a, int32_t kv_dtype, dim3 grid) {
+template <int D, int ROWS>
+void launch_rows(fi_context* ctx, fi::QkvNormArgs& a, int32_t kv_dtype) {
+  const int rows = ROWS * kThreads / (D / 4);  // head rows of a workgroup
+  a.chunks = fi::FastDiv(static_cast<uint32_t>((a.hq + 2 * a.hkv + rows - 1) / rows));
+  const dim3 grid(static_cast<unsigned>(a.tokens) * a.chunks.d);
   if (kv_dtype == FI_DTYPE_F32) {
-    hipLaunchKernelGGL((qkv_norm_rope_append_kernel<D, float>), grid, dim3(kThreads), 0, ctx->stream, a);
+    hipLaunchKernelGGL((qkv_norm_rope_append_kernel<D, float, ROWS>), grid, dim3(kThreads), 0, ctx->stream, a);
   } else if (kv_dtype == FI_DTYPE_BF16) {
-    hipLaunchKernelGGL((qkv_norm_rope_append_kernel<D, uint16_t>), grid, dim3(kThreads), 0, ctx->stream, a);
+    hipLaunchKernelGGL((qkv_norm_rope_append_kernel<D, uint16_t, ROWS>), grid, dim3(kThreads), 0, ctx->stream, a);
   } else {
-    hipLaunchKernelGGL((qkv_norm_rope_append_kernel<D, Fp4Pool>), grid, dim3(kThreads), 0, ctx->stream, a);
+    hipLaunchKernelGGL((qkv_norm_rope_append_kernel<D, Fp4Pool, ROWS>), grid, dim3(kThreads), 0, ctx->stream, a);
+  }
+}
+
+// Where one row a thread would make more workgroups than the device holds at once (eight a CU) and the
+// partials need no sum, as few workgroups a token as six rows a thread allow (2048 tokens of 48 heads
+// of 128, six rows to a thread fill a workgroup: 46.6 us with one row, 31.3 with two, 28.2 with three,
+// 32.4 with four, whose second workgroup is half empty, 26.2 with six).  Smaller launches end sooner
+// with more workgroups.
+template <int D>
+void launch(fi_context* ctx, fi::QkvNormArgs& a, int32_t kv_dtype) {
+  constexpr int STEP = kThreads / (D / 4);
+  const int64_t cus = ctx->compute_units > 0 ? ctx->compute_units : 256;
+  const int heads = a.hq + 2 * a.hkv;
+  const int passes = a.splits == 1 && static_cast<int64_t>(a.tokens) * heads > 8 * cus * STEP ? (heads + STEP - 1) / STEP : 1;
+  switch (passes) {
+    case 1:
+      return launch_rows<D, 1>(ctx, a, kv_dtype);
+    case 2:
+      return launch_rows<D, 2>(ctx, a, kv_dtype);
+    case 3:
+      return launch_rows<D, 3>(ctx, a, kv_dtype);
+    case 4:
+      return launch_rows<D, 4>(ctx, a, kv_dtype);
+    default:
+      return launch_rows<D, 6>(ctx, a, kv_dtype);
   }
 }
 
@@ -155,16 +223,20 @@ int32_t qkv_norm_rope_append(fi_context* ctx, const char* name, QkvNormArgs a, i
              n + ": several position axes need each pair's axis");
   FI_REQUIRE((!a.q_norm && !a.k_norm) || (a.eps >= 0.0f && a.eps < INFINITY), FI_ERR_INVALID_CONFIG,
              n + ": eps must be finite and not negative");
-  for (uint32_t& word : a.pair_axes) word = 0;
+  uint32_t words[4] = {0, 0, 0, 0};
   if (pair_axes) {
     for (int32_t i = 0; i < a.rotary_dims / 2; ++i) {
       FI_REQUIRE(pair_axes[i] >= 0 && pair_axes[i] < a.num_axes, FI_ERR_INVALID_CONFIG,
                  n + ": pair " + std::to_string(i) + " names an axis beyond the positions'");
-      a.pair_axes[i / 16] |= static_cast<uint32_t>(pair_axes[i]) << (2 * (i % 16));
+      words[i / 16] |= static_cast<uint32_t>(pair_axes[i]) << (2 * (i % 16));
     }
   }
-  const int64_t threads = static_cast<int64_t>(a.tokens) * (a.hq + 2 * a.hkv) * (head_dim / 4);
-  const int64_t blocks = (threads + kThreads - 1) / kThreads;
+  a.pair_axes0 = words[0];
+  a.pair_axes1 = words[1];
+  a.pair_axes2 = words[2];
+  a.pair_axes3 = words[3];
+  const int64_t blocks =
+      static_cast<int64_t>(a.tokens) * ((static_cast<int64_t>(a.hq) + 2 * a.hkv) * (head_dim / 4) / kThreads + 1);
   FI_REQUIRE(blocks <= 0x7fffffffLL, FI_ERR_INVALID_SHAPE, n + ": too many tokens for one launch");
   FI_TRY(enter(ctx));
   if (a.tokens == 0) return FI_OK;
@@ -184,16 +256,15 @@ int32_t qkv_norm_rope_append(fi_context* ctx, const char* name, QkvNormArgs a, i
   a.pool_slots = static_cast<int64_t>(num_blocks) * a.block_size;
   a.code_bytes = fp4_code_bytes(num_blocks, a.hkv, a.block_size, head_dim);
   a.faults = ctx->d_faults;
-  const dim3 grid(static_cast<unsigned>(blocks));
   switch (head_dim) {
     case 32:
-      launch<32>(ctx, a, kv_dtype, grid);
+      launch<32>(ctx, a, kv_dtype);
       break;
     case 64:
-      launch<64>(ctx, a, kv_dtype, grid);
+      launch<64>(ctx, a, kv_dtype);
       break;
     default:
-      launch<128>(ctx, a, kv_dtype, grid);
+      launch<128>(ctx, a, kv_dtype);
       break;
   }
   FI_CHECK_LAUNCH("qkv_norm_rope_append_kernel");

@@ -565,7 +565,9 @@ class Context:
             raise FerrisError(4, "qkv_norm_rope_append: positions must be contiguous")
         if pair_axes is not None and len(pair_axes) != int(rotary_dims) // 2:
             raise FerrisError(3, "qkv_norm_rope_append: pair_axes needs rotary_dims / 2 entries")
-        named = None if pair_axes is None else (_I32 * max(len(pair_axes), 1))(*[int(x) for x in pair_axes])
+        if axes == 1 and pair_axes is not None and not any(pair_axes):
+            pair_axes = None  # every pair turns by the one axis
+        named = None if pair_axes is None else (_I32 * max(len(pair_axes), 1))(*pair_axes)
         check(self.lib.fi_qkv_norm_rope_append(self.handle, ptr(parts), int(splits), ptr(bq), ptr(bk), ptr(bv),
                                                ptr(nq), ptr(nk), float(eps), ptr(positions), axes, named,
                                                ptr(cos_t), ptr(sin_t), int(rotary_dims), int(max_positions),
