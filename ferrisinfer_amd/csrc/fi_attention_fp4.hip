@@ -1,6 +1,6 @@
 // Paged decode attention over a 4-bit KV pool (fi_fp4.h) on v_mfma_f32_16x16x32_bf16, in f32
 // accuracy: K and V are exact in bf16, and the f32 operands they meet (query rows,
-// probabilities) are carried as three bf16 pieces whose sum is the f32 value exactly (fi::split3_pk).
+// probabilities) are carried as three bf16 pieces whose sum is the f32 value exactly.
 //
 // The pieces cost no extra products.  A 16x16 MFMA tile has sixteen columns; a kv head serves at
 // most eight query heads.  Column 4 h + p of a tile is piece p of query head h (p = 3 is zero), so
@@ -10,11 +10,13 @@
 //     codes of dims kb * D/4 .. + D/4 - 1, as they lie in memory (16 bytes at D = 128); MFMA j takes
 //     dims kb * D/4 + 8 j + e as its k index 8 kb + e, and Q is read in the same order.
 //   O^T = V^T P^T: dims are the rows.  The scores leave lane (n, kb) with keys 4 kb + r of each
-//     16-key tile for its own column n, which is a B operand over 32 keys once the MFMA's k index
-//     8 kb + e stands for key 4 kb + e (e < 4) or 16 + 4 kb + e - 4: no exchange between lanes.
-//     Lane (m, kb) of A holds those eight keys' codes of dims m * D/16 .. + D/16 - 1; MFMA j takes dim
-//     m * D/16 + j.
-// Rows past the end are clamped to the last valid row and carry probability 0.
+//     16-key tile for its own column n, which is a B operand as it stands: no exchange between lanes.
+//     Lane (m, kb) of A holds those keys' codes of dims m * D/16 .. + D/16 - 1.  A conversion yields two
+//     neighbouring dims of one key in one register, so an operand register is (key, even dim | odd
+//     dim), and the product is taken twice, against (p, 0) for the even dims and (0, p) for the odd
+//     ones: sixteen MFMAs a 32-key step where eight would do, but no instruction to regroup the
+//     values by key (32 a step), and B needs no packing.  The vector pipe is what this kernel runs
+//     short of; the matrix pipe has the room.
 #include <type_traits>
 
 #include "fi_common.h"
@@ -32,7 +34,7 @@ typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 __device__ __forceinline__ float quad_sum(float v) { return fi::group_sum<4>(v); }
 
 // Piece p (0, 1, 2; 3: zero) of eight f32 values, as a bf16 operand.
-__device__ __forceinline__ bf16x8 piece8(const float (&x)[8], int p) {
+__device__ __forceinline__ uint4 piece8(const float (&x)[8], int p) {
   uint32_t w[4];
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
@@ -40,36 +42,38 @@ __device__ __forceinline__ bf16x8 piece8(const float (&x)[8], int p) {
     fi::split3_pk(x[2 * i], x[2 * i + 1], h, m, l);
     w[i] = p == 0 ? h : (p == 1 ? m : (p == 2 ? l : 0u));
   }
-  return __builtin_bit_cast(bf16x8, make_uint4(w[0], w[1], w[2], w[3]));
-}
-
-// The low (kHigh = 0) or high halves of eight dwords, in order.
-template <int kHigh>
-__device__ __forceinline__ bf16x8 halves8(const uint32_t (&x)[8]) {
-  uint32_t w[4];
-#pragma unroll
-  for (int i = 0; i < 4; ++i)
-    w[i] = __builtin_amdgcn_perm(x[2 * i + 1], x[2 * i], kHigh ? 0x07060302u : 0x05040100u);
-  return __builtin_bit_cast(bf16x8, make_uint4(w[0], w[1], w[2], w[3]));
+  return make_uint4(w[0], w[1], w[2], w[3]);
 }
 
 // One workgroup = one (sequence, kv head, partition of 4 WT tokens), or in small launches a share of
 // its query heads; each wave owns WT consecutive tokens, computes all their scores, then their
 // softmax once, then the weighted sum.  T tiles of four query heads.  The waves' (max, sum, acc)
 // are combined through LDS in wave order and the partitions as in decode_partition_kernel.
-template <int D, int T, int WT>
-__global__ __launch_bounds__(kThreads, 2) void decode_fp4_kernel(DecodeArgs a) {
+//
+// QUAD (block sizes that are multiples of four): the pool rows of keys 4 i .. 4 i + 3 follow each
+// other, so a lane's keys need one address and immediate offsets; the rows of the last group that lie past the
+// end are read as they are (they are rows of the same block) and masked.  Otherwise every key has
+// its own address, clamped to the last valid row.
+//
+// The wave's K codes, and V codes two steps ahead, are in flight together (a wave has 10 KB
+// outstanding at D = 128, sixteen waves a CU).
+template <int D, int T, int WT, bool QUAD>
+__global__ __launch_bounds__(kThreads, T == 1 ? 4 : 2) void decode_fp4_kernel(DecodeArgs a) {
   constexpr int kPartTokens = kWaves * WT;
   constexpr int G = 4 * T;        // query heads
   constexpr int STEPS = WT / 32;  // 32-key steps
   constexpr int KB = D / 8;       // bytes of K codes a lane holds of one key
   constexpr int KJ = D / 32;      // MFMAs of a score tile
   constexpr int VB = D / 32;      // bytes of V codes a lane holds of one key
-  constexpr int VJ = D / 16;      // MFMAs of a 32-key step of P V
+  constexpr int VJ = D / 16;      // dims of a lane
+  constexpr int VD = STEPS < 2 ? STEPS : 2;  // steps of V in flight
   constexpr int GROUPS = D / fi::kFp4Group;
+  constexpr int QP = D + 8;  // padded LDS rows of the query operand
+  constexpr int ROWS = QUAD ? kPartTokens / 4 : kPartTokens;
   static_assert(WT % 32 == 0, "a wave's tokens are whole steps");
 
-  __shared__ uint32_t s_row[kPartTokens];
+  __shared__ uint32_t s_row[ROWS];  // pool rows of the partition's tokens (QUAD: of every fourth)
+  __shared__ __align__(16) uint16_t s_q[16 * T][QP];
   __shared__ float s_ml[kWaves][G][2];
   __shared__ __align__(16) float s_acc[kWaves][G][D];
 
@@ -95,7 +99,7 @@ __global__ __launch_bounds__(kThreads, 2) void decode_fp4_kernel(DecodeArgs a) {
   if (t0 >= ctx) return;  // whole workgroup exits together
   const int n_part = min(kPartTokens, ctx - t0);
   const int nparts = (ctx + kPartTokens - 1) / kPartTokens;
-  const int w = tid >> 6;
+  const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int lane = tid & 63;
   const int m = lane & 15, kb = lane >> 4;
   const int piece = m & 3;
@@ -107,94 +111,129 @@ __global__ __launch_bounds__(kThreads, 2) void decode_fp4_kernel(DecodeArgs a) {
   const uint8_t* __restrict__ k_scales = k_codes + code_bytes;
   const uint8_t* __restrict__ v_scales = v_codes + code_bytes;
 
-  // the partition's token -> pool row indices
-  for (int t = tid; t < n_part; t += kThreads) {
-    const int pos = t0 + t;
+  // the partition's pool rows; entries past the end repeat the last one
+  for (int i = tid; i < ROWS; i += kThreads) {
+    const int last = QUAD ? (n_part - 1) & ~3 : n_part - 1;
+    const int pos = t0 + min(QUAD ? 4 * i : i, last);
     const int lb = pos / a.block_size;
     int id = lb < a.max_blocks ? a.block_tables[(size_t)seq * a.max_blocks + lb] : -1;
     if (id < 0 || id >= a.num_blocks) {
       atomicOr(a.faults, FI_FAULT_BLOCK_RANGE);
       id = 0;
     }
-    s_row[t] = (static_cast<uint32_t>(id) * a.hkv + kvh) * a.block_size + (pos - lb * a.block_size);
+    s_row[i] = (static_cast<uint32_t>(id) * a.hkv + kvh) * a.block_size + (pos - lb * a.block_size);
   }
-
-  // query rows: column m of tile t is piece m & 3 of head 4 t + m / 4
-  bf16x8 qf[T][KJ];
-#pragma unroll
-  for (int t = 0; t < T; ++t) {
-    const int g = 4 * t + (m >> 2);
-    const bool live = g < group;
-    const float* qp = a.q + (head0 + (live ? g : 0)) * D + kb * (D / 4);
-#pragma unroll
-    for (int j = 0; j < KJ; ++j) {
-      const float4 lo = *reinterpret_cast<const float4*>(qp + 8 * j);
-      const float4 hi = *reinterpret_cast<const float4*>(qp + 8 * j + 4);
-      const float x[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
-      qf[t][j] = piece8(x, live ? piece : 3);
-    }
+  // the query operand, once for the workgroup: row 4 h + p is piece p of head h
+  for (int i = tid; i < 16 * T * (D / 8); i += kThreads) {
+    const int col = i / (D / 8), d = 8 * (i % (D / 8));
+    const bool live = (col >> 2) < group;
+    const float* qp = a.q + (head0 + (live ? col >> 2 : 0)) * D + d;
+    const float4 lo = *reinterpret_cast<const float4*>(qp), hi = *reinterpret_cast<const float4*>(qp + 4);
+    const float x[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
+    *reinterpret_cast<uint4*>(&s_q[col][d]) = piece8(x, live ? col & 3 : 3);
   }
   __syncthreads();
 
   if (n > 0) {  // wave-uniform
-    const uint32_t* rows = s_row + w * WT;
-    // ---- scores: sc[t][s][8 i + r] ----
+    const uint32_t* rows = s_row + w * (QUAD ? WT / 4 : WT);
+    fi::Codes<KB> kc[2 * STEPS];
+    uint32_t ks[2 * STEPS];
+#pragma unroll
+    for (int i = 0; i < 2 * STEPS; ++i) {
+      const int key = 16 * i + m;
+      const size_t row = QUAD ? (size_t)rows[key >> 2] + (key & 3) : rows[min(key, n - 1)];
+      kc[i].load(k_codes + row * (D / 2) + kb * KB);
+      ks[i] = k_scales[row * GROUPS + kb * GROUPS / 4];
+    }
+    fi::Codes<VB> vc[VD][8];
+    uint32_t vs[VD][8];
+    // V of step s: keys 32 s + 4 kb + r and 16 more
+    auto issue_v = [&](int s, fi::Codes<VB> (&c)[8], uint32_t (&sc)[8]) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const int key = 32 * s + (e < 4 ? 0 : 16) + 4 * kb + (e & 3);
+        const size_t row = QUAD ? (size_t)rows[key >> 2] + (e & 3) : rows[min(key, n - 1)];
+        c[e].load(v_codes + row * (D / 2) + m * VB);
+        sc[e] = v_scales[row * GROUPS + m * GROUPS / 16];
+      }
+    };
+#pragma unroll
+    for (int s = 0; s < VD; ++s) issue_v(s, vc[s], vs[s]);
+    bf16x8 qf[T][KJ];
+#pragma unroll
+    for (int t = 0; t < T; ++t)
+#pragma unroll
+      for (int j = 0; j < KJ; ++j)
+        qf[t][j] = *reinterpret_cast<const bf16x8*>(&s_q[16 * t + m][kb * (D / 4) + 8 * j]);
+    sched_fence();
+
+    // ---- scores in log2 units ----
+    const float c2 = a.scale * 1.4426950408889634f;
     float sc[T][STEPS][8];
+    float mx[T];
+#pragma unroll
+    for (int t = 0; t < T; ++t) mx[t] = -INFINITY;
 #pragma unroll
     for (int s = 0; s < STEPS; ++s) {
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
-        const size_t row = rows[min(32 * s + 16 * i + m, n - 1)];
-        fi::Codes<KB> kc;
-        kc.load(k_codes + row * (D / 2) + kb * KB);
-        const float scale = fi::fp4_scale_f32(k_scales[row * GROUPS + kb * GROUPS / 4]);
+        const float scale = fi::fp4_scale_f32(ks[2 * s + i]);
         v4f acc[T];
 #pragma unroll
         for (int t = 0; t < T; ++t) acc[t] = v4f{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int j = 0; j < KJ; ++j) {
-          const bf16x8 kf = __builtin_bit_cast(bf16x8, fi::fp4_widen8(kc.w[j], scale));
+          const bf16x8 kf = __builtin_bit_cast(bf16x8, fi::fp4_widen8(kc[2 * s + i].w[j], scale));
 #pragma unroll
           for (int t = 0; t < T; ++t) acc[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf, qf[t][j], acc[t], 0, 0, 0);
         }
 #pragma unroll
         for (int t = 0; t < T; ++t)
 #pragma unroll
-          for (int r = 0; r < 4; ++r) {
-            const float v = quad_sum(acc[t][r]) * a.scale;
-            sc[t][s][4 * i + r] = 32 * s + 16 * i + 4 * kb + r < n ? v : -INFINITY;
-          }
+          for (int r = 0; r < 4; ++r) sc[t][s][4 * i + r] = quad_sum(acc[t][r]) * c2;
       }
+      if (32 * s + 32 > n) {  // wave-uniform: the step reaches past the end
+#pragma unroll
+        for (int t = 0; t < T; ++t)
+#pragma unroll
+          for (int e = 0; e < 8; ++e)
+            if (32 * s + (e < 4 ? 0 : 16) + 4 * kb + (e & 3) >= n) sc[t][s][e] = -INFINITY;
+      }
+#pragma unroll
+      for (int t = 0; t < T; ++t)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) mx[t] = fmaxf(mx[t], sc[t][s][e]);
     }
 
-    // ---- softmax over the wave's tokens (the lanes of column m's quad hold one head) ----
+    // ---- softmax over the wave's tokens (the lanes of a column's quad hold one head) ----
 #pragma unroll
     for (int t = 0; t < T; ++t) {
-      float mx = -INFINITY;
-#pragma unroll
-      for (int s = 0; s < STEPS; ++s)
-#pragma unroll
-        for (int e = 0; e < 8; ++e) mx = fmaxf(mx, sc[t][s][e]);
-      mx = fmaxf(mx, fi::lane_xor16(mx, lane));
-      mx = fmaxf(mx, fi::lane_xor32(mx, lane));
+      mx[t] = fmaxf(mx[t], fi::lane_xor16(mx[t], lane));
+      mx[t] = fmaxf(mx[t], fi::lane_xor32(mx[t], lane));
+      // every score -inf or NaN: weights 0 and NaN, against any finite point
+      const float point = mx[t] == -INFINITY ? 0.0f : mx[t];
       float l = 0.0f;
 #pragma unroll
       for (int s = 0; s < STEPS; ++s)
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-          const float p = sc[t][s][e] == -INFINITY ? 0.0f : __expf(sc[t][s][e] - mx);
-          sc[t][s][e] = p;
-          l += p;
+          sc[t][s][e] = __builtin_amdgcn_exp2f(sc[t][s][e] - point);
+          l += sc[t][s][e];
         }
       l += fi::lane_xor16(l, lane);
       l += fi::lane_xor32(l, lane);
       if (kb == 0 && piece == 0) {
-        s_ml[w][4 * t + (m >> 2)][0] = mx;
+        s_ml[w][4 * t + (m >> 2)][0] = mx[t];
         s_ml[w][4 * t + (m >> 2)][1] = l;
       }
     }
 
     // ---- O^T += V^T P^T ----
+    // this lane's piece of x by truncation: x - first h(x), of that - second h(), where h() keeps the
+    // upper 16 bits (8 significant ones); the third piece is what is left, exactly.  Piece 3 is 0 by
+    // the mask.
+    const float first = piece >= 1 ? -1.0f : 0.0f, second = piece >= 2 ? -1.0f : 0.0f;
+    const uint32_t keep = piece == 3 ? 0u : 0xffff0000u;
     v4f o[T][VJ];
 #pragma unroll
     for (int t = 0; t < T; ++t)
@@ -202,35 +241,51 @@ __global__ __launch_bounds__(kThreads, 2) void decode_fp4_kernel(DecodeArgs a) {
       for (int j = 0; j < VJ; ++j) o[t][j] = v4f{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int s = 0; s < STEPS; ++s) {
-      if (32 * s >= n) break;  // wave-uniform: the step holds no key
-      fi::Codes<VB> vc[8];
-      float scale[8];
+      uint32_t be[T][8], bo[T][8];
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const size_t row = rows[min(32 * s + (e < 4 ? 0 : 16) + 4 * kb + (e & 3), n - 1)];
-        vc[e].load(v_codes + row * (D / 2) + m * VB);
-        scale[e] = fi::fp4_scale_f32(v_scales[row * GROUPS + m * GROUPS / 16]);
-      }
-      bf16x8 pf[T];
-#pragma unroll
-      for (int t = 0; t < T; ++t) pf[t] = piece8(sc[t][s], piece);
-#pragma unroll
-      for (int j = 0; j < VJ; j += 2) {
-        uint32_t x[8];
+      for (int t = 0; t < T; ++t)
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-          if (j == 0) x[e] = fi::fp4_widen2<0>(vc[e].w[0], scale[e]);
-          if (j == 2) x[e] = fi::fp4_widen2<1>(vc[e].w[0], scale[e]);
-          if (j == 4) x[e] = fi::fp4_widen2<2>(vc[e].w[0], scale[e]);
-          if (j == 6) x[e] = fi::fp4_widen2<3>(vc[e].w[0], scale[e]);
+          const float x = sc[t][s][e];
+          const float y = fmaf(first, __uint_as_float(__float_as_uint(x) & 0xffff0000u), x);
+          const float z = fmaf(second, __uint_as_float(__float_as_uint(y) & 0xffff0000u), y);
+          bo[t][e] = __float_as_uint(z) & keep;
+          be[t][e] = bo[t][e] >> 16;
         }
-        const bf16x8 even = halves8<0>(x), odd = halves8<1>(x);
+      float scale[8];
 #pragma unroll
-        for (int t = 0; t < T; ++t) {
-          o[t][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(even, pf[t], o[t][j], 0, 0, 0);
-          o[t][j + 1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(odd, pf[t], o[t][j + 1], 0, 0, 0);
+      for (int e = 0; e < 8; ++e) scale[e] = fi::fp4_scale_f32(vs[s % VD][e]);
+      if (QUAD && 32 * s + 32 > n) {  // wave-uniform: rows past the end hold anything, a NaN scale too
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+          if (32 * s + (e < 4 ? 0 : 16) + 4 * kb + (e & 3) >= n) scale[e] = 1.0f;
+      }
+#pragma unroll
+      for (int j = 0; j < VJ; j += 2) {
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          uint32_t x[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const uint32_t c = vc[s % VD][4 * i + e].w[0];
+            const float sv = scale[4 * i + e];
+            if (j == 0) x[e] = fi::fp4_widen2<0>(c, sv);
+            if (j == 2) x[e] = fi::fp4_widen2<1>(c, sv);
+            if (j == 4) x[e] = fi::fp4_widen2<2>(c, sv);
+            if (j == 6) x[e] = fi::fp4_widen2<3>(c, sv);
+          }
+          const bf16x8 va = __builtin_bit_cast(bf16x8, make_uint4(x[0], x[1], x[2], x[3]));
+#pragma unroll
+          for (int t = 0; t < T; ++t) {
+            const bf16x8 even = __builtin_bit_cast(bf16x8, make_uint4(be[t][4 * i], be[t][4 * i + 1], be[t][4 * i + 2], be[t][4 * i + 3]));
+            const bf16x8 odd = __builtin_bit_cast(bf16x8, make_uint4(bo[t][4 * i], bo[t][4 * i + 1], bo[t][4 * i + 2], bo[t][4 * i + 3]));
+            o[t][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(va, even, o[t][j], 0, 0, 0);
+            o[t][j + 1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(va, odd, o[t][j + 1], 0, 0, 0);
+          }
         }
       }
+      if (s + VD < STEPS) issue_v(s + VD, vc[s % VD], vs[s % VD]);
+      sched_fence();
     }
     // lane (n, kb) holds dims (4 kb + r) * D/16 + j of its column; a quad's lanes store one r each
 #pragma unroll
@@ -247,29 +302,34 @@ __global__ __launch_bounds__(kThreads, 2) void decode_fp4_kernel(DecodeArgs a) {
   }
   __syncthreads();
 
-  combine_waves<D, G, WT, true>(a, hu, pairs, pair, part, nparts, n_part, s_ml, s_acc);
+  combine_waves<D, G, WT, true, true>(a, hu, pairs, pair, part, nparts, n_part, s_ml, s_acc);
 }
 
-template <int D, int T, int WT>
+template <int D, int T, int WT, bool QUAD>
 int32_t launch(fi_context* ctx, const DecodeArgs& args, dim3 grid) {
-  hipLaunchKernelGGL((decode_fp4_kernel<D, T, WT>), grid, dim3(kThreads), 0, ctx->stream, args);
+  hipLaunchKernelGGL((decode_fp4_kernel<D, T, WT, QUAD>), grid, dim3(kThreads), 0, ctx->stream, args);
   FI_CHECK_LAUNCH("decode_fp4_kernel");
   if (args.parts_per_seq > 1 && args.counters == nullptr) {
     const dim3 grid2(static_cast<unsigned>(args.num_seqs) * args.hkv, grid.y);
-    hipLaunchKernelGGL((decode_merge_kernel<D, 4 * T, WT>), grid2, dim3(kThreads), 0, ctx->stream, args);
+    hipLaunchKernelGGL((decode_merge_kernel<D, 4 * T, WT, true>), grid2, dim3(kThreads), 0, ctx->stream, args);
     FI_CHECK_LAUNCH("decode_merge_kernel");
   }
   return FI_OK;
+}
+
+template <int D, int T, int WT>
+int32_t launch_quad(fi_context* ctx, const DecodeArgs& args, dim3 grid) {
+  return args.block_size % 4 == 0 ? launch<D, T, WT, true>(ctx, args, grid) : launch<D, T, WT, false>(ctx, args, grid);
 }
 
 template <int D>
 int32_t launch_dim(fi_context* ctx, const DecodeArgs& args, dim3 grid, int wt) {
   const bool wide = wt == FI_DECODE_WIDE_WAVE_TOKENS;
   if (args.heads_per <= 4)
-    return wide ? launch<D, 1, FI_DECODE_WIDE_WAVE_TOKENS>(ctx, args, grid)
-                : launch<D, 1, FI_DECODE_NARROW_WAVE_TOKENS>(ctx, args, grid);
-  return wide ? launch<D, 2, FI_DECODE_WIDE_WAVE_TOKENS>(ctx, args, grid)
-              : launch<D, 2, FI_DECODE_NARROW_WAVE_TOKENS>(ctx, args, grid);
+    return wide ? launch_quad<D, 1, FI_DECODE_WIDE_WAVE_TOKENS>(ctx, args, grid)
+                : launch_quad<D, 1, FI_DECODE_NARROW_WAVE_TOKENS>(ctx, args, grid);
+  return wide ? launch_quad<D, 2, FI_DECODE_WIDE_WAVE_TOKENS>(ctx, args, grid)
+              : launch_quad<D, 2, FI_DECODE_NARROW_WAVE_TOKENS>(ctx, args, grid);
 }
 
 }  // namespace
