@@ -975,7 +975,8 @@ int32_t decode_paged(fi_context* ctx, const float* d_q, const void* d_k_cache, c
   // separate merge, where the merging workgroups' tail costs more than the launch (C2, 2048
   // workgroups: 113.2 against 111.4 us).
   if (parts > 1 && !noalloc && ctx->d_merge_counters != nullptr &&
-      static_cast<int64_t>(num_seqs) * num_kv_heads * shares <= FI_MERGE_COUNTERS && whole <= 6 * cus)
+      static_cast<int64_t>(num_seqs) * num_kv_heads * shares <= FI_MERGE_COUNTERS &&
+      (kv_dtype == FI_DTYPE_MXFP4 ? fi::decode_fp4_merges(whole, parts, cus) : whole <= 6 * cus))
     args.counters = ctx->d_merge_counters;
   if (kv_dtype == FI_DTYPE_MXFP4) return fi::decode_fp4(ctx, args, head_dim, grid, wt);
   switch (head_dim) {

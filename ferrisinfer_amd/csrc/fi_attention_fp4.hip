@@ -30,8 +30,18 @@ namespace {
 typedef float v4f __attribute__((ext_vector_type(4)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 
+// One move inside a quad, in the form that folds into the instruction that reads it (fi::dpp_mov's does
+// not: 32 moves a 32-key step).
+template <int kCtrl>
+__device__ __forceinline__ float quad_move(float v) {
+  return __uint_as_float(__builtin_amdgcn_update_dpp(0, __float_as_uint(v), kCtrl, 0xF, 0xF, true));
+}
+
 // The sum over the four lanes of a quad, in every lane.
-__device__ __forceinline__ float quad_sum(float v) { return fi::group_sum<4>(v); }
+__device__ __forceinline__ float quad_sum(float v) {
+  v += quad_move<0xB1>(v);
+  return v + quad_move<0x4E>(v);
+}
 
 // Piece p (0, 1, 2; 3: zero) of eight f32 values, as a bf16 operand.
 __device__ __forceinline__ uint4 piece8(const float (&x)[8], int p) {
@@ -45,10 +55,173 @@ __device__ __forceinline__ uint4 piece8(const float (&x)[8], int p) {
   return make_uint4(w[0], w[1], w[2], w[3]);
 }
 
-// One workgroup = one (sequence, kv head, partition of 4 WT tokens), or in small launches a share of
+// ---- the merge of a head's partitions ----
+// M = max m_p, L = sum l_p 2^(m_p - M), out = sum acc_p 2^(m_p - M) / L.  The partitions are summed in
+// four strands, strand s taking p = s, s + 4, .. in order, and the strands then in order: the same
+// arithmetic whether four waves take a strand each (decode_merge_fp4_kernel, any number of partitions)
+// or one wave all four (the last-arriving workgroup of a partition launch, at most kMergeInline).
+constexpr int kStrands = 4;
+constexpr int kMergeInline = 16;
+
+// NS strands from s0 on, of this lane's D / 64 dims (D = 32: of the lower half's one): the weighted
+// sums, and the strands' shares of L.  The first partitions' loads go out with the statistics'.
+template <int D, bool COHERENT, int NS>
+__device__ __forceinline__ void merge_strands(const DecodeArgs& a, size_t head, int nparts, int s0, int lane,
+                                              float (&sum)[NS][(D + 63) / 64], float (&share)[NS]) {
+  constexpr int E = (D + 63) / 64;
+  constexpr int BATCH = 8;                       // partitions whose loads are issued together
+  constexpr int STEP = NS == 1 ? kStrands : 1;   // from one of this wave's partitions to the next
+  constexpr int MAXP = NS == 1 ? kMaxParts : kMergeInline;
+  float* ml = a.part_ml + head * a.parts_per_seq * 2;
+  float* acc = a.part_acc + head * a.parts_per_seq * D + (D < 64 ? lane % D : lane * E);
+  const int mine = (nparts - s0 + STEP - 1) / STEP;  // this wave's partitions
+  float v[BATCH][E];
+#pragma unroll
+  for (int b = 0; b < BATCH; ++b) {
+    const int p = min(s0 + b * STEP, nparts - 1);  // past the end: read and dropped
+#pragma unroll
+    for (int e = 0; e < E; ++e) v[b][e] = load_partial<COHERENT>(acc + (size_t)p * D + e);
+  }
+  float mx = -INFINITY;
+#pragma unroll
+  for (int p0 = 0; p0 < MAXP; p0 += 64)
+    if (p0 + lane < nparts) mx = fmaxf(mx, load_partial<COHERENT>(&ml[2 * (p0 + lane)]));
+  // lane i keeps the statistics of this wave's i-th partition
+  const int own = s0 + lane * STEP;
+  const float m_own = own < nparts ? load_partial<COHERENT>(&ml[2 * own]) : -INFINITY;
+  const float l_own = own < nparts ? load_partial<COHERENT>(&ml[2 * own + 1]) : 0.0f;
+  mx = fi::wave_max(mx);
+  const float w_own = __builtin_amdgcn_exp2f(m_own - (mx == -INFINITY ? 0.0f : mx));
+  const float wl = l_own * w_own;
+#pragma unroll
+  for (int s = 0; s < NS; ++s) {
+    share[s] = fi::wave_sum(NS == 1 || lane % NS == s ? wl : 0.0f);
+#pragma unroll
+    for (int e = 0; e < E; ++e) sum[s][e] = 0.0f;
+  }
+  for (int i0 = 0; i0 < mine; i0 += BATCH) {
+    if (i0 > 0) {
+#pragma unroll
+      for (int b = 0; b < BATCH; ++b) {
+        const int p = min(s0 + (i0 + b) * STEP, nparts - 1);
+#pragma unroll
+        for (int e = 0; e < E; ++e) v[b][e] = load_partial<COHERENT>(acc + (size_t)p * D + e);
+      }
+    }
+#pragma unroll
+    for (int b = 0; b < BATCH; ++b) {
+      if (i0 + b < mine) {  // wave-uniform
+        const float w = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(w_own), i0 + b));
+#pragma unroll
+        for (int e = 0; e < E; ++e) sum[b % NS][e] += v[b][e] * w;
+      }
+    }
+  }
+}
+
+// One workgroup per query head, a wave a strand.
+template <int D, int WT>
+__global__ __launch_bounds__(64 * kStrands) void decode_merge_fp4_kernel(DecodeArgs a) {
+  constexpr int E = (D + 63) / 64;
+  __shared__ float s_sum[kStrands][D];
+  __shared__ float s_share[kStrands];
+  const size_t head = blockIdx.x;
+  const int seq = static_cast<int>(blockIdx.x) / a.hq;
+  const int ctx = min(a.context_lens[seq], a.parts_per_seq * kWaves * WT);  // clamped as in the partitions
+  const int nparts = (ctx + kWaves * WT - 1) / (kWaves * WT);
+  if (nparts <= 1) return;
+  const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+  float sum[1][E], share[1];
+  merge_strands<D, false, 1>(a, head, nparts, w, lane, sum, share);
+  if (D >= 64 || lane < D) {
+#pragma unroll
+    for (int e = 0; e < E; ++e) s_sum[w][lane * E + e] = sum[0][e];
+  }
+  if (lane == 0) s_share[w] = share[0];
+  __syncthreads();
+  if (threadIdx.x < D) {
+    float out = s_sum[0][threadIdx.x], l = s_share[0];
+#pragma unroll
+    for (int s = 1; s < kStrands; ++s) {
+      out += s_sum[s][threadIdx.x];
+      l += s_share[s];
+    }
+    a.out[head * D + threadIdx.x] = out * (1.0f / l);
+  }
+}
+
+// The end of a partition workgroup: the waves' (max, sum, acc) in LDS are combined in wave order.
+// A sequence with one partition writes its normalised output; otherwise the partition's partial is
+// stored, and where the launch merges by itself the last of the group's partitions merges them, a wave
+// a head (the counters' protocol is combine_waves').
+template <int D, int G, int WT>
+__device__ __forceinline__ void combine_waves_fp4(const DecodeArgs& a, const HeadUnit& hu, int pairs, int pair, int part,
+                                                  int nparts, int n_part, const float (*s_ml)[G][2],
+                                                  const float (*s_acc)[G][D]) {
+  const int tid = threadIdx.x, group = hu.heads;
+  const int nw = (n_part + WT - 1) / WT;
+  for (int i = tid; i < group * D; i += kThreads) {
+    const int g = i / D, d = i - (i / D) * D;
+    float mx = s_ml[0][g][0];
+    for (int v = 1; v < nw; ++v) mx = fmaxf(mx, s_ml[v][g][0]);
+    const float point = mx == -INFINITY ? 0.0f : mx;
+    float l = 0.0f, sum = 0.0f;
+    for (int v = 0; v < nw; ++v) {
+      const float wgt = __builtin_amdgcn_exp2f(s_ml[v][g][0] - point);
+      l += s_ml[v][g][1] * wgt;
+      sum += s_acc[v][g][d] * wgt;
+    }
+    const size_t head = hu.head0 + g, slot = head * a.parts_per_seq + part;
+    if (nparts == 1) {
+      a.out[head * D + d] = sum * (1.0f / l);
+    } else if (a.counters) {  // read by another workgroup of this launch: device-coherent stores
+      __hip_atomic_store(&a.part_acc[slot * D + d], sum, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+      if (d == 0) {
+        __hip_atomic_store(&a.part_ml[slot * 2], mx, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        __hip_atomic_store(&a.part_ml[slot * 2 + 1], l, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+      }
+    } else {
+      a.part_acc[slot * D + d] = sum;
+      if (d == 0) *reinterpret_cast<float2*>(&a.part_ml[slot * 2]) = make_float2(mx, l);
+    }
+  }
+  if (nparts <= 1 || a.counters == nullptr) return;  // workgroup-uniform
+  __shared__ int s_last;
+  __builtin_amdgcn_s_waitcnt(0);
+  __syncthreads();
+  if (tid == 0) {
+    const int unit = blockIdx.y * pairs + pair;
+    const unsigned arrived =
+        __hip_atomic_fetch_add(&a.counters[unit], 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) + 1u;
+    s_last = arrived == static_cast<unsigned>(nparts);
+    if (s_last) __hip_atomic_store(&a.counters[unit], 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  }
+  __syncthreads();
+  if (!s_last) return;
+  constexpr int E = (D + 63) / 64;
+  const int lane = tid & 63;
+  for (int g = tid >> 6; g < group; g += kWaves) {
+    const size_t head = hu.head0 + g;
+    float sum[kStrands][E], share[kStrands];
+    merge_strands<D, true, kStrands>(a, head, nparts, 0, lane, sum, share);
+#pragma unroll
+    for (int s = 1; s < kStrands; ++s) {
+      share[0] += share[s];
+#pragma unroll
+      for (int e = 0; e < E; ++e) sum[0][e] += sum[s][e];
+    }
+    if (D >= 64 || lane < D) {
+#pragma unroll
+      for (int e = 0; e < E; ++e) a.out[head * D + lane * E + e] = sum[0][e] * (1.0f / share[0]);
+    }
+  }
+}
+
+// One workgroup = one (sequence, kv head, partition of kWaves * WT tokens), or in small launches a share of
 // its query heads; each wave owns WT consecutive tokens, computes all their scores, then their
 // softmax once, then the weighted sum.  T tiles of four query heads.  The waves' (max, sum, acc)
-// are combined through LDS in wave order and the partitions as in decode_partition_kernel.
+// are combined through LDS in wave order, the partitions by the last of them to arrive or in a launch
+// of their own (merge_head).
 //
 // QUAD (block sizes that are multiples of four): the pool rows of keys 4 i .. 4 i + 3 follow each
 // other, so a lane's keys need one address and immediate offsets; the rows of the last group that lie past the
@@ -106,10 +279,13 @@ __global__ __launch_bounds__(kThreads, T == 1 ? 4 : 2) void decode_fp4_kernel(De
   const int n = min(WT, n_part - w * WT);  // the wave's tokens (<= 0: idle wave)
 
   const size_t code_bytes = fi::fp4_code_bytes(a.num_blocks, a.hkv, a.block_size, D);
-  const uint8_t* __restrict__ k_codes = static_cast<const uint8_t*>(a.k_cache);
-  const uint8_t* __restrict__ v_codes = static_cast<const uint8_t*>(a.v_cache);
-  const uint8_t* __restrict__ k_scales = k_codes + code_bytes;
-  const uint8_t* __restrict__ v_scales = v_codes + code_bytes;
+  // this lane's place in a row (QUAD: of key m & 3 of the K group whose row is looked up)
+  const int k_row = QUAD ? m & 3 : 0;
+  const uint8_t* __restrict__ k_codes = static_cast<const uint8_t*>(a.k_cache) + k_row * (D / 2) + kb * KB;
+  const uint8_t* __restrict__ v_codes = static_cast<const uint8_t*>(a.v_cache) + m * VB;
+  const uint8_t* __restrict__ k_scales =
+      static_cast<const uint8_t*>(a.k_cache) + code_bytes + k_row * GROUPS + kb * GROUPS / 4;
+  const uint8_t* __restrict__ v_scales = static_cast<const uint8_t*>(a.v_cache) + code_bytes + m * GROUPS / 16;
 
   // the partition's pool rows; entries past the end repeat the last one
   for (int i = tid; i < ROWS; i += kThreads) {
@@ -141,20 +317,30 @@ __global__ __launch_bounds__(kThreads, T == 1 ? 4 : 2) void decode_fp4_kernel(De
 #pragma unroll
     for (int i = 0; i < 2 * STEPS; ++i) {
       const int key = 16 * i + m;
-      const size_t row = QUAD ? (size_t)rows[key >> 2] + (key & 3) : rows[min(key, n - 1)];
-      kc[i].load(k_codes + row * (D / 2) + kb * KB);
-      ks[i] = k_scales[row * GROUPS + kb * GROUPS / 4];
+      const size_t row = rows[QUAD ? key >> 2 : min(key, n - 1)];
+      kc[i].load(k_codes + row * (D / 2));
+      ks[i] = k_scales[row * GROUPS];
     }
     fi::Codes<VB> vc[VD][8];
     uint32_t vs[VD][8];
     // V of step s: keys 32 s + 4 kb + r and 16 more
     auto issue_v = [&](int s, fi::Codes<VB> (&c)[8], uint32_t (&sc)[8]) {
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const int key = 32 * s + (e < 4 ? 0 : 16) + 4 * kb + (e & 3);
-        const size_t row = QUAD ? (size_t)rows[key >> 2] + (e & 3) : rows[min(key, n - 1)];
-        c[e].load(v_codes + row * (D / 2) + m * VB);
-        sc[e] = v_scales[row * GROUPS + m * GROUPS / 16];
+      for (int i = 0; i < 2; ++i) {
+        const int key = 32 * s + 16 * i + 4 * kb;
+        const size_t row = rows[QUAD ? key >> 2 : min(key, n - 1)];
+        const uint8_t* pc = v_codes + row * (D / 2);
+        const uint8_t* ps = v_scales + row * GROUPS;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          if (!QUAD && e > 0) {
+            const size_t own = rows[min(key + e, n - 1)];
+            pc = v_codes + own * (D / 2) - e * (D / 2);
+            ps = v_scales + own * GROUPS - e * GROUPS;
+          }
+          c[4 * i + e].load(pc + e * (D / 2));
+          sc[4 * i + e] = ps[e * GROUPS];
+        }
       }
     };
 #pragma unroll
@@ -197,7 +383,7 @@ __global__ __launch_bounds__(kThreads, T == 1 ? 4 : 2) void decode_fp4_kernel(De
         for (int t = 0; t < T; ++t)
 #pragma unroll
           for (int e = 0; e < 8; ++e)
-            if (32 * s + (e < 4 ? 0 : 16) + 4 * kb + (e & 3) >= n) sc[t][s][e] = -INFINITY;
+            sc[t][s][e] = 32 * s + (e < 4 ? 0 : 16) + 4 * kb + (e & 3) < n ? sc[t][s][e] : -INFINITY;
       }
 #pragma unroll
       for (int t = 0; t < T; ++t)
@@ -258,7 +444,7 @@ __global__ __launch_bounds__(kThreads, T == 1 ? 4 : 2) void decode_fp4_kernel(De
       if (QUAD && 32 * s + 32 > n) {  // wave-uniform: rows past the end hold anything, a NaN scale too
 #pragma unroll
         for (int e = 0; e < 8; ++e)
-          if (32 * s + (e < 4 ? 0 : 16) + 4 * kb + (e & 3) >= n) scale[e] = 1.0f;
+          scale[e] = 32 * s + (e < 4 ? 0 : 16) + 4 * kb + (e & 3) < n ? scale[e] : 1.0f;
       }
 #pragma unroll
       for (int j = 0; j < VJ; j += 2) {
@@ -302,7 +488,7 @@ __global__ __launch_bounds__(kThreads, T == 1 ? 4 : 2) void decode_fp4_kernel(De
   }
   __syncthreads();
 
-  combine_waves<D, G, WT, true, true>(a, hu, pairs, pair, part, nparts, n_part, s_ml, s_acc);
+  combine_waves_fp4<D, G, WT>(a, hu, pairs, pair, part, nparts, n_part, s_ml, s_acc);
 }
 
 template <int D, int T, int WT, bool QUAD>
@@ -310,9 +496,9 @@ int32_t launch(fi_context* ctx, const DecodeArgs& args, dim3 grid) {
   hipLaunchKernelGGL((decode_fp4_kernel<D, T, WT, QUAD>), grid, dim3(kThreads), 0, ctx->stream, args);
   FI_CHECK_LAUNCH("decode_fp4_kernel");
   if (args.parts_per_seq > 1 && args.counters == nullptr) {
-    const dim3 grid2(static_cast<unsigned>(args.num_seqs) * args.hkv, grid.y);
-    hipLaunchKernelGGL((decode_merge_kernel<D, 4 * T, WT, true>), grid2, dim3(kThreads), 0, ctx->stream, args);
-    FI_CHECK_LAUNCH("decode_merge_kernel");
+    hipLaunchKernelGGL((decode_merge_fp4_kernel<D, WT>), dim3(static_cast<unsigned>(args.num_seqs) * args.hq),
+                       dim3(64 * kStrands), 0, ctx->stream, args);
+    FI_CHECK_LAUNCH("decode_merge_fp4_kernel");
   }
   return FI_OK;
 }
@@ -335,6 +521,10 @@ int32_t launch_dim(fi_context* ctx, const DecodeArgs& args, dim3 grid, int wt) {
 }  // namespace
 
 namespace fi {
+
+bool decode_fp4_merges(int64_t workgroups, int parts, int64_t cus) {
+  return parts <= kMergeInline && workgroups <= 6 * cus;
+}
 
 int32_t decode_fp4(fi_context* ctx, const DecodeArgs& args, int32_t head_dim, dim3 grid, int wave_tokens) {
   switch (head_dim) {

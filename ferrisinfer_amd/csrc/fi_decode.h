@@ -113,19 +113,12 @@ __device__ __forceinline__ float load_partial(float* p) {
   return *p;
 }
 
-// The weight of a partial whose maximum lies x below the largest, in natural or log2 units.
-template <bool LOG2>
-__device__ __forceinline__ float exp_weight(float x) {
-  if constexpr (LOG2) return __builtin_amdgcn_exp2f(x);
-  return __expf(x);
-}
-
 // Combines the partitions of one (sequence, kv_head) group: M = max m_p,
 // L = sum l_p e^(m_p-M), out = sum acc_p e^(m_p-M) / L per query head.  The first
 // partitions' partials are fetched before the weights are known so the loads overlap.  The
 // same arithmetic, in the same order, runs in decode_merge_kernel and in the partition
 // kernel's last-arriving workgroup, so both give identical outputs.
-template <int D, int MAXG, bool COHERENT, bool LOG2 = false>
+template <int D, int MAXG, bool COHERENT>
 __device__ __forceinline__ void merge_unit(const DecodeArgs& a, size_t head0, int group, int nparts,
                                            float (*s_w)[kMaxParts], float* s_inv) {
   constexpr int kPrefetch = 8;
@@ -166,7 +159,7 @@ __device__ __forceinline__ void merge_unit(const DecodeArgs& a, size_t head0, in
     for (int j = 0; j < kPartsPerLane; ++j) {
       const int p = lane + 64 * j;
       if (p < nparts) {
-        const float wgt = exp_weight<LOG2>(mlv[j].x - m);
+        const float wgt = __expf(mlv[j].x - m);
         s_w[g][p] = wgt;
         l += mlv[j].y * wgt;
       }
@@ -192,7 +185,7 @@ __device__ __forceinline__ void merge_unit(const DecodeArgs& a, size_t head0, in
 // The end of a partition workgroup: the waves' (max, sum, acc) in LDS are combined in wave order.
 // A sequence with one partition writes its normalised output; otherwise the partition's partial is
 // stored, and where the launch merges by itself the last of the group's partitions merges them.
-template <int D, int G, int WT, bool SHARES, bool LOG2 = false>
+template <int D, int G, int WT, bool SHARES>
 __device__ __forceinline__ void combine_waves(const DecodeArgs& a, const HeadUnit& hu, int pairs, int pair, int part,
                                               int nparts, int n_part, const float (*s_ml)[G][2],
                                               const float (*s_acc)[G][D]) {
@@ -206,7 +199,7 @@ __device__ __forceinline__ void combine_waves(const DecodeArgs& a, const HeadUni
     for (int v = 1; v < nw; ++v) mx = fmaxf(mx, s_ml[v][g][0]);
     float l = 0.0f, sum = 0.0f;
     for (int v = 0; v < nw; ++v) {
-      const float wgt = exp_weight<LOG2>(s_ml[v][g][0] - mx);
+      const float wgt = __expf(s_ml[v][g][0] - mx);
       l += s_ml[v][g][1] * wgt;
       sum += s_acc[v][g][d] * wgt;
     }
@@ -249,13 +242,13 @@ __device__ __forceinline__ void combine_waves(const DecodeArgs& a, const HeadUni
   }
   __syncthreads();
   if (!s_last) return;
-  merge_unit<D, G, true, LOG2>(a, head0, group, nparts, s_w, s_inv);
+  merge_unit<D, G, true>(a, head0, group, nparts, s_w, s_inv);
 }
 
 // The separate merge launch (used where the partition kernel does not merge): one workgroup
 // per (sequence, kv_head) group; sequences with a single partition were finished by the
 // partition kernel, and the launch boundary orders the partials' stores before these loads.
-template <int D, int MAXG, int WT, bool LOG2 = false>
+template <int D, int MAXG, int WT>
 __global__ __launch_bounds__(kThreads) void decode_merge_kernel(DecodeArgs a) {
   constexpr int kPartTokens = kWaves * WT;
   __shared__ float s_w[MAXG][kMaxParts];
@@ -265,7 +258,7 @@ __global__ __launch_bounds__(kThreads) void decode_merge_kernel(DecodeArgs a) {
   const int ctx = min(a.context_lens[u.seq], a.parts_per_seq * kPartTokens);  // clamped as in the partitions
   const int nparts = (ctx + kPartTokens - 1) / kPartTokens;
   if (nparts <= 1) return;
-  merge_unit<D, MAXG, false, LOG2>(a, u.head0, u.heads, nparts, s_w, s_inv);
+  merge_unit<D, MAXG, false>(a, u.head0, u.heads, nparts, s_w, s_inv);
 }
 
 }  // namespace

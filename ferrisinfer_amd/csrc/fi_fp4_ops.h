@@ -28,6 +28,9 @@ int32_t kv_copy_blocks_fp4(fi_context* ctx, void* k_cache, void* v_cache, const 
 int32_t kv_gather_fp4(fi_context* ctx, const void* k_cache, const void* v_cache, const int32_t* table, int32_t length,
                       int32_t num_blocks, int32_t block_size, int32_t hkv, int32_t d, float* k_out, float* v_out);
 
+// Whether a decode launch of several partitions merges them by itself.
+bool decode_fp4_merges(int64_t workgroups, int parts, int64_t cus);
+
 // Decode attention: the partition launch and, where the launch does not merge by itself, the merge.
 int32_t decode_fp4(fi_context* ctx, const DecodeArgs& args, int32_t head_dim, dim3 grid, int wave_tokens);
 
