@@ -978,7 +978,12 @@ int32_t decode_paged(fi_context* ctx, const float* d_q, const void* d_k_cache, c
       static_cast<int64_t>(num_seqs) * num_kv_heads * shares <= FI_MERGE_COUNTERS &&
       (kv_dtype == FI_DTYPE_MXFP4 ? fi::decode_fp4_merges(whole, parts, cus) : whole <= 6 * cus))
     args.counters = ctx->d_merge_counters;
-  if (kv_dtype == FI_DTYPE_MXFP4) return fi::decode_fp4(ctx, args, head_dim, grid, wt);
+  if (kv_dtype == FI_DTYPE_MXFP4) {
+    args.blocks = fi::FastDiv(static_cast<uint32_t>(block_size));
+    return fi::decode_fp4(ctx, args, head_dim,
+                          dim3(static_cast<unsigned>(num_seqs) * num_kv_heads, static_cast<unsigned>(shares),
+                               static_cast<unsigned>(parts)), wt);
+  }
   switch (head_dim) {
     case 32:
       return launch_decode_dtype<32>(ctx, kv_dtype, args, grid, wt);

@@ -31,16 +31,29 @@ typedef float v4f __attribute__((ext_vector_type(4)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 
 // One move inside a quad, in the form that folds into the instruction that reads it (fi::dpp_mov's does
-// not: 32 moves a 32-key step).
+// not).
 template <int kCtrl>
-__device__ __forceinline__ float quad_move(float v) {
-  return __uint_as_float(__builtin_amdgcn_update_dpp(0, __float_as_uint(v), kCtrl, 0xF, 0xF, true));
+__device__ __forceinline__ uint32_t quad_move(uint32_t v) {
+  return __builtin_amdgcn_update_dpp(0, v, kCtrl, 0xF, 0xF, true);
 }
 
-// The sum over the four lanes of a quad, in every lane.
-__device__ __forceinline__ float quad_sum(float v) {
-  v += quad_move<0xB1>(v);
-  return v + quad_move<0x4E>(v);
+// Lane p of a quad ends with the sum of v[p] over the quad's four lanes: each step hands on the half
+// of the values that the neighbour keeps (nine instructions, where four full sums take eight and the
+// choice between them three, and leave four copies of each).
+__device__ __forceinline__ float quad_scatter_sum(const v4f& v, bool odd, bool high) {
+  float k0 = odd ? v[1] : v[0], x0 = odd ? v[0] : v[1];
+  float k1 = odd ? v[3] : v[2], x1 = odd ? v[2] : v[3];
+  k0 += __uint_as_float(quad_move<0xB1>(__float_as_uint(x0)));
+  k1 += __uint_as_float(quad_move<0xB1>(__float_as_uint(x1)));
+  const float k = high ? k1 : k0, x = high ? k0 : k1;
+  return k + __uint_as_float(quad_move<0x4E>(__float_as_uint(x)));
+}
+
+// What lane r of the quad holds, for this lane's piece: a (pieces 0 and 1) or b (2 and 3).
+template <int r>
+__device__ __forceinline__ uint32_t quad_pick(uint32_t a, uint32_t b, bool high) {
+  const uint32_t x = quad_move<r * 0x55>(a), y = quad_move<r * 0x55>(b);
+  return high ? y : x;
 }
 
 // Piece p (0, 1, 2; 3: zero) of eight f32 values, as a bf16 operand.
@@ -251,8 +264,7 @@ __global__ __launch_bounds__(kThreads, T == 1 ? 4 : 2) void decode_fp4_kernel(De
   __shared__ __align__(16) float s_acc[kWaves][G][D];
 
   const int pairs = a.num_seqs * a.hkv;
-  const int part = blockIdx.x / pairs;
-  const int pair = blockIdx.x - part * pairs;
+  const int part = blockIdx.z, pair = blockIdx.x;
   const HeadUnit hu = head_unit<true>(a, pair);
   const int seq = hu.seq, kvh = hu.kvh, group = hu.heads;
   if (group <= 0) return;  // every partition of the share
@@ -276,6 +288,7 @@ __global__ __launch_bounds__(kThreads, T == 1 ? 4 : 2) void decode_fp4_kernel(De
   const int lane = tid & 63;
   const int m = lane & 15, kb = lane >> 4;
   const int piece = m & 3;
+  const bool odd = piece & 1, high = piece >> 1;
   const int n = min(WT, n_part - w * WT);  // the wave's tokens (<= 0: idle wave)
 
   const size_t code_bytes = fi::fp4_code_bytes(a.num_blocks, a.hkv, a.block_size, D);
@@ -291,7 +304,7 @@ __global__ __launch_bounds__(kThreads, T == 1 ? 4 : 2) void decode_fp4_kernel(De
   for (int i = tid; i < ROWS; i += kThreads) {
     const int last = QUAD ? (n_part - 1) & ~3 : n_part - 1;
     const int pos = t0 + min(QUAD ? 4 * i : i, last);
-    const int lb = pos / a.block_size;
+    const int lb = static_cast<int>(a.blocks.div(pos));
     int id = lb < a.max_blocks ? a.block_tables[(size_t)seq * a.max_blocks + lb] : -1;
     if (id < 0 || id >= a.num_blocks) {
       atomicOr(a.faults, FI_FAULT_BLOCK_RANGE);
@@ -353,59 +366,48 @@ __global__ __launch_bounds__(kThreads, T == 1 ? 4 : 2) void decode_fp4_kernel(De
         qf[t][j] = *reinterpret_cast<const bf16x8*>(&s_q[16 * t + m][kb * (D / 4) + 8 * j]);
     sched_fence();
 
-    // ---- scores in log2 units ----
+    // ---- scores in log2 units: lane (4 h + r, kb) keeps keys 16 i + 4 kb + r of head h ----
     const float c2 = a.scale * 1.4426950408889634f;
-    float sc[T][STEPS][8];
+    float sc[T][2 * STEPS];
     float mx[T];
 #pragma unroll
     for (int t = 0; t < T; ++t) mx[t] = -INFINITY;
 #pragma unroll
-    for (int s = 0; s < STEPS; ++s) {
+    for (int i = 0; i < 2 * STEPS; ++i) {
+      const float scale = fi::fp4_scale_f32(ks[i]);
+      v4f acc[T];
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const float scale = fi::fp4_scale_f32(ks[2 * s + i]);
-        v4f acc[T];
+      for (int t = 0; t < T; ++t) acc[t] = v4f{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int t = 0; t < T; ++t) acc[t] = v4f{0.f, 0.f, 0.f, 0.f};
+      for (int j = 0; j < KJ; ++j) {
+        const bf16x8 kf = __builtin_bit_cast(bf16x8, fi::fp4_widen8(kc[i].w[j], scale));
 #pragma unroll
-        for (int j = 0; j < KJ; ++j) {
-          const bf16x8 kf = __builtin_bit_cast(bf16x8, fi::fp4_widen8(kc[2 * s + i].w[j], scale));
-#pragma unroll
-          for (int t = 0; t < T; ++t) acc[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf, qf[t][j], acc[t], 0, 0, 0);
-        }
-#pragma unroll
-        for (int t = 0; t < T; ++t)
-#pragma unroll
-          for (int r = 0; r < 4; ++r) sc[t][s][4 * i + r] = quad_sum(acc[t][r]) * c2;
-      }
-      if (32 * s + 32 > n) {  // wave-uniform: the step reaches past the end
-#pragma unroll
-        for (int t = 0; t < T; ++t)
-#pragma unroll
-          for (int e = 0; e < 8; ++e)
-            sc[t][s][e] = 32 * s + (e < 4 ? 0 : 16) + 4 * kb + (e & 3) < n ? sc[t][s][e] : -INFINITY;
+        for (int t = 0; t < T; ++t) acc[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf, qf[t][j], acc[t], 0, 0, 0);
       }
 #pragma unroll
-      for (int t = 0; t < T; ++t)
-#pragma unroll
-        for (int e = 0; e < 8; ++e) mx[t] = fmaxf(mx[t], sc[t][s][e]);
+      for (int t = 0; t < T; ++t) {
+        const float v = quad_scatter_sum(acc[t], odd, high) * c2;
+        sc[t][i] = 16 * i + 4 * kb + piece < n ? v : -INFINITY;
+        mx[t] = fmaxf(mx[t], sc[t][i]);
+      }
     }
 
-    // ---- softmax over the wave's tokens (the lanes of a column's quad hold one head) ----
+    // ---- softmax over the wave's tokens ----
 #pragma unroll
     for (int t = 0; t < T; ++t) {
+      mx[t] = fmaxf(mx[t], __uint_as_float(quad_move<0xB1>(__float_as_uint(mx[t]))));
+      mx[t] = fmaxf(mx[t], __uint_as_float(quad_move<0x4E>(__float_as_uint(mx[t]))));
       mx[t] = fmaxf(mx[t], fi::lane_xor16(mx[t], lane));
       mx[t] = fmaxf(mx[t], fi::lane_xor32(mx[t], lane));
       // every score -inf or NaN: weights 0 and NaN, against any finite point
       const float point = mx[t] == -INFINITY ? 0.0f : mx[t];
       float l = 0.0f;
 #pragma unroll
-      for (int s = 0; s < STEPS; ++s)
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          sc[t][s][e] = __builtin_amdgcn_exp2f(sc[t][s][e] - point);
-          l += sc[t][s][e];
-        }
+      for (int i = 0; i < 2 * STEPS; ++i) {
+        sc[t][i] = __builtin_amdgcn_exp2f(sc[t][i] - point);
+        l += sc[t][i];
+      }
+      l = fi::group_sum<4>(l);
       l += fi::lane_xor16(l, lane);
       l += fi::lane_xor32(l, lane);
       if (kb == 0 && piece == 0) {
@@ -415,11 +417,12 @@ __global__ __launch_bounds__(kThreads, T == 1 ? 4 : 2) void decode_fp4_kernel(De
     }
 
     // ---- O^T += V^T P^T ----
-    // this lane's piece of x by truncation: x - first h(x), of that - second h(), where h() keeps the
-    // upper 16 bits (8 significant ones); the third piece is what is left, exactly.  Piece 3 is 0 by
-    // the mask.
-    const float first = piece >= 1 ? -1.0f : 0.0f, second = piece >= 2 ? -1.0f : 0.0f;
-    const uint32_t keep = piece == 3 ? 0u : 0xffff0000u;
+    // A probability's pieces by truncation: h keeps the upper 16 bits of x (8 significant ones), m those
+    // of x - h, and l = x - h - m is what is left, exactly (weights near 2^-126, whose pieces have fewer
+    // bits, lose what lies below; the mask keeps it out of the lower half).  The lane that holds x packs (h, m) and (l, 0);
+    // column 4 h + p takes piece p of the four keys from its quad's lanes, into the upper half (odd
+    // dims) and the lower half (even dims) of a register.
+    const uint32_t to_high = odd ? 0x05040c0cu : 0x07060c0cu, to_low = odd ? 0x0c0c0504u : 0x0c0c0706u;
     v4f o[T][VJ];
 #pragma unroll
     for (int t = 0; t < T; ++t)
@@ -431,12 +434,20 @@ __global__ __launch_bounds__(kThreads, T == 1 ? 4 : 2) void decode_fp4_kernel(De
 #pragma unroll
       for (int t = 0; t < T; ++t)
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const float x = sc[t][s][e];
-          const float y = fmaf(first, __uint_as_float(__float_as_uint(x) & 0xffff0000u), x);
-          const float z = fmaf(second, __uint_as_float(__float_as_uint(y) & 0xffff0000u), y);
-          bo[t][e] = __float_as_uint(z) & keep;
-          be[t][e] = bo[t][e] >> 16;
+        for (int i = 0; i < 2; ++i) {
+          const float x = sc[t][2 * s + i];
+          const uint32_t h = __float_as_uint(x) & 0xffff0000u;
+          const float y = x - __uint_as_float(h);
+          const uint32_t mid = __float_as_uint(y) & 0xffff0000u;
+          const uint32_t rest = __float_as_uint(y - __uint_as_float(mid)) & 0xffff0000u;
+          const uint32_t hm = __builtin_amdgcn_perm(h, mid, 0x07060302u);
+          const uint32_t own[4] = {quad_pick<0>(hm, rest, high), quad_pick<1>(hm, rest, high),
+                                   quad_pick<2>(hm, rest, high), quad_pick<3>(hm, rest, high)};
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            bo[t][4 * i + r] = __builtin_amdgcn_perm(own[r], 0u, to_high);
+            be[t][4 * i + r] = __builtin_amdgcn_perm(own[r], 0u, to_low);
+          }
         }
       float scale[8];
 #pragma unroll
@@ -478,12 +489,7 @@ __global__ __launch_bounds__(kThreads, T == 1 ? 4 : 2) void decode_fp4_kernel(De
     for (int t = 0; t < T; ++t) {
       float* dst = &s_acc[w][4 * t + (m >> 2)][(4 * kb + piece) * VJ];
 #pragma unroll
-      for (int j = 0; j < VJ; ++j) {
-        float sum[4];
-#pragma unroll
-        for (int r = 0; r < 4; ++r) sum[r] = quad_sum(o[t][j][r]);
-        dst[j] = piece == 0 ? sum[0] : (piece == 1 ? sum[1] : (piece == 2 ? sum[2] : sum[3]));
-      }
+      for (int j = 0; j < VJ; ++j) dst[j] = quad_scatter_sum(o[t][j], odd, high);
     }
   }
   __syncthreads();

@@ -45,6 +45,7 @@ struct DecodeArgs {
   int block_size;
   int num_blocks;
   float scale;
+  FastDiv blocks;  // 4-bit pools: by block_size
 };
 
 }  // namespace fi
