@@ -9,8 +9,15 @@
 // lazily moved reference point of the exponents are those kernels'.
 //
 // A chunk is 64 keys: thread (lane, wave) stages key `lane`, elements wave * D/4 .. + D/4 - 1, one load
-// of codes and one scale byte each for K and V.  Two LDS buffers, one barrier a chunk; the next
-// chunk's codes are in registers (10 of them at D = 128) while the current one is multiplied.
+// of codes and one scale byte each for K and V; the next chunk's codes are in registers (10 of them at
+// D = 128) while the current one is multiplied.  One LDS buffer (36 KB at D = 128) and two barriers a chunk
+// leave room for three workgroups a CU: 222 us for 16 prompts of 32 to 1024 tokens after up to 512 cached ones
+// (32/8 heads of 128; 240 with two buffers and two workgroups), 359 TFLOP/s, three products a product:
+// 1.08 PFLOP/s of bf16 products, where a large library product reaches 1.26 on the same card.  Measured and
+// no faster: 32 rows a wave on 32x32x16 products (250), two 16-row groups a wave (234, at 256 registers),
+// the next chunk's scores beside this one's softmax (255), K and V fragments read ahead (246).  The products
+// take 45-50% of the time, the vector instructions about as much, and beside each other they overlap
+// little: a 16x16x32 product costs another wave's vector instructions 5.8 ns of its 7.2.
 //
 // A NaN group of V must reach only the rows that see its key, though a chunk's product multiplies every
 // key by every row (0 * NaN is NaN): it is staged as zeros, its key noted in a 64-bit mask of the
@@ -23,24 +30,108 @@
 
 namespace {
 
-constexpr int kKeys = 64;  // keys per staged chunk
+// A chunk's way from the pool to LDS: KB keys, thread tid stages key tid % KB, elements
+// seg * SEG .. + SEG - 1.  One block lookup per chunk, a chunk ahead of its loads; loads unconditional
+// (clamped key), codes and scales in registers until they are widened into the chunk's planes.
+template <int D, int KB>
+struct ChunkLoader {
+  static constexpr int SEG = D * KB / kThreads;
+  static constexpr int GROUPS = D / fi::kFp4Group;
+  static constexpr int KPK = D == 128 ? D + 16 : D + 8;  // padded LDS rows of K (see prefill_bf16_kernel)
+  static constexpr int KP = D + 8;                       // of V (transposing reads)
+  static_assert(KB == 64 && SEG % 8 == 0, "a wave stages a column quarter of every key, in whole dwords of codes");
 
-template <int D, int G, int RG, bool SPLIT>
-__global__ __launch_bounds__(kThreads, 2) void prefill_fp4_kernel(PrefillArgs a) {
-  constexpr int QT = kRows * RG / G;    // query tokens per workgroup (RG 16-row groups a wave)
-  constexpr int KB = kKeys;
+  const uint8_t *k_codes, *v_codes, *k_scales, *v_scales;  // of this thread's segment
+  const int* table;                                        // the sequence's blocks
+  int max_blocks, num_blocks, hkv, kvh, block_size;
+  int skey, kend, nchunks;
+  bool aligned;  // blocks that divide the chunk: the key's block within it and its offset are constants
+  int key_blk, key_off, chunk_blks;
+  fi::Codes<SEG / 2> kc, vc;
+  uint32_t k_scale, v_scale;
+  int id_next, off_next;
+  bool bad_block, part_next, valid_next;
+
+  __device__ __forceinline__ void init(const PrefillArgs& a, int seq, int kv_head, int tid, int end, int chunks) {
+    const size_t code_bytes = fi::fp4_code_bytes(a.num_blocks, a.hkv, a.block_size, D);
+    const int seg = tid / KB;
+    skey = tid % KB;
+    k_codes = static_cast<const uint8_t*>(a.k_cache) + seg * (SEG / 2);
+    v_codes = static_cast<const uint8_t*>(a.v_cache) + seg * (SEG / 2);
+    k_scales = static_cast<const uint8_t*>(a.k_cache) + code_bytes + seg * SEG / fi::kFp4Group;
+    v_scales = static_cast<const uint8_t*>(a.v_cache) + code_bytes + seg * SEG / fi::kFp4Group;
+    table = a.block_tables + (size_t)seq * a.max_blocks;
+    max_blocks = a.max_blocks;
+    num_blocks = a.num_blocks;
+    hkv = a.hkv;
+    kvh = kv_head;
+    block_size = a.block_size;
+    kend = end;
+    nchunks = chunks;
+    aligned = KB % block_size == 0;  // workgroup-uniform
+    key_blk = aligned ? skey / block_size : 0;
+    key_off = aligned ? skey - key_blk * block_size : 0;
+    chunk_blks = aligned ? KB / block_size : 0;
+    bad_block = false;
+  }
+  __device__ __forceinline__ void lookup(int c) {
+    c = min(c, nchunks - 1);
+    const int kpc = max(min(c * KB + skey, kend - 1), 0);
+    const bool exact = aligned && c * KB + skey < kend;
+    const int lb = exact ? c * chunk_blks + key_blk : kpc / block_size;
+    const bool in_table = lb < max_blocks;
+    const int id = table[in_table ? lb : 0];
+    id_next = in_table ? id : -1;
+    off_next = exact ? key_off : kpc - lb * block_size;
+  }
+  __device__ __forceinline__ void fetch(int c) {
+    c = min(c, nchunks - 1);
+    part_next = (c + 1) * KB > kend;  // workgroup-uniform: the chunk has padding keys
+    valid_next = c * KB + skey < kend;
+    const bool bad = id_next < 0 || id_next >= num_blocks;
+    bad_block |= bad;
+    const size_t row = ((size_t)(bad ? 0 : id_next) * hkv + kvh) * block_size + off_next;
+    kc.load(k_codes + row * (D / 2));
+    vc.load(v_codes + row * (D / 2));
+    k_scale = k_scales[row * GROUPS];
+    v_scale = v_scales[row * GROUPS];
+  }
+  // Padding keys of a partial chunk are stored as zero (their clamped loads hold a valid row); so is a
+  // NaN group of V, whose key goes into nan_keys[wave] (a wave stages a quarter of the columns).
+  __device__ __forceinline__ void stage(uint16_t (*ks)[KPK], uint16_t (*vs)[KP], uint64_t* nan_keys, int tid) {
+    const bool pad = part_next && !valid_next;
+    const bool nan = !pad && v_scale == 255u;
+    const uint64_t nans = __builtin_amdgcn_ballot_w64(nan);
+    if ((tid & 63) == 0) nan_keys[tid >> 6] = nans;
+    const float k2 = fi::fp4_scale_f32(pad ? 127u : k_scale), v2 = fi::fp4_scale_f32(pad || nan ? 127u : v_scale);
+    const int col = tid / KB * SEG;
+#pragma unroll
+    for (int j = 0; j < SEG / 8; ++j) {
+      *reinterpret_cast<uint4*>(&ks[skey][col + 8 * j]) = fi::fp4_widen8(pad ? 0u : kc.w[j], k2);
+      *reinterpret_cast<uint4*>(&vs[skey][col + 8 * j]) = fi::fp4_widen8(pad || nan ? 0u : vc.w[j], v2);
+    }
+  }
+};
+
+// The keys of a chunk from k0 on that a row at position qpos sees, as a mask.
+__device__ __forceinline__ uint64_t seen_keys(int qpos, int ctx, int k0) {
+  const int last = min(qpos, ctx - 1) - k0;
+  return last < 0 ? 0 : (last >= 63 ? ~0ull : (2ull << last) - 1);
+}
+
+template <int D, int G, bool SPLIT>
+__global__ __launch_bounds__(kThreads, 3) void prefill_fp4_kernel(PrefillArgs a) {
+  constexpr int QT = kRows / G;    // query tokens per workgroup
+  constexpr int KB = 64;
   constexpr int DS = D / 32;             // 32-wide d steps of Q K^T
   constexpr int DT = D / 16;             // 16-wide output d tiles of P V
   constexpr int JT = KB / 16;            // 16-key score tiles per chunk
   constexpr int KS = KB / 32;            // 32-key steps of P V
-  constexpr int SEG = D / 4;             // elements a thread stages of its key
-  constexpr int GROUPS = D / fi::kFp4Group;
   constexpr int DB = DT < 4 ? DT : 4;    // d tiles whose V fragments are held at once
-  constexpr int KP = D + 8;              // padded LDS rows of V (transposing reads)
-  constexpr int KPK = D == 128 ? D + 16 : D + 8;  // of K (see prefill_bf16_kernel)
-  __shared__ __align__(16) uint16_t Ks[2][KB][KPK];
-  __shared__ __align__(16) uint16_t Vs[2][KB][KP];
-  __shared__ uint64_t s_nan[2][4];  // keys whose V group is NaN, by column quarter
+  using Loader = ChunkLoader<D, KB>;
+  __shared__ __align__(16) uint16_t Ks[KB][Loader::KPK];
+  __shared__ __align__(16) uint16_t Vs[KB][Loader::KP];
+  __shared__ uint64_t s_nan[4];  // keys whose V group is NaN, by column quarter
 
   const int ntiles = (a.max_query_len + QT - 1) / QT;
   const int wg = blockIdx.x / a.hkv, kvh = blockIdx.x % a.hkv;
@@ -57,41 +148,28 @@ __global__ __launch_bounds__(kThreads, 2) void prefill_fp4_kernel(PrefillArgs a)
   const int start = ctx - qlen;
   const int tid = threadIdx.x, w = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
   const int li = lane & 15, lk = lane >> 4;
+  const int row = 16 * w + li;
+  const int qpos = start + q0 + row % QT;
 
-  const size_t code_bytes = fi::fp4_code_bytes(a.num_blocks, a.hkv, a.block_size, D);
-  const uint8_t* __restrict__ k_codes = static_cast<const uint8_t*>(a.k_cache);
-  const uint8_t* __restrict__ v_codes = static_cast<const uint8_t*>(a.v_cache);
-  const uint8_t* __restrict__ k_scales = k_codes + code_bytes;
-  const uint8_t* __restrict__ v_scales = v_codes + code_bytes;
-
-  // Q pieces: B operand row li of group g, d = 32 t + 8 lk .. + 7
-  int qpos[RG];
-  bf16x8 qf[RG][DS][3];
-#pragma unroll
-  for (int g = 0; g < RG; ++g) {
-    const int row = 16 * (w + 4 * g) + li;
+  // Q pieces: B operand row li, d = 32 t + 8 lk .. + 7
+  bf16x8 qf[DS][3];
+  {
     const int ah = row / QT, at = row % QT;
-    qpos[g] = start + q0 + at;
     const bool a_ok = ah < a.group && q0 + at < qlen;
-    const float* qp = a.q + ((size_t)(qs + q0 + (a_ok ? at : 0)) * a.hq + kvh * a.group + (a_ok ? ah : 0)) * D;
+    const float* qp = a.q + ((size_t)(qs + q0 + (a_ok ? at : 0)) * a.hq + kvh * a.group + (a_ok ? ah : 0)) * D + 8 * lk;
 #pragma unroll
     for (int t = 0; t < DS; ++t) {
-      const float4 lo = *reinterpret_cast<const float4*>(qp + 32 * t + 8 * lk);
-      const float4 hi = *reinterpret_cast<const float4*>(qp + 32 * t + 8 * lk + 4);
+      const float4 lo = *reinterpret_cast<const float4*>(qp + 32 * t);
+      const float4 hi = *reinterpret_cast<const float4*>(qp + 32 * t + 4);
       const f32x8 v = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
       const f32x8 z = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-      split3(a_ok ? v : z, qf[g][t]);
+      split3(a_ok ? v : z, qf[t]);
     }
   }
-  v4f o[RG][DT];  // O^T tile dt of group g: d = 16 dt + 4 lk + v, row li
-  float m_row[RG], l_part[RG];
+  v4f o[DT];  // O^T tile dt: d = 16 dt + 4 lk + v, row li
 #pragma unroll
-  for (int g = 0; g < RG; ++g) {
-#pragma unroll
-    for (int dt = 0; dt < DT; ++dt) o[g][dt] = v4f{0.f, 0.f, 0.f, 0.f};
-    m_row[g] = -INFINITY;
-    l_part[g] = 0.0f;
-  }
+  for (int dt = 0; dt < DT; ++dt) o[dt] = v4f{0.f, 0.f, 0.f, 0.f};
+  float m_row = -INFINITY, l_part = 0.0f;
   const float c2 = a.scale * 1.4426950408889634f;  // scores -> log2 units
   constexpr float kLazy = 8.0f;  // headroom of the exponents' reference point (log2 units)
 
@@ -99,138 +177,82 @@ __global__ __launch_bounds__(kThreads, 2) void prefill_fp4_kernel(PrefillArgs a)
   const int nchunks = max((kend + KB - 1) / KB, 1);
   const int c_lo = SPLIT ? split * nchunks / a.kv_splits : 0;
   const int c_hi = SPLIT ? (split + 1) * nchunks / a.kv_splits : nchunks;
+  Loader in;
+  in.init(a, seq, kvh, tid, kend, nchunks);
 
-  // staging: one block lookup per chunk, looked up a chunk ahead; loads unconditional (clamped key)
-  fi::Codes<SEG / 2> kc, vc;
-  uint32_t k_scale = 0, v_scale = 0;
-  int id_next = 0, off_next = 0;
-  bool bad_block = false;
-  bool part_next = false, valid_next = true;
-  const bool aligned = KB % a.block_size == 0;  // workgroup-uniform
-  const int lane_blk = aligned ? lane / a.block_size : 0;
-  const int lane_off = aligned ? lane - lane_blk * a.block_size : 0;
-  const int chunk_blks = aligned ? KB / a.block_size : 0;
-  auto lookup = [&](int c) {
-    c = min(c, nchunks - 1);
-    const int kpc = max(min(c * KB + lane, kend - 1), 0);
-    const bool exact = aligned && c * KB + lane < kend;
-    const int lb = exact ? c * chunk_blks + lane_blk : kpc / a.block_size;
-    const bool in_table = lb < a.max_blocks;
-    const int id = a.block_tables[(size_t)seq * a.max_blocks + (in_table ? lb : 0)];
-    id_next = in_table ? id : -1;
-    off_next = exact ? lane_off : kpc - lb * a.block_size;
-  };
-  auto fetch = [&](int c) {
-    c = min(c, nchunks - 1);
-    part_next = (c + 1) * KB > kend;  // workgroup-uniform: the chunk has padding keys
-    valid_next = c * KB + lane < kend;
-    const bool bad = id_next < 0 || id_next >= a.num_blocks;
-    bad_block |= bad;
-    const size_t row = ((size_t)(bad ? 0 : id_next) * a.hkv + kvh) * a.block_size + off_next;
-    kc.load(k_codes + row * (D / 2) + w * (SEG / 2));
-    vc.load(v_codes + row * (D / 2) + w * (SEG / 2));
-    k_scale = k_scales[row * GROUPS + w * GROUPS / 4];
-    v_scale = v_scales[row * GROUPS + w * GROUPS / 4];
-  };
-  // padding keys of a partial chunk are stored as zero (their clamped loads hold a valid row)
-  auto stage = [&](int buf) {
-    const bool pad = part_next && !valid_next;
-    const bool nan = !pad && v_scale == 255u;
-    const uint64_t nans = __builtin_amdgcn_ballot_w64(nan);
-    if (lane == 0) s_nan[buf][w] = nans;
-    const float ks = fi::fp4_scale_f32(pad ? 127u : k_scale), vs = fi::fp4_scale_f32(pad || nan ? 127u : v_scale);
-#pragma unroll
-    for (int j = 0; j < SEG / 8; ++j) {
-      *reinterpret_cast<uint4*>(&Ks[buf][lane][w * SEG + 8 * j]) = fi::fp4_widen8(pad ? 0u : kc.w[j], ks);
-      *reinterpret_cast<uint4*>(&Vs[buf][lane][w * SEG + 8 * j]) = fi::fp4_widen8(pad || nan ? 0u : vc.w[j], vs);
-    }
-  };
-
-  lookup(c_lo);
-  fetch(c_lo);
-  lookup(c_lo + 1);
-  stage(0);
+  in.lookup(c_lo);
+  in.fetch(c_lo);
+  in.lookup(c_lo + 1);
+  in.stage(Ks, Vs, s_nan, tid);
   __syncthreads();
   for (int c = c_lo; c < c_hi; ++c) {
     const int k0 = c * KB;
-    const int buf = (c - c_lo) & 1;
-    fetch(c + 1);  // the last chunk re-reads itself: the loads stay unconditional
-    lookup(c + 2);
+    in.fetch(c + 1);  // the last chunk re-reads itself: the loads stay unconditional
+    in.lookup(c + 2);
     __builtin_amdgcn_sched_barrier(0);
 
-    // ---- S^T = K Q^T: 64 keys x 16 rows per group ----
-    v4f s_acc[RG][JT];
+    // ---- S^T = K Q^T: 64 keys x 16 rows ----
+    v4f s[JT];
 #pragma unroll
-    for (int g = 0; g < RG; ++g)
-#pragma unroll
-      for (int jt = 0; jt < JT; ++jt) s_acc[g][jt] = v4f{0.f, 0.f, 0.f, 0.f};
+    for (int jt = 0; jt < JT; ++jt) s[jt] = v4f{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int t = 0; t < DS; ++t) {
       bf16x8 kf[JT];
 #pragma unroll
-      for (int jt = 0; jt < JT; ++jt) kf[jt] = *reinterpret_cast<const bf16x8*>(&Ks[buf][16 * jt + li][32 * t + 8 * lk]);
+      for (int jt = 0; jt < JT; ++jt) kf[jt] = *reinterpret_cast<const bf16x8*>(&Ks[16 * jt + li][32 * t + 8 * lk]);
 #pragma unroll
       for (int p = 2; p >= 0; --p)
 #pragma unroll
-        for (int g = 0; g < RG; ++g)
-#pragma unroll
-          for (int jt = 0; jt < JT; ++jt)
-            s_acc[g][jt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf[jt], qf[g][t][p], s_acc[g][jt], 0, 0, 0);
+        for (int jt = 0; jt < JT; ++jt)
+          s[jt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf[jt], qf[t][p], s[jt], 0, 0, 0);
     }
     // causal / context mask only where the chunk reaches past the tile's first query position
     if (k0 + KB - 1 > start + q0) {
 #pragma unroll
-      for (int g = 0; g < RG; ++g)
-#pragma unroll
-        for (int jt = 0; jt < JT; ++jt)
-#pragma unroll
-          for (int v = 0; v < 4; ++v) {
-            const int kp = k0 + 16 * jt + 4 * lk + v;
-            s_acc[g][jt][v] = (kp <= qpos[g] && kp < ctx) ? s_acc[g][jt][v] : -INFINITY;
-          }
-    }
-#pragma unroll
-    for (int g = 0; g < RG; ++g) {
-      float mx = -INFINITY;
-#pragma unroll
-      for (int jt = 0; jt < JT; ++jt)
-#pragma unroll
-        for (int v = 0; v < 4; ++v) mx = fmaxf(mx, s_acc[g][jt][v]);
-      mx = fmaxf(mx, fi::lane_xor16(mx, lane));
-      mx = fmaxf(mx, fi::lane_xor32(mx, lane));
-      const float m_chunk = mx * c2;
-      const float m_new = m_chunk > m_row[g] + kLazy ? m_chunk : m_row[g];
-      // no key seen yet (a split that starts past the row's position, keys that are NaN): the
-      // reference point stays -inf; masked scores weigh 0 and NaN ones NaN against any finite point
-      const float point = m_new == -INFINITY ? 0.0f : m_new;
-      const float alpha = m_new == m_row[g] ? 1.0f : __builtin_amdgcn_exp2f(m_row[g] - m_new);
-      m_row[g] = m_new;
-      float ls = 0.0f;
-#pragma unroll
       for (int jt = 0; jt < JT; ++jt)
 #pragma unroll
         for (int v = 0; v < 4; ++v) {
-          const float pexp = __builtin_amdgcn_exp2f(fmaf(s_acc[g][jt][v], c2, -point));
-          s_acc[g][jt][v] = pexp;
-          ls += pexp;
+          const int kp = k0 + 16 * jt + 4 * lk + v;
+          s[jt][v] = (kp <= qpos && kp < ctx) ? s[jt][v] : -INFINITY;
         }
-      l_part[g] = l_part[g] * alpha + ls;
-      if (__builtin_amdgcn_ballot_w64(alpha != 1.0f) != 0) {
-#pragma unroll
-        for (int dt = 0; dt < DT; ++dt) o[g][dt] *= alpha;
-      }
     }
+    float mx = -INFINITY;
+#pragma unroll
+    for (int jt = 0; jt < JT; ++jt)
+#pragma unroll
+      for (int v = 0; v < 4; ++v) mx = fmaxf(mx, s[jt][v]);
+    mx = fmaxf(mx, fi::lane_xor16(mx, lane));
+    mx = fmaxf(mx, fi::lane_xor32(mx, lane));
+    const float m_chunk = mx * c2;
+    const float m_new = m_chunk > m_row + kLazy ? m_chunk : m_row;
+    // no key seen yet (a split that starts past the row's position, keys that are NaN): the
+    // reference point stays -inf; masked scores weigh 0 and NaN ones NaN against any finite point
+    const float point = m_new == -INFINITY ? 0.0f : m_new;
+    // rows whose point moved (after the first chunks, hardly any)
+    if (__builtin_amdgcn_ballot_w64(m_new != m_row) != 0) {
+      const float alpha = m_new == m_row ? 1.0f : __builtin_amdgcn_exp2f(m_row - m_new);
+      l_part *= alpha;
+#pragma unroll
+      for (int dt = 0; dt < DT; ++dt) o[dt] *= alpha;
+    }
+    m_row = m_new;
+    float ls = 0.0f;
+#pragma unroll
+    for (int jt = 0; jt < JT; ++jt)
+#pragma unroll
+      for (int v = 0; v < 4; ++v) {
+        s[jt][v] = __builtin_amdgcn_exp2f(fmaf(s[jt][v], c2, -point));
+        ls += s[jt][v];
+      }
+    l_part += ls;
 
     // ---- O^T += V^T P^T (k index 8 lk + e of step u: key 32 u + 4 lk + e, e < 4, or 32 u + 16 + 4 lk + e - 4) ----
 #pragma unroll
     for (int u = 0; u < KS; ++u) {
-      bf16x8 pp[RG][3];
-#pragma unroll
-      for (int g = 0; g < RG; ++g) {
-        const f32x8 pf = {s_acc[g][2 * u][0],     s_acc[g][2 * u][1],     s_acc[g][2 * u][2],     s_acc[g][2 * u][3],
-                          s_acc[g][2 * u + 1][0], s_acc[g][2 * u + 1][1], s_acc[g][2 * u + 1][2], s_acc[g][2 * u + 1][3]};
-        split3(pf, pp[g]);
-      }
+      const f32x8 pf = {s[2 * u][0],     s[2 * u][1],     s[2 * u][2],     s[2 * u][3],
+                        s[2 * u + 1][0], s[2 * u + 1][1], s[2 * u + 1][2], s[2 * u + 1][3]};
+      bf16x8 pp[3];
+      split3(pf, pp);
       // transposing reads as in prefill_bf16_kernel
       const int vrow = 32 * u + 4 * lk + (li >> 2), vcol = 4 * (li & 3);
 #pragma unroll
@@ -238,124 +260,103 @@ __global__ __launch_bounds__(kThreads, 2) void prefill_fp4_kernel(PrefillArgs a)
         bf16x8 vf[DB];
 #pragma unroll
         for (int i = 0; i < DB; ++i) {
-          const v4s lo = lds_read_tr16(&Vs[buf][vrow][16 * (d0 + i) + vcol]);
-          const v4s hi = lds_read_tr16(&Vs[buf][vrow + 16][16 * (d0 + i) + vcol]);
+          const v4s lo = lds_read_tr16(&Vs[vrow][16 * (d0 + i) + vcol]);
+          const v4s hi = lds_read_tr16(&Vs[vrow + 16][16 * (d0 + i) + vcol]);
           vf[i] = __builtin_bit_cast(bf16x8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
         }
 #pragma unroll
         for (int p = 2; p >= 0; --p)
 #pragma unroll
           for (int i = 0; i < DB; ++i)
-#pragma unroll
-            for (int g = 0; g < RG; ++g)
-              o[g][d0 + i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf[i], pp[g][p], o[g][d0 + i], 0, 0, 0);
+            o[d0 + i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf[i], pp[p], o[d0 + i], 0, 0, 0);
       }
     }
     // rows that see a key with a NaN group of V
-    if ((s_nan[buf][0] | s_nan[buf][1] | s_nan[buf][2] | s_nan[buf][3]) != 0) {  // workgroup-uniform
-#pragma unroll
-      for (int g = 0; g < RG; ++g) {
-        const int last = min(qpos[g], ctx - 1) - k0;  // the last key of the chunk that the row sees
-        const uint64_t seen = last < 0 ? 0 : (last >= 63 ? ~0ull : (2ull << last) - 1);
-#pragma unroll
-        for (int dt = 0; dt < DT; ++dt)
-          if (s_nan[buf][dt * 4 / DT] & seen) o[g][dt] = v4f{NAN, NAN, NAN, NAN};
-      }
-    }
-    // the other buffer was last read in the chunk before, which every wave finished before the
-    // previous barrier; this barrier publishes the next chunk and retires this one's buffer
-    if (c + 1 < c_hi) stage(buf ^ 1);  // workgroup-uniform
-    __syncthreads();
-  }
-
-  if (bad_block) atomicOr(a.faults, FI_FAULT_BLOCK_RANGE);
-
-  // ---- normalise and store: lane holds row li of each group, d = 16 dt + 4 lk + v ----
-#pragma unroll
-  for (int g = 0; g < RG; ++g) {
-    float l_row = l_part[g] + fi::lane_xor16(l_part[g], lane);
-    l_row += fi::lane_xor32(l_row, lane);
-    const int row = 16 * (w + 4 * g) + li;
-    if constexpr (SPLIT) {
-      // this split's partials: O [rows][D] unnormalised, then (reference point, row sum) [rows].  A NaN
-      // sum takes a finite point, which the merge does not skip; a row without any key is O = 0 over 1
-      constexpr int ROWS = kRows * RG;
-      const size_t unit = ((size_t)tile * a.kv_splits + split) * a.hkv + kvh;
-      float* po = a.part + unit * ROWS * D + (size_t)row * D;
-      float* pml = a.part + (size_t)gridDim.x * ROWS * D + (unit * ROWS + row) * 2;
+    if ((s_nan[0] | s_nan[1] | s_nan[2] | s_nan[3]) != 0) {  // workgroup-uniform
+      const uint64_t seen = seen_keys(qpos, ctx, k0);
 #pragma unroll
       for (int dt = 0; dt < DT; ++dt)
-        *reinterpret_cast<float4*>(po + 16 * dt + 4 * lk) = make_float4(o[g][dt][0], o[g][dt][1], o[g][dt][2], o[g][dt][3]);
-      if (lk == 0)
-        *reinterpret_cast<float2*>(pml) = qpos[g] < 0 ? make_float2(0.f, 1.f)
-                                                      : make_float2(l_row != l_row ? 0.f : m_row[g], l_row);
-    } else {
-      const int h = row / QT, t = row % QT;
-      if (h < a.group && q0 + t < qlen) {
-        const float inv = qpos[g] < 0 ? 0.0f : 1.0f / l_row;
-        float* op = a.out + ((size_t)(qs + q0 + t) * a.hq + kvh * a.group + h) * D;
+        if (s_nan[dt * 4 / DT] & seen) o[dt] = v4f{NAN, NAN, NAN, NAN};
+    }
+    __syncthreads();  // every wave is done with this chunk's K and V
+    if (c + 1 < c_hi) {  // workgroup-uniform
+      in.stage(Ks, Vs, s_nan, tid);
+      __syncthreads();
+    }
+  }
+
+  if (in.bad_block) atomicOr(a.faults, FI_FAULT_BLOCK_RANGE);
+
+  float l_row = l_part + fi::lane_xor16(l_part, lane);
+  l_row += fi::lane_xor32(l_row, lane);
+  if constexpr (SPLIT) {
+    // this split's partials: O [rows][D] unnormalised, then (reference point, row sum) [rows].  A NaN
+    // sum takes a finite point, which the merge does not skip; a row without any key is O = 0 over 1
+    const size_t unit = ((size_t)tile * a.kv_splits + split) * a.hkv + kvh;
+    float* po = a.part + unit * kRows * D + (size_t)row * D;
+    float* pml = a.part + (size_t)gridDim.x * kRows * D + (unit * kRows + row) * 2;
 #pragma unroll
-        for (int dt = 0; dt < DT; ++dt)
-          *reinterpret_cast<float4*>(op + 16 * dt + 4 * lk) =
-              make_float4(o[g][dt][0] * inv, o[g][dt][1] * inv, o[g][dt][2] * inv, o[g][dt][3] * inv);
-      }
+    for (int dt = 0; dt < DT; ++dt)
+      *reinterpret_cast<float4*>(po + 16 * dt + 4 * lk) = make_float4(o[dt][0], o[dt][1], o[dt][2], o[dt][3]);
+    if (lk == 0)
+      *reinterpret_cast<float2*>(pml) = qpos < 0 ? make_float2(0.f, 1.f) : make_float2(l_row != l_row ? 0.f : m_row, l_row);
+  } else {
+    const int h = row / QT, t = row % QT;
+    if (h < a.group && q0 + t < qlen) {
+      const float inv = qpos < 0 ? 0.0f : 1.0f / l_row;
+      float* op = a.out + ((size_t)(qs + q0 + t) * a.hq + kvh * a.group + h) * D;
+#pragma unroll
+      for (int dt = 0; dt < DT; ++dt)
+        *reinterpret_cast<float4*>(op + 16 * dt + 4 * lk) =
+            make_float4(o[dt][0] * inv, o[dt][1] * inv, o[dt][2] * inv, o[dt][3] * inv);
     }
   }
 }
 
-template <int D, int RG, bool SPLIT>
-void launch_g(fi_context* ctx, const PrefillArgs& args, dim3 grid, int g) {
-  switch (g) {
-    case 1:
-      hipLaunchKernelGGL((prefill_fp4_kernel<D, 1, RG, SPLIT>), grid, dim3(kThreads), 0, ctx->stream, args);
-      break;
-    case 2:
-      hipLaunchKernelGGL((prefill_fp4_kernel<D, 2, RG, SPLIT>), grid, dim3(kThreads), 0, ctx->stream, args);
-      break;
-    case 4:
-      hipLaunchKernelGGL((prefill_fp4_kernel<D, 4, RG, SPLIT>), grid, dim3(kThreads), 0, ctx->stream, args);
-      break;
-    default:
-      hipLaunchKernelGGL((prefill_fp4_kernel<D, 8, RG, SPLIT>), grid, dim3(kThreads), 0, ctx->stream, args);
-      break;
+template <int D, int G>
+void launch_group(fi_context* ctx, const PrefillArgs& args, dim3 grid) {
+  if (args.kv_splits > 1) {
+    hipLaunchKernelGGL((prefill_fp4_kernel<D, G, true>), grid, dim3(kThreads), 0, ctx->stream, args);
+  } else {
+    hipLaunchKernelGGL((prefill_fp4_kernel<D, G, false>), grid, dim3(kThreads), 0, ctx->stream, args);
   }
-}
-
-template <int D, int RG>
-int32_t launch_rg(fi_context* ctx, PrefillArgs& args, int g) {
-  const int qt = kRows * RG / g;
-  // Key splits for launches that leave most workgroup slots empty, as for f32 pools: up to four
-  // workgroups a CU, each with at least two chunks (a tile's keys are at least max_query_len).
-  int splits = 1;
-  if (RG == 1) {
-    const long cus = ctx->compute_units > 0 ? ctx->compute_units : 256;
-    const long wgs = (long)((args.max_query_len + qt - 1) / qt) * args.num_seqs * args.hkv;
-    splits = static_cast<int>(std::min<long>(FI_PREFILL_MAX_SPLITS, (4 * cus) / std::max<long>(wgs, 1)));
-    splits = std::max(1, std::min(splits, args.max_query_len / (2 * kKeys)));
-  }
-  dim3 grid;
-  FI_TRY(plan_tiles(ctx, args, qt, kKeys, "fi_attn_prefill_paged", &grid, splits, kRows * RG * (D + 2)));
-  if constexpr (RG == 1) {
-    if (splits > 1) {
-      launch_g<D, RG, true>(ctx, args, grid, g);
-      FI_CHECK_LAUNCH("prefill_fp4_kernel");
-      const int ntiles = (args.max_query_len + qt - 1) / qt;
-      hipLaunchKernelGGL((prefill_split_merge_kernel<D, RG>), dim3(grid.x / splits), dim3(kThreads), 0, ctx->stream,
-                         args, qt, ntiles);
-      FI_CHECK_LAUNCH("prefill_split_merge_kernel");
-      return FI_OK;
-    }
-  }
-  launch_g<D, RG, false>(ctx, args, grid, g);
-  FI_CHECK_LAUNCH("prefill_fp4_kernel");
-  return FI_OK;
 }
 
 template <int D>
 int32_t launch_dim(fi_context* ctx, const PrefillArgs& args_in) {
   PrefillArgs args = args_in;
   const int g = args.group <= 1 ? 1 : (args.group <= 2 ? 2 : (args.group <= 4 ? 4 : 8));
-  return row_groups(ctx, args, g) == 2 ? launch_rg<D, 2>(ctx, args, g) : launch_rg<D, 1>(ctx, args, g);
+  const int qt = kRows / g;
+  // Key splits for launches that leave most workgroup slots empty, as for f32 pools: up to four
+  // workgroups a CU, each with 128 keys or more (a tile's keys are at least max_query_len).
+  const long cus = ctx->compute_units > 0 ? ctx->compute_units : 256;
+  const long wgs = (long)((args.max_query_len + qt - 1) / qt) * args.num_seqs * args.hkv;
+  int splits = static_cast<int>(std::min<long>(FI_PREFILL_MAX_SPLITS, (4 * cus) / std::max<long>(wgs, 1)));
+  splits = std::max(1, std::min(splits, args.max_query_len / 128));
+  dim3 grid;
+  FI_TRY(plan_tiles(ctx, args, qt, 64, "fi_attn_prefill_paged", &grid, splits, kRows * (D + 2)));
+  switch (g) {
+    case 1:
+      launch_group<D, 1>(ctx, args, grid);
+      break;
+    case 2:
+      launch_group<D, 2>(ctx, args, grid);
+      break;
+    case 4:
+      launch_group<D, 4>(ctx, args, grid);
+      break;
+    default:
+      launch_group<D, 8>(ctx, args, grid);
+      break;
+  }
+  FI_CHECK_LAUNCH("prefill_fp4_kernel");
+  if (splits > 1) {
+    const int ntiles = (args.max_query_len + qt - 1) / qt;
+    hipLaunchKernelGGL((prefill_split_merge_kernel<D, 1>), dim3(grid.x / splits), dim3(kThreads), 0, ctx->stream, args,
+                       qt, ntiles);
+    FI_CHECK_LAUNCH("prefill_split_merge_kernel");
+  }
+  return FI_OK;
 }
 
 }  // namespace
