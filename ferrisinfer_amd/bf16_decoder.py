@@ -28,12 +28,17 @@ rounded to nearest even where they are produced: the residual norms write them d
 and the first norm are narrowed by fi_convert_f32_to_bf16.  The GEMMs round f32 activations
 the same way, so the step's results are bit-identical either way; bf16 inputs halve the bytes
 the projections stage per K step.
+
+The K/V pools are bf16 or, with `kv_dtype` DTYPE_MXFP4, 4-bit; the prefill chunk then goes through
+fi_attn_prefill_paged, which attends a 4-bit pool in f32 accuracy.  A layer with query and key head
+norms, or a decoder whose positions have several axes (`pair_axes`), consumes its q|k|v projection
+with fi_qkv_norm_rope_append.
 """
 from __future__ import annotations
 
 from dataclasses import dataclass
 
-from .kernel import DTYPE_BF16, FerrisError
+from .kernel import DTYPE_BF16, DTYPE_MXFP4, FerrisError, kv_pool_bytes
 
 LLAMA3_8B_C5 = dict(hidden=4096, intermediate=14336, layers=32, heads=32, kv_heads=8, vocab=128256,
                     max_pos=8192 + 2048, eps=1e-6, theta=500000.0, tie=False)
@@ -43,7 +48,7 @@ LLAMA3_8B_C5 = dict(hidden=4096, intermediate=14336, layers=32, heads=32, kv_hea
 class StepBatch:
     """Device metadata of one mixed step: rows [0, num_decode) are one decode token per
     sequence, rows [num_decode, T) the prefill chunks packed by cu_seqlens."""
-    positions: object          # int32 [T]
+    positions: object          # int32 [T] (or [axes, T], contiguous, for a decoder with pair_axes)
     slot_mapping: object       # int64 [T]
     num_decode: int
     dec_block_tables: object   # int32 [Bd, max_blocks]
@@ -57,12 +62,19 @@ class StepBatch:
 
 
 class Bf16Decoder:
-    """Packed bf16 weights, per-layer bf16 K/V pools and the step buffers for up to
-    `max_tokens` rows."""
+    """Packed bf16 weights, per-layer K/V pools (bf16, or 4-bit with kv_dtype DTYPE_MXFP4) and the
+    step buffers for up to `max_tokens` rows.  pair_axes: the position axis of each rotary pair, for
+    positions of several axes."""
 
     def __init__(self, ctx, cfg: dict, num_blocks: int, block_size: int, max_tokens: int,
-                 max_last_rows: int, bf16_activations: bool = True):
+                 max_last_rows: int, bf16_activations: bool = True, kv_dtype: int = DTYPE_BF16,
+                 pair_axes=None):
         import torch
+
+        if kv_dtype not in (DTYPE_BF16, DTYPE_MXFP4):
+            raise FerrisError(5, "decoder KV dtype must be bf16 or mxfp4")
+        self.kv_dtype = kv_dtype
+        self.pair_axes = None if pair_axes is None else [int(a) for a in pair_axes]
 
         self.ctx, self.cfg = ctx, cfg
         self.bf16_activations = bool(bf16_activations)
@@ -75,9 +87,11 @@ class Bf16Decoder:
         self.final_norm = None
         self.lm_head = None
         dev = "cuda"
-        pool = (num_blocks, self.hkv, block_size, self.d)
-        self.k_pools = [torch.empty(pool, dtype=torch.int16, device=dev) for _ in range(cfg["layers"])]
-        self.v_pools = [torch.empty(pool, dtype=torch.int16, device=dev) for _ in range(cfg["layers"])]
+        pool, cell = (num_blocks, self.hkv, block_size, self.d), torch.int16
+        if kv_dtype == DTYPE_MXFP4:  # codes, then scales
+            pool, cell = (kv_pool_bytes(kv_dtype, num_blocks, block_size, self.hkv, self.d),), torch.uint8
+        self.k_pools = [torch.empty(pool, dtype=cell, device=dev) for _ in range(cfg["layers"])]
+        self.v_pools = [torch.empty(pool, dtype=cell, device=dev) for _ in range(cfg["layers"])]
         t = max_tokens
         self.hidden = [torch.empty(t, self.h, device=dev), torch.empty(t, self.h, device=dev)]
         self.normed = torch.empty(t, self.h, device=dev)
@@ -102,15 +116,17 @@ class Bf16Decoder:
         self.parts = None
 
     # ---- weights ----
-    def set_layer(self, wq, wk, wv, wo, w1, w2, w3, attention_norm, ffn_norm):
-        """Packs one layer's [in, out] weights (bf16 bits as int16 / torch.bfloat16, or f32)."""
+    def set_layer(self, wq, wk, wv, wo, w1, w2, w3, attention_norm, ffn_norm, q_norm=None, k_norm=None):
+        """Packs one layer's [in, out] weights (bf16 bits as int16 / torch.bfloat16, or f32); q_norm and
+        k_norm: f32 [D] weights of the query and key heads' RMS norms."""
         c = self.ctx
         self.layers.append(dict(
             qkv=c.weight_pack_bf16_columns([wq, wk, wv], self.h),
             wo=c.weight_pack_bf16(wo, self.h, self.h),
             w13=c.weight_pack_bf16_pair(w1, w3, self.h, self.f),
             w2=c.weight_pack_bf16(w2, self.f, self.h),
-            attention_norm=attention_norm, ffn_norm=ffn_norm))
+            attention_norm=attention_norm, ffn_norm=ffn_norm,
+            head_norms=None if q_norm is None and k_norm is None else (q_norm, k_norm)))
 
     def set_head(self, final_norm, output_weight):
         """Final norm [H] and the [vocab, hidden] output weight."""
@@ -155,17 +171,24 @@ class Bf16Decoder:
             w = self.layers[li]
             parts = self._parts(t, self.nqkv, s_qkv)
             c.gemm_bf16(xin, w["qkv"], h, self.nqkv, s_qkv, parts)
-            c.qkv_rope_append(parts, s_qkv, None, b.positions, self.cos, self.sin, self.d, self.max_pos,
-                              b.slot_mapping, self.k_pools[li], self.v_pools[li], DTYPE_BF16,
-                              self.num_blocks, self.block_size, self.hq, self.hkv, self.d, q)
+            kv = (b.slot_mapping, self.k_pools[li], self.v_pools[li], self.kv_dtype, self.num_blocks,
+                  self.block_size, self.hq, self.hkv, self.d, q)
+            if w["head_norms"] is None and self.pair_axes is None:
+                c.qkv_rope_append(parts, s_qkv, None, b.positions, self.cos, self.sin, self.d, self.max_pos, *kv)
+            else:
+                c.qkv_norm_rope_append(parts, s_qkv, None, w["head_norms"], eps, b.positions, self.pair_axes,
+                                       self.cos, self.sin, self.d, self.max_pos, *kv)
             if nd > 0:
-                c.attn_decode_paged(q[:nd], self.k_pools[li], self.v_pools[li], DTYPE_BF16,
+                c.attn_decode_paged(q[:nd], self.k_pools[li], self.v_pools[li], self.kv_dtype,
                                     b.dec_block_tables, b.dec_context_lens, b.dec_max_context, self.hkv,
                                     self.block_size, self.num_blocks, scale, attn[:nd])
             if t > nd:
-                c.attn_prefill_paged_bf16(q[nd:], self.k_pools[li], self.v_pools[li], b.pf_block_tables,
-                                          b.pf_cu_seqlens, b.pf_context_lens, b.pf_max_query, self.hkv,
-                                          self.block_size, self.num_blocks, scale, attn[nd:])
+                chunk = (b.pf_block_tables, b.pf_cu_seqlens, b.pf_context_lens, b.pf_max_query, self.hkv,
+                         self.block_size, self.num_blocks, scale, attn[nd:])
+                if self.kv_dtype == DTYPE_BF16:
+                    c.attn_prefill_paged_bf16(q[nd:], self.k_pools[li], self.v_pools[li], *chunk)
+                else:
+                    c.attn_prefill_paged(q[nd:], self.k_pools[li], self.v_pools[li], self.kv_dtype, *chunk)
             if b16:
                 c.convert_f32_to_bf16(attn, ain)
             parts = self._parts(t, h, s_o)

@@ -60,6 +60,13 @@ const char* fr_last_error(void) { return g_err.c_str(); }
 int32_t fr_create(int32_t ordinal, const fr_model_config* mc, const fr_runtime_config* rc, void** out) {
   return guard([&] {
     if (!mc || !rc || !out) fr::fail(fr::ErrorKind::InvalidConfig, "fr_create: null argument");
+    if (rc->kv_dtype == FI_DTYPE_MXFP4 && mc->num_attention_heads > 0) {
+      const int32_t d = mc->hidden_size / mc->num_attention_heads;
+      if ((d != 32 && d != 64 && d != 128) || mc->rotary_dims % 8 != 0) {
+        fr::fail(fr::ErrorKind::Unsupported,
+                 "a 4-bit KV pool is served for head dims 32, 64 and 128 with rotary dims a multiple of 8");
+      }
+    }
     auto r = std::make_unique<Runtime>();
     fr::check(fi_ctx_create(ordinal, &r->ctx));
     fr::ModelConfig c;

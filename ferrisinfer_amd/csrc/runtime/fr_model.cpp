@@ -241,12 +241,14 @@ BlockPool::BlockPool(fi_context* ctx, int32_t layers, int32_t num_blocks, int32_
   if (layers <= 0 || num_blocks <= 0 || block_size <= 0 || kv_heads <= 0 || head_dim <= 0) {
     fail(ErrorKind::InvalidConfig, "KV cache dimensions must be greater than zero");
   }
-  if (kv_dtype != FI_DTYPE_F32 && kv_dtype != FI_DTYPE_BF16) fail(ErrorKind::InvalidType, "KV dtype must be f32 or bf16");
+  if (kv_dtype != FI_DTYPE_F32 && kv_dtype != FI_DTYPE_BF16 && kv_dtype != FI_DTYPE_MXFP4) {
+    fail(ErrorKind::InvalidType, "KV dtype must be f32, bf16 or mxfp4");
+  }
   free_.reserve(num_blocks);
   for (int32_t b = num_blocks - 1; b >= 0; --b) free_.push_back(b);
   refs_.assign(num_blocks, 0);
-  const size_t elem = kv_dtype == FI_DTYPE_F32 ? 4 : 2;
-  const size_t bytes = static_cast<size_t>(num_blocks) * kv_heads * block_size * head_dim * elem;
+  size_t bytes = 0;
+  check(fi_kv_pool_bytes(kv_dtype, num_blocks, block_size, kv_heads, head_dim, &bytes));
   for (int32_t l = 0; l < layers; ++l) {
     k_.emplace_back(ctx, bytes);
     v_.emplace_back(ctx, bytes);

@@ -9,7 +9,7 @@ import time
 
 import numpy as np
 
-from .kernel import DTYPE_BF16, DTYPE_F16, DTYPE_F32, FerrisError, PKG_DIR, load as load_kernel
+from .kernel import DTYPE_BF16, DTYPE_F16, DTYPE_F32, DTYPE_MXFP4, FerrisError, PKG_DIR, load as load_kernel
 
 LIB_PATH = os.path.join(PKG_DIR, "libferrisinfer_runtime.so")
 
@@ -147,7 +147,8 @@ class Runtime:
                  max_consecutive_prefill=2, min_share=64, num_blocks=4096, block_size=16,
                  kv_dtype="f32", ordinal=0, sampler=None, weight_dtype="f32", graph_decode=False):
         """sampler: None (greedy) or (temperature, top_k, top_p, seed), the SamplerConfig of
-        every session (runtime/sampler.rs:3-43).  weight_dtype "f32" or "bf16": storage of the
+        every session (runtime/sampler.rs:3-43).  kv_dtype "f32", "bf16" or "mxfp4" (4-bit KV
+        pool): storage of the KV pool.  weight_dtype "f32" or "bf16": storage of the
         packed projections and head.  graph_decode: replay decode ticks from HIP graphs."""
         L = load()
         temperature, top_k, top_p, seed = (0.0, 1, 1.0, 0) if sampler is None else sampler
@@ -156,7 +157,7 @@ class Runtime:
                          head_dim if rotary_dims is None else rotary_dims, 1 if tie else 0)
         rc = RuntimeConfig(max_seq, max_gen, max_batch, max_chunk, max_batch_tokens,
                            max_consecutive_prefill, min_share, num_blocks, block_size,
-                           DTYPE_F32 if kv_dtype == "f32" else DTYPE_BF16,
+                           {"f32": DTYPE_F32, "mxfp4": DTYPE_MXFP4}.get(kv_dtype, DTYPE_BF16),
                            temperature, top_k, top_p, 1.0, seed,
                            DTYPE_F32 if weight_dtype == "f32" else DTYPE_BF16,
                            1 if graph_decode else 0)

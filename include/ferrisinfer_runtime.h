@@ -43,7 +43,7 @@ typedef struct fr_runtime_config {
   int64_t min_prefix_share_tokens;
   int32_t num_blocks;
   int32_t block_size;
-  int32_t kv_dtype; /* FI_DTYPE_F32 or FI_DTYPE_BF16 */
+  int32_t kv_dtype; /* FI_DTYPE_F32, FI_DTYPE_BF16 or FI_DTYPE_MXFP4 (head_dim 32, 64 or 128, rotary_dims % 8 == 0) */
   /* SamplerConfig of every session (sampler.rs:3-43, session.rs:29-46).  Greedy when
    * temperature <= 0, top_k == 1 or top_p <= 0 (a zero-filled struct is greedy): the fused
    * argmax head.  Otherwise sample_last_token on the device (fi_sample_tokens) with one
