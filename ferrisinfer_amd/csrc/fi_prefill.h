@@ -31,6 +31,7 @@ struct PrefillArgs {
   // row sum per row) that prefill_split_merge_kernel combines in split order
   int kv_splits;
   float* part;
+  int split_chunks;  // 4-bit pools: a tile is cut into kv_splits ranges, or as many of this many chunks as it has
 };
 
 }  // namespace fi

@@ -119,10 +119,23 @@ __device__ __forceinline__ uint64_t seen_keys(int qpos, int ctx, int k0) {
   return last < 0 ? 0 : (last >= 63 ? ~0ull : (2ull << last) - 1);
 }
 
+constexpr int kChunk = 64;      // keys
+constexpr int kMaxSplits = 32;  // key splits of a tile, at most
+
+// How many key splits a tile of `chunks` chunks runs as; the launch's other workgroups of it end at once.
+__device__ __forceinline__ int tile_splits(const PrefillArgs& a, int chunks) {
+  return max(1, min(a.kv_splits, chunks / a.split_chunks));
+}
+
+// Chunks of the keys that a tile's last row sees: at least one, of rows without keys too.
+__device__ __forceinline__ int tile_chunks(int start, int qlen, int q_end) {
+  return max((start + min(qlen, q_end) + kChunk - 1) / kChunk, 1);
+}
+
 template <int D, int G, bool SPLIT>
 __global__ __launch_bounds__(kThreads, 3) void prefill_fp4_kernel(PrefillArgs a) {
   constexpr int QT = kRows / G;    // query tokens per workgroup
-  constexpr int KB = 64;
+  constexpr int KB = kChunk;
   constexpr int DS = D / 32;             // 32-wide d steps of Q K^T
   constexpr int DT = D / 16;             // 16-wide output d tiles of P V
   constexpr int JT = KB / 16;            // 16-key score tiles per chunk
@@ -150,6 +163,9 @@ __global__ __launch_bounds__(kThreads, 3) void prefill_fp4_kernel(PrefillArgs a)
   const int li = lane & 15, lk = lane >> 4;
   const int row = 16 * w + li;
   const int qpos = start + q0 + row % QT;
+  const int nchunks = tile_chunks(start, qlen, q0 + QT);
+  const int splits = SPLIT ? tile_splits(a, nchunks) : 1;
+  if (SPLIT && split >= splits) return;
 
   // Q pieces: B operand row li, d = 32 t + 8 lk .. + 7
   bf16x8 qf[DS][3];
@@ -174,9 +190,8 @@ __global__ __launch_bounds__(kThreads, 3) void prefill_fp4_kernel(PrefillArgs a)
   constexpr float kLazy = 8.0f;  // headroom of the exponents' reference point (log2 units)
 
   const int kend = start + min(qlen, q0 + QT);
-  const int nchunks = max((kend + KB - 1) / KB, 1);
-  const int c_lo = SPLIT ? split * nchunks / a.kv_splits : 0;
-  const int c_hi = SPLIT ? (split + 1) * nchunks / a.kv_splits : nchunks;
+  const int c_lo = SPLIT ? split * nchunks / splits : 0;
+  const int c_hi = SPLIT ? (split + 1) * nchunks / splits : nchunks;
   Loader in;
   in.init(a, seq, kvh, tid, kend, nchunks);
 
@@ -313,6 +328,51 @@ __global__ __launch_bounds__(kThreads, 3) void prefill_fp4_kernel(PrefillArgs a)
   }
 }
 
+// One output row quad a thread: the splits' partials of its row combined in split order, four loaded at a
+// time, each rescaled from its own reference point to the largest so far (a split without a key that the
+// row sees carries -inf and adds nothing; the one with key 0 always has one), divided by the combined sum.
+template <int D>
+__global__ __launch_bounds__(kThreads) void prefill_merge_fp4_kernel(PrefillArgs a, int qt_tokens, int ntiles) {
+  constexpr int DQ = D / 4, BLOCKS = kRows * DQ / kThreads;  // workgroups a (tile, kv head)
+  constexpr int N = 4;
+  const int pair = blockIdx.x / BLOCKS, idx = blockIdx.x % BLOCKS * kThreads + threadIdx.x;
+  const int tile = pair / a.hkv, kvh = pair % a.hkv;
+  const int seq = tile / ntiles, q0 = (tile % ntiles) * qt_tokens;
+  const int qs = a.cu_seqlens[seq], qlen = a.cu_seqlens[seq + 1] - qs;
+  const int r = idx / DQ, dq = idx % DQ;
+  const int h = r / qt_tokens, t = r % qt_tokens;
+  if (h >= a.group || q0 + t >= qlen) return;
+  const int splits = tile_splits(a, tile_chunks(a.context_lens[seq] - qlen, qlen, q0 + qt_tokens));
+  const size_t units = (size_t)(gridDim.x / BLOCKS) * a.kv_splits;
+  const float* pml = a.part + units * kRows * D;
+  const size_t first = (size_t)tile * a.kv_splits * a.hkv + kvh;  // split s: first + s * hkv
+  float mx = -INFINITY, l = 0.0f;
+  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int s0 = 0; s0 < splits; s0 += N) {
+    float2 ml[N];
+    float4 o[N];
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const size_t unit = first + (size_t)min(s0 + i, splits - 1) * a.hkv;
+      ml[i] = *reinterpret_cast<const float2*>(pml + (unit * kRows + r) * 2);
+      o[i] = *reinterpret_cast<const float4*>(a.part + (unit * kRows + r) * D + 4 * dq);
+    }
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      if (s0 + i >= splits || ml[i].x == -INFINITY) continue;
+      const float to = fmaxf(mx, ml[i].x);
+      const float old = __builtin_amdgcn_exp2f(mx - to), now = __builtin_amdgcn_exp2f(ml[i].x - to);
+      mx = to;
+      l = l * old + now * ml[i].y;
+      acc = make_float4(acc.x * old + now * o[i].x, acc.y * old + now * o[i].y, acc.z * old + now * o[i].z,
+                        acc.w * old + now * o[i].w);
+    }
+  }
+  const float inv = 1.0f / l;
+  *reinterpret_cast<float4*>(a.out + ((size_t)(qs + q0 + t) * a.hq + kvh * a.group + h) * D + 4 * dq) =
+      make_float4(acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv);
+}
+
 template <int D, int G>
 void launch_group(fi_context* ctx, const PrefillArgs& args, dim3 grid) {
   if (args.kv_splits > 1) {
@@ -327,12 +387,19 @@ int32_t launch_dim(fi_context* ctx, const PrefillArgs& args_in) {
   PrefillArgs args = args_in;
   const int g = args.group <= 1 ? 1 : (args.group <= 2 ? 2 : (args.group <= 4 ? 4 : 8));
   const int qt = kRows / g;
-  // Key splits for launches that leave most workgroup slots empty, as for f32 pools: up to four
-  // workgroups a CU, each with 128 keys or more (a tile's keys are at least max_query_len).
-  const long cus = ctx->compute_units > 0 ? ctx->compute_units : 256;
-  const long wgs = (long)((args.max_query_len + qt - 1) / qt) * args.num_seqs * args.hkv;
-  int splits = static_cast<int>(std::min<long>(FI_PREFILL_MAX_SPLITS, (4 * cus) / std::max<long>(wgs, 1)));
-  splits = std::max(1, std::min(splits, args.max_query_len / 128));
+  // Key splits for launches that leave workgroup slots empty: up to three workgroups a CU, the most that
+  // run at a time, and (tile_splits) four chunks of keys or more each; the block tables' width is the
+  // bound of a tile's chunks that the host knows.  32/8 heads of 128, us cut against whole: 64 rows after
+  // 1000 cached 20.9 against 44, after 4000 33 against 124, after 16000 60 against 468.  Where the launch has a workgroup for
+  // half the CUs without them, sixteen chunks: the partials' way through memory costs a range 3 us (300
+  // rows after 8000 114 against 246, 500 after 2000 68 against 79; but 500 after none 26.6 in two against 21.6, 1000
+  // after 4000, two workgroups a CU without them, 194 against 188).
+  const int64_t cus = ctx->compute_units > 0 ? ctx->compute_units : 256;
+  const int64_t wgs = static_cast<int64_t>((args.max_query_len + qt - 1) / qt) * args.num_seqs * args.hkv;
+  const int64_t chunks = (static_cast<int64_t>(args.max_blocks) * args.block_size + kChunk - 1) / kChunk;
+  args.split_chunks = 2 * wgs <= cus ? 4 : 16;
+  const int splits = static_cast<int>(std::max<int64_t>(
+      1, std::min<int64_t>({kMaxSplits, 3 * cus / std::max<int64_t>(wgs, 1), chunks / args.split_chunks})));
   dim3 grid;
   FI_TRY(plan_tiles(ctx, args, qt, 64, "fi_attn_prefill_paged", &grid, splits, kRows * (D + 2)));
   switch (g) {
@@ -352,9 +419,10 @@ int32_t launch_dim(fi_context* ctx, const PrefillArgs& args_in) {
   FI_CHECK_LAUNCH("prefill_fp4_kernel");
   if (splits > 1) {
     const int ntiles = (args.max_query_len + qt - 1) / qt;
-    hipLaunchKernelGGL((prefill_split_merge_kernel<D, 1>), dim3(grid.x / splits), dim3(kThreads), 0, ctx->stream, args,
+    const unsigned blocks = kRows * (D / 4) / kThreads;  // of the merge, a (tile, kv head)
+    hipLaunchKernelGGL((prefill_merge_fp4_kernel<D>), dim3(grid.x / splits * blocks), dim3(kThreads), 0, ctx->stream, args,
                        qt, ntiles);
-    FI_CHECK_LAUNCH("prefill_split_merge_kernel");
+    FI_CHECK_LAUNCH("prefill_merge_fp4_kernel");
   }
   return FI_OK;
 }

@@ -265,3 +265,49 @@ def test_prefill_replayed(gpu_ctx, seqs, hq, hkv, d):
     own.check_faults()
     kernel.check(lib.fi_graph_destroy(graph))
     own.close()
+
+
+@pytest.mark.parametrize("seqs,hq,hkv,d,bs", [
+    ([(16000, 5)], 32, 8, 128, 16),                         # 24 ranges of one tile's keys
+    ([(20000, 1)], 1, 1, 32, 16),                           # 32 ranges, as many as a tile is cut into
+    ([(3000, 40), (0, 3), (255, 1), (256, 1), (511, 2), (0, 0)], 14, 2, 64, 16),  # cut, whole and absent beside each other
+    ([(1500, 70), (100, 257)], 6, 2, 128, 5),               # tiles of 1, 2, .. ranges
+    ([(9000, 300)], 14, 2, 64, 64),                         # more tiles: ranges of 16 chunks
+])
+def test_prefill_of_few_rows_over_long_prefixes(gpu_ctx, seqs, hq, hkv, d, bs):
+    print(f"prefill over prefixes {seqs}", flush=True)
+    new, lens = [n for _, n in seqs], [p + n for p, n in seqs]
+    rng = np.random.default_rng(sum(lens) + d)
+    nb = sum(-(-n // bs) for n in lens) + 3
+    (kb, kv), (vb, vv) = random_pool(rng, nb, hkv, bs, d), random_pool(rng, nb, hkv, bs, d)
+    tables = tables_of(rng, lens, bs, nb)
+    wide = np.concatenate([tables, np.full((len(lens), 40000 // bs), -1, np.int32)], 1)  # far wider than its sequences
+    q = rng.standard_normal((sum(new), hq, d)).astype(np.float32)
+    scale = d ** -0.5
+    for table in (tables, wide):
+        got = prefill(gpu_ctx, q, (dev(kb), dev(vb)), table, new, lens, hkv, bs, nb, scale)
+        at = 0
+        for b, (p, n) in enumerate(seqs):
+            if n == 0:
+                continue
+            k, v = (fp4.rows_of(x, tables[b], p + n, bs) for x in (kv, vv))
+            want = attention64(q[at:at + n], k, v, p, scale)
+            assert np.abs(got[at:at + n] - want).max() <= fp4.attention_tolerance(q[at:at + n], k, v, scale, p + n), b
+            at += n
+
+
+def test_prefill_nan_in_one_range_of_a_long_prefix(gpu_ctx):
+    """Ranges of keys of which one holds a NaN group of V, and one of K in another kv head."""
+    rng = np.random.default_rng(50)
+    hq, hkv, d, bs, n, p = 8, 2, 64, 16, 6, 2500
+    nb = -(-(n + p) // bs) + 1
+    (kb, _), (vb, _) = random_pool(rng, nb, hkv, bs, d), random_pool(rng, nb, hkv, bs, d)
+    tables = tables_of(rng, [n + p], bs, nb)
+    fp4.split_pool(kb, nb, hkv, bs, d)[1][tables[0, 70], 0, 3, 1] = 255
+    fp4.split_pool(vb, nb, hkv, bs, d)[1][tables[0, 20], 1, 9, 0] = 255
+    q = rng.standard_normal((n, hq, d)).astype(np.float32)
+    got = prefill(gpu_ctx, q, (dev(kb), dev(vb)), tables, [n], [n + p], hkv, bs, nb, d ** -0.5)
+    want = np.zeros((n, hkv, hq // hkv, d), bool)
+    want[:, 0] = True
+    want[:, 1, :, :32] = True
+    assert np.array_equal(np.isnan(got), want.reshape(n, hq, d))
