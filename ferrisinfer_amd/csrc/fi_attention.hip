@@ -842,8 +842,10 @@ int head_split(int64_t whole, int group, int parts, bool bf16, int64_t cus) {
 }
 
 // Over a 4-bit pool a workgroup's arithmetic goes by tiles of four heads: groups of more are cut in
-// two where that leaves every workgroup a CU.
-int head_split_fp4(int64_t whole, int group, int64_t cus) { return group > 4 && 2 * whole <= cus ? 2 : 1; }
+// two in launches of up to two workgroups a CU (14/2 heads of 64, us cut against whole: one sequence of
+// 700 tokens 7.4 against 9.4, 8 of 1000 8.5 against 10.2, 64 of 1000 (two a CU) 10.9 against 11.8, 64 of 2000 15.3
+// against 15.1, 256 of 1000 24.5 against 21.7).
+int head_split_fp4(int64_t whole, int group, int64_t cus) { return group > 4 && whole <= 2 * cus ? 2 : 1; }
 
 // Shared by both decode entry points: validation, launch shape and launches.  With
 // `noalloc` the partials go to the library's fixed scratch array instead of the context
@@ -902,6 +904,8 @@ int32_t decode_paged(fi_context* ctx, const float* d_q, const void* d_k_cache, c
                "fi_attn_decode_paged: q must be 16-byte aligned (vector accesses)");
     FI_REQUIRE(num_q_heads / num_kv_heads <= 8, FI_ERR_UNSUPPORTED,
                "decode attention supports at most 8 query heads per KV head");
+    FI_REQUIRE(static_cast<int64_t>(num_seqs) * num_q_heads < (1 << 24), FI_ERR_UNSUPPORTED,
+               "fi_attn_decode_paged: 4-bit pools are served for fewer than 2^24 query rows a launch");
   }
   if (qkv) {
     auto aligned16 = [](const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; };
@@ -976,7 +980,7 @@ int32_t decode_paged(fi_context* ctx, const float* d_q, const void* d_k_cache, c
   // workgroups: 113.2 against 111.4 us).
   if (parts > 1 && !noalloc && ctx->d_merge_counters != nullptr &&
       static_cast<int64_t>(num_seqs) * num_kv_heads * shares <= FI_MERGE_COUNTERS &&
-      (kv_dtype == FI_DTYPE_MXFP4 ? fi::decode_fp4_merges(whole, parts, cus) : whole <= 6 * cus))
+      (kv_dtype == FI_DTYPE_MXFP4 ? fi::decode_fp4_merges(whole, parts, args.heads_per, cus) : whole <= 6 * cus))
     args.counters = ctx->d_merge_counters;
   if (kv_dtype == FI_DTYPE_MXFP4) {
     args.blocks = fi::FastDiv(static_cast<uint32_t>(block_size));

@@ -528,8 +528,8 @@ int32_t launch_dim(fi_context* ctx, const DecodeArgs& args, dim3 grid, int wt) {
 
 namespace fi {
 
-bool decode_fp4_merges(int64_t workgroups, int parts, int64_t cus) {
-  return parts <= kMergeInline && workgroups <= 6 * cus;
+bool decode_fp4_merges(int64_t workgroups, int parts, int heads, int64_t cus) {
+  return parts <= kMergeInline / 2 || (parts <= kMergeInline && heads <= 4 && workgroups > 2 * cus);
 }
 
 int32_t decode_fp4(fi_context* ctx, const DecodeArgs& args, int32_t head_dim, dim3 grid, int wave_tokens) {

@@ -28,8 +28,15 @@ int32_t kv_copy_blocks_fp4(fi_context* ctx, void* k_cache, void* v_cache, const 
 int32_t kv_gather_fp4(fi_context* ctx, const void* k_cache, const void* v_cache, const int32_t* table, int32_t length,
                       int32_t num_blocks, int32_t block_size, int32_t hkv, int32_t d, float* k_out, float* v_out);
 
-// Whether a decode launch of several partitions merges them by itself.
-bool decode_fp4_merges(int64_t workgroups, int parts, int64_t cus);
+// Whether a decode launch of several partitions (up to `heads` heads a workgroup) merges them by itself:
+// the workgroup that ends a sequence's last partition does, instead of a launch of its own.  One
+// strand of the merge holds a sequence's weights, up to 16 partitions.  Up to 8 that is the faster way
+// (us merging by itself against by a launch: 64 sequences of 128 to 2048 tokens over 8 heads of 128 24.2
+// against 26.0, 64 of 4000 66.2 against 68.7, one of 700 over 2 heads of 64 7.4 against 10.0).  Of 9 to 16 it is
+// for large launches with few heads a workgroup (128 of 512 to 8192 142.5 against 145.0, 16 of 5500 26.5 against
+// 27.4), not for small ones, which end in the merge of a few workgroups (one of 8000 11.6 against 10.8), nor
+// for more heads a workgroup (14/2 heads of 64, 8 of 4000 13.0 against 9.9, 64 of 4000 22.9 against 22.1).
+bool decode_fp4_merges(int64_t workgroups, int parts, int heads, int64_t cus);
 
 // Decode attention: the partition launch and, where the launch does not merge by itself, the merge.
 int32_t decode_fp4(fi_context* ctx, const DecodeArgs& args, int32_t head_dim, dim3 grid, int wave_tokens);
