@@ -869,7 +869,8 @@ int32_t decode_paged(fi_context* ctx, const float* d_q, const void* d_k_cache, c
                      int32_t kv_dtype, const int32_t* d_block_tables, int32_t max_blocks_per_seq,
                      const int32_t* d_context_lens, int32_t num_seqs, int32_t max_context_len,
                      int32_t num_q_heads, int32_t num_kv_heads, int32_t head_dim, int32_t block_size,
-                     int32_t num_blocks, float scale, float* d_out, bool noalloc, const QkvIn* qkv = nullptr) {
+                     int32_t num_blocks, float scale, float* d_out, bool noalloc, const QkvIn* qkv = nullptr,
+                     bool check_only = false) {
   FI_TRY(fi::enter(ctx));
   FI_REQUIRE(num_seqs >= 0 && max_context_len >= 0, FI_ERR_INVALID_SHAPE,
              "fi_attn_decode_paged: negative sizes");
@@ -906,6 +907,9 @@ int32_t decode_paged(fi_context* ctx, const float* d_q, const void* d_k_cache, c
                "decode attention supports at most 8 query heads per KV head");
     FI_REQUIRE(static_cast<int64_t>(num_seqs) * num_q_heads < (1 << 24), FI_ERR_UNSUPPORTED,
                "fi_attn_decode_paged: 4-bit pools are served for fewer than 2^24 query rows a launch");
+    // the kernel keeps pool rows in 32 bits (2^32 of them are 73 GB of an array at head_dim 32)
+    FI_REQUIRE(static_cast<int64_t>(num_blocks) * block_size <= (int64_t{1} << 32) / num_kv_heads, FI_ERR_UNSUPPORTED,
+               "fi_attn_decode_paged: 4-bit pools are served up to 2^32 rows of one head");
   }
   if (qkv) {
     auto aligned16 = [](const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; };
@@ -918,6 +922,7 @@ int32_t decode_paged(fi_context* ctx, const float* d_q, const void* d_k_cache, c
                    (qkv->rotary_dims == 0 || (aligned16(qkv->cos_t) && aligned16(qkv->sin_t))),
                FI_ERR_INVALID_CONFIG, "fi_attn_decode_paged_qkv: partials, biases and rope tables must be 16-byte aligned");
   }
+  if (check_only) return FI_OK;
   const int32_t parts = max_context_len == 0 ? 1 : (max_context_len + part_tokens - 1) / part_tokens;
   DecodeArgs args{};
   args.q = d_q;
@@ -1034,6 +1039,10 @@ int32_t fi_attn_decode_paged_qkv(fi_context* ctx, const float* d_qkv_parts, int3
   const int64_t cus = ctx->compute_units > 0 ? ctx->compute_units : 256;
   if (kv_dtype == FI_DTYPE_MXFP4 || static_cast<int64_t>(num_seqs) * num_kv_heads * parts > 6 * cus) {
     FI_REQUIRE(d_q_out != nullptr, FI_ERR_INVALID_CONFIG, "fi_attn_decode_paged_qkv: null q_out");
+    if (kv_dtype == FI_DTYPE_MXFP4)  // what the attention refuses is refused before rows are appended
+      FI_TRY(decode_paged(ctx, d_q_out, d_k_cache, d_v_cache, kv_dtype, d_block_tables, max_blocks_per_seq,
+                          d_context_lens, num_seqs, max_context_len, num_q_heads, num_kv_heads, head_dim, block_size,
+                          num_blocks, scale, d_out, false, nullptr, true));
     FI_TRY(fi_qkv_rope_append(ctx, d_qkv_parts, splits, d_bias_q, d_bias_k, d_bias_v, d_positions, d_cos, d_sin,
                               rotary_dims, max_positions, d_slot_mapping, d_k_cache, d_v_cache, kv_dtype, num_blocks,
                               block_size, num_seqs, num_q_heads, num_kv_heads, head_dim, d_q_out));

@@ -235,6 +235,8 @@ int32_t qkv_norm_rope_append(fi_context* ctx, const char* name, QkvNormArgs a, i
   a.pair_axes1 = words[1];
   a.pair_axes2 = words[2];
   a.pair_axes3 = words[3];
+  FI_REQUIRE((static_cast<int64_t>(a.hq) + 2 * static_cast<int64_t>(a.hkv)) * head_dim <= 0x7fffffffLL, FI_ERR_INVALID_SHAPE,
+             n + ": rows are too wide");
   const int64_t blocks =
       static_cast<int64_t>(a.tokens) * ((static_cast<int64_t>(a.hq) + 2 * a.hkv) * (head_dim / 4) / kThreads + 1);
   FI_REQUIRE(blocks <= 0x7fffffffLL, FI_ERR_INVALID_SHAPE, n + ": too many tokens for one launch");

@@ -96,6 +96,7 @@ def _consume(**change):
     (dict(weight=16, eps=float("nan")), "InvalidConfig", "eps"),
     (dict(weight=16, eps=float("inf")), "InvalidConfig", "eps"),
     (dict(tokens=2 ** 31 - 1, hq=64, hkv=64, d=128, rotary=128), "InvalidShape", "too many tokens"),
+    (dict(tokens=1, hq=2 ** 24, hkv=2 ** 24, d=128, rotary=128), "InvalidShape", "too wide"),
 ])
 def test_consumer_refusals(change, kind, words):
     got, message = _consume(**change)

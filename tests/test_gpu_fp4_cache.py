@@ -370,3 +370,64 @@ def test_decode_replayed_and_on_another_stream(gpu_ctx, lens, hq, hkv, d):
         assert torch.equal(other, want[2])
     kernel.check(lib.fi_graph_destroy(graph))
     own.close()
+
+
+def test_launch_limits_and_refusals_before_rows_are_written(gpu_ctx):
+    import torch
+
+    from ferrisinfer_amd import DTYPE_MXFP4, FerrisError
+
+    pool = torch.full((1 << 16,), 7, dtype=torch.uint8, device="cuda")
+    x = torch.zeros(1, 2, 32, device="cuda")
+    slots = torch.zeros(1, dtype=torch.int64, device="cuda")
+    bt = torch.zeros(1, 4, dtype=torch.int32, device="cuda")
+    ints = torch.zeros(1, dtype=torch.int32, device="cuda")
+    many = torch.empty(1 << 23, 2, 32, device="cuda")
+    calls = [  # sizes that the checks refuse before anything is read
+        ("2^24", lambda: gpu_ctx.attn_decode_paged(many, pool, pool, DTYPE_MXFP4, bt, ints, 4, 2, 4, 4, 1.0, x)),
+        ("2^32", lambda: gpu_ctx.attn_decode_paged(x, pool, pool, DTYPE_MXFP4, bt, ints, 4, 2, 1 << 12, 1 << 20, 1.0, x)),
+    ]
+    for words, call in calls:
+        with pytest.raises(FerrisError) as e:
+            call()
+        assert e.value.kind == "Unsupported" and words in e.value.message
+    table = torch.ones(64, 16, device="cuda")
+    before = pool.clone()
+    for hq, longest, kind in ((9, 4, "Unsupported"), (4, 17, "InvalidShape")):  # too many heads a kv head, too short a table
+        parts, q = torch.ones(1, (hq + 2) * 32, device="cuda"), torch.zeros(1, hq, 32, device="cuda")
+        with pytest.raises(FerrisError) as e:
+            gpu_ctx.attn_decode_paged_qkv(parts, 1, None, ints, table, table, 32, 64, slots, pool, pool, DTYPE_MXFP4, bt, ints,
+                                          longest, hq, 1, 32, 4, 4, 1.0, q.clone(), q)
+        assert e.value.kind == kind
+    gpu_ctx.sync()
+    assert torch.equal(pool, before)
+
+
+def test_two_contexts_decode_at_once(gpu_ctx):
+    """Calls of two contexts on streams of their own, each merging its partitions by itself."""
+    import torch
+
+    from ferrisinfer_amd import DTYPE_MXFP4, Context
+
+    rng = np.random.default_rng(60)
+    hq, hkv, d, bs, lens = 8, 2, 128, 16, [2000, 900, 1500]
+    nb = sum(-(-n // bs) for n in lens) + 1
+    pools = [tuple(dev(random_pool(rng, nb, hkv, bs, d)[0]) for _ in range(2)) for _ in range(2)]
+    tables = dev(tables_of(rng, lens, bs, nb))
+    q = dev(rng.standard_normal((3, hq, d)).astype(np.float32))
+    ints = dev(np.array(lens, np.int32))
+    other = Context(0, use_torch_stream=False)
+    want = []
+    for k, v in pools:
+        want.append(torch.empty_like(q))
+        gpu_ctx.attn_decode_paged(q, k, v, DTYPE_MXFP4, tables, ints, 2000, hkv, bs, nb, d ** -0.5, want[-1])
+    gpu_ctx.sync()
+    outs = [[torch.empty_like(q) for _ in range(20)] for _ in range(2)]
+    torch.cuda.synchronize()
+    for i in range(20):
+        for ctx, (k, v), out in zip((gpu_ctx, other), pools, outs):
+            ctx.attn_decode_paged(q, k, v, DTYPE_MXFP4, tables, ints, 2000, hkv, bs, nb, d ** -0.5, out[i])
+    gpu_ctx.sync()
+    other.sync()
+    other.close()
+    assert all(torch.equal(o, w) for out, w in zip(outs, want) for o in out)
