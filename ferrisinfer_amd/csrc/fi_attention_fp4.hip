@@ -77,13 +77,13 @@ constexpr int kStrands = 4;
 constexpr int kMergeInline = 16;
 
 // NS strands from s0 on, of this lane's D / 64 dims (D = 32: of the lower half's one): the weighted
-// sums, and the strands' shares of L.  The first partitions' loads go out with the statistics'.
-template <int D, bool COHERENT, int NS>
+// sums, and the strands' shares of L.  BATCH partitions' loads are issued together, the first ones' with the
+// statistics'.
+template <int D, bool COHERENT, int NS, int BATCH>
 __device__ __forceinline__ void merge_strands(const DecodeArgs& a, size_t head, int nparts, int s0, int lane,
                                               float (&sum)[NS][(D + 63) / 64], float (&share)[NS]) {
   constexpr int E = (D + 63) / 64;
-  constexpr int BATCH = 8;                       // partitions whose loads are issued together
-  constexpr int STEP = NS == 1 ? kStrands : 1;   // from one of this wave's partitions to the next
+  constexpr int STEP = NS == 1 ? kStrands : 1;  // from one of this wave's partitions to the next
   constexpr int MAXP = NS == 1 ? kMaxParts : kMergeInline;
   float* ml = a.part_ml + head * a.parts_per_seq * 2;
   float* acc = a.part_acc + head * a.parts_per_seq * D + (D < 64 ? lane % D : lane * E);
@@ -132,8 +132,11 @@ __device__ __forceinline__ void merge_strands(const DecodeArgs& a, size_t head, 
   }
 }
 
-// One workgroup per query head, a wave a strand.
-template <int D, int WT>
+// One workgroup per query head, a wave a strand.  Bound by the chain of its loads: 64 heads of 196 partitions
+// of 128 dims, 6.7 MB, in 6.6 us with 32 partitions' loads at a time (8.2 with 8, which is the faster one up
+// to 64 partitions: one sequence of 60000 tokens over 2 heads of 64 15.0 against 18.1 us in all, 8 of 4000 9.4
+// against 9.0).
+template <int D, int WT, int BATCH>
 __global__ __launch_bounds__(64 * kStrands) void decode_merge_fp4_kernel(DecodeArgs a) {
   constexpr int E = (D + 63) / 64;
   __shared__ float s_sum[kStrands][D];
@@ -145,7 +148,7 @@ __global__ __launch_bounds__(64 * kStrands) void decode_merge_fp4_kernel(DecodeA
   if (nparts <= 1) return;
   const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
   float sum[1][E], share[1];
-  merge_strands<D, false, 1>(a, head, nparts, w, lane, sum, share);
+  merge_strands<D, false, 1, BATCH>(a, head, nparts, w, lane, sum, share);
   if (D >= 64 || lane < D) {
 #pragma unroll
     for (int e = 0; e < E; ++e) s_sum[w][lane * E + e] = sum[0][e];
@@ -216,7 +219,7 @@ __device__ __forceinline__ void combine_waves_fp4(const DecodeArgs& a, const Hea
   for (int g = tid >> 6; g < group; g += kWaves) {
     const size_t head = hu.head0 + g;
     float sum[kStrands][E], share[kStrands];
-    merge_strands<D, true, kStrands>(a, head, nparts, 0, lane, sum, share);
+    merge_strands<D, true, kStrands, 8>(a, head, nparts, 0, lane, sum, share);
 #pragma unroll
     for (int s = 1; s < kStrands; ++s) {
       share[0] += share[s];
@@ -234,7 +237,7 @@ __device__ __forceinline__ void combine_waves_fp4(const DecodeArgs& a, const Hea
 // its query heads; each wave owns WT consecutive tokens, computes all their scores, then their
 // softmax once, then the weighted sum.  T tiles of four query heads.  The waves' (max, sum, acc)
 // are combined through LDS in wave order, the partitions by the last of them to arrive or in a launch
-// of their own (merge_head).
+// of their own.
 //
 // QUAD (block sizes that are multiples of four): the pool rows of keys 4 i .. 4 i + 3 follow each
 // other, so a lane's keys need one address and immediate offsets; the rows of the last group that lie past the
@@ -242,7 +245,11 @@ __device__ __forceinline__ void combine_waves_fp4(const DecodeArgs& a, const Hea
 // its own address, clamped to the last valid row.
 //
 // The wave's K codes, and V codes two steps ahead, are in flight together (a wave has 10 KB
-// outstanding at D = 128, sixteen waves a CU).
+// outstanding at D = 128, sixteen waves a CU).  Bound by the pool's bytes in large launches: 128 sequences
+// of 512 to 8192 tokens over 8 heads of 128, 610 MB of codes and scales (679 read), 142.5 us with the merge,
+// 4.3 TB/s, where a plain sum over an array reads 4.0 and the matrix pipe is busy 16 %; 64 of 128 to 2048
+// (78 MB) 23.9 us, 3.3 TB/s, by the workgroups' own chain (rows, codes, scores, softmax, sum), of which a CU
+// has a round and a half.
 template <int D, int T, int WT, bool QUAD>
 __global__ __launch_bounds__(kThreads, T == 1 ? 4 : 2) void decode_fp4_kernel(DecodeArgs a) {
   constexpr int kPartTokens = kWaves * WT;
@@ -502,8 +509,9 @@ int32_t launch(fi_context* ctx, const DecodeArgs& args, dim3 grid) {
   hipLaunchKernelGGL((decode_fp4_kernel<D, T, WT, QUAD>), grid, dim3(kThreads), 0, ctx->stream, args);
   FI_CHECK_LAUNCH("decode_fp4_kernel");
   if (args.parts_per_seq > 1 && args.counters == nullptr) {
-    hipLaunchKernelGGL((decode_merge_fp4_kernel<D, WT>), dim3(static_cast<unsigned>(args.num_seqs) * args.hq),
-                       dim3(64 * kStrands), 0, ctx->stream, args);
+    auto merge = args.parts_per_seq > 64 ? decode_merge_fp4_kernel<D, WT, 32> : decode_merge_fp4_kernel<D, WT, 8>;
+    hipLaunchKernelGGL(merge, dim3(static_cast<unsigned>(args.num_seqs) * args.hq), dim3(64 * kStrands), 0, ctx->stream,
+                       args);
     FI_CHECK_LAUNCH("decode_merge_fp4_kernel");
   }
   return FI_OK;

@@ -53,6 +53,8 @@ __device__ __forceinline__ size_t table_row(const fi::QkvNormArgs& a, int t, uin
 // uniform, and a thread's ROWS rows (the same elements of heads kThreads / LPR apart) share its
 // weights, cosines and sines.  Every load is issued before the first is waited for, but for the table
 // rows, which wait for the positions: the chain of dependent loads, not the arithmetic, bounds this.
+// 2048 tokens of 32 + 16 heads of 128 (one split, three axes, norms, bf16 pool; 92 MB) 25.7 us, 3.6 TB/s;
+// 64 tokens of four splits 4.9 us, one token of 14 + 4 heads of 64 and seven splits 3.2 us.
 template <int D, typename Pool, int ROWS>
 __global__ __launch_bounds__(kThreads) void qkv_norm_rope_append_kernel(fi::QkvNormArgs a) {
   constexpr int LPR = D / 4;            // lanes per head row

@@ -431,3 +431,23 @@ def test_two_contexts_decode_at_once(gpu_ctx):
     other.sync()
     other.close()
     assert all(torch.equal(o, w) for out, w in zip(outs, want) for o in out)
+
+
+@pytest.mark.parametrize("lens,hq,hkv,d", [([17000, 300, 65536], 2, 1, 32), ([40000], 8, 4, 128), ([16384], 7, 1, 64)])
+def test_decode_of_many_partitions(gpu_ctx, lens, hq, hkv, d):
+    """64 partitions, more, and as many as a launch takes (65536 tokens of narrow rows)."""
+    print(f"decode {lens} {hq} {hkv} {d}", flush=True)
+    rng = np.random.default_rng(sum(lens))
+    bs = 16
+    nb = sum(-(-n // bs) for n in lens) + 1
+    (kb, kv), (vb, vv) = random_pool(rng, nb, hkv, bs, d), random_pool(rng, nb, hkv, bs, d)
+    tables = tables_of(rng, lens, bs, nb)
+    q = rng.standard_normal((len(lens), hq, d)).astype(np.float32)
+    scale = d ** -0.5
+    got = decode(gpu_ctx, q, (dev(kb), dev(vb)), tables, lens, hkv, bs, nb, scale)
+    for b, n in enumerate(lens):
+        k, v = (fp4.rows_of(x, tables[b], n, bs) for x in (kv, vv))
+        want = fp4.attention(q[b:b + 1], k, v, n - 1, scale)
+        assert np.abs(got[b] - want[0]).max() <= fp4.attention_tolerance(q[b:b + 1], k, v, scale, n), b
+    alone = decode(gpu_ctx, q[:1], (dev(kb), dev(vb)), tables[:1], lens[:1], hkv, bs, nb, scale)
+    assert np.array_equal(alone[0], got[0])  # whatever the launch's other sequences are
