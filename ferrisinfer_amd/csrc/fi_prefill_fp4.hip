@@ -127,10 +127,14 @@ __device__ __forceinline__ int tile_splits(const PrefillArgs& a, int chunks) {
   return max(1, min(a.kv_splits, chunks / a.split_chunks));
 }
 
-// Chunks of the keys that a tile's last row sees: at least one, of rows without keys too.
-__device__ __forceinline__ int tile_chunks(int start, int qlen, int q_end) {
-  return max((start + min(qlen, q_end) + kChunk - 1) / kChunk, 1);
+// The end of the keys that a tile's last row sees, none past the block table's width (rows that ask for
+// more are reported: a context length that is wrong must not make a loop of a billion chunks), and
+// their chunks: at least one, of rows without keys too.
+__device__ __forceinline__ int tile_end(const PrefillArgs& a, int start, int qlen, int q_end) {
+  const int64_t width = (int64_t)a.max_blocks * a.block_size;
+  return static_cast<int>(min((int64_t)start + min(qlen, q_end), min(width, (int64_t)0x7fffffff - kChunk)));
 }
+__device__ __forceinline__ int tile_chunks(int end) { return max((end + kChunk - 1) / kChunk, 1); }
 
 template <int D, int G, bool SPLIT>
 __global__ __launch_bounds__(kThreads, 3) void prefill_fp4_kernel(PrefillArgs a) {
@@ -163,7 +167,8 @@ __global__ __launch_bounds__(kThreads, 3) void prefill_fp4_kernel(PrefillArgs a)
   const int li = lane & 15, lk = lane >> 4;
   const int row = 16 * w + li;
   const int qpos = start + q0 + row % QT;
-  const int nchunks = tile_chunks(start, qlen, q0 + QT);
+  const int kend = tile_end(a, start, qlen, q0 + QT);
+  const int nchunks = tile_chunks(kend);
   const int splits = SPLIT ? tile_splits(a, nchunks) : 1;
   if (SPLIT && split >= splits) return;
 
@@ -189,7 +194,6 @@ __global__ __launch_bounds__(kThreads, 3) void prefill_fp4_kernel(PrefillArgs a)
   const float c2 = a.scale * 1.4426950408889634f;  // scores -> log2 units
   constexpr float kLazy = 8.0f;  // headroom of the exponents' reference point (log2 units)
 
-  const int kend = start + min(qlen, q0 + QT);
   const int c_lo = SPLIT ? split * nchunks / splits : 0;
   const int c_hi = SPLIT ? (split + 1) * nchunks / splits : nchunks;
   Loader in;
@@ -300,7 +304,7 @@ __global__ __launch_bounds__(kThreads, 3) void prefill_fp4_kernel(PrefillArgs a)
     }
   }
 
-  if (in.bad_block) atomicOr(a.faults, FI_FAULT_BLOCK_RANGE);
+  if (in.bad_block || kend < (int64_t)start + min(qlen, q0 + QT)) atomicOr(a.faults, FI_FAULT_BLOCK_RANGE);
 
   float l_row = l_part + fi::lane_xor16(l_part, lane);
   l_row += fi::lane_xor32(l_row, lane);
@@ -342,7 +346,7 @@ __global__ __launch_bounds__(kThreads) void prefill_merge_fp4_kernel(PrefillArgs
   const int r = idx / DQ, dq = idx % DQ;
   const int h = r / qt_tokens, t = r % qt_tokens;
   if (h >= a.group || q0 + t >= qlen) return;
-  const int splits = tile_splits(a, tile_chunks(a.context_lens[seq] - qlen, qlen, q0 + qt_tokens));
+  const int splits = tile_splits(a, tile_chunks(tile_end(a, a.context_lens[seq] - qlen, qlen, q0 + qt_tokens)));
   const size_t units = (size_t)(gridDim.x / BLOCKS) * a.kv_splits;
   const float* pml = a.part + units * kRows * D;
   const size_t first = (size_t)tile * a.kv_splits * a.hkv + kvh;  // split s: first + s * hkv

@@ -311,3 +311,22 @@ def test_prefill_nan_in_one_range_of_a_long_prefix(gpu_ctx):
     want[:, 0] = True
     want[:, 1, :, :32] = True
     assert np.array_equal(np.isnan(got), want.reshape(n, hq, d))
+
+
+@pytest.mark.parametrize("n,seen", [(5, 1000), (5, 2 ** 31 - 1), (200, 2 ** 30), (5, -2 ** 31 + 64)])
+def test_prefill_context_beyond_the_block_table(gpu_ctx, n, seen):
+    """Keys end with the table, whatever the context length says: the call ends and reports it."""
+    from ferrisinfer_amd import FerrisError
+
+    rng = np.random.default_rng(51)
+    hq, hkv, d, bs, nb = 4, 2, 64, 16, 20
+    pools = tuple(dev(random_pool(rng, nb, hkv, bs, d)[0]) for _ in range(2))
+    tables = np.arange(nb, dtype=np.int32)[None]
+    q = rng.standard_normal((n, hq, d)).astype(np.float32)
+    if seen < 0:  # rows without keys
+        assert (prefill(gpu_ctx, q, pools, tables, [n], [seen], hkv, bs, nb, d ** -0.5) == 0).all()
+        return
+    with pytest.raises(FerrisError) as e:
+        prefill(gpu_ctx, q, pools, tables, [n], [seen], hkv, bs, nb, d ** -0.5)
+    assert e.value.kind == "Runtime"
+    prefill(gpu_ctx, q, pools, tables, [n], [nb * bs], hkv, bs, nb, d ** -0.5)  # the whole table is served
