@@ -177,17 +177,18 @@ void launch_rows(fi_context* ctx, fi::QkvNormArgs& a, int32_t kv_dtype) {
   }
 }
 
-// Where one row a thread would make more workgroups than the device holds at once (eight a CU) and the
-// partials need no sum, as few workgroups a token as six rows a thread allow (2048 tokens of 48 heads
+// Where one row a thread would make more workgroups than the device holds at once (eight a CU) and at
+// most two splits are summed, as few workgroups a token as six rows a thread allow (2048 tokens of 48 heads
 // of 128, six rows to a thread fill a workgroup: 46.6 us with one row, 31.3 with two, 28.2 with three,
-// 32.4 with four, whose second workgroup is half empty, 26.2 with six).  Smaller launches end sooner
-// with more workgroups.
+// 32.4 with four, whose second workgroup is half empty, 26.2 with six; two splits 46.9 against 50.9 with one
+// row).  Smaller launches end sooner with more workgroups, and a thread's rows wait for each other's
+// splits (four splits 61.6 against 59.0).
 template <int D>
 void launch(fi_context* ctx, fi::QkvNormArgs& a, int32_t kv_dtype) {
   constexpr int STEP = kThreads / (D / 4);
   const int64_t cus = ctx->compute_units > 0 ? ctx->compute_units : 256;
   const int heads = a.hq + 2 * a.hkv;
-  const int passes = a.splits == 1 && static_cast<int64_t>(a.tokens) * heads > 8 * cus * STEP ? (heads + STEP - 1) / STEP : 1;
+  const int passes = a.splits <= 2 && static_cast<int64_t>(a.tokens) * heads > 8 * cus * STEP ? (heads + STEP - 1) / STEP : 1;
   switch (passes) {
     case 1:
       return launch_rows<D, 1>(ctx, a, kv_dtype);

@@ -244,3 +244,19 @@ def test_bad_slots_positions_and_layouts(gpu_ctx):
         call(axes=x["pair_axes"][:-1])
     assert e.value.kind == "InvalidShape"
     call()
+
+
+@pytest.mark.parametrize("kind", ["f32", "bf16", "mxfp4"])
+@pytest.mark.parametrize("case", [
+    # head rows past what one row a thread keeps resident: two, three, four, five and six rows a thread
+    (1101, 8, 4, 128, 1, 3, 128, True, True, 16),
+    (1101, 8, 4, 128, 2, 1, 64, False, True, 16),
+    (701, 12, 6, 128, 1, 1, 128, True, True, 16),
+    (520, 16, 8, 128, 2, 4, 128, True, False, 5),
+    (430, 24, 8, 128, 1, 2, 128, False, True, 16),
+    (350, 32, 8, 128, 1, 3, 128, True, True, 16),
+    (1900, 14, 2, 64, 1, 3, 64, True, True, 16),     # two rows a thread, heads that do not fill the second
+    (2100, 30, 2, 32, 1, 1, 32, True, True, 16),
+])
+def test_consumer_of_many_tokens(gpu_ctx, case, kind):
+    test_consumer(gpu_ctx, case, kind)
