@@ -231,7 +231,8 @@ int32_t fi_ctx_check_faults(fi_context* ctx);
  * decode_causal_attention_f32 (kernel/cpu/attention.rs:520-686).
  * q/out: f32 [num_seqs, Hq, D]; scale is 1/sqrt(D) in the reference (attention.rs:659).  Scores,
  * softmax and sums are f32 whatever the pool's dtype, and the pool's values enter them exactly;
- * over an mxfp4 pool q must be 16-byte aligned (InvalidLayout otherwise).
+ * over an mxfp4 pool q must be 16-byte aligned (InvalidLayout otherwise), and num_blocks * Hkv *
+ * block_size may be 2^32 and num_seqs * Hq below 2^24 (Unsupported otherwise).
  * max_context_len must bound every context_lens entry (it sizes the grid); an entry beyond
  * the partitions it sizes is clamped to them on device and reported as Runtime by
  * fi_ctx_check_faults. */
@@ -294,8 +295,9 @@ int32_t fi_attn_decode_paged_noalloc(fi_context* ctx, const float* d_q, const vo
  * longer qlen_b is reported as Runtime by fi_ctx_check_faults and its rows past the tiles that
  * max_query_len sized are left unwritten.  q, out and the pools must be 16-byte aligned
  * (InvalidLayout otherwise).  Every pool dtype is attended in f32 accuracy.  Over an mxfp4 pool a
- * query row at a negative position (context_lens[b] below qlen_b) sees no key and gets zeros, and
- * scale must be positive and finite (InvalidConfig otherwise). */
+ * query row at a negative position (context_lens[b] below qlen_b) sees no key and gets zeros, a
+ * context length beyond the block table's width is cut off there and reported as Runtime by
+ * fi_ctx_check_faults, and scale must be positive and finite (InvalidConfig otherwise). */
 int32_t fi_attn_prefill_paged(fi_context* ctx, const float* d_q, const void* d_k_cache,
                               const void* d_v_cache, int32_t kv_dtype,
                               const int32_t* d_block_tables, int32_t max_blocks_per_seq,
