@@ -392,16 +392,19 @@ int32_t launch_dim(fi_context* ctx, const PrefillArgs& args_in) {
   const int g = args.group <= 1 ? 1 : (args.group <= 2 ? 2 : (args.group <= 4 ? 4 : 8));
   const int qt = kRows / g;
   // Key splits for launches that leave workgroup slots empty: up to three workgroups a CU, the most that
-  // run at a time, and (tile_splits) four chunks of keys or more each; the block tables' width is the
-  // bound of a tile's chunks that the host knows.  32/8 heads of 128, us cut against whole: 64 rows after
-  // 1000 cached 20.9 against 44, after 4000 33 against 124, after 16000 60 against 468.  Where the launch has a workgroup for
-  // half the CUs without them, sixteen chunks: the partials' way through memory costs a range 3 us (300
-  // rows after 8000 114 against 246, 500 after 2000 68 against 79; but 500 after none 26.6 in two against 21.6, 1000
-  // after 4000, two workgroups a CU without them, 194 against 188).
+  // run at a time, and (tile_splits) four chunks of keys or more each.  What the host knows of a tile's
+  // chunks is the block tables' width less half of the new rows, the mean over a sequence's tiles (500 rows
+  // after none over 14/2 heads of 64, tiles of one to eight chunks: 17.9 us with the longer ones cut, 14.6
+  // whole).  32/8 heads of 128, us cut against whole: 64 rows after 1000 cached 20.9 against 44, after 4000 33 against
+  // 124, after 16000 60 against 468.  Where the launch has a workgroup for half the CUs without them, eight
+  // chunks: the partials' way through memory costs a range 3 us (300 rows after 8000 112 against 246, 300
+  // after 2000 50 and with sixteen chunks 59, 500 after 500 36 and with six 45; 1000 after 4000, two workgroups a
+  // CU without splits, 194 against 188).
   const int64_t cus = ctx->compute_units > 0 ? ctx->compute_units : 256;
   const int64_t wgs = static_cast<int64_t>((args.max_query_len + qt - 1) / qt) * args.num_seqs * args.hkv;
-  const int64_t chunks = (static_cast<int64_t>(args.max_blocks) * args.block_size + kChunk - 1) / kChunk;
-  args.split_chunks = 2 * wgs <= cus ? 4 : 16;
+  const int64_t chunks = (static_cast<int64_t>(args.max_blocks) * args.block_size + kChunk - 1) / kChunk -
+                         args.max_query_len / (2 * kChunk);
+  args.split_chunks = 2 * wgs <= cus ? 4 : 8;
   const int splits = static_cast<int>(std::max<int64_t>(
       1, std::min<int64_t>({kMaxSplits, 3 * cus / std::max<int64_t>(wgs, 1), chunks / args.split_chunks})));
   dim3 grid;

@@ -272,7 +272,7 @@ def test_prefill_replayed(gpu_ctx, seqs, hq, hkv, d):
     ([(20000, 1)], 1, 1, 32, 16),                           # 32 ranges, as many as a tile is cut into
     ([(3000, 40), (0, 3), (255, 1), (256, 1), (511, 2), (0, 0)], 14, 2, 64, 16),  # cut, whole and absent beside each other
     ([(1500, 70), (100, 257)], 6, 2, 128, 5),               # tiles of 1, 2, .. ranges
-    ([(9000, 300)], 14, 2, 64, 64),                         # more tiles: ranges of 16 chunks
+    ([(9000, 300)], 14, 2, 64, 64),                         # more tiles: longer ranges
 ])
 def test_prefill_of_few_rows_over_long_prefixes(gpu_ctx, seqs, hq, hkv, d, bs):
     print(f"prefill over prefixes {seqs}", flush=True)
