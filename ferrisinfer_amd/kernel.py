@@ -175,6 +175,12 @@ def ptr(t) -> int | None:
     return t.data_ptr()
 
 
+def check_slots(name, rows, slot_mapping) -> None:
+    """A consumer of `rows` tokens reads a slot for each."""
+    if slot_mapping is not None and not isinstance(slot_mapping, int) and slot_mapping.numel() < rows:
+        raise FerrisError(3, f"{name}: {rows} positions need a slot each")
+
+
 def kv_pool_bytes(kv_dtype, num_blocks, block_size, num_kv_heads, head_dim) -> int:
     """Bytes of one K or V pool array of a layer."""
     out = _SZ()
@@ -543,6 +549,7 @@ class Context:
                         max_positions, slot_mapping, k_cache, v_cache, kv_dtype, num_blocks,
                         block_size, num_q_heads, num_kv_heads, head_dim, q_out):
         bq, bk, bv = biases if biases is not None else (None, None, None)
+        check_slots("qkv_rope_append", positions.numel(), slot_mapping)
         check(self.lib.fi_qkv_rope_append(self.handle, ptr(parts), int(splits), ptr(bq), ptr(bk),
                                           ptr(bv),
                                           ptr(positions), ptr(cos_t), ptr(sin_t), int(rotary_dims),
@@ -560,7 +567,11 @@ class Context:
         rotary pair's axis (a sequence of rotary_dims / 2 ints, or None with one axis)."""
         bq, bk, bv = biases if biases is not None else (None, None, None)
         nq, nk = norms if norms is not None else (None, None)
-        axes = 1 if positions.dim() == 1 else int(positions.shape[0])
+        shape = positions.shape
+        if not 1 <= len(shape) <= 2:
+            raise FerrisError(3, "qkv_norm_rope_append: positions must be [T] or [axes, T]")
+        tokens, axes = shape[-1], 1 if len(shape) == 1 else shape[0]
+        check_slots("qkv_norm_rope_append", tokens, slot_mapping)
         if not positions.is_contiguous():
             raise FerrisError(4, "qkv_norm_rope_append: positions must be contiguous")
         if pair_axes is not None and len(pair_axes) != int(rotary_dims) // 2:
@@ -572,6 +583,6 @@ class Context:
                                                ptr(nq), ptr(nk), float(eps), ptr(positions), axes, named,
                                                ptr(cos_t), ptr(sin_t), int(rotary_dims), int(max_positions),
                                                ptr(slot_mapping), ptr(k_cache), ptr(v_cache), int(kv_dtype),
-                                               int(num_blocks), int(block_size), int(positions.shape[-1]),
+                                               int(num_blocks), int(block_size), tokens,
                                                int(num_q_heads), int(num_kv_heads), int(head_dim),
                                                ptr(q_out)))
