@@ -114,8 +114,8 @@ struct ChunkLoader {
 };
 
 // The keys of a chunk from k0 on that a row at position qpos sees, as a mask.
-__device__ __forceinline__ uint64_t seen_keys(int qpos, int ctx, int k0) {
-  const int last = min(qpos, ctx - 1) - k0;
+__device__ __forceinline__ uint64_t seen_keys(int qpos, int kend, int k0) {
+  const int last = min(qpos, kend - 1) - k0;
   return last < 0 ? 0 : (last >= 63 ? ~0ull : (2ull << last) - 1);
 }
 
@@ -225,14 +225,14 @@ __global__ __launch_bounds__(kThreads, 3) void prefill_fp4_kernel(PrefillArgs a)
         for (int jt = 0; jt < JT; ++jt)
           s[jt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf[jt], qf[t][p], s[jt], 0, 0, 0);
     }
-    // causal / context mask only where the chunk reaches past the tile's first query position
-    if (k0 + KB - 1 > start + q0) {
+    // causal / context mask only where the chunk reaches past the tile's first query position or its keys
+    if (k0 + KB - 1 > min(start + q0, kend - 1)) {
 #pragma unroll
       for (int jt = 0; jt < JT; ++jt)
 #pragma unroll
         for (int v = 0; v < 4; ++v) {
           const int kp = k0 + 16 * jt + 4 * lk + v;
-          s[jt][v] = (kp <= qpos && kp < ctx) ? s[jt][v] : -INFINITY;
+          s[jt][v] = (kp <= qpos && kp < kend) ? s[jt][v] : -INFINITY;
         }
     }
     float mx = -INFINITY;
@@ -292,7 +292,7 @@ __global__ __launch_bounds__(kThreads, 3) void prefill_fp4_kernel(PrefillArgs a)
     }
     // rows that see a key with a NaN group of V
     if ((s_nan[0] | s_nan[1] | s_nan[2] | s_nan[3]) != 0) {  // workgroup-uniform
-      const uint64_t seen = seen_keys(qpos, ctx, k0);
+      const uint64_t seen = seen_keys(qpos, kend, k0);
 #pragma unroll
       for (int dt = 0; dt < DT; ++dt)
         if (s_nan[dt * 4 / DT] & seen) o[dt] = v4f{NAN, NAN, NAN, NAN};

@@ -1,0 +1,42 @@
+"""Prefill attention over a 4-bit KV pool where keys end: at the block table's width."""
+import numpy as np
+import pytest
+
+import fp4_accuracy as acc
+import fp4_reference as fp4
+from test_gpu_fp4_cache import dev, random_pool
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize("n,seen,bs,blocks", [
+    (5, 1000, 16, 19),        # 304 keys: the last chunk of 64 is not full
+    (200, 310, 16, 19),       # rows before, at and past the table's last key
+    (7, 2 ** 31 - 1, 5, 13),  # 65 keys
+    (70, 66, 1, 3),
+    (6, 9000, 8, 1025),       # 8200 keys in ranges
+])
+def test_keys_end_with_the_block_table(gpu_ctx, n, seen, bs, blocks):
+    """A context length past the table's width is reported, and the keys of the table are what counts."""
+    import torch
+
+    from ferrisinfer_amd import DTYPE_MXFP4, FerrisError
+
+    print(f"prefill past the table {n} {seen} {bs} {blocks}", flush=True)
+    rng = np.random.default_rng(52)
+    hq, hkv, d = 8, 2, 64
+    (kb, kv), (vb, vv) = random_pool(rng, blocks, hkv, bs, d), random_pool(rng, blocks, hkv, bs, d)
+    tables = rng.permutation(blocks).astype(np.int32)[None]
+    q = rng.standard_normal((n, hq, d)).astype(np.float32)
+    out = torch.full(q.shape, -7.0, device="cuda")
+    gpu_ctx.attn_prefill_paged(dev(q), dev(kb), dev(vb), DTYPE_MXFP4, dev(tables), dev(np.array([0, n], np.int32)),
+                               dev(np.array([seen], np.int32)), n, hkv, bs, blocks, d ** -0.5, out)
+    gpu_ctx.sync()
+    with pytest.raises(FerrisError) as e:
+        gpu_ctx.check_faults()
+    assert e.value.kind == "Runtime"
+    k, v = (fp4.rows_of(x, tables[0], blocks * bs, bs) for x in (kv, vv))
+    first = seen - n
+    got, skip = out.cpu().numpy(), max(0, -first)
+    assert (got[:skip] == 0).all()
+    acc.check(got[skip:], q[skip:], k, v, first + skip, d ** -0.5, acc.prefill_additions(blocks * bs))
