@@ -89,7 +89,7 @@ struct ChunkLoader {
     part_next = (c + 1) * KB > kend;  // workgroup-uniform: the chunk has padding keys
     valid_next = c * KB + skey < kend;
     const bool bad = id_next < 0 || id_next >= num_blocks;
-    bad_block |= bad;
+    bad_block |= bad && valid_next;  // a tile without keys looks up one block all the same
     const size_t row = ((size_t)(bad ? 0 : id_next) * hkv + kvh) * block_size + off_next;
     kc.load(k_codes + row * (D / 2));
     vc.load(v_codes + row * (D / 2));

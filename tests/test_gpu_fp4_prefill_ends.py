@@ -1,10 +1,12 @@
-"""Prefill attention over a 4-bit KV pool where keys end: at the block table's width."""
+"""Prefill attention over a 4-bit KV pool where keys end: at the block table's width, and
+before a row's position."""
 import numpy as np
 import pytest
 
 import fp4_accuracy as acc
 import fp4_reference as fp4
-from test_gpu_fp4_cache import dev, random_pool
+from test_gpu_fp4_cache import dev, random_pool, tables_of
+from test_gpu_fp4_prefill import prefill
 
 pytestmark = pytest.mark.gpu
 
@@ -40,3 +42,41 @@ def test_keys_end_with_the_block_table(gpu_ctx, n, seen, bs, blocks):
     got, skip = out.cpu().numpy(), max(0, -first)
     assert (got[:skip] == 0).all()
     acc.check(got[skip:], q[skip:], k, v, first + skip, d ** -0.5, acc.prefill_additions(blocks * bs))
+
+
+@pytest.mark.parametrize("long", [0, 3000])
+@pytest.mark.parametrize("seen", [0, -5])
+def test_a_sequence_without_keys_names_no_block(gpu_ctx, seen, long):
+    """New rows at negative positions get zeros, whatever their row of the block table holds; in a launch
+    whose other sequence is cut into ranges of keys, too."""
+    rng = np.random.default_rng(53)
+    hq, hkv, d, bs = 4, 1, 128, 16
+    new, lens = [20, 40], [seen, long + 40]
+    nb = -(-lens[1] // bs) + 2
+    (kb, kv), (vb, vv) = random_pool(rng, nb, hkv, bs, d), random_pool(rng, nb, hkv, bs, d)
+    tables = tables_of(rng, [0, lens[1]], bs, nb)
+    assert (tables[0] == -1).all()
+    q = rng.standard_normal((60, hq, d)).astype(np.float32)
+    got = prefill(gpu_ctx, q, (dev(kb), dev(vb)), tables, new, lens, hkv, bs, nb, d ** -0.5)
+    assert (got[:20] == 0).all()
+    k, v = (fp4.rows_of(x, tables[1], lens[1], bs) for x in (kv, vv))
+    acc.check(got[20:], q[20:], k, v, long, d ** -0.5, acc.prefill_additions(lens[1]))
+
+
+@pytest.mark.parametrize("cached,n", [(0, 12), (0, 70), (1300, 6)])
+def test_a_block_out_of_range_is_still_reported(gpu_ctx, cached, n):
+    """At the sequence's first key, and at its last, in a chunk that is not full."""
+    from ferrisinfer_amd import FerrisError
+
+    rng = np.random.default_rng(54)
+    hq, hkv, d, bs = 4, 1, 64, 16
+    nb = -(-(cached + n) // bs)
+    pools = tuple(dev(random_pool(rng, nb, hkv, bs, d)[0]) for _ in range(2))
+    q = rng.standard_normal((n, hq, d)).astype(np.float32)
+    for at in (0, -1):
+        for bad in (nb, -1):
+            tables = tables_of(rng, [cached + n], bs, nb)
+            tables[0, at] = bad
+            with pytest.raises(FerrisError) as e:
+                prefill(gpu_ctx, q, pools, tables, [n], [cached + n], hkv, bs, nb, 1.0)
+            assert e.value.kind == "Runtime"
