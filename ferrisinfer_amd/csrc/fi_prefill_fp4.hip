@@ -127,6 +127,12 @@ __device__ __forceinline__ int tile_splits(const PrefillArgs& a, int chunks) {
   return max(1, min(a.kv_splits, chunks / a.split_chunks));
 }
 
+// The position of a sequence's first new row.  Below 0 its row sees no key; context lengths below 0 count as 0,
+// for the difference to stay in 32 bits.
+__device__ __forceinline__ int first_position(const PrefillArgs& a, int seq, int qlen) {
+  return max(a.context_lens[seq], 0) - qlen;
+}
+
 // The end of the keys that a tile's last row sees, none past the block table's width (rows that ask for
 // more are reported: a context length that is wrong must not make a loop of a billion chunks), and
 // their chunks: at least one, of rows without keys too.
@@ -161,8 +167,7 @@ __global__ __launch_bounds__(kThreads, 3) void prefill_fp4_kernel(PrefillArgs a)
   check_query_length(a, qt, qlen, ntiles * QT);
   const int q0 = qt * QT;
   if (q0 >= qlen) return;
-  const int ctx = a.context_lens[seq];
-  const int start = ctx - qlen;
+  const int start = first_position(a, seq, qlen);
   const int tid = threadIdx.x, w = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
   const int li = lane & 15, lk = lane >> 4;
   const int row = 16 * w + li;
@@ -346,7 +351,7 @@ __global__ __launch_bounds__(kThreads) void prefill_merge_fp4_kernel(PrefillArgs
   const int r = idx / DQ, dq = idx % DQ;
   const int h = r / qt_tokens, t = r % qt_tokens;
   if (h >= a.group || q0 + t >= qlen) return;
-  const int splits = tile_splits(a, tile_chunks(tile_end(a, a.context_lens[seq] - qlen, qlen, q0 + qt_tokens)));
+  const int splits = tile_splits(a, tile_chunks(tile_end(a, first_position(a, seq, qlen), qlen, q0 + qt_tokens)));
   const size_t units = (size_t)(gridDim.x / BLOCKS) * a.kv_splits;
   const float* pml = a.part + units * kRows * D;
   const size_t first = (size_t)tile * a.kv_splits * a.hkv + kvh;  // split s: first + s * hkv

@@ -45,7 +45,7 @@ def test_keys_end_with_the_block_table(gpu_ctx, n, seen, bs, blocks):
 
 
 @pytest.mark.parametrize("long", [0, 3000])
-@pytest.mark.parametrize("seen", [0, -5])
+@pytest.mark.parametrize("seen", [0, -5, -2 ** 31])
 def test_a_sequence_without_keys_names_no_block(gpu_ctx, seen, long):
     """New rows at negative positions get zeros, whatever their row of the block table holds; in a launch
     whose other sequence is cut into ranges of keys, too."""
