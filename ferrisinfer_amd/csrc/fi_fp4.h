@@ -20,6 +20,7 @@
 namespace fi {
 
 constexpr int kFp4Group = 32;  // elements that share a scale
+constexpr uint32_t kFp4MaxScale = 252;  // the largest scale byte of values: 6 * 2^(E - 127) may be infinite above
 
 // One pool array: codes [num_blocks][Hkv][block_size][D / 2] (element 2 i in the low half of byte
 // i), then scales [num_blocks][Hkv][block_size][D / 32].  Codes and scales are apart so that a
@@ -58,7 +59,7 @@ __device__ __forceinline__ uint32_t group_max(uint32_t v) {
 __device__ __forceinline__ uint32_t fp4_scale(uint32_t top) {
   if (top >= 0x7f800000u) return 255u;
   const int e = static_cast<int>(top >> 23) - 2 + ((top & 0x7fffffu) >= 0x600000u ? 1 : 0);
-  return static_cast<uint32_t>(min(max(e, 2), 252));
+  return static_cast<uint32_t>(min(max(e, 2), static_cast<int>(kFp4MaxScale)));
 }
 
 // A scale byte as the f32 whose exponent field it is (255: an infinity, which the conversions

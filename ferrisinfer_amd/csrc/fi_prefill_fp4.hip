@@ -21,7 +21,8 @@
 //
 // A NaN group of V must reach only the rows that see its key, though a chunk's product multiplies every
 // key by every row (0 * NaN is NaN): it is staged as zeros, its key noted in a 64-bit mask of the
-// chunk and column quarter, and the rows that see a noted key are set to NaN afterwards.
+// chunk and column quarter, and the rows that see a noted key are set to NaN afterwards.  So is a group with a
+// scale that appending never writes, 253 or 254, whose values may be infinite.
 #include "fi_common.h"
 #include "fi_device.h"
 #include "fi_fp4.h"
@@ -97,10 +98,10 @@ struct ChunkLoader {
     v_scale = v_scales[row * GROUPS];
   }
   // Padding keys of a partial chunk are stored as zero (their clamped loads hold a valid row); so is a
-  // NaN group of V, whose key goes into nan_keys[wave] (a wave stages a quarter of the columns).
+  // NaN (or overflowing) group of V, whose key goes into nan_keys[wave] (a wave stages a quarter of the columns).
   __device__ __forceinline__ void stage(uint16_t (*ks)[KPK], uint16_t (*vs)[KP], uint64_t* nan_keys, int tid) {
     const bool pad = part_next && !valid_next;
-    const bool nan = !pad && v_scale == 255u;
+    const bool nan = !pad && v_scale > fi::kFp4MaxScale;
     const uint64_t nans = __builtin_amdgcn_ballot_w64(nan);
     if ((tid & 63) == 0) nan_keys[tid >> 6] = nans;
     const float k2 = fi::fp4_scale_f32(pad ? 127u : k_scale), v2 = fi::fp4_scale_f32(pad || nan ? 127u : v_scale);

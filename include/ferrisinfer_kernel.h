@@ -59,7 +59,9 @@ enum {
  *
  * FI_DTYPE_MXFP4, 4-bit KV storage: each group of 32 consecutive elements of a head's row holds 32
  * e2m1 codes (bit 3 the sign, bits 0-2 the magnitude 0, 0.5, 1, 1.5, 2, 3, 4, 6) and one scale byte
- * E; an element's value is magnitude * 2^(E - 127), exactly, and E = 255 makes the group NaN.  17
+ * E; an element's value is magnitude * 2^(E - 127), exactly, for E up to 252, and E = 255 makes the
+ * group NaN.  253 and 254, whose values can pass f32's largest, are not for a host to write: a row
+ * that sees such a group has no defined result, other rows are not affected.  17
  * bytes for 32 elements.  A pool array (K or V of one layer, fi_kv_pool_bytes bytes, 16-byte
  * aligned) is the codes [num_blocks, Hkv, block_size, D / 2], element 2 i of a row in the low half
  * of its byte i, followed by the scales [num_blocks, Hkv, block_size, D / 32].  Appending takes the

@@ -1,5 +1,5 @@
-"""Prefill attention over a 4-bit KV pool where keys end: at the block table's width, and
-before a row's position."""
+"""Prefill attention over a 4-bit KV pool where keys end: at the block table's width,
+before a row's position, and at scales that appending never writes."""
 import numpy as np
 import pytest
 
@@ -80,3 +80,26 @@ def test_a_block_out_of_range_is_still_reported(gpu_ctx, cached, n):
             with pytest.raises(FerrisError) as e:
                 prefill(gpu_ctx, q, pools, tables, [n], [cached + n], hkv, bs, nb, 1.0)
             assert e.value.kind == "Runtime"
+
+
+@pytest.mark.parametrize("e", [253, 254, 255])
+def test_scales_past_the_formats_reach_only_rows_that_see_them(gpu_ctx, e):
+    """Appending writes no scale above 252 but 255; a pool that holds one, from elsewhere, harms the rows that
+    see its key and no others."""
+    rng = np.random.default_rng(55)
+    n, hq, hkv, d, bs = 90, 8, 2, 64, 16
+    nb = -(-n // bs) + 1
+    (kb, kv), (vb, vv) = random_pool(rng, nb, hkv, bs, d), random_pool(rng, nb, hkv, bs, d)
+    tables = tables_of(rng, [n], bs, nb)
+    q = rng.standard_normal((n, hq, d)).astype(np.float32)
+    k, v = (fp4.rows_of(x, tables[0], n, bs) for x in (kv, vv))
+    for at_k, at_v in ((41, n), (n, 41), (70, 30)):
+        ks, vs = kb.copy(), vb.copy()
+        for pool, at in ((ks, at_k), (vs, at_v)):
+            if at < n:
+                codes, scales = fp4.split_pool(pool, nb, hkv, bs, d)
+                codes[tables[0, at // bs], :, at % bs] |= 0x77  # magnitudes of 6 scales
+                scales[tables[0, at // bs], :, at % bs] = e
+        got = prefill(gpu_ctx, q, (dev(ks), dev(vs)), tables, [n], [n], hkv, bs, nb, d ** -0.5)
+        clean = min(at_k, at_v)
+        acc.check(got[:clean], q[:clean], k, v, 0, d ** -0.5, acc.prefill_additions(n))
