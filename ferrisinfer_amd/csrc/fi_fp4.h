@@ -67,8 +67,9 @@ __device__ __forceinline__ uint32_t fp4_scale(uint32_t top) {
 __device__ __forceinline__ float fp4_scale_f32(uint32_t e) { return __uint_as_float(e << 23); }
 
 // Codes of two values divided by the scale (nearest even, cut off at 6) into byte kByte of `old`.
-// The instruction's results equal the format's rule for every scale byte from 2 to 252, ties and
-// values above 6 scales among them; non-finite groups do not come here.
+// The instruction's results equal the format's rule for every scale byte from 2 to 252, ties, their
+// neighbours, subnormals and values above 6 scales among them (tests/test_gpu_fp4_scales.py); non-finite
+// groups do not come here.
 template <int kByte>
 __device__ __forceinline__ uint32_t fp4_pack2(uint32_t old, float a, float b, float scale) {
   return __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(old, a, b, scale, kByte);
