@@ -13,6 +13,9 @@ from .kernel import DTYPE_BF16, DTYPE_F16, DTYPE_F32, DTYPE_MXFP4, FerrisError, 
 
 LIB_PATH = os.path.join(PKG_DIR, "libferrisinfer_runtime.so")
 
+#: the KV pools that a runtime serves from, by name
+KV_DTYPES = {"f32": DTYPE_F32, "bf16": DTYPE_BF16, "mxfp4": DTYPE_MXFP4}
+
 
 class ModelConfig(C.Structure):
     _fields_ = [("hidden_size", C.c_int32), ("intermediate_size", C.c_int32),
@@ -151,13 +154,15 @@ class Runtime:
         pool): storage of the KV pool.  weight_dtype "f32" or "bf16": storage of the
         packed projections and head.  graph_decode: replay decode ticks from HIP graphs."""
         L = load()
+        if kv_dtype not in KV_DTYPES:
+            raise FerrisError(5, f"KV dtype {kv_dtype!r} is none of {', '.join(KV_DTYPES)}")
         temperature, top_k, top_p, seed = (0.0, 1, 1.0, 0) if sampler is None else sampler
         head_dim = hidden // heads
         mc = ModelConfig(hidden, intermediate, layers, heads, kv_heads, vocab, max_pos, eps, theta,
                          head_dim if rotary_dims is None else rotary_dims, 1 if tie else 0)
         rc = RuntimeConfig(max_seq, max_gen, max_batch, max_chunk, max_batch_tokens,
                            max_consecutive_prefill, min_share, num_blocks, block_size,
-                           {"f32": DTYPE_F32, "mxfp4": DTYPE_MXFP4}.get(kv_dtype, DTYPE_BF16),
+                           KV_DTYPES[kv_dtype],
                            temperature, top_k, top_p, 1.0, seed,
                            DTYPE_F32 if weight_dtype == "f32" else DTYPE_BF16,
                            1 if graph_decode else 0)
