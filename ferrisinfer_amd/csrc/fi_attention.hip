@@ -886,8 +886,9 @@ int32_t decode_paged(fi_context* ctx, const float* d_q, const void* d_k_cache, c
              "fi_attn_decode_paged: head_dim must be 32, 64 or 128");
   const int wt = wave_tokens_for(num_kv_heads, head_dim);
   const int part_tokens = kWaves * wt;
-  FI_REQUIRE(max_context_len <= part_tokens * kMaxParts, FI_ERR_UNSUPPORTED,
-             "fi_attn_decode_paged: context longer than " + std::to_string(part_tokens * kMaxParts) + " tokens");
+  const int longest = kv_dtype == FI_DTYPE_MXFP4 ? fi::kFp4MaxContext : part_tokens * kMaxParts;
+  FI_REQUIRE(max_context_len <= longest, FI_ERR_UNSUPPORTED,
+             "fi_attn_decode_paged: context longer than " + std::to_string(longest) + " tokens");
   if (qkv) {
     FI_REQUIRE(qkv->splits >= 1, FI_ERR_INVALID_SHAPE, "fi_attn_decode_paged_qkv: splits must be at least 1");
     FI_REQUIRE(qkv->rotary_dims >= 0 && qkv->rotary_dims <= head_dim && qkv->rotary_dims % 2 == 0,

@@ -78,13 +78,14 @@ constexpr int kMergeInline = 16;
 
 // NS strands from s0 on, of this lane's D / 64 dims (D = 32: of the lower half's one): the weighted
 // sums, and the strands' shares of L.  BATCH partitions' loads are issued together, the first ones' with the
-// statistics'.
-template <int D, bool COHERENT, int NS, int BATCH>
+// statistics'.  MAXP: the partitions that a sequence may have.
+template <int D, bool COHERENT, int NS, int BATCH, int MAXP>
 __device__ __forceinline__ void merge_strands(const DecodeArgs& a, size_t head, int nparts, int s0, int lane,
                                               float (&sum)[NS][(D + 63) / 64], float (&share)[NS]) {
   constexpr int E = (D + 63) / 64;
   constexpr int STEP = NS == 1 ? kStrands : 1;  // from one of this wave's partitions to the next
-  constexpr int MAXP = NS == 1 ? kMaxParts : kMergeInline;
+  constexpr int PER = (MAXP / STEP + 63) / 64;  // partitions whose statistics a lane keeps
+  static_assert(64 % BATCH == 0, "a batch's weights lie in one register");
   float* ml = a.part_ml + head * a.parts_per_seq * 2;
   float* acc = a.part_acc + head * a.parts_per_seq * D + (D < 64 ? lane % D : lane * E);
   const int mine = (nparts - s0 + STEP - 1) / STEP;  // this wave's partitions
@@ -99,13 +100,22 @@ __device__ __forceinline__ void merge_strands(const DecodeArgs& a, size_t head, 
 #pragma unroll
   for (int p0 = 0; p0 < MAXP; p0 += 64)
     if (p0 + lane < nparts) mx = fmaxf(mx, load_partial<COHERENT>(&ml[2 * (p0 + lane)]));
-  // lane i keeps the statistics of this wave's i-th partition
-  const int own = s0 + lane * STEP;
-  const float m_own = own < nparts ? load_partial<COHERENT>(&ml[2 * own]) : -INFINITY;
-  const float l_own = own < nparts ? load_partial<COHERENT>(&ml[2 * own + 1]) : 0.0f;
+  // lane i keeps the statistics of this wave's partitions i, i + 64, ..
+  float w_own[PER], l_own[PER];
+#pragma unroll
+  for (int k = 0; k < PER; ++k) {
+    const int own = s0 + (lane + 64 * k) * STEP;
+    w_own[k] = own < nparts ? load_partial<COHERENT>(&ml[2 * own]) : -INFINITY;
+    l_own[k] = own < nparts ? load_partial<COHERENT>(&ml[2 * own + 1]) : 0.0f;
+  }
   mx = fi::wave_max(mx);
-  const float w_own = __builtin_amdgcn_exp2f(m_own - (mx == -INFINITY ? 0.0f : mx));
-  const float wl = l_own * w_own;
+  const float point = mx == -INFINITY ? 0.0f : mx;
+  float wl = 0.0f;
+#pragma unroll
+  for (int k = 0; k < PER; ++k) {
+    w_own[k] = __builtin_amdgcn_exp2f(w_own[k] - point);
+    wl += l_own[k] * w_own[k];
+  }
 #pragma unroll
   for (int s = 0; s < NS; ++s) {
     share[s] = fi::wave_sum(NS == 1 || lane % NS == s ? wl : 0.0f);
@@ -121,10 +131,11 @@ __device__ __forceinline__ void merge_strands(const DecodeArgs& a, size_t head, 
         for (int e = 0; e < E; ++e) v[b][e] = load_partial<COHERENT>(acc + (size_t)p * D + e);
       }
     }
+    const float weights = PER == 1 || i0 < 64 ? w_own[0] : w_own[PER - 1];
 #pragma unroll
     for (int b = 0; b < BATCH; ++b) {
       if (i0 + b < mine) {  // wave-uniform
-        const float w = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(w_own), i0 + b));
+        const float w = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(weights), (i0 + b) % 64));
 #pragma unroll
         for (int e = 0; e < E; ++e) sum[b % NS][e] += v[b][e] * w;
       }
@@ -136,7 +147,7 @@ __device__ __forceinline__ void merge_strands(const DecodeArgs& a, size_t head, 
 // of 128 dims, 6.7 MB, in 6.6 us with 32 partitions' loads at a time (8.2 with 8, which is the faster one up
 // to 64 partitions: one sequence of 60000 tokens over 2 heads of 64 15.0 against 18.1 us in all, 8 of 4000 9.4
 // against 9.0).
-template <int D, int WT, int BATCH>
+template <int D, int WT, int BATCH, int MAXP>
 __global__ __launch_bounds__(64 * kStrands) void decode_merge_fp4_kernel(DecodeArgs a) {
   constexpr int E = (D + 63) / 64;
   __shared__ float s_sum[kStrands][D];
@@ -148,7 +159,7 @@ __global__ __launch_bounds__(64 * kStrands) void decode_merge_fp4_kernel(DecodeA
   if (nparts <= 1) return;
   const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
   float sum[1][E], share[1];
-  merge_strands<D, false, 1, BATCH>(a, head, nparts, w, lane, sum, share);
+  merge_strands<D, false, 1, BATCH, MAXP>(a, head, nparts, w, lane, sum, share);
   if (D >= 64 || lane < D) {
 #pragma unroll
     for (int e = 0; e < E; ++e) s_sum[w][lane * E + e] = sum[0][e];
@@ -219,7 +230,7 @@ __device__ __forceinline__ void combine_waves_fp4(const DecodeArgs& a, const Hea
   for (int g = tid >> 6; g < group; g += kWaves) {
     const size_t head = hu.head0 + g;
     float sum[kStrands][E], share[kStrands];
-    merge_strands<D, true, kStrands, 8>(a, head, nparts, 0, lane, sum, share);
+    merge_strands<D, true, kStrands, 8, kMergeInline>(a, head, nparts, 0, lane, sum, share);
 #pragma unroll
     for (int s = 1; s < kStrands; ++s) {
       share[0] += share[s];
@@ -509,7 +520,11 @@ int32_t launch(fi_context* ctx, const DecodeArgs& args, dim3 grid) {
   hipLaunchKernelGGL((decode_fp4_kernel<D, T, WT, QUAD>), grid, dim3(kThreads), 0, ctx->stream, args);
   FI_CHECK_LAUNCH("decode_fp4_kernel");
   if (args.parts_per_seq > 1 && args.counters == nullptr) {
-    auto merge = args.parts_per_seq > 64 ? decode_merge_fp4_kernel<D, WT, 32> : decode_merge_fp4_kernel<D, WT, 8>;
+    auto merge = args.parts_per_seq > 64 ? decode_merge_fp4_kernel<D, WT, 32, kMaxParts> : decode_merge_fp4_kernel<D, WT, 8, kMaxParts>;
+    constexpr int kLongest = fi::kFp4MaxContext / (kWaves * WT);
+    if constexpr (kLongest > kMaxParts) {  // narrow rows: two statistics a lane
+      if (args.parts_per_seq > kMaxParts) merge = decode_merge_fp4_kernel<D, WT, 32, kLongest>;
+    }
     hipLaunchKernelGGL(merge, dim3(static_cast<unsigned>(args.num_seqs) * args.hq), dim3(64 * kStrands), 0, ctx->stream,
                        args);
     FI_CHECK_LAUNCH("decode_merge_fp4_kernel");

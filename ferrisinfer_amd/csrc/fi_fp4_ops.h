@@ -28,6 +28,10 @@ int32_t kv_copy_blocks_fp4(fi_context* ctx, void* k_cache, void* v_cache, const 
 int32_t kv_gather_fp4(fi_context* ctx, const void* k_cache, const void* v_cache, const int32_t* table, int32_t length,
                       int32_t num_blocks, int32_t block_size, int32_t hkv, int32_t d, float* k_out, float* v_out);
 
+// Tokens of a sequence that decode serves over a 4-bit pool: 256 partitions of 512 tokens, or 512 of 256 where
+// the rows are narrow (wave_tokens_for).
+constexpr int kFp4MaxContext = 131072;
+
 // Whether a decode launch of several partitions (up to `heads` heads a workgroup) merges them by itself:
 // the workgroup that ends a sequence's last partition does, instead of a launch of its own.  One
 // strand of the merge holds a sequence's weights, up to 16 partitions.  Up to 8 that is the faster way

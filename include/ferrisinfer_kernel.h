@@ -234,7 +234,8 @@ int32_t fi_ctx_check_faults(fi_context* ctx);
  * q/out: f32 [num_seqs, Hq, D]; scale is 1/sqrt(D) in the reference (attention.rs:659).  Scores,
  * softmax and sums are f32 whatever the pool's dtype, and the pool's values enter them exactly;
  * over an mxfp4 pool q must be 16-byte aligned (InvalidLayout otherwise), and num_blocks * Hkv *
- * block_size may be 2^32 and num_seqs * Hq below 2^24 (Unsupported otherwise).
+ * block_size may be 2^32 and num_seqs * Hq below 2^24 (Unsupported otherwise).  max_context_len may be
+ * 131072, and 65536 over an f32 or bf16 pool where Hkv * D is below 512 (Unsupported otherwise).
  * max_context_len must bound every context_lens entry (it sizes the grid); an entry beyond
  * the partitions it sizes is clamped to them on device and reported as Runtime by
  * fi_ctx_check_faults. */
