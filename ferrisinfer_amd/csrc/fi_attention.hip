@@ -674,12 +674,14 @@ int32_t fi_kv_pool_bytes(int32_t kv_dtype, int32_t num_blocks, int32_t block_siz
   FI_REQUIRE(kv_dtype == FI_DTYPE_F32 || kv_dtype == FI_DTYPE_BF16 || kv_dtype == FI_DTYPE_MXFP4, FI_ERR_INVALID_TYPE,
              "fi_kv_pool_bytes: KV dtype must be f32, bf16 or mxfp4");
   FI_REQUIRE(bytes != nullptr, FI_ERR_INVALID_CONFIG, "fi_kv_pool_bytes: null pointer");
-  if (kv_dtype == FI_DTYPE_MXFP4) {
-    FI_TRY(fi::check_fp4_pool("fi_kv_pool_bytes", nullptr, nullptr, head_dim));
-    *bytes = fi::fp4_pool_bytes(num_blocks, num_kv_heads, block_size, head_dim);
-  } else {
-    *bytes = static_cast<size_t>(num_blocks) * num_kv_heads * block_size * head_dim * (kv_dtype == FI_DTYPE_F32 ? 4 : 2);
-  }
+  if (kv_dtype == FI_DTYPE_MXFP4) FI_TRY(fi::check_fp4_pool("fi_kv_pool_bytes", nullptr, nullptr, head_dim));
+  const uint64_t row = kv_dtype == FI_DTYPE_MXFP4 ? fi::fp4_pool_bytes(1, 1, 1, head_dim)
+                                                  : static_cast<uint64_t>(head_dim) * (kv_dtype == FI_DTYPE_F32 ? 4 : 2);
+  uint64_t rows = static_cast<uint64_t>(num_blocks) * static_cast<uint64_t>(block_size), total = 0;  // below 2^62
+  FI_REQUIRE(!__builtin_mul_overflow(rows, static_cast<uint64_t>(num_kv_heads), &rows) &&
+                 !__builtin_mul_overflow(rows, row, &total) && total <= INT64_MAX,
+             FI_ERR_INVALID_SHAPE, "fi_kv_pool_bytes: the pool's size passes 63 bits");
+  *bytes = total;
   return FI_OK;
 }
 

@@ -177,7 +177,8 @@ int32_t fi_token_feed(fi_context* ctx, const int32_t* d_prev_tokens, int32_t pre
 /* ---------------------------------------------------------------- KV pool ops */
 
 /* Bytes of one K or V pool array of a layer (num_blocks * Hkv * block_size rows of head_dim
- * elements of kv_dtype).  Host arithmetic only; no counterpart in the reference. */
+ * elements of kv_dtype; InvalidShape past 63 bits).  Host arithmetic only; no counterpart in the
+ * reference. */
 int32_t fi_kv_pool_bytes(int32_t kv_dtype, int32_t num_blocks, int32_t block_size, int32_t num_kv_heads,
                          int32_t head_dim, size_t* bytes);
 
