@@ -1,5 +1,5 @@
 // Varlen causal prefill attention over the paged pool: what the kernels of every pool type share
-// (launch arguments, tile order, grid, three-piece operands, the merge of key splits).
+// (launch arguments, tile order, grid, three-piece operands).
 #pragma once
 
 #include <algorithm>
@@ -26,9 +26,10 @@ struct PrefillArgs {
   int max_query_len;
   const int* order;          // (sequence, query tile) pairs, largest first; null: tile_of's own order
   int fold;                  // that order pairs long and short tiles (see prefill_plan_kernel)
-  // prefill_x3_kernel with key splits: each (tile, kv head) runs as kv_splits workgroups over
-  // consecutive ranges of its key chunks, writing partials (unnormalised O, reference point and
-  // row sum per row) that prefill_split_merge_kernel combines in split order
+  // prefill_x3_kernel and prefill_fp4_kernel with key splits: each (tile, kv head) runs as kv_splits
+  // workgroups over consecutive ranges of its key chunks, writing partials (unnormalised O, reference
+  // point and row sum per row) that prefill_split_merge_kernel (prefill_merge_fp4_kernel) combines in
+  // split order
   int kv_splits;
   float* part;
   int split_chunks;  // 4-bit pools: a tile is cut into kv_splits ranges, or as many of this many chunks as it has
@@ -164,16 +165,6 @@ int32_t plan_tiles(fi_context* ctx, PrefillArgs& args, int qt, int kb, const cha
   return FI_OK;
 }
 
-// Row groups per wave: two when the grid still gives every CU two workgroups (every K/V
-// fragment read from LDS then feeds two MFMAs), one for launches with few (sequence, tile,
-// kv head) triples, such as a prefill chunk over two kv heads.
-int row_groups(fi_context* ctx, const PrefillArgs& args, int g) {
-  const long cus = ctx->compute_units > 0 ? ctx->compute_units : 256;
-  const int qt2 = kRows * 2 / g;
-  const long tiles2 = (long)((args.max_query_len + qt2 - 1) / qt2) * args.num_seqs * args.hkv;
-  return tiles2 >= 2 * cus ? 2 : 1;
-}
-
 // An f32 operand as its three bf16 pieces (fi::split3_pk).
 __device__ __forceinline__ void split3(const f32x8& x, bf16x8 (&p)[3]) {
   uint4 h, m, l;
@@ -184,71 +175,6 @@ __device__ __forceinline__ void split3(const f32x8& x, bf16x8 (&p)[3]) {
   p[0] = __builtin_bit_cast(bf16x8, h);
   p[1] = __builtin_bit_cast(bf16x8, m);
   p[2] = __builtin_bit_cast(bf16x8, l);
-}
-
-#ifndef FI_PREFILL_MAX_SPLITS
-#define FI_PREFILL_MAX_SPLITS 4  // key splits of a small f32-pool prefill launch, at most
-#endif
-
-// One workgroup per (tile, kv head) of a split launch: each row's output is the splits'
-// partials combined in split order, each rescaled from its own reference point to the largest
-// (a split with no key the row sees carries -inf and adds nothing; the split holding key 0
-// always sees one), then normalised by the combined row sum.
-template <int D, int RG>
-__global__ __launch_bounds__(kThreads) void prefill_split_merge_kernel(PrefillArgs a, int qt_tokens, int ntiles) {
-  constexpr int ROWS = kRows * RG, DQ = D / 4;
-  constexpr int ITER = ROWS * DQ / kThreads;  // (row, column quad) items a thread
-  constexpr int BATCH = ITER < 4 ? ITER : 4;  // items whose loads are issued together
-  constexpr int MAXS = FI_PREFILL_MAX_SPLITS;
-  static_assert(ROWS * DQ % kThreads == 0 && ITER % BATCH == 0, "items must split over the workgroup");
-  const int tile = blockIdx.x / a.hkv, kvh = blockIdx.x % a.hkv;
-  const int seq = tile / ntiles, q0 = (tile % ntiles) * qt_tokens;
-  const int qs = a.cu_seqlens[seq], qlen = a.cu_seqlens[seq + 1] - qs;
-  if (q0 >= qlen) return;
-  const int S = a.kv_splits;
-  const float* pml = a.part + (size_t)gridDim.x * S * ROWS * D;
-  const size_t unit0 = (size_t)tile * S * a.hkv + kvh;  // split sp: unit0 + sp * hkv
-  for (int it0 = 0; it0 < ITER; it0 += BATCH) {
-    // every split's (point, sum) and O quad of BATCH items are loaded before any is combined
-    // (splits past S read split 0 and are dropped)
-    float2 ml[BATCH][MAXS];
-    float4 ov[BATCH][MAXS];
-#pragma unroll
-    for (int b = 0; b < BATCH; ++b) {
-      const int idx = threadIdx.x + (it0 + b) * kThreads;
-      const int r = idx / DQ, dq = idx - (idx / DQ) * DQ;
-#pragma unroll
-      for (int sp = 0; sp < MAXS; ++sp) {
-        const size_t unit = unit0 + (size_t)(sp < S ? sp : 0) * a.hkv;
-        ml[b][sp] = *reinterpret_cast<const float2*>(pml + (unit * ROWS + r) * 2);
-        ov[b][sp] = *reinterpret_cast<const float4*>(a.part + (unit * ROWS + r) * D + 4 * dq);
-      }
-    }
-#pragma unroll
-    for (int b = 0; b < BATCH; ++b) {
-      const int idx = threadIdx.x + (it0 + b) * kThreads;
-      const int r = idx / DQ, dq = idx - (idx / DQ) * DQ;
-      const int h = r / qt_tokens, t = r - (r / qt_tokens) * qt_tokens;
-      if (h >= a.group || q0 + t >= qlen) continue;
-      float mx = -INFINITY;
-#pragma unroll
-      for (int sp = 0; sp < MAXS; ++sp)
-        if (sp < S) mx = fmaxf(mx, ml[b][sp].x);
-      float l = 0.0f;
-      float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll
-      for (int sp = 0; sp < MAXS; ++sp) {
-        if (sp >= S || ml[b][sp].x == -INFINITY) continue;
-        const float wgt = __builtin_amdgcn_exp2f(ml[b][sp].x - mx);
-        const float4 o = ov[b][sp];
-        l = l + wgt * ml[b][sp].y;
-        acc = make_float4(acc.x + wgt * o.x, acc.y + wgt * o.y, acc.z + wgt * o.z, acc.w + wgt * o.w);
-      }
-      const float inv = 1.0f / l;
-      *reinterpret_cast<float4*>(a.out + ((size_t)(qs + q0 + t) * a.hq + kvh * a.group + h) * D + 4 * dq) =
-          make_float4(acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv);
-    }
-  }
 }
 
 }  // namespace
