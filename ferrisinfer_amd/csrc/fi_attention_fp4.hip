@@ -146,7 +146,8 @@ __device__ __forceinline__ void merge_strands(const DecodeArgs& a, size_t head, 
 // One workgroup per query head, a wave a strand.  Bound by the chain of its loads: 64 heads of 196 partitions
 // of 128 dims, 6.7 MB, in 6.6 us with 32 partitions' loads at a time (8.2 with 8, which is the faster one up
 // to 64 partitions: one sequence of 60000 tokens over 2 heads of 64 15.0 against 18.1 us in all, 8 of 4000 9.4
-// against 9.0).
+// against 9.0).  Past 256 partitions (MAXP 512): 14 heads of 391 partitions of 64 dims, 1.4 MB, 8.5 us, of 256
+// 5.0.
 template <int D, int WT, int BATCH, int MAXP>
 __global__ __launch_bounds__(64 * kStrands) void decode_merge_fp4_kernel(DecodeArgs a) {
   constexpr int E = (D + 63) / 64;
@@ -256,11 +257,11 @@ __device__ __forceinline__ void combine_waves_fp4(const DecodeArgs& a, const Hea
 // its own address, clamped to the last valid row.
 //
 // The wave's K codes, and V codes two steps ahead, are in flight together (a wave has 10 KB
-// outstanding at D = 128, sixteen waves a CU).  Bound by the pool's bytes in large launches: 128 sequences
-// of 512 to 8192 tokens over 8 heads of 128, 610 MB of codes and scales (679 read), 142.5 us with the merge,
-// 4.3 TB/s, where a plain sum over an array reads 4.0 and the matrix pipe is busy 16 %; 64 of 128 to 2048
-// (78 MB) 23.9 us, 3.3 TB/s, by the workgroups' own chain (rows, codes, scores, softmax, sum), of which a CU
-// has a round and a half.
+// outstanding at D = 128).  114 registers at D = 128 and four heads leave four workgroups a CU, 24 of them
+// hold one scale byte each, and 40 of a wave's 80 pool loads fetch one.  128 sequences of 512 to 8192 tokens over 8
+// heads of 128, 610 MB of codes and scales (679 read), 142 us with the merge, 4.3 TB/s, where a large copy
+// moves 4.7, a pure read of paged blocks 5.8, and the matrix pipe is busy 16 %; 64 of 128 to 2048 (78 MB) 24 us, 3.3
+// TB/s, by the workgroups' own chain (rows, codes, scores, softmax, sum): 1328 of them with keys, 1024 at a time.
 template <int D, int T, int WT, bool QUAD>
 __global__ __launch_bounds__(kThreads, T == 1 ? 4 : 2) void decode_fp4_kernel(DecodeArgs a) {
   constexpr int kPartTokens = kWaves * WT;

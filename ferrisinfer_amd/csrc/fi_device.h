@@ -109,7 +109,8 @@ __device__ __forceinline__ float add(float a, float b) { return a + b; }
 __device__ __forceinline__ float4 add(float4 a, float4 b) { return make_float4(a.x + b.x, a.y + b.y, a.z + b.z, a.w + b.w); }
 
 // sum over z < splits of p[z * plane], added in split order; the split loads are issued in
-// batches of eight before their adds (one memory latency per batch)
+// batches of eight before their adds (one memory latency per batch; a batch's loads past the last
+// split read split 0 and are dropped)
 template <typename T>
 __device__ __forceinline__ T sum_splits(const T* __restrict__ p, size_t plane, int splits) {
   T x = p[0];

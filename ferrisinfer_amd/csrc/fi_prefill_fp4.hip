@@ -402,10 +402,11 @@ int32_t launch_dim(fi_context* ctx, const PrefillArgs& args_in) {
   // chunks is the block tables' width less half of the new rows, the mean over a sequence's tiles (500 rows
   // after none over 14/2 heads of 64, tiles of one to eight chunks: 17.9 us with the longer ones cut, 14.6
   // whole).  32/8 heads of 128, us cut against whole: 64 rows after 1000 cached 20.9 against 44, after 4000 33 against
-  // 124, after 16000 60 against 468.  Where the launch has a workgroup for half the CUs without them, eight
+  // 124, after 16000 59 against 468.  Where the launch has a workgroup for half the CUs without them, eight
   // chunks: the partials' way through memory costs a range 3 us (300 rows after 8000 112 against 246, 300
-  // after 2000 50 and with sixteen chunks 59, 500 after 500 36 and with six 45; 1000 after 4000, two workgroups a
-  // CU without splits, 194 against 188).
+  // after 2000 50 and with sixteen chunks 59, four sequences of 100 after up to 4000 67 and with sixteen 80, but of
+  // 100 after up to 1000 43 and with sixteen 40, 500 after 500 36 and with six 45; 1000 after 4000, two workgroups
+  // a CU without splits, 194 against 188).
   const int64_t cus = ctx->compute_units > 0 ? ctx->compute_units : 256;
   const int64_t wgs = static_cast<int64_t>((args.max_query_len + qt - 1) / qt) * args.num_seqs * args.hkv;
   const int64_t chunks = (static_cast<int64_t>(args.max_blocks) * args.block_size + kChunk - 1) / kChunk -

@@ -51,10 +51,13 @@ __device__ __forceinline__ size_t table_row(const fi::QkvNormArgs& a, int t, uin
 
 // One workgroup = ROWS * kThreads / LPR head rows of one token: the token's slot, block and positions are
 // uniform, and a thread's ROWS rows (the same elements of heads kThreads / LPR apart) share its
-// weights, cosines and sines.  Every load is issued before the first is waited for, but for the table
-// rows, which wait for the positions: the chain of dependent loads, not the arithmetic, bounds this.
-// 2048 tokens of 32 + 16 heads of 128 (one split, three axes, norms, bf16 pool; 92 MB) 25.7 us, 3.6 TB/s;
-// 64 tokens of four splits 4.9 us, one token of 14 + 4 heads of 64 and seven splits 3.2 us.
+// weights, cosines and sines.  With one split every load is issued before the first is waited for, but for the
+// table rows, which wait for the positions; several splits are loaded after the table rows, eight at a time
+// (fi::sum_splits), one latency more.  The chain of dependent loads, not the arithmetic, bounds this.
+// 2048 tokens of 32 + 16 heads of 128 (one split, three axes, norms, bf16 pool; 92 MB) 25.7 us, 3.6 TB/s (80
+// registers with six rows: 1536 of its 2048 workgroups run at a time), into a 4-bit pool (86 MB) 26.3;
+// 64 tokens of four splits 4.9 us (4-bit pool: 4.8, without norms 4.5), one token of 14 + 4 heads of 64 and seven
+// splits 3.2 us (4-bit pool 3.8).
 template <int D, typename Pool, int ROWS>
 __global__ __launch_bounds__(kThreads) void qkv_norm_rope_append_kernel(fi::QkvNormArgs a) {
   constexpr int LPR = D / 4;            // lanes per head row
