@@ -36,6 +36,19 @@ def test_decoder_step_refuses_positions_of_other_rows(pair_axes, positions, slot
     assert e.value.kind == "InvalidShape"
 
 
+@pytest.mark.parametrize("pair_axes,positions,slots", [(None, (T,), T), (None, (T,), T + 3), (None, (1, T), T),
+                                                       ([0, 1, 2, 0], (3, T), T), ([0, 0, 0, 0], (T,), T)])
+def test_decoder_step_takes_positions_of_its_rows(pair_axes, positions, slots):
+    dec = object.__new__(Bf16Decoder)
+    dec.ctx, dec.cfg, dec.max_tokens, dec.pair_axes, dec.layers = None, {}, 64, pair_axes, []
+    batch = StepBatch(positions=ints(*positions), slot_mapping=torch.zeros(slots, dtype=torch.int64), num_decode=T,
+                      dec_block_tables=None, dec_context_lens=None, dec_max_context=0, pf_block_tables=None,
+                      pf_cu_seqlens=None, pf_context_lens=None, pf_max_query=0, last_rows=None)
+    with pytest.raises(FerrisError) as e:  # the next check: a decoder without layers
+        dec.step(torch.zeros(T, 4), batch)
+    assert e.value.kind != "InvalidShape" and "layers" in e.value.message
+
+
 def context():
     """A context without a device: what reaches the library is refused there as InvalidConfig."""
     ctx = object.__new__(kernel.Context)
