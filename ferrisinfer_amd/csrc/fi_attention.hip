@@ -1192,7 +1192,7 @@ int32_t fi_attn_decode_paged_qkv(fi_context* ctx, const float* d_qkv_parts, int3
   const int part_tokens = kWaves * wave_tokens_for(num_kv_heads, head_dim);
   const int64_t parts = max_context_len == 0 ? 1 : (max_context_len + part_tokens - 1) / part_tokens;
   const int64_t cus = ctx->compute_units > 0 ? ctx->compute_units : 256;
-  if (kv_dtype == FI_DTYPE_MXFP4 || static_cast<int64_t>(num_seqs) * num_kv_heads * parts > 6 * cus) {
+  if (num_seqs > 0 && (kv_dtype == FI_DTYPE_MXFP4 || static_cast<int64_t>(num_seqs) * num_kv_heads * parts > 6 * cus)) {
     FI_REQUIRE(d_q_out != nullptr, FI_ERR_INVALID_CONFIG, "fi_attn_decode_paged_qkv: null q_out");
     if (kv_dtype == FI_DTYPE_MXFP4)  // what the attention refuses is refused before rows are appended
       FI_TRY(decode_paged(ctx, d_q_out, d_k_cache, d_v_cache, kv_dtype, d_block_tables, max_blocks_per_seq,
