@@ -23,6 +23,9 @@ SOURCES = [
     "fi_qkv_norm.hip",
     "fi_prefill.hip",
     "fi_prefill_fp4.hip",
+    "fi_attn_tree.hip",
+    "fi_tree.hip",
+    "fi_verify.hip",
     "fi_ops.hip",
     "fi_gemm.hip",
     "fi_gemm_packed.hip",

@@ -18,6 +18,7 @@ enum : uint32_t {
   FI_FAULT_CONTEXT_RANGE = 1u << 5,     // decode attention: a context length beyond the partitions max_context_len sized
   FI_FAULT_QUERY_RANGE = 1u << 6,       // prefill attention: a query length beyond the tiles max_query_len sized
   FI_FAULT_POSITION_RANGE = 1u << 7,    // RoPE: a position outside the cos/sin table
+  FI_FAULT_TREE_RANGE = 1u << 8,        // drafted tokens: a parent not before its node, a path that does not rise
 };
 
 // Arrival counters a context holds for decode attention's in-kernel merge: launches with more

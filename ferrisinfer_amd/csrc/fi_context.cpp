@@ -385,6 +385,7 @@ int32_t fi_ctx_check_faults(fi_context* ctx) {
   if (bits & FI_FAULT_CONTEXT_RANGE) msg += " context length beyond max_context_len;";
   if (bits & FI_FAULT_QUERY_RANGE) msg += " query length beyond max_query_len (its rows past the tiles were not computed);";
   if (bits & FI_FAULT_POSITION_RANGE) msg += " position outside the RoPE table;";
+  if (bits & FI_FAULT_TREE_RANGE) msg += " draft parent not before its node, or path that does not rise through the tree;";
   return fi::set_error(FI_ERR_RUNTIME, msg);
 }
 

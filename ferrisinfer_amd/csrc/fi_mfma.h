@@ -1,0 +1,32 @@
+// Operands of the bf16 matrix products that the attention kernels share: register vectors, transposing
+// LDS reads, three-piece splits.
+#pragma once
+
+#include "fi_device.h"
+
+namespace {
+
+typedef float v4f __attribute__((ext_vector_type(4)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef float f32x8 __attribute__((ext_vector_type(8)));
+typedef short v4s __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) v4s lds_v4s;
+
+// ds_read_b64_tr_b16 at an LDS address (8-byte aligned)
+__device__ __forceinline__ v4s lds_read_tr16(const uint16_t* p) {
+  return __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s*)(p));
+}
+
+// An f32 operand as its three bf16 pieces (fi::split3_pk).
+__device__ __forceinline__ void split3(const f32x8& x, bf16x8 (&p)[3]) {
+  uint4 h, m, l;
+  fi::split3_pk(x[0], x[1], h.x, m.x, l.x);
+  fi::split3_pk(x[2], x[3], h.y, m.y, l.y);
+  fi::split3_pk(x[4], x[5], h.z, m.z, l.z);
+  fi::split3_pk(x[6], x[7], h.w, m.w, l.w);
+  p[0] = __builtin_bit_cast(bf16x8, h);
+  p[1] = __builtin_bit_cast(bf16x8, m);
+  p[2] = __builtin_bit_cast(bf16x8, l);
+}
+
+}  // namespace

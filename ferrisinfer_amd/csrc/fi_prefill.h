@@ -1,11 +1,12 @@
 // Varlen causal prefill attention over the paged pool: what the kernels of every pool type share
-// (launch arguments, tile order, grid, three-piece operands).
+// (launch arguments, tile order, grid).
 #pragma once
 
 #include <algorithm>
 
 #include "fi_common.h"
 #include "fi_device.h"
+#include "fi_mfma.h"
 
 namespace fi {
 
@@ -40,17 +41,6 @@ struct PrefillArgs {
 namespace {
 
 using fi::PrefillArgs;
-
-typedef float v4f __attribute__((ext_vector_type(4)));
-typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
-typedef float f32x8 __attribute__((ext_vector_type(8)));
-typedef short v4s __attribute__((ext_vector_type(4)));
-typedef __attribute__((address_space(3))) v4s lds_v4s;
-
-// ds_read_b64_tr_b16 at an LDS address (8-byte aligned)
-__device__ __forceinline__ v4s lds_read_tr16(const uint16_t* p) {
-  return __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s*)(p));
-}
 
 constexpr int kThreads = 256;
 constexpr int kRows = 64;     // (head, token) rows per workgroup
@@ -163,18 +153,6 @@ int32_t plan_tiles(fi_context* ctx, PrefillArgs& args, int qt, int kb, const cha
   }
   *grid = dim3(static_cast<unsigned>(wgs));
   return FI_OK;
-}
-
-// An f32 operand as its three bf16 pieces (fi::split3_pk).
-__device__ __forceinline__ void split3(const f32x8& x, bf16x8 (&p)[3]) {
-  uint4 h, m, l;
-  fi::split3_pk(x[0], x[1], h.x, m.x, l.x);
-  fi::split3_pk(x[2], x[3], h.y, m.y, l.y);
-  fi::split3_pk(x[4], x[5], h.z, m.z, l.z);
-  fi::split3_pk(x[6], x[7], h.w, m.w, l.w);
-  p[0] = __builtin_bit_cast(bf16x8, h);
-  p[1] = __builtin_bit_cast(bf16x8, m);
-  p[2] = __builtin_bit_cast(bf16x8, l);
 }
 
 }  // namespace

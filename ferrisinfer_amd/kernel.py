@@ -114,6 +114,13 @@ _SIGNATURES = {
     "fi_convert_f32_to_bf16": [_P, _P, C.c_int64, _P],
     "fi_sample_tokens": [_P, _P, _I32, _I32, _I32, _P, _P, _P, _P, _P, _P],
     "fi_sample_reserve": [_P, _I32, _I32],
+    "fi_tree_plan": [_P, _P, _P, _P, _I32, _I32, _I32, _P, _P],
+    "fi_attn_tree_paged": [_P, _P, _P, _P, _I32, _P, _I32, _P, _P, _P, _I32, _I32, _I32, _I32, _I32, _I32, _I32,
+                           _I32, _I32, _F32, _P],
+    "fi_verify_drafts": [_P, _P, _I32, _I32, _P, _P, _P, _I32, _I32, _P, _P, _I32, _I32, _P, _P, _I32, _P, _P, _P,
+                         _P],
+    "fi_kv_keep_path": [_P, C.POINTER(_P), C.POINTER(_P), _I32, _I32, _P, _I32, _P, _P, _P, _I32, _I32, _I32, _I32,
+                        _I32, _I32],
 }
 _RESTYPES = {"fi_ctx_stream": _P, "fi_last_error": C.c_char_p}
 
@@ -179,6 +186,35 @@ def check_slots(name, rows, slot_mapping) -> None:
     """A consumer of `rows` tokens reads a slot for each."""
     if slot_mapping is not None and not isinstance(slot_mapping, int) and slot_mapping.numel() < rows:
         raise FerrisError(3, f"{name}: {rows} positions need a slot each")
+
+
+def check_arrays(name, kind, **arrays) -> None:
+    """Arrays of a drafted step, (tensor, leading shape) each: of the element type that the kernels read, contiguous,
+    and at least as long as the rows they are read for."""
+    for what, (t, shape) in arrays.items():
+        if t is None or isinstance(t, int):
+            continue
+        if str(t.dtype) != "torch." + kind:
+            raise FerrisError(5, f"{name}: {what} must be {kind}, not {str(t.dtype)[6:]}")
+        if len(t.shape) < len(shape) or int(t.shape[0]) < shape[0] or tuple(t.shape[1:len(shape)]) != tuple(shape[1:]):
+            raise FerrisError(3, f"{name}: {what} must be of shape {list(shape)}, not {list(t.shape)}")
+        if not t.is_contiguous():
+            raise FerrisError(4, f"{name}: {what} must be contiguous")
+
+
+def check_logit_rows(name, what, t, rows, vocab) -> None:
+    """Rows of `vocab` f32 logits (probabilities), each contiguous, any row stride."""
+    if str(t.dtype) != "torch.float32":
+        raise FerrisError(5, f"{name}: {what} must be float32, not {str(t.dtype)[6:]}")
+    if len(t.shape) != 2 or int(t.shape[0]) < rows or int(t.shape[1]) != vocab:
+        raise FerrisError(3, f"{name}: {what} must be of shape {[rows, vocab]}, not {list(t.shape)}")
+    if vocab > 1 and int(t.stride(1)) != 1:
+        raise FerrisError(4, f"{name}: the rows of {what} must be contiguous")
+
+
+def row_stride(t) -> int:
+    """Elements from a row to the next (a tensor of one row may give any number for it)."""
+    return int(t.stride(0)) if int(t.shape[0]) > 1 else int(t.shape[1])
 
 
 def kv_pool_bytes(kv_dtype, num_blocks, block_size, num_kv_heads, head_dim) -> int:
@@ -537,6 +573,71 @@ class Context:
         """Room for sample_tokens to serve top_k above 1024 (up to the vocabulary) in calls of
         up to `rows` rows of `vocab` logits."""
         check(self.lib.fi_sample_reserve(self.handle, int(rows), int(vocab)))
+
+    # ---- drafted tokens ----
+
+    def tree_plan(self, parents, cu_seqlens, context_lens, max_query_len, mask_out, positions_out):
+        """Masks (int64 [T, words], the bits of uint64) and positions int32 [T] of the trees' nodes from their
+        parents int32 [T]."""
+        rows, seqs, words = int(parents.numel()), int(context_lens.numel()), int(mask_out.shape[1])
+        check_arrays("tree_plan", "int32", parents=(parents, (rows,)), cu_seqlens=(cu_seqlens, (seqs + 1,)),
+                     context_lens=(context_lens, (seqs,)), positions_out=(positions_out, (rows,)))
+        check_arrays("tree_plan", "int64", mask_out=(mask_out, (rows, words)))
+        check(self.lib.fi_tree_plan(self.handle, ptr(parents), ptr(cu_seqlens), ptr(context_lens), seqs,
+                                    int(max_query_len), words, ptr(mask_out), ptr(positions_out)))
+
+    def attn_tree_paged(self, q, k_cache, v_cache, kv_dtype, block_tables, cu_seqlens, context_lens, tree_mask,
+                        max_query_len, max_context_len, num_kv_heads, block_size, num_blocks, scale, out):
+        """Attention of the trees' rows q [T, Hq, D] over the cached prefixes and the nodes of their masks
+        (int64 [T, words])."""
+        t, num_q_heads, head_dim = (int(n) for n in q.shape)
+        seqs, words, blocks = int(context_lens.numel()), int(tree_mask.shape[1]), int(block_tables.shape[1])
+        check_arrays("attn_tree_paged", "float32", q=(q, (t, num_q_heads, head_dim)), out=(out, (t, num_q_heads, head_dim)))
+        check_arrays("attn_tree_paged", "int32", block_tables=(block_tables, (seqs, blocks)),
+                     cu_seqlens=(cu_seqlens, (seqs + 1,)), context_lens=(context_lens, (seqs,)))
+        check_arrays("attn_tree_paged", "int64", tree_mask=(tree_mask, (t, words)))
+        check(self.lib.fi_attn_tree_paged(self.handle, ptr(q), ptr(k_cache), ptr(v_cache), int(kv_dtype),
+                                          ptr(block_tables), blocks, ptr(cu_seqlens), ptr(context_lens), ptr(tree_mask),
+                                          words, seqs, int(max_query_len), int(max_context_len), num_q_heads,
+                                          int(num_kv_heads), head_dim, int(block_size), int(num_blocks), float(scale),
+                                          ptr(out)))
+
+    def verify_drafts(self, logits, tokens, parents, cu_seqlens, max_query_len, temperature, accept_u, pick_u,
+                      draft_probs, distinct, tokens_out, path_out, count_out, prob_out):
+        """Accepts drafted tokens against logits [T, vocab] (any row stride) and draws one more a sequence;
+        draft_probs [T, vocab] or None; tokens_out [B, max_path + 1], path_out [B, max_path]."""
+        name = "verify_drafts"
+        rows, vocab = (int(n) for n in logits.shape)
+        seqs, longest = int(temperature.numel()), int(path_out.shape[1])
+        check_logit_rows(name, "logits", logits, rows, vocab)
+        if draft_probs is not None:
+            check_logit_rows(name, "draft_probs", draft_probs, rows, vocab)
+        check_arrays(name, "int32", tokens=(tokens, (rows,)), parents=(parents, (rows,)), cu_seqlens=(cu_seqlens, (seqs + 1,)),
+                     tokens_out=(tokens_out, (seqs, longest + 1)), path_out=(path_out, (seqs, longest)),
+                     count_out=(count_out, (seqs,)))
+        check_arrays(name, "float32", temperature=(temperature, (seqs,)), accept_u=(accept_u, (rows,)),
+                     pick_u=(pick_u, (seqs,)), prob_out=(prob_out, (seqs,)))
+        check(self.lib.fi_verify_drafts(self.handle, ptr(logits), row_stride(logits), vocab, ptr(tokens), ptr(parents),
+                                        ptr(cu_seqlens), seqs, int(max_query_len), ptr(temperature), ptr(draft_probs),
+                                        0 if draft_probs is None else row_stride(draft_probs), 1 if distinct else 0,
+                                        ptr(accept_u), ptr(pick_u), longest, ptr(tokens_out), ptr(path_out),
+                                        ptr(count_out), ptr(prob_out)))
+
+    def kv_keep_path(self, k_caches, v_caches, kv_dtype, block_tables, cu_seqlens, context_lens, path, num_blocks,
+                     block_size, num_kv_heads, head_dim):
+        """Moves the rows of the accepted nodes path [B, max_path] behind each sequence's node 0, in every
+        layer's pools (two lists)."""
+        if len(k_caches) != len(v_caches):
+            raise FerrisError(3, "kv_keep_path: as many K pools as V pools")
+        seqs, longest = (int(n) for n in path.shape)
+        blocks = int(block_tables.shape[1])
+        check_arrays("kv_keep_path", "int32", block_tables=(block_tables, (seqs, blocks)), cu_seqlens=(cu_seqlens, (seqs + 1,)),
+                     context_lens=(context_lens, (seqs,)), path=(path, (seqs, longest)))
+        pools = _P * max(len(k_caches), 1)
+        check(self.lib.fi_kv_keep_path(self.handle, pools(*[ptr(t) for t in k_caches]), pools(*[ptr(t) for t in v_caches]),
+                                       len(k_caches), int(kv_dtype), ptr(block_tables), blocks, ptr(cu_seqlens),
+                                       ptr(context_lens), ptr(path), longest, seqs, int(num_blocks), int(block_size),
+                                       int(num_kv_heads), int(head_dim)))
 
     def convert_to_f32(self, src, src_dtype, rows, cols, transpose, dst):
         """dst (f32) = the widening of src, a [rows, cols] row-major tensor of src_dtype

@@ -587,6 +587,91 @@ int32_t fi_sample_tokens(fi_context* ctx, const float* d_logits, int32_t ld, int
  * beforehand.  Not during graph capture; a reallocation bumps fi_ctx_workspace_generation. */
 int32_t fi_sample_reserve(fi_context* ctx, int32_t rows, int32_t vocab);
 
+/* ---------------------------------------------------------------- drafted tokens
+ * A step that scores a tree of drafted tokens a sequence and keeps the path that the model would have
+ * taken.  No counterpart in the reference, whose sessions feed one sampled token a step
+ * (runtime/session.rs:246-262).
+ *
+ * The step's rows are packed as prefill's: sequence b's tree is the rows [cu_seqlens[b], cu_seqlens[b + 1]),
+ * node i of it row cu_seqlens[b] + i.  Node 0 is the sequence's last token, the others are drafted; a node's
+ * parent (its index in the tree) comes before it.  The nodes' K/V rows are appended in their order behind
+ * the cached prefix (fi_qkv_rope_append and its like): node i at position context_lens[b] - nodes + i of
+ * the block table.  A step is
+ *   fi_tree_plan, then in every layer the q|k|v consumer (positions from the plan) and fi_attn_tree_paged,
+ *   fi_verify_drafts on the logits of all rows, fi_kv_keep_path on all layers' pools;
+ * the sequence then has context_lens[b] - nodes + 1 + count[b] cached positions, and the last token of
+ * out_tokens is the next step's node 0.
+ * max_query_len (at most 1024, Unsupported otherwise) must bound every tree's nodes; rows of a longer tree
+ * past it are left as they were and reported as Runtime by fi_ctx_check_faults. */
+
+/* d_tree_mask[t] = the nodes that row t may attend, its ancestors and itself, as bits of its sequence's
+ * nodes (uint64 [T, mask_words], node j bit j % 64 of word j / 64); d_positions[t] = context_lens[b] - nodes +
+ * depth of the node.  d_parents int32 [T], -1 for node 0 (and any other node without a parent, which starts a
+ * tree of its own).  A parent that is not before its node counts as -1 and is reported as Runtime by
+ * fi_ctx_check_faults.  64 * mask_words must be at least max_query_len. */
+int32_t fi_tree_plan(fi_context* ctx, const int32_t* d_parents, const int32_t* d_cu_seqlens, const int32_t* d_context_lens,
+                     int32_t num_seqs, int32_t max_query_len, int32_t mask_words, uint64_t* d_tree_mask,
+                     int32_t* d_positions);
+
+/* Attention of the trees' rows over the paged pool: row t of sequence b attends the positions before
+ * context_lens[b] - nodes and those of the nodes whose bits d_tree_mask[t] has set (any mask, not only
+ * fi_tree_plan's; bits past the tree are ignored).  q/out f32 [T, Hq, D]; scores, softmax and sums are
+ * f32, and f32, bf16 and mxfp4 pools are attended in f32 accuracy; any number of query heads per KV head.  A row that
+ * sees no key is zero; K and V of a node that a row does not see do not reach it, whatever they hold.
+ * max_context_len must bound every context_lens entry (it sizes the grid); positions of a longer one past it
+ * are not attended, and it is reported as Runtime by fi_ctx_check_faults.  Keys are cut into parts by the launch's
+ * sizes and joined in order, so equal calls give equal bits.  head_dim 32, 64 or 128 and max_context_len up to
+ * 2^30 (Unsupported otherwise); q, out and the pools 16-byte aligned (InvalidLayout); scale positive and
+ * finite (InvalidConfig).  Uses the context workspace. */
+int32_t fi_attn_tree_paged(fi_context* ctx, const float* d_q, const void* d_k_cache, const void* d_v_cache, int32_t kv_dtype,
+                           const int32_t* d_block_tables, int32_t max_blocks_per_seq, const int32_t* d_cu_seqlens,
+                           const int32_t* d_context_lens, const uint64_t* d_tree_mask, int32_t mask_words, int32_t num_seqs,
+                           int32_t max_query_len, int32_t max_context_len, int32_t num_q_heads, int32_t num_kv_heads,
+                           int32_t head_dim, int32_t block_size, int32_t num_blocks, float scale, float* d_out);
+
+/* Walks each sequence's tree from node 0, accepting drafted tokens so that the emitted ones are distributed as
+ * sampling from the model's logits (d_logits f32 [T, ld], row t scores what follows node t) gives them.
+ * At a node with the distribution p = softmax(logits / max(temperature[b], 2^-23)), or all on the first of the
+ * largest logits where temperature[b] <= 0, its children are tried in order against the rest of p (at first
+ * rho = p):
+ *   d_draft_probs NULL (drafts that were not drawn: looked up, the draft's best): x is accepted when
+ *     accept_u * sum(rho) < rho(x), and rho(x) becomes 0 otherwise;
+ *   d_draft_probs f32 [T, draft_ld] (row t the distribution that node t's children were drawn from): x is
+ *     accepted when accept_u * c * q(x) < rho(x), c = sum(rho) / (1 - s), and rho becomes max(rho - c q, 0) otherwise; s is 0 when the children
+ *     were drawn independently and the sum of q over the earlier ones when they were drawn without
+ *     repetition (distinct != 0; a child behind s >= 1 is passed over).
+ * An accepted child is the next node; where none is, there is none, or max_path were accepted (the children
+ * of the last are not tried then), the last token is the first index whose running sum of rho passes pick_u * sum(rho) (rho = p where
+ * nothing is left; the last index with any for a pick_u of 1 or more).  d_accept_u f32 [T] (of the drafted nodes) and d_pick_u
+ * f32 [B] are uniform in [0, 1), and do not count where temperature[b] <= 0 (a child is accepted when it is the first of the
+ * largest).  Comparisons are decided in 64-bit accuracy.  Logits of -inf have no
+ * probability: mask them to sample from a top-k or top-p set.
+ * Outputs: d_out_tokens int32 [B, max_path + 1], the accepted tokens, then the last one, then -1; d_out_path
+ * int32 [B, max_path], the accepted nodes, then -1; d_out_count int32 [B], how many; d_out_prob f32 [B], the last
+ * token's probability under rho / sum(rho) (greedy: p's softmax at temperature 1).  A sequence without rows
+ * gets -1, 0 and 0.  Where a sampled row that decides holds NaN or +inf, or a row nothing but -inf, the walk ends without a last
+ * token (-1) and is reported as Runtime by fi_ctx_check_faults; so is a drafted token outside the vocabulary,
+ * which is passed over, and a parent that is not before its node.  vocab at most 1048576 (Unsupported otherwise);
+ * at most 65535 sequences.  Uses the context workspace. */
+int32_t fi_verify_drafts(fi_context* ctx, const float* d_logits, int32_t ld, int32_t vocab, const int32_t* d_tokens,
+                         const int32_t* d_parents, const int32_t* d_cu_seqlens, int32_t num_seqs, int32_t max_query_len,
+                         const float* d_temperature, const float* d_draft_probs, int32_t draft_ld, int32_t distinct,
+                         const float* d_accept_u, const float* d_pick_u, int32_t max_path, int32_t* d_out_tokens,
+                         int32_t* d_out_path, int32_t* d_out_count, float* d_out_prob);
+
+/* Moves the K/V rows of each sequence's accepted path to the positions behind its node 0, in num_layers pools of
+ * one shape in one launch (64 layers each): the row of node path[b][i] to position context_lens[b] - nodes + 1 + i.
+ * k_caches and v_caches are HOST arrays of device pointers, read during the call.  d_path int32 [B, max_path] as
+ * fi_verify_drafts writes it: nodes in rising order, ended by a negative entry or max_path; an entry that does
+ * not rise or is no node of the tree ends the path and is reported as Runtime by fi_ctx_check_faults, as is a block id
+ * outside the pool, whose rows stay.  Rows move as if all were read before any is written; other rows are left
+ * as they were.  The blocks of these positions must be the sequence's own (fi_kv_copy_blocks first where a
+ * block is shared). */
+int32_t fi_kv_keep_path(fi_context* ctx, void* const* k_caches, void* const* v_caches, int32_t num_layers, int32_t kv_dtype,
+                        const int32_t* d_block_tables, int32_t max_blocks_per_seq, const int32_t* d_cu_seqlens,
+                        const int32_t* d_context_lens, const int32_t* d_path, int32_t max_path, int32_t num_seqs,
+                        int32_t num_blocks, int32_t block_size, int32_t num_kv_heads, int32_t head_dim);
+
 /* ---------------------------------------------------------------- checkpoint import
  * d_dst = the f32 widening of d_src, a [rows, cols] row-major tensor of src_dtype (FI_DTYPE_F32,
  * _BF16 or _F16; rank-1 tensors as rows = 1); transpose != 0 writes the [cols, rows] transpose
