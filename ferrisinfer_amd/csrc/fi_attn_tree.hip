@@ -38,26 +38,26 @@ struct TreeArgs {
   const int* context_lens;   // [B]
   const uint64_t* mask;      // [T, words]
   float* out;                // [T, Hq, D]
-  float* part_acc;           // [B * max_query_len * Hq * parts, D]
-  float* part_ml;            // [.., 2]
+  // what a cut launch joins: each workgroup's unnormalised rows [pieces, 64, D], their reference points and
+  // sums [pieces, 64, 2], and each sequence's pieces (its first, its parts) for a join in a launch of its own
+  float* part_acc;
+  float* part_ml;
+  int2* plan;          // null: the last workgroup of a tile joins its parts
+  unsigned* counters;  // of them, one a tile: those that are done, zero between launches
   uint32_t* faults;
   int words, max_blocks, hq, hkv, group, block_size, num_blocks;
   int num_seqs, max_query_len, max_context_len;
-  int ntiles, parts, part_chunks;
+  int ntiles;      // tiles of a tree of max_query_len nodes
+  int slots;       // pieces of a cut launch, at most; 0: none is cut
+  int cus, least;  // the least chunks of a part
   float scale;
   fi::FastDiv by_block, by_group;
 };
 
-// The keys of a sequence that the launch reads (lengths past max_context_len are cut off there), and the
-// parts that they make: one at least, for rows without keys too.
+// The keys of a sequence that the launch reads: lengths past max_context_len are cut off there.
 __device__ __forceinline__ int key_end(const TreeArgs& a, const fi::TreeSpan& t) {
   return min(t.prefix + t.nodes, a.max_context_len);
 }
-template <int KB>
-__device__ __forceinline__ int key_parts(const TreeArgs& a, int kend) {
-  return max(1, (kend + KB * a.part_chunks - 1) / (KB * a.part_chunks));
-}
-
 // Whether a row sees no key at all: then it is zero, where a row whose scores are all -inf is NaN.
 __device__ __forceinline__ bool sees_nothing(const TreeArgs& a, const fi::TreeSpan& t, int kend, const uint64_t* mask) {
   if (t.prefix > 0) return false;
@@ -185,36 +185,165 @@ __device__ __forceinline__ v4f product(const bf16x8 (&x)[PLANES], const bf16x8 (
   return __builtin_amdgcn_mfma_f32_16x16x32_bf16(x[0], f[0], acc, 0, 0, 0);
 }
 
-// What a workgroup does: 64 rows of one (part, sequence, kv head), its chunks [c_lo, c_hi).
+// What a workgroup does: 64 rows of one (sequence, kv head), chunks [c_lo, c_hi) of its keys.
 struct Unit {
-  int seq, kvh, part, tile;
+  int seq, kvh, part, tile, nparts;
+  int piece;   // among the launch's
+  int tiles;   // of the sequence
   fi::TreeSpan t;
-  int nodes, kend, nparts, c_lo, c_hi;
+  int nodes, kend, c_lo, c_hi;
 };
 
-// False: nothing (the whole workgroup).  The tiles of a (part, sequence, kv head) run one after the other on one XCD
-// (workgroup L runs on XCD L % 8), whose L2 then holds the keys that they share.
+constexpr int kPlanned = kThreads;  // sequences of a planned launch, at most: a thread each
+
+struct PlanShared {
+  uint32_t key[kPlanned];  // chunks, then the place in the batch: the order of the sequences
+  int count[kPlanned];     // pieces a kv head
+  int sums[2][kThreads / 64][3];
+  int found[4];  // sequence, its first piece, parts, tiles
+};
+
+// Lane 63's combination of a wave's values (none below 0), in a scalar register.
+template <typename F>
+__device__ __forceinline__ int wave_combine(int v, F f) {
+  v = f(v, __builtin_amdgcn_update_dpp(0, v, 0x111, 0xf, 0xf, true));  // row_shr:1, 2, 4, 8
+  v = f(v, __builtin_amdgcn_update_dpp(0, v, 0x112, 0xf, 0xf, true));
+  v = f(v, __builtin_amdgcn_update_dpp(0, v, 0x114, 0xf, 0xf, true));
+  v = f(v, __builtin_amdgcn_update_dpp(0, v, 0x118, 0xf, 0xf, true));
+  v = f(v, __builtin_amdgcn_update_dpp(0, v, 0x142, 0xa, 0xf, false));  // row_bcast:15, 31
+  v = f(v, __builtin_amdgcn_update_dpp(0, v, 0x143, 0xc, 0xf, false));
+  return __builtin_amdgcn_readlane(v, 63);
+}
+__device__ __forceinline__ int add_int(int x, int y) { return x + y; }
+__device__ __forceinline__ int max_int(int x, int y) { return max(x, y); }
+
+// The launch's pieces, which every workgroup lays out for itself from the lengths, a thread a sequence.  Tiles that
+// fill the device are not cut: they are taken as they are, those of long sequences first, folded where they all
+// run at once, so that a CU gets a long one and a short one.  Otherwise, where the longest sequence's tile has more
+// chunks than a CU's share of them all, sequences are cut into parts of as few chunks as make no more pieces
+// than run at a time.
+// False: this workgroup has none.
 template <int KB>
 __device__ __forceinline__ bool find_unit(const TreeArgs& a, Unit& u) {
-  const int slot = blockIdx.x >> 3;
-  const int unit = slot / a.ntiles * 8 + (blockIdx.x & 7);
-  u.tile = slot % a.ntiles;
-  if (unit >= a.parts * a.num_seqs * a.hkv) return false;
-  u.kvh = unit % a.hkv;
-  u.seq = unit / a.hkv % a.num_seqs;
-  u.part = unit / a.hkv / a.num_seqs;
+  int at = blockIdx.x;  // the piece
+  u.piece = at;
+  u.part = 0;
+  u.nparts = 1;
+  int cut = 0x7fffffff;  // chunks of a part
+  auto chunks_of = [&](const fi::TreeSpan& t) { return max((key_end(a, t) + KB - 1) / KB, 1); };
+  auto tiles_of = [&](const fi::TreeSpan& t) { return (min(t.nodes, a.max_query_len) * a.group + kRows - 1) / kRows; };
+  if (a.num_seqs == 1 || a.num_seqs > kPlanned) {
+    u.kvh = at % a.hkv;
+    at /= a.hkv;
+    if (a.num_seqs == 1) {
+      u.seq = 0;
+      const fi::TreeSpan t = fi::tree_span(a.cu_seqlens, a.context_lens, 0);
+      const int chunks = chunks_of(t), tiles = max(tiles_of(t), 1), all = tiles * a.hkv;
+      if (a.slots > 0 && chunks > a.least) cut = max(a.least, (chunks + a.slots / all - 1) / max(a.slots / all, 1));
+      u.part = at / tiles;
+      u.tile = at - u.part * tiles;
+      u.nparts = (chunks + min(cut, chunks) - 1) / min(cut, chunks);
+      if (u.part >= u.nparts) return false;
+      if (a.plan && blockIdx.x == 0 && threadIdx.x == 0) a.plan[0] = make_int2(0, u.nparts);
+    } else {
+      u.tile = at % a.ntiles;
+      u.seq = at / a.ntiles;
+    }
+  } else {
+    __shared__ PlanShared sh;
+    const int tid = threadIdx.x, w = tid >> 6;
+    int chunks = 0, tiles = 0;
+    if (tid < a.num_seqs) {
+      const fi::TreeSpan t = fi::tree_span(a.cu_seqlens, a.context_lens, tid);
+      tiles = tiles_of(t);
+      chunks = tiles > 0 ? chunks_of(t) : 0;
+    }
+    // of the workgroup's threads: sums of x and y, the largest z
+    int turn = 0;
+    auto combine = [&](int& x, int& y, int& z) {
+      int(*sums)[3] = sh.sums[turn];
+      turn ^= 1;  // one barrier a turn: the one before last has been read
+      const int wx = wave_combine(x, add_int), wy = wave_combine(y, add_int), wz = wave_combine(z, max_int);
+      if ((tid & 63) == 0) {
+        sums[w][0] = wx;
+        sums[w][1] = wy;
+        sums[w][2] = wz;
+      }
+      __syncthreads();
+      x = y = z = 0;
+      for (int i = 0; i < kThreads / 64; ++i) {
+        x += sums[i][0];
+        y += sums[i][1];
+        z = max(z, sums[i][2]);
+      }
+      x = __builtin_amdgcn_readfirstlane(x);
+      y = __builtin_amdgcn_readfirstlane(y);
+      z = __builtin_amdgcn_readfirstlane(z);
+    };
+    // (a sequence counts for 2^22 chunks at most, which keeps the sum in 32 bits)
+    int all = tiles, work = static_cast<int>(min(static_cast<int64_t>(chunks) * tiles, int64_t{1} << 22)), longest = chunks;
+    combine(all, work, longest);
+    all *= a.hkv;
+    int pieces = all;
+    const float total = static_cast<float>(work) * a.hkv;
+    if (a.slots > all && static_cast<float>(longest) * a.cus > total) {
+      int want = max(a.least, static_cast<int>(total / a.slots));
+      for (int round = 0; round < 8 && want < longest; ++round) {
+        int n = tiles * ((chunks + want - 1) / want), none = 0, zero = 0;
+        combine(n, none, zero);
+        n *= a.hkv;
+        if (n <= a.slots) {
+          cut = want;
+          pieces = n;
+          break;
+        }
+        want = max(want + 1, static_cast<int>(static_cast<float>(want) * n / a.slots));
+      }
+    }
+    if (at >= pieces) return false;
+    if (cut >= longest && pieces <= 3 * a.cus && (at / a.cus) % 2 == 1) {  // folded: rows of a workgroup a CU
+      const int first = at / a.cus * a.cus;
+      at = first + min(a.cus, pieces - first) - 1 - (at - first);
+    }
+    u.kvh = at % a.hkv;
+    at /= a.hkv;
+    const uint32_t key = static_cast<uint32_t>(min(chunks, 0xffffff)) * kPlanned + (kPlanned - 1 - tid);
+    const int parts = cut >= longest ? min(chunks, 1) : (chunks + cut - 1) / cut, mine = tiles * parts;
+    sh.key[tid] = tid < a.num_seqs ? key : 0;
+    sh.count[tid] = mine;
+    __syncthreads();
+    int before = 0;  // pieces of the sequences that come first
+    for (int j = 0; j < a.num_seqs; j += 4) {
+      const uint4 k = *reinterpret_cast<const uint4*>(&sh.key[j]);
+      const int4 n = *reinterpret_cast<const int4*>(&sh.count[j]);
+      before += (k.x > key ? n.x : 0) + (k.y > key ? n.y : 0) + (k.z > key ? n.z : 0) + (k.w > key ? n.w : 0);
+    }
+    if (before <= at && at < before + mine) {
+      sh.found[0] = tid;
+      sh.found[1] = before;
+      sh.found[2] = parts;
+      sh.found[3] = tiles;
+    }
+    if (a.plan && blockIdx.x == 0 && tid < a.num_seqs) a.plan[tid] = make_int2(before, parts);
+    __syncthreads();
+    u.seq = __builtin_amdgcn_readfirstlane(sh.found[0]);
+    u.nparts = __builtin_amdgcn_readfirstlane(sh.found[2]);
+    const int n = __builtin_amdgcn_readfirstlane(sh.found[3]), place = at - __builtin_amdgcn_readfirstlane(sh.found[1]);
+    u.part = place / n;
+    u.tile = place - u.part * n;
+  }
   u.t = fi::tree_span(a.cu_seqlens, a.context_lens, u.seq);
   u.nodes = min(u.t.nodes, a.max_query_len);
   if (u.part == 0 && u.tile == 0 && u.kvh == 0 && threadIdx.x == 0) {
     if (u.t.nodes > a.max_query_len) atomicOr(a.faults, FI_FAULT_QUERY_RANGE);
     if (u.t.prefix + u.t.nodes > a.max_context_len) atomicOr(a.faults, FI_FAULT_CONTEXT_RANGE);
   }
-  if (u.tile * kRows >= u.nodes * a.group) return false;
+  u.tiles = tiles_of(u.t);
+  if (u.tile >= u.tiles) return false;
   u.kend = key_end(a, u.t);
-  u.nparts = key_parts<KB>(a, u.kend);
-  if (u.part >= u.nparts) return false;
-  u.c_lo = u.part * a.part_chunks;
-  u.c_hi = min(u.c_lo + a.part_chunks, (u.kend + KB - 1) / KB);
+  const int chunks = (u.kend + KB - 1) / KB;
+  u.c_lo = u.nparts > 1 ? u.part * cut : 0;
+  u.c_hi = u.nparts > 1 ? min(u.c_lo + cut, chunks) : chunks;
   return true;
 }
 
@@ -222,6 +351,116 @@ __device__ __forceinline__ bool find_unit(const TreeArgs& a, Unit& u) {
 template <int KB>
 __device__ __forceinline__ bool reaches(const Unit& u, int c) {
   return (c + 1) * KB > min(u.t.prefix, u.kend);
+}
+
+// ---- parts ----
+// A piece's partials, and the join of a tile's.  Where the last workgroup of a tile joins them, they are read by
+// another workgroup of the launch: device-coherent stores and loads (past the XCDs' private L2s), eight
+// bytes each.
+
+__device__ __forceinline__ void put2(float* p, float x, float y, bool coherent) {
+  const uint64_t v = static_cast<uint64_t>(__float_as_uint(x)) | (static_cast<uint64_t>(__float_as_uint(y)) << 32);
+  if (coherent)
+    __hip_atomic_store(reinterpret_cast<uint64_t*>(p), v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  else
+    *reinterpret_cast<uint64_t*>(p) = v;
+}
+template <bool COHERENT>
+__device__ __forceinline__ float2 get2(const float* p) {
+  uint64_t v;
+  if constexpr (COHERENT)
+    v = __hip_atomic_load(reinterpret_cast<const uint64_t*>(p), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  else
+    v = *reinterpret_cast<const uint64_t*>(p);
+  return make_float2(__uint_as_float(static_cast<uint32_t>(v)), __uint_as_float(static_cast<uint32_t>(v >> 32)));
+}
+
+// A lane's share of row r: O at d = 16 dt + 4 lk .. + 3; its reference point (a finite one where the sum is NaN,
+// which the join does not skip) and sum.
+template <int D>
+__device__ __forceinline__ void store_part(const TreeArgs& a, const Unit& u, int r, int lk, const v4f (&o)[D / 16], float m,
+                                           float sum) {
+  const bool coherent = a.plan == nullptr;
+  float* acc = a.part_acc + ((size_t)u.piece * kRows + r) * D + 4 * lk;
+#pragma unroll
+  for (int dt = 0; dt < D / 16; ++dt) {
+    put2(acc + 16 * dt, o[dt][0], o[dt][1], coherent);
+    put2(acc + 16 * dt + 2, o[dt][2], o[dt][3], coherent);
+  }
+  if (lk == 0) put2(a.part_ml + ((size_t)u.piece * kRows + r) * 2, m, sum, coherent);
+}
+
+// Row r's elements 4 dq .. + 3 of the tile whose parts are the pieces first + step * part, joined in part order, each
+// rescaled from its own reference point to the largest so far (a part without a key that the row sees carries
+// -inf and adds nothing), divided by the combined sum.
+template <int D, int ITEMS, bool COHERENT>
+__device__ __forceinline__ void join_parts(const TreeArgs& a, const fi::TreeSpan& t, int kvh, int tile, int first, int step,
+                                           int nparts, int from, int stride) {
+  constexpr int N = 16 / ITEMS < 8 ? 16 / ITEMS : 8, DQ = D / 4;  // N parts' loads are issued together
+  float mx[ITEMS], l[ITEMS];
+  float4 acc[ITEMS];
+#pragma unroll
+  for (int i = 0; i < ITEMS; ++i) {
+    mx[i] = -INFINITY;
+    l[i] = 0.0f;
+    acc[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+  }
+  for (int s0 = 0; s0 < nparts; s0 += N) {
+    float2 ml[N][ITEMS], lo[N][ITEMS], hi[N][ITEMS];
+#pragma unroll
+    for (int n = 0; n < N; ++n)
+#pragma unroll
+      for (int i = 0; i < ITEMS; ++i) {
+        const int idx = from + i * stride;
+        const size_t row = (size_t)(first + step * min(s0 + n, nparts - 1)) * kRows + idx / DQ;
+        ml[n][i] = get2<COHERENT>(a.part_ml + row * 2);
+        lo[n][i] = get2<COHERENT>(a.part_acc + row * D + 4 * (idx % DQ));
+        hi[n][i] = get2<COHERENT>(a.part_acc + row * D + 4 * (idx % DQ) + 2);
+      }
+#pragma unroll
+    for (int n = 0; n < N; ++n)
+#pragma unroll
+      for (int i = 0; i < ITEMS; ++i) {
+        if (s0 + n >= nparts || ml[n][i].x == -INFINITY) continue;
+        const float to = fmaxf(mx[i], ml[n][i].x);
+        const float old = __builtin_amdgcn_exp2f(mx[i] - to), now = __builtin_amdgcn_exp2f(ml[n][i].x - to);
+        mx[i] = to;
+        l[i] = l[i] * old + now * ml[n][i].y;
+        acc[i] = make_float4(acc[i].x * old + now * lo[n][i].x, acc[i].y * old + now * lo[n][i].y,
+                             acc[i].z * old + now * hi[n][i].x, acc[i].w * old + now * hi[n][i].y);
+      }
+  }
+#pragma unroll
+  for (int i = 0; i < ITEMS; ++i) {
+    const int idx = from + i * stride, r = tile * kRows + idx / DQ;
+    const int node = static_cast<int>(a.by_group.div(r)), head = kvh * a.group + (r - node * a.group);
+    if (node >= min(t.nodes, a.max_query_len)) continue;
+    // (several parts and no prefix: a tree longer than a part)
+    const float inv = l[i] == 0.0f && sees_nothing(a, t, key_end(a, t), a.mask + (size_t)(t.first + node) * a.words) ? 0.0f : 1.0f / l[i];
+    *reinterpret_cast<float4*>(a.out + ((size_t)(t.first + node) * a.hq + head) * D + 4 * (idx % DQ)) =
+        make_float4(acc[i].x * inv, acc[i].y * inv, acc[i].z * inv, acc[i].w * inv);
+  }
+}
+
+// The end of a workgroup of a cut tile where the launch joins by itself: the tile's last joins its parts.  Each
+// thread waits until its coherent stores have completed, so when the counter shows every part's arrival, every
+// partial can be read.  The last resets the counter for the next launch or graph replay.
+template <int D>
+__device__ __forceinline__ void join_last(const TreeArgs& a, const Unit& u) {
+  if (u.nparts <= 1 || a.plan != nullptr) return;  // workgroup-uniform
+  __shared__ int s_last;
+  __builtin_amdgcn_s_waitcnt(0);
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    unsigned* counter = a.counters + ((size_t)u.seq * a.ntiles + u.tile) * a.hkv + u.kvh;
+    const unsigned arrived = __hip_atomic_fetch_add(counter, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) + 1u;
+    s_last = arrived == static_cast<unsigned>(u.nparts);
+    if (s_last) __hip_atomic_store(counter, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  }
+  __syncthreads();
+  if (!s_last) return;
+  const int step = u.tiles * a.hkv;
+  join_parts<D, kRows * (D / 4) / kThreads, true>(a, u.t, u.kvh, u.tile, u.piece - u.part * step, step, u.nparts, threadIdx.x, kThreads);
 }
 
 // A lane's row: row li of its wave's sixteen, shared by four lanes (lk).
@@ -347,17 +586,12 @@ struct Row {
   __device__ __forceinline__ void finish(const TreeArgs& a, const Unit& u) {
     float sum = l + fi::lane_xor16(l, lane);
     sum += fi::lane_xor32(sum, lane);
-    const Place p = place(a, u);
-    if (!p.live) return;
     if (u.nparts > 1) {
-      const size_t at = (((size_t)u.seq * a.max_query_len + p.node) * a.hq + p.head) * a.parts + u.part;
-#pragma unroll
-      for (int dt = 0; dt < DT; ++dt)
-        *reinterpret_cast<float4*>(a.part_acc + at * D + 16 * dt + 4 * lk) = make_float4(o[dt][0], o[dt][1], o[dt][2], o[dt][3]);
-      // a NaN sum takes a finite point, which the merge does not skip
-      if (lk == 0) *reinterpret_cast<float2*>(a.part_ml + at * 2) = make_float2(sum != sum ? 0.f : m, sum);
+      store_part<D>(a, u, 16 * (threadIdx.x >> 6) + li, lk, o, sum != sum ? 0.f : m, sum);
       return;
     }
+    const Place p = place(a, u);
+    if (!p.live) return;
     const float inv = sum == 0.0f && sees_nothing(a, u.t, u.kend, a.mask + p.row * a.words) ? 0.0f : 1.0f / sum;
     float* out = a.out + p.index * D + 4 * lk;
 #pragma unroll
@@ -551,6 +785,7 @@ __global__ __launch_bounds__(kThreads, 3) void attn_tree_bf16_kernel(TreeArgs a)
   }
   if (bad_block) atomicOr(a.faults, FI_FAULT_BLOCK_RANGE);
   row.finish(a, u);
+  join_last<D>(a, u);
 }
 
 // ---- f32 and 4-bit pools: through registers, which convert them ----
@@ -667,53 +902,23 @@ __global__ __launch_bounds__(kThreads, D == 128 && POOL == FI_DTYPE_F32 ? 2 : 3)
   }
   if (bad_block) atomicOr(a.faults, FI_FAULT_BLOCK_RANGE);
   row.finish(a, u);
+  join_last<D>(a, u);
 }
 
-// One output row quad a thread: the partials of its row joined in part order, four loaded at a time, each
-// rescaled from its own reference point to the largest so far (a part without a key that the row sees
-// carries -inf and adds nothing), divided by the combined sum.
-template <int D, int KB>
-__global__ __launch_bounds__(kThreads) void tree_merge_kernel(TreeArgs a, int64_t quads) {
-  constexpr int N = 4;
-  const int64_t idx = (int64_t)blockIdx.x * kThreads + threadIdx.x;
-  if (idx >= quads) return;
-  const int64_t prow = idx / (D / 4);  // (sequence, node, head)
-  const int dq = static_cast<int>(idx % (D / 4));
-  const int64_t at_node = prow / a.hq;
-  const int head = static_cast<int>(prow - at_node * a.hq);
-  const int seq = static_cast<int>(at_node / a.max_query_len), node = static_cast<int>(at_node - (int64_t)seq * a.max_query_len);
-  const fi::TreeSpan t = fi::tree_span(a.cu_seqlens, a.context_lens, seq);
-  if (node >= t.nodes) return;
-  const int kend = key_end(a, t), nparts = key_parts<KB>(a, kend);
-  if (nparts <= 1) return;  // written by the launch before
-  const float* acc_at = a.part_acc + prow * a.parts * D + 4 * dq;
-  const float* ml_at = a.part_ml + prow * a.parts * 2;
-  float mx = -INFINITY, l = 0.0f;
-  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-  for (int s0 = 0; s0 < nparts; s0 += N) {
-    float2 ml[N];
-    float4 o[N];
-#pragma unroll
-    for (int i = 0; i < N; ++i) {
-      const int s = min(s0 + i, nparts - 1);
-      ml[i] = *reinterpret_cast<const float2*>(ml_at + 2 * s);
-      o[i] = *reinterpret_cast<const float4*>(acc_at + (size_t)s * D);
-    }
-#pragma unroll
-    for (int i = 0; i < N; ++i) {
-      if (s0 + i >= nparts || ml[i].x == -INFINITY) continue;
-      const float to = fmaxf(mx, ml[i].x);
-      const float old = __builtin_amdgcn_exp2f(mx - to), now = __builtin_amdgcn_exp2f(ml[i].x - to);
-      mx = to;
-      l = l * old + now * ml[i].y;
-      acc = make_float4(acc.x * old + now * o[i].x, acc.y * old + now * o[i].y, acc.z * old + now * o[i].z,
-                        acc.w * old + now * o[i].w);
-    }
+// The join in a launch of its own: 256 quads of a (sequence, tile, kv head) at a time.
+template <int D>
+__global__ __launch_bounds__(kThreads) void tree_join_kernel(TreeArgs a, int units) {
+  constexpr int BLOCKS = kRows * (D / 4) / kThreads;
+  for (int i = blockIdx.x; i < units * BLOCKS; i += gridDim.x) {
+    const int share = i % BLOCKS, kvh = i / BLOCKS % a.hkv;
+    const int tile = i / BLOCKS / a.hkv % a.ntiles, seq = i / BLOCKS / a.hkv / a.ntiles;
+    const int2 plan = a.plan[seq];
+    if (plan.y <= 1) continue;  // written by the launch before
+    const fi::TreeSpan t = fi::tree_span(a.cu_seqlens, a.context_lens, seq);
+    const int tiles = (min(t.nodes, a.max_query_len) * a.group + kRows - 1) / kRows;
+    if (tile >= tiles) continue;
+    join_parts<D, 1, false>(a, t, kvh, tile, (plan.x + tile) * a.hkv + kvh, tiles * a.hkv, plan.y, share * kThreads + threadIdx.x, 0);
   }
-  // (several parts and no prefix: a tree longer than a part)
-  const float inv = l == 0.0f && sees_nothing(a, t, kend, a.mask + (size_t)(t.first + node) * a.words) ? 0.0f : 1.0f / l;
-  *reinterpret_cast<float4*>(a.out + ((size_t)(t.first + node) * a.hq + head) * D + 4 * dq) =
-      make_float4(acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv);
 }
 
 template <int D, int POOL>
@@ -724,31 +929,42 @@ int32_t launch_tree(fi_context* ctx, TreeArgs& a) {
   FI_REQUIRE(rows < (1 << 30), FI_ERR_INVALID_SHAPE, "fi_attn_tree_paged: too many rows");
   a.ntiles = static_cast<int>((rows + kRows - 1) / kRows);
   const int64_t tiles = static_cast<int64_t>(a.num_seqs) * a.hkv * a.ntiles;
-  const int64_t chunks = std::max<int64_t>(1, (static_cast<int64_t>(a.max_context_len) + KB - 1) / KB);
-  const int64_t wanted = std::max<int64_t>(1, 8 * cus / tiles);
-  a.part_chunks = static_cast<int>(std::max<int64_t>(256 / KB, (chunks + wanted - 1) / wanted));
-  a.parts = static_cast<int>((chunks + a.part_chunks - 1) / a.part_chunks);
-  const int64_t units = static_cast<int64_t>(a.parts) * a.num_seqs * a.hkv;
-  const int64_t grid = (units + 7) / 8 * 8 * a.ntiles;
-  FI_REQUIRE(grid <= 0x7fffffff, FI_ERR_INVALID_SHAPE, "fi_attn_tree_paged: grid too large");
-  const int64_t prows = static_cast<int64_t>(a.num_seqs) * a.max_query_len * a.hq;
-  if (a.parts > 1) {
-    const size_t acc = static_cast<size_t>(prows) * a.parts * D * sizeof(float);
-    FI_TRY(fi::ensure_workspace(ctx, acc + static_cast<size_t>(prows) * a.parts * 2 * sizeof(float)));
+  FI_REQUIRE(tiles <= 0x7fffffff, FI_ERR_INVALID_SHAPE, "fi_attn_tree_paged: grid too large");
+  const int64_t chunks = (static_cast<int64_t>(a.max_context_len) + KB - 1) / KB;
+  a.cus = static_cast<int>(cus);
+  // Parts of four chunks and more (us with two, three and four: 8 sequences of 200 to 1000 tokens, 32/8 heads of 128,
+  // 29.4, 25.6, 25.2; 16 of 200 to 1500 over 14/2 heads of 64, f32, 24.1, 22.9, 21.1; one of 4000 25.2, 25.0, 23.4).
+  a.least = 4;
+  // Workgroups that run at a time: three a CU, two where f32 rows of 128 take the registers.  Launches of two tiles a CU
+  // are not cut (64 sequences of 128 to 2048: 80 us, cut into parts of 16 chunks 81 and the join).
+  const int64_t slots = (D == 128 && POOL == FI_DTYPE_F32 ? 2 : 3) * cus;
+  int64_t grid = tiles;
+  bool join = false;
+  if (a.num_seqs <= kPlanned && tiles < 2 * cus && chunks > a.least) {  // may be cut
+    a.slots = static_cast<int>(slots);
+    grid = slots;
+    const size_t acc = static_cast<size_t>(slots) * kRows * D * sizeof(float), ml = static_cast<size_t>(slots) * kRows * 2 * sizeof(float);
+    FI_TRY(fi::ensure_workspace(ctx, acc + ml + kPlanned * sizeof(int2)));
     a.part_acc = static_cast<float*>(ctx->workspace);
     a.part_ml = reinterpret_cast<float*>(static_cast<char*>(ctx->workspace) + acc);
+    // The last workgroup of a tile joins up to eight parts by itself; more take it longer than a launch of its own
+    // (one sequence of 4000 tokens, 16 parts: 38.3 us against 27.2; of 700, six parts: 18.6 against 20.1).
+    join = chunks > 8 * a.least;
+    if (join)
+      a.plan = reinterpret_cast<int2*>(static_cast<char*>(ctx->workspace) + acc + ml);
+    else
+      a.counters = ctx->d_merge_counters;  // a tile each: fewer than slots
   }
   if constexpr (POOL == FI_DTYPE_BF16)
     hipLaunchKernelGGL((attn_tree_bf16_kernel<D>), dim3(static_cast<unsigned>(grid)), dim3(kThreads), 0, ctx->stream, a);
   else
     hipLaunchKernelGGL((attn_tree_kernel<D, POOL>), dim3(static_cast<unsigned>(grid)), dim3(kThreads), 0, ctx->stream, a);
   FI_CHECK_LAUNCH("attn_tree_kernel");
-  if (a.parts > 1) {
-    const int64_t quads = prows * (D / 4);
-    FI_REQUIRE(quads / kThreads < 0x7fffffff, FI_ERR_INVALID_SHAPE, "fi_attn_tree_paged: too many rows");
-    hipLaunchKernelGGL((tree_merge_kernel<D, KB>), dim3(static_cast<unsigned>((quads + kThreads - 1) / kThreads)),
-                       dim3(kThreads), 0, ctx->stream, a, quads);
-    FI_CHECK_LAUNCH("tree_merge_kernel");
+  if (join) {
+    const int64_t blocks = std::min<int64_t>(tiles * (kRows * (D / 4) / kThreads), 8 * cus);
+    hipLaunchKernelGGL((tree_join_kernel<D>), dim3(static_cast<unsigned>(blocks)), dim3(kThreads), 0, ctx->stream, a,
+                       static_cast<int>(tiles));
+    FI_CHECK_LAUNCH("tree_join_kernel");
   }
   return FI_OK;
 }
