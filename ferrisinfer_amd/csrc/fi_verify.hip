@@ -10,22 +10,20 @@
 //     q' = q without the s of the earlier children where they are distinct); otherwise rho becomes
 //     max(rho - c q, 0).
 // max(max(p - a q, 0) - c q, 0) = max(p - (a + c) q, 0) for q, c >= 0, so rho is never stored: it is
-// max(p - a q, 0) with a number a, and each rejection that a further child follows costs one pass over the
-// two rows.  (A rejected child's rho is 0 from then on: it was below c q.  So taking it out of q as well
-// changes nothing.)  The token at the end is the first index at which the running sum of rho passes u Z.
+// max(p - a q, 0) with a number a, and each rejection costs one pass over the two rows.  (A rejected child's rho is 0
+// from then on: it was below c q.  So taking it out of q as well changes nothing.)  The token at the end is
+// the first index at which the running sum of rho passes u Z.
 //
 // Tokens are compared with u at borders that lie 1e-7 and less apart in a flat row, so what decides is in 64
-// bits: exponentials and sums to 1e-14.  The walk itself takes sums of f32 exponentials, with a bound on
-// their error, and repeats a node in 64 bits where a comparison falls within it (one in 30000).
+// bits: exponentials and sums to 1e-14.
 //
-// verify_walk_kernel walks, one workgroup a sequence: it reads the rows of the path's nodes that have
-// children.  verify_end_kernel draws the last token, one workgroup a (segment of a row, sequence): the
-// segments' sums, then the last workgroup of a sequence to finish finds the segment and the token in it.
-// The numbers a that the walk took rho by are off as its sums are, so the segments also sum what rho changes by
-// with a: f(a) = sum(max(w - a q, 0)) = f(a') - (a - a') sum(q where w > a' q) but for the elements whose w / q lies
-// between a' and a, 1e-7 apart, each of which is off by 1e-7 of a q.  From the exact sum of w the exact a's follow one
-// by one.
+// A workgroup reads a row at 50 GB/s at most, whatever it keeps in flight (12 us for 600 KB), so a row is split over
+// one workgroup a segment of 4096, and a walk goes from launch to launch: in each, a sequence's segments are summed
+// for the row that its walk is at, and the last workgroup to finish takes the walk on, to the next row or to
+// the end.  No workgroup waits for another.  The host knows how many launches a walk can need; those of
+// sequences that have ended are left at once.
 #include <algorithm>
+#include <type_traits>
 
 #include "fi_common.h"
 #include "fi_device.h"
@@ -46,35 +44,37 @@ struct VerifyArgs {
   int* out_path;             // [B, max_path]
   int* out_count;            // [B]
   float* out_prob;           // [B]
-  struct EndState* ends;     // [B]
-  struct SegmentSums* sums;  // [B, segments]
-  unsigned* counters;        // [B], zero between launches
+  struct Walk* walks;        // [B]
+  struct RowSums* sums;      // [B, segments] of the row that the walk is at, or [B * max_query_len, segments] of all
+  double* rests;             // [B, segments] of what is left of it
+  unsigned* counters;        // [B] (and [B * max_query_len] behind them, where all rows are summed), `apart` apart; zero between launches
   uint32_t* faults;
   int64_t ld, ld_probs;
   int vocab, distinct, max_path, max_query_len, segments;
+  int all_rows;  // sums are of all rows
+  int apart;
 };
 
-constexpr int kMaxSteps = 4;  // values of a that the end follows; past them the walk's are of 64 bits
-
-// The values of a at a node (times the sum of the weights w): a_1 = sum(w), a_(i + 1) = a_i + f(a_i) / room_(i + 1),
-// one each time a drawn token was rejected; only the last where they are exact.
-struct Offs {
-  int steps, exact;
-  double off[kMaxSteps], room[kMaxSteps];
+enum Phase : int {
+  kTotal,  // the row's sums are asked for
+  kRest,   // children were rejected: the sums of what is left
+  kDone,
 };
 
-// Where a sequence's walk ended.
-struct EndState {
-  int node;   // -1: nothing to draw
-  int count;  // tokens accepted
-  int tried;  // its children were tried and rejected
-  float ref;  // the reference point of the row's weights
-  Offs offs;
+// Where a sequence's walk is.
+struct Walk {
+  int node, count;  // the node; how many tokens are accepted
+  int phase;
+  int child;     // the last one rejected (tokens drawn)
+  float ref;     // the reference point of the row's weights
+  double total;  // their sum
+  double off, taken;  // a and s
 };
 
-// A row's weights are 2^(k (l - ref)): k = log2(e) / temperature, l the logit.
+// A row's weights are 2^(k l - c): k = log2(e) / temperature, l the logit, c = k times the reference point.  (c is one
+// rounded number for the whole row, so that its rounding is a common factor of them.)
 struct Weights {
-  double k, ref;
+  double k, c;
 };
 
 constexpr double kLog2E = 1.4426950408889634;
@@ -84,43 +84,80 @@ __device__ __forceinline__ double row_scale(float temperature) {
   return kLog2E / static_cast<double>(fmaxf(temperature, kMinTemperature));
 }
 
-// 2^x for x in [-1100, 1000]: 2^n times the series of e^(f ln 2), |f| <= 1/2; its twelfth term is 6e-15.
+// 2^x for x in [-1100, 1000]: 2^n times a polynomial in f, |f| <= 1/2, through 2^f at the eleven Chebyshev
+// points; it is within 3.2e-16 of 2^f.
 __device__ __forceinline__ double exp2_64(double x) {
-  constexpr double L = 0.69314718055994530942;
-  const double n = __builtin_rint(x), f = (x - n) * L;
-  double s = 1.0 / 39916800;
-  s = __builtin_fma(s, f, 1.0 / 3628800);
-  s = __builtin_fma(s, f, 1.0 / 362880);
-  s = __builtin_fma(s, f, 1.0 / 40320);
-  s = __builtin_fma(s, f, 1.0 / 5040);
-  s = __builtin_fma(s, f, 1.0 / 720);
-  s = __builtin_fma(s, f, 1.0 / 120);
-  s = __builtin_fma(s, f, 1.0 / 24);
-  s = __builtin_fma(s, f, 1.0 / 6);
-  s = __builtin_fma(s, f, 0.5);
-  s = __builtin_fma(s, f, 1.0);
+  const double n = __builtin_rint(x), f = x - n;
+  double s = 7.072585949269223e-09;
+  s = __builtin_fma(s, f, 1.0208690299958306e-07);
+  s = __builtin_fma(s, f, 1.321544258792169e-06);
+  s = __builtin_fma(s, f, 1.5252657260200837e-05);
+  s = __builtin_fma(s, f, 0.0001540353044173605);
+  s = __builtin_fma(s, f, 0.0013333558230164974);
+  s = __builtin_fma(s, f, 0.009618129107606888);
+  s = __builtin_fma(s, f, 0.05550410866444772);
+  s = __builtin_fma(s, f, 0.24022650695910097);
+  s = __builtin_fma(s, f, 0.69314718055995);
   s = __builtin_fma(s, f, 1.0);
   return __builtin_ldexp(s, static_cast<int>(n));
 }
 
-// A logit's weight; one of -inf (and, where k is 0, NaN from it) weighs nothing.
+// A logit's weight, by a reference point that no logit of the row passes; one of -inf (and, where k is 0, NaN from
+// it) weighs nothing.
 __device__ __forceinline__ double weight(double l, const Weights& w) {
-  return exp2_64(__builtin_fmin(__builtin_fmax((l - w.ref) * w.k, -1100.0), 1000.0));
+  return exp2_64(__builtin_fmax(__builtin_fma(l, w.k, -w.c), -1100.0));
 }
 
-// What weights by `from` are multiplied with to be weights by `to`.
+// What weights by `from` are multiplied with to be weights by `to`, which is no less.
 __device__ __forceinline__ double change_of_ref(double k, float from, float to) {
-  return exp2_64(__builtin_fmin(__builtin_fmax((static_cast<double>(from) - to) * k, -1100.0), 1000.0));
+#pragma clang fp contract(off)  // the difference of the two c, as they are
+  const double c_from = k * from, c_to = k * to;
+  return exp2_64(__builtin_fmax(c_from - c_to, -1100.0));
 }
 
 __device__ __forceinline__ float finite_or_zero(float x) { return fabsf(x) <= 3.402823466e38f ? x : 0.0f; }
 
 __device__ __forceinline__ bool unusable(float l) { return !(l <= 3.402823466e38f); }  // NaN or +inf
 
-__device__ __forceinline__ double wave_sum64(double v) {
-#pragma unroll
-  for (int m = 32; m >= 1; m >>= 1) v += __shfl_xor(v, m, 64);
+// What another lane holds, or `otherwise`, on the vector pipe (a shuffle is an LDS round trip).
+template <int kCtrl, int kRows>
+__device__ __forceinline__ int from_lane(int v, int otherwise) {
+  return __builtin_amdgcn_update_dpp(otherwise, v, kCtrl, kRows, 0xf, false);
+}
+// f over the lanes up to each one, in order, and so over the wave in its last: within rows of 16 lanes (row_shr:1, 2, 4, 8),
+// then a row's last to the next (row_bcast:15) and the half's last to the next half (:31).
+template <typename F>
+__device__ __forceinline__ void up_the_wave(F f) {
+  f(std::integral_constant<int, 0x111>{}, std::integral_constant<int, 0xf>{});
+  f(std::integral_constant<int, 0x112>{}, std::integral_constant<int, 0xf>{});
+  f(std::integral_constant<int, 0x114>{}, std::integral_constant<int, 0xf>{});
+  f(std::integral_constant<int, 0x118>{}, std::integral_constant<int, 0xf>{});
+  f(std::integral_constant<int, 0x142>{}, std::integral_constant<int, 0xa>{});
+  f(std::integral_constant<int, 0x143>{}, std::integral_constant<int, 0xc>{});
+}
+__device__ __forceinline__ double wave_scan64(double v) {
+  up_the_wave([&](auto ctrl, auto rows) {
+    const int2 x = __builtin_bit_cast(int2, v);
+    v += __builtin_bit_cast(double, make_int2(from_lane<ctrl.value, rows.value>(x.x, 0), from_lane<ctrl.value, rows.value>(x.y, 0)));
+  });
   return v;
+}
+__device__ __forceinline__ double wave_sum64(double v) {
+  const int2 x = __builtin_bit_cast(int2, wave_scan64(v));
+  return __builtin_bit_cast(double, make_int2(__builtin_amdgcn_readlane(x.x, 63), __builtin_amdgcn_readlane(x.y, 63)));
+}
+__device__ __forceinline__ float wave_top(float v) {
+  up_the_wave([&](auto ctrl, auto rows) {
+    const int x = __builtin_bit_cast(int, v);
+    v = fmaxf(v, __builtin_bit_cast(float, from_lane<ctrl.value, rows.value>(x, x)));
+  });
+  return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), 63));
+}
+// The least of the wave's indexes whose value is the wave's largest.
+__device__ __forceinline__ int first_of(float value, float top, int index) {
+  int at = value == top ? index : 0x7fffffff;
+  up_the_wave([&](auto ctrl, auto rows) { at = min(at, from_lane<ctrl.value, rows.value>(at, at)); });
+  return __builtin_amdgcn_readlane(at, 63);
 }
 
 // Four logits (probabilities) from `at` on, those past the row's end as `pad`; VEC: rows of whole,
@@ -135,139 +172,231 @@ __device__ __forceinline__ float4 quad_at(const float* __restrict__ row, int at,
   }
 }
 
-// ---------------------------------------------------------------- the walk
+// ---------------------------------------------------------------- segments of a row
 
-constexpr int kWalkThreads = 512;
-constexpr int kWalkWaves = kWalkThreads / 64;
-constexpr int kAhead = 4;  // quads of a row that a lane has in flight
+constexpr int kEndThreads = 256;
+constexpr int kEndElems = 16;                          // consecutive elements a thread
+constexpr int kSegment = kEndThreads * kEndElems;      // 4096
+constexpr int kMaxSegments = 256;                      // a thread each when they are joined
+constexpr int kMaxVocab = kSegment * kMaxSegments;     // 1048576
 
-// What a wave finds in its part of a row.
-struct PartStats {
-  double sum;  // of the weights by the point k * ref
-  float ref, top;
-  int first;  // the index of the first logit of value top
-  int bad;    // a logit that is NaN or +inf, or (fast sums) nothing that can be relied on
+constexpr int64_t kAllRows = 20000000;  // logits up to which every row is summed in the first launch
+constexpr int kRejections = 4;          // launches for rejected drawn children
+
+// Of a segment: the weights' sum by its maximum (by 0 where that is not finite; NaN if there is a logit that is NaN or
+// +inf), the maximum and its first index.
+struct alignas(16) RowSums {
+  double sum;
+  float top;
+  int first;
 };
 
-struct WalkShared {
-  int tokens[fi::kMaxTreeNodes];
-  int parents[fi::kMaxTreeNodes];
-  float accept[fi::kMaxTreeNodes];
+struct SegmentShared {
+  double scan[kEndThreads / 64];
+  float tops[kEndThreads / 64];
+  int firsts[kEndThreads / 64];
+};
+
+// The workgroup's maximum; its first index too, if that is asked for.
+__device__ __forceinline__ void segment_top(SegmentShared& sh, float& top, int& first, bool index) {
+  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+  const float wave = wave_top(top);
+  const int at = index ? first_of(top, wave, first) : 0;
+  __syncthreads();  // the last use is over
+  if (lane == 0) {
+    sh.tops[w] = wave;
+    sh.firsts[w] = at;
+  }
+  __syncthreads();
+  top = -INFINITY;
+  first = 0x7fffffff;
+  for (int i = 0; i < kEndThreads / 64; ++i)
+    if (sh.tops[i] > top) {
+      top = sh.tops[i];
+      first = sh.firsts[i];
+    }
+}
+// The workgroup's sum of x.
+__device__ __forceinline__ double segment_sum(SegmentShared& sh, double x) {
+  x = wave_sum64(x);
+  __syncthreads();  // the last use is over
+  if ((threadIdx.x & 63) == 0) sh.scan[threadIdx.x >> 6] = x;
+  __syncthreads();
+  double all = 0.0;
+  for (int i = 0; i < kEndThreads / 64; ++i) all += sh.scan[i];
+  return all;
+}
+
+// A thread's 16 elements of a segment: quads 256 apart (whole lines a wave), or one behind the other (in order).
+template <bool VEC, bool IN_ORDER>
+__device__ __forceinline__ void segment_load(const float* __restrict__ row, int begin, int vocab, float pad, float (&v)[kEndElems]) {
+#pragma unroll
+  for (int j = 0; j < kEndElems / 4; ++j) {
+    const float4 x = quad_at<VEC>(row, begin + (IN_ORDER ? threadIdx.x * kEndElems + 4 * j : 4 * threadIdx.x + 4 * kEndThreads * j), vocab, pad);
+    v[4 * j] = x.x;
+    v[4 * j + 1] = x.y;
+    v[4 * j + 2] = x.z;
+    v[4 * j + 3] = x.w;
+  }
+}
+// The place in the segment of a thread's element e, as they are loaded out of order.
+__device__ __forceinline__ int element_at(int e) { return 4 * threadIdx.x + 4 * kEndThreads * (e / 4) + e % 4; }
+
+// ---------------------------------------------------------------- a launch's part
+
+struct VerifyShared {
+  SegmentShared seg;
+  uint32_t out[kSegment / 32];            // tokens given and rejected
   uint64_t kids[fi::kMaxTreeNodes / 64];  // the node's children, as bits
-  PartStats parts[kWalkWaves];
-  double rest[kWalkWaves];
+  int tokens[fi::kMaxTreeNodes];
+  float accept[fi::kMaxTreeNodes];
+  float probs[fi::kMaxTreeNodes];
+  double mass[fi::kMaxTreeNodes];  // weights of the children's tokens
+  int last;
 };
 
-// The fast sums' error, relative to the sum.  A term's exponent t = (l - ref) k is off by three roundings, its value
-// by ln 2 * 3 * 2^-24 |t| + 2^-23 of itself.  The maximum lies within 40 of the reference point, so that |t| <= 80 (1.0e-5)
-// for all but terms below 2^-40 of the largest, a million of which are worth 1e-6.  A lane adds 16 terms in f32
-// (2^-20), the rest in f64.  Together below 2^-16.
-constexpr double kFastError = 1.52587890625e-5;
-
-// One pass of a wave over row[begin, end): maximum, its first index and, unless GREEDY, the weights' sum by a reference
-// point from the first quads of the part.  That serves as long as the maximum lies within 900 (fast: 40) binary
-// orders of it; a part where it does not is summed again by its maximum.
-template <bool VEC, bool FAST, bool GREEDY>
-__device__ __forceinline__ PartStats part_stats(const float* __restrict__ row, int begin, int end, double k, int lane) {
-  PartStats r{0.0, 0.0f, -INFINITY, 0x7fffffff, 0};
-  const float k32 = static_cast<float>(k);
-  for (int round = 0; round < 2; ++round) {
-    float ref = r.top, top = -INFINITY;
-    int first = 0x7fffffff;
-    double sum = 0.0;
-    bool bad = false;
-    for (int at0 = begin + 4 * lane; at0 - 4 * lane < end; at0 += 256 * kAhead) {  // wave-uniform
-      float4 x[kAhead];
-#pragma unroll
-      for (int j = 0; j < kAhead; ++j) x[j] = quad_at<VEC>(row, at0 + 256 * j < end ? at0 + 256 * j : 0x7ffffff0, end, -INFINITY);
-      if (!GREEDY && round == 0 && at0 - 4 * lane == begin) {
-        float m = -INFINITY;
-#pragma unroll
-        for (int j = 0; j < kAhead; ++j) m = fmaxf(m, fmaxf(fmaxf(x[j].x, x[j].y), fmaxf(x[j].z, x[j].w)));
-        ref = fi::wave_max(m);
-        if (!(fabsf(ref) <= 3.402823466e38f)) ref = 0.0f;
-      }
-      const Weights w{k, ref};
-      float quick = 0.0f;
-#pragma unroll
-      for (int j = 0; j < kAhead; ++j) {
-        const float v[4] = {x[j].x, x[j].y, x[j].z, x[j].w};
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          if (v[e] > top) {
-            top = v[e];
-            first = at0 + 256 * j + e;
-          }
-          if constexpr (!GREEDY) {
-            if constexpr (FAST) {
-              quick += __builtin_amdgcn_exp2f((v[e] - ref) * k32);
-            } else {
-              bad |= unusable(v[e]);
-              sum += weight(v[e], w);
-            }
-          }
-        }
-      }
-      if constexpr (FAST && !GREEDY) sum += quick;
-    }
-    const float wave_top = fi::wave_max(top);
-    int at = top == wave_top ? first : 0x7fffffff;
-#pragma unroll
-    for (int m = 32; m >= 1; m >>= 1) at = min(at, __shfl_xor(at, m, 64));
-    r.top = wave_top;
-    r.first = at;
-    r.ref = ref;
-    if constexpr (GREEDY) return r;
-    r.sum = wave_sum64(sum);
-    const bool over = wave_top != -INFINITY && __builtin_fabs((static_cast<double>(wave_top) - ref) * k) > (FAST ? 40.0 : 900.0);
-    r.bad = __builtin_amdgcn_ballot_w64(bad) != 0 || !(r.sum <= 1.7976931348623157e308);
-    if (!over || unusable(wave_top)) return r;
-  }
-  return r;
+template <typename T>
+__device__ __forceinline__ void put(T* to, T x) {  // for another workgroup of this launch
+  __hip_atomic_store(to, x, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+template <typename T>
+__device__ __forceinline__ T get(T* from) {
+  return __hip_atomic_load(from, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
 }
 
-// sum of max(weight - off * q, 0) over a wave's part of the rows
-template <bool VEC, bool FAST>
-__device__ __forceinline__ double part_rest(const float* __restrict__ row, const float* __restrict__ probs, int begin, int end,
-                                            const Weights& w, double off, int lane) {
+// A sequence: its nodes, its row scale, its outputs.
+struct Sequence {
+  int index, first, n;
+  bool greedy;
+  double k;
+};
+
+__device__ __forceinline__ Sequence sequence_of(const VerifyArgs& a, int index) {
+  const fi::TreeSpan t = fi::tree_span(a.cu_seqlens, nullptr, index);
+  const float temperature = a.temperature[index];
+  const bool greedy = temperature <= 0.0f;
+  return Sequence{index, t.first, min(t.nodes, a.max_query_len), greedy, greedy ? kLog2E : row_scale(temperature)};
+}
+
+// A node, and its token's logit and draft probability where it is a child of the node that the walk is at.
+struct Node {
+  int parent, token;
+  float accept, logit, prob;
+  bool child;
+};
+
+__device__ __forceinline__ Node node_at(const VerifyArgs& a, const Sequence& s, int j) {
+  Node x{-2, -1, 0.0f, 0.0f, 0.0f, false};
+  if (j < s.n) {
+    x.parent = a.parents[s.first + j];
+    x.token = a.tokens[s.first + j];
+    x.accept = a.accept_u[s.first + j];
+  }
+  return x;
+}
+__device__ __forceinline__ void look_up(const VerifyArgs& a, const Sequence& s, int node, int j, Node& x) {
+  x.child = j > node && x.parent == node && x.token >= 0 && x.token < a.vocab;  // (no token: as if it were not there)
+  if (x.child && !s.greedy) {
+    x.logit = a.logits[(int64_t)(s.first + node) * a.ld + x.token];
+    if (a.probs) x.prob = a.probs[(int64_t)(s.first + node) * a.ld_probs + x.token];
+  }
+}
+
+// Marks the tokens of a segment that were tried (tokens given, and rejected).
+__device__ __forceinline__ void mark_tried(const VerifyArgs& a, VerifyShared& sh, const Sequence& q, int node, int begin) {
+  __syncthreads();
+  for (int i = threadIdx.x; i < kSegment / 32; i += kEndThreads) sh.out[i] = 0;
+  __syncthreads();
+  for (int j = node + 1 + threadIdx.x; j < q.n; j += kEndThreads) {
+    const int x = a.tokens[q.first + j];
+    if (a.parents[q.first + j] == node && x >= begin && x < min(begin + kSegment, a.vocab))
+      atomicOr(&sh.out[(x - begin) >> 5], 1u << ((x - begin) & 31));
+  }
+  __syncthreads();
+}
+__device__ __forceinline__ bool was_tried(const VerifyShared& sh, int e) { return ((sh.out[e >> 5] >> (e & 31)) & 1) != 0; }
+
+// The sums of a segment that the walk asks for; thread 0 stores them.  Meanwhile the thread's node is looked up, as a child of
+// node `from`: only the last workgroup needs it, but that then waits for nothing.
+template <bool VEC>
+__device__ __forceinline__ void sum_segment(const VerifyArgs& a, VerifyShared& sh, const Sequence& s, const Walk& walk, int segment,
+                                            int from, Node& mine) {
+  const int begin = segment * kSegment;
+  const bool less = walk.phase == kRest && a.probs;
+  float v[kEndElems], q[kEndElems];
+  segment_load<VEC, false>(a.logits + (int64_t)(s.first + walk.node) * a.ld, begin, a.vocab, -INFINITY, v);
+  if (less) segment_load<VEC, false>(a.probs + (int64_t)(s.first + walk.node) * a.ld_probs, begin, a.vocab, 0.0f, q);
+  mine = node_at(a, s, threadIdx.x);
+  look_up(a, s, from, threadIdx.x, mine);
   double sum = 0.0;
-  const float k32 = static_cast<float>(w.k), off32 = static_cast<float>(off), ref32 = static_cast<float>(w.ref);
-  for (int at0 = begin + 4 * lane; at0 - 4 * lane < end; at0 += 256 * kAhead) {
-    float4 x[kAhead], q[kAhead];
+  if (less) {
+    const Weights by{s.k, s.k * walk.ref};
 #pragma unroll
-    for (int j = 0; j < kAhead; ++j) {
-      const int at = at0 + 256 * j < end ? at0 + 256 * j : 0x7ffffff0;
-      x[j] = quad_at<VEC>(row, at, end, -INFINITY);
-      q[j] = quad_at<VEC>(probs, at, end, 0.0f);
-    }
-    float quick = 0.0f;
-#pragma unroll
-    for (int j = 0; j < kAhead; ++j) {
-      const float v[4] = {x[j].x, x[j].y, x[j].z, x[j].w}, p[4] = {q[j].x, q[j].y, q[j].z, q[j].w};
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        if constexpr (FAST)
-          quick += fmaxf(__builtin_amdgcn_exp2f((v[e] - ref32) * k32) - off32 * p[e], 0.0f);
-        else
-          sum += __builtin_fmax(weight(v[e], w) - off * p[e], 0.0);
-      }
-    }
-    if constexpr (FAST) sum += quick;
+    for (int e = 0; e < kEndElems; ++e) sum += __builtin_fmax(weight(v[e], by) - walk.off * q[e], 0.0);
+    sum = segment_sum(sh.seg, sum);
+    if (threadIdx.x == 0) put(&a.rests[(size_t)s.index * a.segments + segment], sum);
+    return;
   }
-  return wave_sum64(sum);
+  float top = walk.ref;
+  int first = 0x7fffffff;
+  bool bad = false;
+  if (walk.phase == kRest) {
+    mark_tried(a, sh, s, walk.node, begin);
+#pragma unroll
+    for (int e = 0; e < kEndElems; ++e) v[e] = was_tried(sh, element_at(e)) ? -INFINITY : v[e];
+  } else {
+    top = -INFINITY;
+#pragma unroll
+    for (int e = 0; e < kEndElems; ++e) {
+      bad |= unusable(v[e]);
+      top = fmaxf(top, v[e]);
+    }
+    if (s.greedy) {
+#pragma unroll
+      for (int e = kEndElems - 1; e >= 0; --e)  // (a thread's elements rise)
+        if (v[e] == top) first = begin + element_at(e);
+    }
+    segment_top(sh.seg, top, first, s.greedy);
+  }
+  const Weights by{s.k, s.k * finite_or_zero(top)};
+#pragma unroll
+  for (int e = 0; e < kEndElems; ++e) sum += weight(v[e], by);
+  sum = segment_sum(sh.seg, bad ? NAN : sum);
+  if (threadIdx.x != 0) return;
+  if (walk.phase == kRest) {
+    put(&a.rests[(size_t)s.index * a.segments + segment], sum);
+  } else {
+    RowSums* to = a.sums + (a.all_rows ? (size_t)s.index * a.max_query_len + walk.node : (size_t)s.index) * a.segments + segment;
+    put(&to->sum, sum);
+    put(reinterpret_cast<uint64_t*>(&to->top), __builtin_bit_cast(uint64_t, make_int2(__float_as_int(top), first)));
+  }
 }
 
-// What a node's trial gives.
-struct Trial {
-  int child;    // the accepted child, or -1
-  int unsure;   // a comparison within the fast sums' error, or a row that they do not serve
-  int failed;   // no distribution: a logit that is NaN or +inf, or none that is finite
-  float ref;
-  Offs offs;
-};
+// The node's children: their tokens' weights, draft probabilities and random numbers.  `mine` is the thread's own
+// node, looked up before.
+__device__ __forceinline__ void find_children(const VerifyArgs& a, VerifyShared& sh, const Sequence& s, const Walk& walk, const Weights& by,
+                                              const Node& mine) {
+  __syncthreads();  // the last use is over
+  for (int j = threadIdx.x; j < (s.n + 63) / 64 * 64; j += kEndThreads) {  // whole waves
+    Node x = mine;
+    if (j >= kEndThreads) {
+      x = node_at(a, s, j);
+      look_up(a, s, walk.node, j, x);
+    }
+    if (x.child) {
+      sh.tokens[j] = x.token;
+      sh.accept[j] = x.accept;
+      sh.mass[j] = weight(x.logit, by);
+      sh.probs[j] = x.prob;
+    }
+    const uint64_t bits = __builtin_amdgcn_ballot_w64(x.child);
+    if ((j & 63) == 0) sh.kids[j >> 6] = bits;
+  }
+  __syncthreads();
+}
 
-// The first child (a bit of sh.kids) behind node j, or -1.
-__device__ __forceinline__ int next_child(const WalkShared& sh, int n, int j) {
+// The first child behind node j, or -1.
+__device__ __forceinline__ int next_child(const VerifyShared& sh, int n, int j) {
   ++j;
   for (int word = j >> 6; word < (n + 63) >> 6; ++word) {
     const uint64_t bits = sh.kids[word] & (word == j >> 6 ? ~0ull << (j & 63) : ~0ull);
@@ -276,502 +405,303 @@ __device__ __forceinline__ int next_child(const WalkShared& sh, int n, int j) {
   return -1;
 }
 
-// Tries the children of `node`, sh.kids, of which there is one.  Every thread of the workgroup takes the same way.
-template <bool VEC, bool FAST>
-__device__ __forceinline__ Trial try_node(const VerifyArgs& a, WalkShared& sh, const fi::TreeSpan& t, int n, int node,
-                                          float temperature) {
-  const int tid = threadIdx.x, w = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
-  const int part = ((a.vocab + kWalkWaves - 1) / kWalkWaves + 255) & ~255;
-  const int begin = min(w * part, a.vocab), end = min(begin + part, a.vocab);
-  const float* row = a.logits + (int64_t)(t.first + node) * a.ld;
-  const bool greedy = temperature <= 0.0f;
-  const double k = row_scale(temperature);
-  const PartStats mine = greedy ? part_stats<VEC, true, true>(row, begin, end, k, lane)
-                                : part_stats<VEC, FAST, false>(row, begin, end, k, lane);
-  __syncthreads();  // the last trial's readers are done
-  if (lane == 0) sh.parts[w] = mine;
-  __syncthreads();
-  Trial r{};
-  r.child = -1;
-  float top = -INFINITY;
-  int first = 0x7fffffff, bad = 0;
-  for (int i = 0; i < kWalkWaves; ++i) {
-    const PartStats p = sh.parts[i];
-    if (p.top > top) {
-      top = p.top;
-      first = p.first;
-    }
-    bad |= p.bad;
-  }
-  if (greedy) {
-    r.child = next_child(sh, n, node);
-    while (r.child >= 0 && (sh.tokens[r.child] != first || first >= a.vocab)) r.child = next_child(sh, n, r.child);
-    return r;
-  }
-  r.unsure = FAST && bad;
-  r.failed = !FAST && (bad || top == -INFINITY);
-  if (bad || top == -INFINITY) {
-    r.unsure = FAST;
-    return r;
-  }
-  const Weights by{k, top};
-  r.ref = top;
-  double total = 0.0;  // 1 at least: the largest logit's
-  for (int i = 0; i < kWalkWaves; ++i) {
-    const PartStats p = sh.parts[i];
-    if (p.sum > 0.0) total += p.sum * change_of_ref(k, p.ref, top);
-  }
-  const float* probs = a.probs ? a.probs + (int64_t)(t.first + node) * a.ld_probs : nullptr;
-  double rest = total, rest_error = FAST ? kFastError * total : 0.0;  // Z
-  double off = 0.0, off_error = 0.0, taken = 0.0;
-  int next = next_child(sh, n, node);
-  while (next >= 0) {
-    const int j = next, x = sh.tokens[j];
-    next = next_child(sh, n, j);
-    if (x < 0 || x >= a.vocab || !(taken < 1.0)) continue;
-    const double mass = weight(row[x], by), u = sh.accept[j];
-    if (!probs) {
-      // an earlier child of the same token has been taken out
-      bool out = false;
-      for (int i = next_child(sh, n, node); i < j; i = next_child(sh, n, i)) out |= sh.tokens[i] == x;
-      const double left = out ? 0.0 : mass;
-      if (FAST && __builtin_fabs(u * rest - left) <= u * rest_error + 1e-9 * left) r.unsure = 1;
-      if (u * rest < left) {
-        r.child = j;
-        break;
-      }
-      rest -= left;
-    } else {
-      const double q = probs[x], c = rest / (1.0 - taken), c_error = rest_error / (1.0 - taken);
-      const double left = __builtin_fmax(mass - off * q, 0.0);
-      if (FAST && __builtin_fabs(u * c * q - left) <= (u * c_error + off_error) * q + 1e-9 * (left + off * q)) r.unsure = 1;
-      if (u * c * q < left) {
-        r.child = j;
-        break;
-      }
-      off += c;
-      off_error += c_error;
-      if constexpr (FAST) {
-        // the end takes it from here; more steps than it follows: the node once more, in 64 bits
-        if (r.offs.steps == kMaxSteps) r.unsure = 1;
+// What a segment's sums come to by the row's reference point; a lane has those of kPer segments on end, every wave all.
+constexpr int kPer = kMaxSegments / 64;
+constexpr double kNothing = 1e-290;  // less than this is no share (a million of the least normal numbers)
+
+__device__ __forceinline__ int lane_of(uint64_t some, uint64_t any) {
+  return some != 0 ? __builtin_ctzll(some) : any != 0 ? 63 - __builtin_clzll(any) : 0;
+}
+__device__ __forceinline__ double of_lane(double v, int lane) {
+  const int2 x = __builtin_bit_cast(int2, v);
+  return __builtin_bit_cast(double, make_int2(__builtin_amdgcn_readlane(x.x, lane), __builtin_amdgcn_readlane(x.y, lane)));
+}
+
+// Draws the last token by the segments' shares: the segment, wave, lane and element at which the running sum of what is
+// left passes u times all of it, each of those that have anything; past the last of them (u of 1 and more, or the sums'
+// roundings) the last.
+template <bool VEC>
+__device__ __forceinline__ void pick_token(const VerifyArgs& a, VerifyShared& sh, const Sequence& s, const Walk& walk,
+                                           const double (&part)[kPer], bool rest, float pick_u) {
+  const int tid = threadIdx.x, lane = tid & 63, per = (a.segments + 63) / 64;
+  const float* row = a.logits + (int64_t)(s.first + walk.node) * a.ld;
+  const bool less = rest && a.probs, without = rest && !a.probs;
+  double share = 0.0;
 #pragma unroll
-        for (int i = 0; i < kMaxSteps; ++i)
-          if (i == r.offs.steps) {
-            r.offs.off[i] = off;
-            r.offs.room[i] = 1.0 - taken;
-          }
-        ++r.offs.steps;
-      } else {
-        r.offs.steps = r.offs.exact = 1;
-        r.offs.off[0] = off;
-      }
-      if (a.distinct) taken += q;
-      if (next >= 0 && !r.unsure) {
-        const double wave = part_rest<VEC, FAST>(row, probs, begin, end, by, off, lane);
-        __syncthreads();
-        if (lane == 0) sh.rest[w] = wave;
-        __syncthreads();
-        rest = 0.0;
-        for (int i = 0; i < kWalkWaves; ++i) rest += sh.rest[i];
-        rest_error = FAST ? kFastError * total + off_error + 1e-6 * off : 0.0;
-      }
-    }
-    if (r.unsure) return r;
-  }
-  return r;
-}
-
-template <bool VEC>
-__global__ __launch_bounds__(kWalkThreads) void verify_walk_kernel(VerifyArgs a) {
-  __shared__ WalkShared sh;
-  const int seq = blockIdx.x, tid = threadIdx.x;
-  const fi::TreeSpan t = fi::tree_span(a.cu_seqlens, nullptr, seq);
-  const int n = min(t.nodes, a.max_query_len);
-  if (tid == 0 && t.nodes > a.max_query_len) atomicOr(a.faults, FI_FAULT_QUERY_RANGE);
-  for (int i = tid; i < n; i += kWalkThreads) {
-    const int p = a.parents[t.first + i], x = a.tokens[t.first + i];
-    if (p < -1 || p >= i) atomicOr(a.faults, FI_FAULT_TREE_RANGE);
-    if (i > 0 && (x < 0 || x >= a.vocab)) atomicOr(a.faults, FI_FAULT_TOKEN_RANGE);
-    sh.parents[i] = p >= i ? -1 : p;
-    sh.tokens[i] = x;
-    sh.accept[i] = a.accept_u[t.first + i];
-  }
-  int* tokens = a.out_tokens + (size_t)seq * (a.max_path + 1);
-  int* path = a.out_path + (size_t)seq * a.max_path;
-  __syncthreads();
-  const float temperature = a.temperature[seq];
-  EndState end{};
-  end.node = n > 0 ? 0 : -1;
-  while (end.node >= 0 && end.count < a.max_path) {
-    for (int i = tid; i < (n + 63) / 64 * 64; i += kWalkThreads) {  // whole waves
-      const uint64_t bits = __builtin_amdgcn_ballot_w64(i < n && sh.parents[i] == end.node);
-      if ((tid & 63) == 0) sh.kids[i >> 6] = bits;
-    }
-    __syncthreads();
-    if (next_child(sh, n, end.node) < 0) break;
-    Trial r = try_node<VEC, true>(a, sh, t, n, end.node, temperature);
-    if (r.unsure) r = try_node<VEC, false>(a, sh, t, n, end.node, temperature);
-    if (r.failed) {
-      if (tid == 0) atomicOr(a.faults, FI_FAULT_SAMPLE_NONFINITE);
-      end.node = -1;
-    } else if (r.child < 0) {
-      end.tried = 1;
-      end.offs = r.offs;
-      end.ref = r.ref;
-      break;
-    } else {
-      if (tid == 0) {
-        path[end.count] = r.child;
-        tokens[end.count] = sh.tokens[r.child];
-      }
-      end.node = r.child;
-      ++end.count;
-    }
-    __syncthreads();  // sh.kids is read no more
-  }
-  for (int i = end.count + tid; i < a.max_path; i += kWalkThreads) path[i] = -1;
-  for (int i = end.count + tid; i <= a.max_path; i += kWalkThreads) tokens[i] = -1;
-  if (tid == 0) {
-    a.out_count[seq] = end.count;
-    a.out_prob[seq] = 0.0f;
-    a.ends[seq] = end;
-  }
-}
-
-// ---------------------------------------------------------------- the token at the end
-
-constexpr int kEndThreads = 256;
-constexpr int kEndElems = 16;                          // consecutive elements a thread
-constexpr int kSegment = kEndThreads * kEndElems;      // 4096
-constexpr int kMaxSegments = 256;                      // a thread each when they are joined
-constexpr int kMaxVocab = kSegment * kMaxSegments;     // 1048576
-
-struct SegmentSums {
-  double sum;              // of the weights
-  double rest[kMaxSteps];  // of what is left of them, at each a
-  double part[kMaxSteps];  // of q where something is left
-  float top;               // the reference point of the weights (0 where it is not finite)
-  int first, bad, pad;
-};
-
-struct EndShared {
-  uint32_t out[kSegment / 32];  // tokens given and rejected
-  double scan[kEndThreads / 64];
-  float tops[kEndThreads / 64];
-  int firsts[kEndThreads / 64], bads[kEndThreads / 64];
-  double total;
-  int last, pick, segment;
-};
-
-// The 16 elements of a thread.
-template <bool VEC>
-__device__ __forceinline__ void end_load(const float* __restrict__ row, int begin, int vocab, float pad, float (&v)[kEndElems]) {
+  for (int i = 0; i < kPer; ++i) share += part[i];
+  double run = wave_scan64(share);
+  const double total = of_lane(run, 63), target = static_cast<double>(pick_u) * total;
+  int from = lane_of(__builtin_amdgcn_ballot_w64(share > kNothing && run > target), __builtin_amdgcn_ballot_w64(share > kNothing));
+  int segment = 0;
+  double before = 0.0, at = run - share;
+  bool passed = false;
 #pragma unroll
-  for (int j = 0; j < kEndElems / 4; ++j) {
-    const float4 x = quad_at<VEC>(row, begin + 4 * j, vocab, pad);
-    v[4 * j] = x.x;
-    v[4 * j + 1] = x.y;
-    v[4 * j + 2] = x.z;
-    v[4 * j + 3] = x.w;
-  }
-}
-
-template <bool VEC>
-__global__ __launch_bounds__(kEndThreads) void verify_end_kernel(VerifyArgs a) {
-  __shared__ EndShared sh;
-  const int seq = blockIdx.y, tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
-  const EndState end = a.ends[seq];
-  if (end.node < 0) return;  // every segment of the sequence
-  const fi::TreeSpan t = fi::tree_span(a.cu_seqlens, nullptr, seq);
-  const int n = min(t.nodes, a.max_query_len);
-  const float* row = a.logits + (int64_t)(t.first + end.node) * a.ld;
-  const float* probs = a.probs ? a.probs + (int64_t)(t.first + end.node) * a.ld_probs : nullptr;
-  const float temperature = a.temperature[seq];
-  const bool greedy = temperature <= 0.0f;
-  const double k = greedy ? kLog2E : row_scale(temperature);
-  const bool less = end.tried && !greedy && probs && end.offs.steps > 0;  // max(w - a q, 0)
-  const bool without = end.tried && !greedy && !probs;                    // w, but for the tokens tried
-  const int steps = less ? end.offs.steps : 1;
-
-  // marks the segment's tokens that were tried, and loads it
-  auto open = [&](int segment, float (&v)[kEndElems], float (&q)[kEndElems]) {
-    const int begin = segment * kSegment;
-    end_load<VEC>(row, begin + tid * kEndElems, a.vocab, -INFINITY, v);
-    if (less) end_load<VEC>(probs, begin + tid * kEndElems, a.vocab, 0.0f, q);
-    if (without) {  // workgroup-uniform
-      for (int i = tid; i < kSegment / 32; i += kEndThreads) sh.out[i] = 0;
-      __syncthreads();
-      for (int j = end.node + 1 + tid; j < n; j += kEndThreads) {
-        const int x = a.tokens[t.first + j];
-        if (a.parents[t.first + j] == end.node && x >= begin && x < min(begin + kSegment, a.vocab))
-          atomicOr(&sh.out[(x - begin) >> 5], 1u << ((x - begin) & 31));
-      }
-      __syncthreads();
+  for (int i = 0; i < kPer; ++i) {
+    if (part[i] > kNothing && !passed) {
+      segment = per * lane + i;
+      before = at;
+      passed = at + part[i] > target;
     }
-  };
-
-  auto tried = [&](int e) { return ((sh.out[e >> 5] >> (e & 31)) & 1) != 0; };
-
+    at += part[i];
+  }
+  segment = __builtin_amdgcn_readlane(segment, from);
+  before = of_lane(before, from);
   float v[kEndElems], q[kEndElems];
-  const int segment = blockIdx.x;
-  open(segment, v, q);
-  float top = -INFINITY;
-  int first = 0x7fffffff;
-  bool bad = false;
-#pragma unroll
-  for (int e = 0; e < kEndElems; ++e) {
-    bad |= unusable(v[e]);
-    if (v[e] > top) {
-      top = v[e];
-      first = segment * kSegment + tid * kEndElems + e;
-    }
-  }
-  {
-    const float wave_top = fi::wave_max(top);
-    int at = top == wave_top ? first : 0x7fffffff;
-#pragma unroll
-    for (int m = 32; m >= 1; m >>= 1) at = min(at, __shfl_xor(at, m, 64));
-    const bool any = __builtin_amdgcn_ballot_w64(bad) != 0;
-    if (lane == 0) {
-      sh.tops[w] = wave_top;
-      sh.firsts[w] = at;
-      sh.bads[w] = any;
-    }
-  }
-  __syncthreads();
-  top = -INFINITY;
-  bad = false;
-  for (int i = 0; i < kEndThreads / 64; ++i) {
-    if (sh.tops[i] > top) {
-      top = sh.tops[i];
-      first = sh.firsts[i];
-    }
-    bad |= sh.bads[i] != 0;
-  }
-  const Weights by{k, finite_or_zero(top)};
-  double sum = 0.0, rest[kMaxSteps] = {}, in_part[kMaxSteps] = {}, off[kMaxSteps];
-  {
-    const double change = less ? change_of_ref(k, end.ref, finite_or_zero(top)) : 0.0;
-#pragma unroll
-    for (int i = 0; i < kMaxSteps; ++i) off[i] = less && i < steps ? end.offs.off[i] * change : 0.0;
-  }
-#pragma unroll
-  for (int e = 0; e < kEndElems; ++e) {
-    const double x = weight(v[e], by);
-    sum += x;
-    if (less) {
-#pragma unroll
-      for (int i = 0; i < kMaxSteps; ++i)
-        if (i < steps) {
-          const double left = x - off[i] * q[e];
-          rest[i] += __builtin_fmax(left, 0.0);
-          in_part[i] += left > 0.0 ? static_cast<double>(q[e]) : 0.0;
-        }
-    } else {
-      rest[0] += without && tried(tid * kEndElems + e) ? 0.0 : x;
-    }
-  }
-  // the workgroup's sum of x, in thread 0
-  auto gather = [&](double x) {
-    x = wave_sum64(x);
-    __syncthreads();  // the last use of sh.scan is over
-    if (lane == 0) sh.scan[w] = x;
-    __syncthreads();
-    double all = 0.0;
-    for (int i = 0; i < kEndThreads / 64; ++i) all += sh.scan[i];
-    return all;
-  };
-  sum = gather(sum);
-#pragma unroll
-  for (int i = 0; i < kMaxSteps; ++i)
-    if (i < steps) {
-      rest[i] = gather(rest[i]);
-      if (less) in_part[i] = gather(in_part[i]);
-    }
-  if (tid == 0) {
-    SegmentSums* to = a.sums + (size_t)seq * a.segments + segment;
-    // read by another workgroup of this launch: device-coherent stores, complete before the arrival
-    __hip_atomic_store(&to->sum, sum, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-#pragma unroll
-    for (int i = 0; i < kMaxSteps; ++i)
-      if (i < steps) {
-        __hip_atomic_store(&to->rest[i], rest[i], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-        __hip_atomic_store(&to->part[i], in_part[i], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-      }
-    __hip_atomic_store(&to->top, top, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    __hip_atomic_store(&to->first, first, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    __hip_atomic_store(&to->bad, bad ? 1 : 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    __builtin_amdgcn_s_waitcnt(0);
-    const unsigned arrived = __hip_atomic_fetch_add(&a.counters[seq], 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) + 1u;
-    sh.last = arrived == static_cast<unsigned>(a.segments);
-    if (sh.last) __hip_atomic_store(&a.counters[seq], 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-  }
-  __syncthreads();
-  if (!sh.last) return;
-
-  // ---- the last workgroup of the sequence: a thread a segment ----
-  SegmentSums mine{};
-  mine.top = -INFINITY;
-  mine.first = 0x7fffffff;
-  if (tid < a.segments) {
-    SegmentSums* from = a.sums + (size_t)seq * a.segments + tid;
-    mine.sum = __hip_atomic_load(&from->sum, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-#pragma unroll
-    for (int i = 0; i < kMaxSteps; ++i)
-      if (i < steps) {
-        mine.rest[i] = __hip_atomic_load(&from->rest[i], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-        mine.part[i] = __hip_atomic_load(&from->part[i], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-      }
-    mine.top = __hip_atomic_load(&from->top, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    mine.first = __hip_atomic_load(&from->first, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    mine.bad = __hip_atomic_load(&from->bad, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-  }
-  {
-    const float wave_top = fi::wave_max(mine.top);
-    int at = mine.top == wave_top ? mine.first : 0x7fffffff;
-#pragma unroll
-    for (int m = 32; m >= 1; m >>= 1) at = min(at, __shfl_xor(at, m, 64));
-    const bool any = __builtin_amdgcn_ballot_w64(mine.bad != 0) != 0;
-    if (lane == 0) {
-      sh.tops[w] = wave_top;
-      sh.firsts[w] = at;
-      sh.bads[w] = any;
-    }
-  }
-  __syncthreads();
-  top = -INFINITY;
-  bad = false;
-  for (int i = 0; i < kEndThreads / 64; ++i) {
-    if (sh.tops[i] > top) {
-      top = sh.tops[i];
-      first = sh.firsts[i];
-    }
-    bad |= sh.bads[i] != 0;
-  }
-  int* token = a.out_tokens + (size_t)seq * (a.max_path + 1) + end.count;
-  if ((bad && !greedy) || top == -INFINITY) {
-    if (tid == 0) atomicOr(a.faults, FI_FAULT_SAMPLE_NONFINITE);
-    return;  // the token stays -1
-  }
-  // the segments' sums by one reference point
-  const float ref = finite_or_zero(top);
-  const double scale = tid < a.segments ? change_of_ref(k, finite_or_zero(mine.top), ref) : 0.0;
-  // running sums of `x` over the threads, in order; the total in sh.total
-  auto running = [&](double x) {
-    double run = x;
-#pragma unroll
-    for (int m = 1; m < 64; m <<= 1) {
-      const double y = __shfl_up(run, m, 64);
-      if (lane >= m) run += y;
-    }
-    __syncthreads();  // the last use of sh.scan is over
-    if (lane == 63) sh.scan[w] = run;
-    __syncthreads();
-    double before = 0.0, all = 0.0;
-    for (int i = 0; i < kEndThreads / 64; ++i) {
-      if (i < w) before += sh.scan[i];
-      all += sh.scan[i];
-    }
-    if (tid == 0) sh.total = all;
-    return before + run;
-  };
-  if (greedy) {
-    running(mine.sum * scale);
-    if (tid == 0) {
-      *token = first;
-      a.out_prob[seq] = bad ? NAN : static_cast<float>(1.0 / sh.total);
-    }
-    return;
-  }
-  // the exact a, step by step, and what is left of the segment's weights there
-  double exact = 0.0, left_here = mine.rest[0] * scale;
+  const int begin = segment * kSegment;
+  segment_load<VEC, true>(row, begin, a.vocab, -INFINITY, v);
   if (less) {
-    const double change = change_of_ref(k, end.ref, ref);
-    if (end.offs.exact) {
-      exact = end.offs.off[0] * change;
-    } else {
-      const double all = gather(mine.sum * scale);
+    segment_load<VEC, true>(a.probs + (int64_t)(s.first + walk.node) * a.ld_probs, begin, a.vocab, 0.0f, q);
+  } else {
 #pragma unroll
-      for (int i = 0; i < kMaxSteps; ++i)
-        if (i < steps) {
-          exact = i == 0 ? all : exact + gather(left_here) / end.offs.room[i];
-          left_here = __builtin_fmax(mine.rest[i] * scale - (exact - end.offs.off[i] * change) * mine.part[i], 0.0);
-        }
-    }
+    for (int e = 0; e < kEndElems; ++e) q[e] = 0.0f;
   }
-  // nothing left (p = a q but for rounding): the draw is from the distribution itself
-  double run = running(left_here);
-  __syncthreads();
-  const bool whole = !(sh.total > 0.0);
-  if (whole) run = running(mine.sum * scale);
-  if (tid == 0) {
-    sh.segment = a.segments;
-    sh.pick = 0x7fffffff;
+  if (without) {
+    mark_tried(a, sh, s, walk.node, begin);
+#pragma unroll
+    for (int e = 0; e < kEndElems; ++e) v[e] = was_tried(sh, tid * kEndElems + e) ? -INFINITY : v[e];
   }
-  __syncthreads();
-  const double total = sh.total, target = static_cast<double>(a.pick_u[seq]) * total;
-  const double share = whole ? mine.sum * scale : left_here;
-  if (tid < a.segments && share > 0.0 && run > target) atomicMin(&sh.segment, tid);
-  __syncthreads();
-  int chosen = sh.segment;
-  __syncthreads();             // every wave has read it
-  if (chosen >= a.segments) {  // u of 1 and more (or NaN): the last segment that has anything
-    if (tid == 0) sh.segment = -1;
-    __syncthreads();
-    if (tid < a.segments && share > 0.0) atomicMax(&sh.segment, tid);
-    __syncthreads();
-    chosen = sh.segment;
-  }
-  __shared__ double s_before;
-  __shared__ float s_top;
-  if (tid == chosen) {
-    s_before = run - share;
-    s_top = mine.top;
-  }
-  __syncthreads();
-  // ---- the token in the segment ----
-  open(chosen, v, q);
-  const Weights in{k, finite_or_zero(s_top)};
-  const double to_ref = change_of_ref(k, finite_or_zero(s_top), ref);
-  const double off_in = less ? exact * change_of_ref(k, ref, finite_or_zero(s_top)) : 0.0;
+  const Weights by{s.k, s.k * walk.ref};
+  const double off = less ? walk.off : 0.0;
   double left[kEndElems], here = 0.0;
 #pragma unroll
   for (int e = 0; e < kEndElems; ++e) {
-    const double x = weight(v[e], in);
-    left[e] = to_ref * (whole  ? x
-                        : less ? __builtin_fmax(x - off_in * q[e], 0.0)
-                               : (without && tried(tid * kEndElems + e) ? 0.0 : x));
+    left[e] = __builtin_fmax(weight(v[e], by) - off * q[e], 0.0);
     here += left[e];
   }
-  const double before = s_before;
-  double at = before + running(here) - here;
-  int found = 0x7fffffff, last = -1;
+  run = wave_scan64(here);
+  __syncthreads();  // the last use is over
+  if (lane == 63) sh.seg.scan[tid >> 6] = run;
+  __syncthreads();
+  int wave = 0;
+  passed = false;
+#pragma unroll
+  for (int i = 0; i < kEndThreads / 64; ++i) {
+    const double all = sh.seg.scan[i];
+    if (all > 0.0 && !passed) {
+      wave = i;
+      at = before;
+      passed = before + all > target;
+    }
+    before += all;
+  }
+  if (tid >> 6 != wave) return;
+  run += at;
+  from = lane_of(__builtin_amdgcn_ballot_w64(here > 0.0 && run > target), __builtin_amdgcn_ballot_w64(here > 0.0));
+  if (lane != from) return;
+  at = run - here;
+  int token = -1;
+  double mass = 0.0;
+  passed = false;
 #pragma unroll
   for (int e = 0; e < kEndElems; ++e) {
     at += left[e];
-    if (left[e] > 0.0) {
-      last = e;
-      if (at > target && found == 0x7fffffff) found = e;
+    if (left[e] > 0.0 && !passed) {
+      token = begin + tid * kEndElems + e;
+      mass = left[e];
+      passed = at > target;
     }
   }
-  if (found != 0x7fffffff) atomicMin(&sh.pick, tid * kEndElems + found);
-  __syncthreads();
-  if (sh.pick == 0x7fffffff) {  // the sums' roundings, or u of 1 and more: the last that has anything
-    if (tid == 0) sh.segment = -1;
-    __syncthreads();
-    if (last >= 0) atomicMax(&sh.segment, tid * kEndElems + last);
-    __syncthreads();
-    if (tid == 0) sh.pick = sh.segment;
-    __syncthreads();
-  }
-  const int pick = sh.pick;
-  if (pick >= 0 && pick / kEndElems == tid) {
-    double mass = 0.0;
+  // (behind barriers from where other threads cleared them)
+  a.out_tokens[(size_t)s.index * (a.max_path + 1) + walk.count] = token;
+  a.out_prob[s.index] = static_cast<float>(mass / total);
+}
+
+// Takes the walk on from the sums that it asked for, until it asks for others or ends.  Every wave does, so that what they
+// need of each other is their lanes' nodes.
+template <bool VEC>
+__device__ __forceinline__ void advance(const VerifyArgs& a, VerifyShared& sh, const Sequence& s, Walk& walk, Node& mine, float pick_u) {
+  const int tid = threadIdx.x, lane = tid & 63, per = (a.segments + 63) / 64;
+  while (true) {  // mine is looked up at the walk's node
+    const bool rest = walk.phase == kRest;
+    double part[kPer] = {}, total;
+    float top = -INFINITY;
+    int first = 0x7fffffff;
+    auto row_parts = [&]() {
+      const RowSums* sums = a.sums + (a.all_rows ? (size_t)s.index * a.max_query_len + walk.node : (size_t)s.index) * a.segments;
+      float tops[kPer];
+      top = -INFINITY;
 #pragma unroll
-    for (int e = 0; e < kEndElems; ++e)
-      if (e == pick % kEndElems) mass = left[e];
-    *token = chosen * kSegment + pick;
-    a.out_prob[seq] = static_cast<float>(mass / total);
+      for (int i = 0; i < kPer; ++i) {
+        tops[i] = -INFINITY;
+        if (i < per && per * lane + i < a.segments) {
+          const RowSums* from = sums + per * lane + i;
+          part[i] = get(&from->sum);
+          const int2 at = __builtin_bit_cast(int2, get(reinterpret_cast<const uint64_t*>(&from->top)));
+          tops[i] = __int_as_float(at.x);
+          if (tops[i] > top) {
+            top = tops[i];
+            first = at.y;
+          }
+        }
+      }
+      const float mine_top = top;
+      top = wave_top(top);
+      if (s.greedy) first = first_of(mine_top, top, first);
+      walk.ref = finite_or_zero(top);
+#pragma unroll
+      for (int i = 0; i < kPer; ++i)
+        if (i < per && tops[i] != -INFINITY) part[i] *= change_of_ref(s.k, finite_or_zero(tops[i]), walk.ref);
+    };
+    if (rest) {
+#pragma unroll
+      for (int i = 0; i < kPer; ++i)
+        if (i < per && per * lane + i < a.segments) part[i] = get(&a.rests[(size_t)s.index * a.segments + per * lane + i]);
+    } else {
+      row_parts();
+    }
+    total = (part[0] + part[1]) + (part[2] + part[3]);
+    total = wave_sum64(total);
+    if (!rest) {
+      if ((!s.greedy && !(total == total)) || top == -INFINITY) {
+        if (tid == 0) atomicOr(a.faults, FI_FAULT_SAMPLE_NONFINITE);
+        walk.phase = kDone;
+        return;
+      }
+      walk.total = total;  // 1 at least: the largest logit's
+    }
+    // the children
+    int accepted = -1;
+    bool rejected = false;
+    if (walk.count < a.max_path && (!rest || a.probs)) {
+      find_children(a, sh, s, walk, Weights{s.k, s.k * walk.ref}, mine);
+      if (s.greedy) {
+        int best = 0x7fffffff;
+        for (int j = lane; j < s.n; j += 64)
+          if ((sh.kids[j >> 6] >> lane & 1) != 0 && sh.tokens[j] == first) best = min(best, j);
+        best = first_of(0.0f, 0.0f, best);
+        accepted = best == 0x7fffffff ? -1 : best;
+      } else if (!a.probs) {
+        double left = total;
+        for (int j = next_child(sh, s.n, walk.node); j >= 0; j = next_child(sh, s.n, j)) {
+          bool out = false;  // an earlier child of the same token has been taken out
+          for (int i = next_child(sh, s.n, walk.node); i < j; i = next_child(sh, s.n, i)) out |= sh.tokens[i] == sh.tokens[j];
+          const double mass = out ? 0.0 : sh.mass[j];
+          if (sh.accept[j] * left < mass) {
+            accepted = j;
+            break;
+          }
+          left -= mass;
+          rejected = true;
+        }
+      } else {
+        const int j = walk.taken < 1.0 ? next_child(sh, s.n, max(walk.child, walk.node)) : -1;
+        if (j >= 0) {
+          const double q = sh.probs[j], c = total / (1.0 - walk.taken);
+          if (sh.accept[j] * c * q < __builtin_fmax(sh.mass[j] - walk.off * q, 0.0)) {
+            accepted = j;
+          } else {
+            rejected = true;
+            walk.off += c;
+            if (a.distinct) walk.taken += q;
+            walk.child = j;
+          }
+        }
+      }
+    }
+    if (accepted >= 0) {
+      if (tid == walk.count % kEndThreads) {  // the thread that has cleared these
+        a.out_path[(size_t)s.index * a.max_path + walk.count] = accepted;
+        a.out_tokens[(size_t)s.index * (a.max_path + 1) + walk.count] = sh.tokens[accepted];
+      }
+      if (tid == 0) a.out_count[s.index] = walk.count + 1;
+      walk = Walk{accepted, walk.count + 1, kTotal, -1, 0.0f, 0.0, 0.0, 0.0};
+      if (!a.all_rows) return;
+      look_up(a, s, walk.node, tid, mine);
+      continue;
+    }
+    if (rejected) {
+      walk.phase = kRest;
+      return;
+    }
+    // the end
+    if (s.greedy) {
+      if (tid == walk.count % kEndThreads) a.out_tokens[(size_t)s.index * (a.max_path + 1) + walk.count] = first;
+      if (tid == 0) a.out_prob[s.index] = static_cast<float>(1.0 / total);
+    } else {
+      const bool whole = rest && !(total > kNothing);  // nothing left (p = a q but for rounding): the draw is from the distribution itself
+      if (whole) row_parts();
+      pick_token<VEC>(a, sh, s, walk, part, rest && !whole, pick_u);
+    }
+    walk.phase = kDone;
+    return;
+  }
+}
+
+// What a sequence's first advance finds: nothing accepted yet.
+__device__ __forceinline__ void begin_outputs(const VerifyArgs& a, const Sequence& s, const Node& mine) {
+  const int tid = threadIdx.x;
+  for (int i = tid; i < a.max_path; i += kEndThreads) a.out_path[(size_t)s.index * a.max_path + i] = -1;
+  for (int i = tid; i <= a.max_path; i += kEndThreads) a.out_tokens[(size_t)s.index * (a.max_path + 1) + i] = -1;
+  if (tid == 0) {
+    a.out_count[s.index] = 0;
+    a.out_prob[s.index] = 0.0f;
+    if (a.cu_seqlens[s.index + 1] - a.cu_seqlens[s.index] > a.max_query_len) atomicOr(a.faults, FI_FAULT_QUERY_RANGE);
+  }
+  for (int i = tid; i < s.n; i += kEndThreads) {
+    const Node x = i < kEndThreads ? mine : node_at(a, s, i);
+    if (x.parent < -1 || x.parent >= i) atomicOr(a.faults, FI_FAULT_TREE_RANGE);
+    if (i > 0 && (x.token < 0 || x.token >= a.vocab)) atomicOr(a.faults, FI_FAULT_TOKEN_RANGE);
+  }
+}
+
+// One launch of the walks: a workgroup a (segment, sequence), or, the first launch where all rows are summed,
+// a (segment, row).  What bounds it: the rows of 64 sequences of 128k logits, 33 MB, take 16 us.  8 us of that are the
+// exponentials, 1.05e12 a second in 64 bits (as many bytes of logits as 4.2 TB/s); the rest is the arrival and the
+// last workgroup's way, one memory latency after the other.  16 sequences take 9 us, one 8.
+template <bool VEC, bool FIRST>
+__global__ __launch_bounds__(kEndThreads) void verify_pass_kernel(VerifyArgs a) {
+  __shared__ VerifyShared sh;
+  const bool rows = FIRST && a.all_rows;
+  const int seq = rows ? blockIdx.y / a.max_query_len : blockIdx.y;
+  const int node = rows ? blockIdx.y - seq * a.max_query_len : 0;
+  Walk walk{node, 0, kTotal, -1, 0.0f, 0.0, 0.0, 0.0};
+  if (!FIRST) walk = a.walks[seq];
+  const Sequence s = sequence_of(a, seq);
+  const float pick_u = a.pick_u[seq];
+  if (!FIRST && walk.phase == kDone) return;
+  if (FIRST && node >= s.n) {
+    if (node == 0 && blockIdx.x == 0) {  // no nodes at all
+      begin_outputs(a, s, Node{});
+      if (threadIdx.x == 0) a.walks[seq].phase = kDone;
+    }
+    return;
+  }
+  const int from = FIRST ? 0 : walk.node;
+  Node mine;
+  sum_segment<VEC>(a, sh, s, walk, blockIdx.x, from, mine);
+  if (threadIdx.x == 0) {
+    __builtin_amdgcn_s_waitcnt(0);  // the sums are there before the arrival
+    // (the last of `of` to arrive)
+    auto last_of = [&](int counter, int of) {
+      unsigned* at = a.counters + (size_t)counter * a.apart;
+      const bool last = __hip_atomic_fetch_add(at, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) + 1u == static_cast<unsigned>(of);
+      if (last) put(at, 0u);
+      return last;
+    };
+    sh.last = rows ? last_of(gridDim.y / a.max_query_len + blockIdx.y, a.segments) && last_of(seq, s.n) : last_of(seq, a.segments);
+  }
+  __syncthreads();
+  if (!sh.last) return;
+  if (FIRST) begin_outputs(a, s, mine);
+  walk.node = from;
+  advance<VEC>(a, sh, s, walk, mine, pick_u);
+  if (threadIdx.x == 0) a.walks[seq] = walk;
+}
+
+// The walks that are left, a workgroup each.
+template <bool VEC>
+__global__ __launch_bounds__(kEndThreads) void verify_finish_kernel(VerifyArgs a) {
+  __shared__ VerifyShared sh;
+  Walk walk = a.walks[blockIdx.x];
+  if (walk.phase == kDone) return;
+  const Sequence s = sequence_of(a, blockIdx.x);
+  while (walk.phase != kDone) {  // each round tries a child, goes to one, or ends the walk
+    Node mine;
+    for (int i = 0; i < a.segments; ++i) sum_segment<VEC>(a, sh, s, walk, i, walk.node, mine);
+    if (threadIdx.x == 0) __builtin_amdgcn_s_waitcnt(0);
+    __syncthreads();
+    advance<VEC>(a, sh, s, walk, mine, a.pick_u[blockIdx.x]);
+    __syncthreads();
   }
 }
 
@@ -819,24 +749,46 @@ int32_t fi_verify_drafts(fi_context* ctx, const float* d_logits, int32_t ld, int
   a.max_path = max_path;
   a.max_query_len = max_query_len;
   a.segments = (vocab + kSegment - 1) / kSegment;
-  const size_t sums = static_cast<size_t>(num_seqs) * a.segments * sizeof(SegmentSums);
-  FI_TRY(fi::ensure_workspace(ctx, sums + static_cast<size_t>(num_seqs) * sizeof(EndState)));
-  a.sums = static_cast<SegmentSums*>(ctx->workspace);
-  a.ends = reinterpret_cast<EndState*>(static_cast<char*>(ctx->workspace) + sums);
+  const int64_t rows = static_cast<int64_t>(num_seqs) * max_query_len;
+  // Few rows are all summed in the first launch, so that a walk goes through accepted tokens without further ones: one
+  // sequence of 8 rows of 152k logits 22 us, 37 with a launch a row; 24 sequences of 5 rows of 128k 51 and 57; 32 of
+  // them 61 and 63; 24 of 8 rows of 152k 62 and 59; 64 of 5 rows of 128k 93 and 88.
+  a.all_rows = max_path > 0 && max_query_len > 1 && rows <= 65535 && rows + num_seqs <= FI_MERGE_COUNTERS && rows * vocab <= kAllRows;
+  // Arrivals at one line follow each other at 11 ns: counters a line each, as far as there are lines (64 sequences of five rows,
+  // all rows summed: 63 us, 117 with the counters side by side).
+  for (a.apart = 32; (num_seqs + (a.all_rows ? rows : 0)) * a.apart > FI_MERGE_COUNTERS;) a.apart /= 2;
+  const size_t sums = static_cast<size_t>(a.all_rows ? rows : num_seqs) * a.segments * sizeof(RowSums);
+  const size_t rests = static_cast<size_t>(num_seqs) * a.segments * sizeof(double);
+  FI_TRY(fi::ensure_workspace(ctx, sums + rests + static_cast<size_t>(num_seqs) * sizeof(Walk)));
+  a.sums = static_cast<RowSums*>(ctx->workspace);
+  a.rests = reinterpret_cast<double*>(static_cast<char*>(ctx->workspace) + sums);
+  a.walks = reinterpret_cast<Walk*>(static_cast<char*>(ctx->workspace) + sums + rests);
   a.counters = ctx->d_merge_counters;
   const bool vec = vocab % 4 == 0 && ld % 4 == 0 && reinterpret_cast<uintptr_t>(d_logits) % 16 == 0 &&
                    (!d_draft_probs || (draft_ld % 4 == 0 && reinterpret_cast<uintptr_t>(d_draft_probs) % 16 == 0));
-  const dim3 ends(static_cast<unsigned>(a.segments), static_cast<unsigned>(num_seqs));
-  if (vec) {
-    hipLaunchKernelGGL((verify_walk_kernel<true>), dim3(num_seqs), dim3(kWalkThreads), 0, ctx->stream, a);
-    FI_CHECK_LAUNCH("verify_walk_kernel");
-    hipLaunchKernelGGL((verify_end_kernel<true>), ends, dim3(kEndThreads), 0, ctx->stream, a);
-  } else {
-    hipLaunchKernelGGL((verify_walk_kernel<false>), dim3(num_seqs), dim3(kWalkThreads), 0, ctx->stream, a);
-    FI_CHECK_LAUNCH("verify_walk_kernel");
-    hipLaunchKernelGGL((verify_end_kernel<false>), ends, dim3(kEndThreads), 0, ctx->stream, a);
-  }
-  FI_CHECK_LAUNCH("verify_end_kernel");
+  // The launches behind the first.  A walk visits depth + 1 rows at most; a node all of whose given children are
+  // rejected costs a pass and ends the walk, so that it never needs more than that.  Each drawn child that is
+  // rejected costs a pass; a walk has nodes - 1 children to try in all.
+  const int depth = std::min(max_path, std::max(max_query_len - 1, 0));
+  const int needed = a.all_rows ? (d_draft_probs ? max_query_len - 1 : 1)
+                                : (d_draft_probs && depth > 0 ? max_query_len - 1 : depth);
+  // Launches for four rejections, then one that takes what is left, a workgroup a walk: 16 trees of 32 nodes 96 us
+  // (109 with launches for eight, 280 with none).
+  const int passes = std::min(needed, (a.all_rows ? 0 : depth) + kRejections);
+  auto launch = [&](auto vec_rows) {
+    constexpr bool VEC = decltype(vec_rows)::value;
+    const unsigned segments = static_cast<unsigned>(a.segments);
+    hipLaunchKernelGGL((verify_pass_kernel<VEC, true>), dim3(segments, static_cast<unsigned>(a.all_rows ? rows : num_seqs)),
+                       dim3(kEndThreads), 0, ctx->stream, a);
+    for (int i = 0; i < passes; ++i)
+      hipLaunchKernelGGL((verify_pass_kernel<VEC, false>), dim3(segments, num_seqs), dim3(kEndThreads), 0, ctx->stream, a);
+    if (passes < needed) hipLaunchKernelGGL((verify_finish_kernel<VEC>), dim3(num_seqs), dim3(kEndThreads), 0, ctx->stream, a);
+  };
+  if (vec)
+    launch(std::true_type{});
+  else
+    launch(std::false_type{});
+  FI_CHECK_LAUNCH("verify_pass_kernel");
   return FI_OK;
 }
 
