@@ -188,13 +188,26 @@ def check_slots(name, rows, slot_mapping) -> None:
         raise FerrisError(3, f"{name}: {rows} positions need a slot each")
 
 
+_DTYPES = {}
+
+
+def _dtype(kind):
+    if kind not in _DTYPES:
+        import torch
+
+        _DTYPES[kind] = getattr(torch, kind)
+    return _DTYPES[kind]
+
+
 def check_arrays(name, kind, **arrays) -> None:
     """Arrays of a drafted step, (tensor, leading shape) each: of the element type that the kernels read, contiguous,
     and at least as long as the rows they are read for."""
+    dtype = _dtype(kind)
     for what, (t, shape) in arrays.items():
-        if t is None or isinstance(t, int):
+        # (most calls' arrays are of just that shape; a call has up to thirteen, and the host's time is all of a small one's)
+        if t is None or isinstance(t, int) or (t.dtype is dtype and t.shape == shape and t.is_contiguous()):
             continue
-        if str(t.dtype) != "torch." + kind:
+        if t.dtype is not dtype:
             raise FerrisError(5, f"{name}: {what} must be {kind}, not {str(t.dtype)[6:]}")
         if len(t.shape) < len(shape) or int(t.shape[0]) < shape[0] or tuple(t.shape[1:len(shape)]) != tuple(shape[1:]):
             raise FerrisError(3, f"{name}: {what} must be of shape {list(shape)}, not {list(t.shape)}")
@@ -204,7 +217,7 @@ def check_arrays(name, kind, **arrays) -> None:
 
 def check_logit_rows(name, what, t, rows, vocab) -> None:
     """Rows of `vocab` f32 logits (probabilities), each contiguous, any row stride."""
-    if str(t.dtype) != "torch.float32":
+    if t.dtype is not _dtype("float32"):
         raise FerrisError(5, f"{name}: {what} must be float32, not {str(t.dtype)[6:]}")
     if len(t.shape) != 2 or int(t.shape[0]) < rows or int(t.shape[1]) != vocab:
         raise FerrisError(3, f"{name}: {what} must be of shape {[rows, vocab]}, not {list(t.shape)}")
@@ -634,7 +647,8 @@ class Context:
         check_arrays("kv_keep_path", "int32", block_tables=(block_tables, (seqs, blocks)), cu_seqlens=(cu_seqlens, (seqs + 1,)),
                      context_lens=(context_lens, (seqs,)), path=(path, (seqs, longest)))
         pools = _P * max(len(k_caches), 1)
-        check(self.lib.fi_kv_keep_path(self.handle, pools(*[ptr(t) for t in k_caches]), pools(*[ptr(t) for t in v_caches]),
+        k_at, v_at = ([t if t is None or isinstance(t, int) else t.data_ptr() for t in pool] for pool in (k_caches, v_caches))
+        check(self.lib.fi_kv_keep_path(self.handle, pools(*k_at), pools(*v_at),
                                        len(k_caches), int(kv_dtype), ptr(block_tables), blocks, ptr(cu_seqlens),
                                        ptr(context_lens), ptr(path), longest, seqs, int(num_blocks), int(block_size),
                                        int(num_kv_heads), int(head_dim)))
