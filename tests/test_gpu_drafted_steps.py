@@ -348,3 +348,53 @@ def test_launch_layouts(gpu_ctx, layout, kind):
                 shown = ref.visible(ref.ancestors(trees[b]), p, p + n)
                 ref.check_attention(got[at:at + n], q[at:at + n], keys, values, shown, d ** -0.5, PIECES[kind], (b, kind, layout))
                 at += n
+
+
+# what the scales of a 4-bit pool's groups are, as (K, V) of a group (block, head, row, group) of a context of 500 rows
+SCALES = {
+    "the least that f16 holds": lambda rng, n: (rng.integers(104, 108, n), rng.integers(104, 108, n)),
+    "the largest": lambda rng, n: (rng.integers(137, 141, n), rng.integers(137, 141, n)),
+    "all that it holds": lambda rng, n: (rng.integers(104, 141, n), rng.integers(104, 141, n)),
+    "the least that is normal": lambda rng, n: (rng.integers(109, 112, n), rng.integers(109, 112, n)),
+    "the largest of those": lambda rng, n: (rng.integers(133, 136, n), rng.integers(133, 136, n)),
+    "all of those": lambda rng, n: (rng.integers(109, 136, n), rng.integers(109, 136, n)),
+    "less": lambda rng, n: (rng.integers(80, 104, n), rng.integers(1, 104, n)),
+    "more": lambda rng, n: (rng.integers(141, 160, n), rng.integers(141, 200, n)),
+    "one K group beyond": lambda rng, n: (np.where(np.arange(n) == n // 2, 150, 127), np.full(n, 127)),
+    "one V group below": lambda rng, n: (np.full(n, 127), np.where(np.arange(n) == n // 3, 90, 127)),
+    "any": lambda rng, n: (rng.integers(60, 150, n), rng.integers(1, 220, n)),
+}
+
+
+@pytest.mark.parametrize("d,prefix", [(32, 500), (64, 490), (128, 497), (128, 5000)])
+@pytest.mark.parametrize("scales", list(SCALES))
+def test_scales_of_four_bit_groups(gpu_ctx, scales, d, prefix):
+    rng = np.random.default_rng(d + prefix)
+    hq, hkv, n = 8, 2, 11
+    keys = prefix + n
+    nb = -(-keys // BS) + 1
+    tables = tables_of(rng, [keys], BS, nb)
+    pools, values = [], []
+    for which in range(2):
+        raw, value = pool_of(rng, "mxfp4", nb, hkv, BS, d)
+        at = nb * hkv * BS * (d // 2)
+        old = raw[at:].cpu().numpy().astype(np.int64)
+        new = np.asarray(SCALES[scales](rng, old.size)[which], np.int64)
+        if "one" in scales:  # in a row that is seen
+            seen = np.zeros((nb, hkv, BS, d // 32), bool)
+            seen[tables[0, 7], 1, 3, 0] = True
+            new = np.where(seen.reshape(-1), np.unique(new)[np.argmax(np.abs(np.unique(new) - 127))], 127)
+        raw[at:] = dev(new.astype(np.uint8))
+        pools.append(raw)
+        values.append((value.reshape(-1, 32) * np.exp2((new - old).astype(np.float64))[:, None]).reshape(value.shape))
+    trees, mask = trees_of(rng, [n])
+    q = rng.standard_normal((n, hq, d)).astype(np.float32)
+    k, v = (fp4.rows_of(x, tables[0], keys, BS) for x in values)
+    # scores of a few units, whatever K's scales: rows of Q of very different sizes
+    q /= np.float32(np.sqrt((k * k).mean()))
+    q[3] = 0.0
+    q[5] *= np.float32(1e-9)
+    q[6] *= 3
+    got = checked(gpu_ctx, attend(gpu_ctx, "mxfp4", q, pools, tables, [n], [keys], mask, hkv, BS, nb, d ** -0.5))
+    shown = ref.visible(ref.ancestors(trees[0]), prefix, keys)
+    ref.check_attention(got, q, k, v, shown, d ** -0.5, PIECES["mxfp4"], scales)
