@@ -4,9 +4,9 @@
 // (crates/ferrisinfer-runtime/src/session.rs:246-262).
 //
 // Rows are packed: row r of a (sequence, kv head) is head r % G of node r / G, so that any group size fills
-// 64-row tiles (four waves of 16 rows).  The keys are cut into parts of part_chunks chunks, one workgroup a
-// (part, sequence, kv head, tile); a sequence of several parts stores unnormalised partials that
-// tree_merge_kernel joins.  The products are the prefill kernels': S^T = K Q^T leaves a lane the scores of
+// 64-row tiles (four waves of 16 rows).  One workgroup a (sequence, kv head, tile), or, where those leave CUs
+// idle, a part of its keys: the lengths are on the device, so each workgroup works out the cut from them
+// (find_unit), and a tile's unnormalised partials are joined by its last workgroup or by tree_join_kernel.  The products are the prefill kernels': S^T = K Q^T leaves a lane the scores of
 // one row, O^T = V^T P^T takes them as its B operand from registers, the f32 operands go as three bf16
 // pieces (x = hi + mid + lo exactly), and the exponents' reference point moves only when a chunk's maximum
 // passes it by 2^8.  K and V of bf16 pools are exact in bf16 (three products a product), f32 pools' are split as well

@@ -617,12 +617,13 @@ int32_t fi_tree_plan(fi_context* ctx, const int32_t* d_parents, const int32_t* d
  * context_lens[b] - nodes and those of the nodes whose bits d_tree_mask[t] has set (any mask, not only
  * fi_tree_plan's; bits past the tree are ignored).  q/out f32 [T, Hq, D]; scores, softmax and sums are
  * f32, and f32, bf16 and mxfp4 pools are attended in f32 accuracy; any number of query heads per KV head.  A row that
- * sees no key is zero; K and V of a node that a row does not see do not reach it, whatever they hold.
+ * sees no key is zero; K and V of a node that a row does not see do not reach it, whatever they hold (over an mxfp4
+ * pool a scale outside [2^-18, 2^8], seen or not, changes the roundings of the rows of its 64-row tile).
  * max_context_len must bound every context_lens entry (it sizes the grid); positions of a longer one past it
  * are not attended, and it is reported as Runtime by fi_ctx_check_faults.  Keys are cut into parts by the launch's
  * sizes and joined in order, so equal calls give equal bits.  head_dim 32, 64 or 128 and max_context_len up to
- * 2^30 (Unsupported otherwise); q, out and the pools 16-byte aligned (InvalidLayout); scale positive and
- * finite (InvalidConfig).  Uses the context workspace. */
+ * 2^30, pools of up to 2^32 head rows (Unsupported otherwise); q, out and the pools 16-byte aligned
+ * (InvalidLayout); scale positive and finite (InvalidConfig).  Uses the context workspace. */
 int32_t fi_attn_tree_paged(fi_context* ctx, const float* d_q, const void* d_k_cache, const void* d_v_cache, int32_t kv_dtype,
                            const int32_t* d_block_tables, int32_t max_blocks_per_seq, const int32_t* d_cu_seqlens,
                            const int32_t* d_context_lens, const uint64_t* d_tree_mask, int32_t mask_words, int32_t num_seqs,
@@ -636,7 +637,7 @@ int32_t fi_attn_tree_paged(fi_context* ctx, const float* d_q, const void* d_k_ca
  * rho = p):
  *   d_draft_probs NULL (drafts that were not drawn: looked up, the draft's best): x is accepted when
  *     accept_u * sum(rho) < rho(x), and rho(x) becomes 0 otherwise;
- *   d_draft_probs f32 [T, draft_ld] (row t the distribution that node t's children were drawn from): x is
+ *   d_draft_probs f32 [T, draft_ld] (row t the distribution that node t's children were drawn from, finite and not negative): x is
  *     accepted when accept_u * c * q(x) < rho(x), c = sum(rho) / (1 - s), and rho becomes max(rho - c q, 0) otherwise; s is 0 when the children
  *     were drawn independently and the sum of q over the earlier ones when they were drawn without
  *     repetition (distinct != 0; a child behind s >= 1 is passed over).
@@ -652,7 +653,9 @@ int32_t fi_attn_tree_paged(fi_context* ctx, const float* d_q, const void* d_k_ca
  * gets -1, 0 and 0.  Where a sampled row that decides holds NaN or +inf, or a row nothing but -inf, the walk ends without a last
  * token (-1) and is reported as Runtime by fi_ctx_check_faults; so is a drafted token outside the vocabulary,
  * which is passed over, and a parent that is not before its node.  vocab at most 1048576 (Unsupported otherwise);
- * at most 65535 sequences.  Uses the context workspace. */
+ * at most 65535 sequences.  A walk goes from launch to launch: 1 + min(max_path, max_query_len - 1) of them, with
+ * d_draft_probs up to five more; at most two and six where num_seqs * max_query_len * vocab is up to 2 * 10^7.  Uses the context
+ * workspace. */
 int32_t fi_verify_drafts(fi_context* ctx, const float* d_logits, int32_t ld, int32_t vocab, const int32_t* d_tokens,
                          const int32_t* d_parents, const int32_t* d_cu_seqlens, int32_t num_seqs, int32_t max_query_len,
                          const float* d_temperature, const float* d_draft_probs, int32_t draft_ld, int32_t distinct,
