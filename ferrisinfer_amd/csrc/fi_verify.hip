@@ -67,7 +67,6 @@ struct Walk {
   int phase;
   int child;     // the last one rejected (tokens drawn)
   float ref;     // the reference point of the row's weights
-  double total;  // their sum
   double off, taken;  // a and s
 };
 
@@ -182,6 +181,12 @@ constexpr int kMaxVocab = kSegment * kMaxSegments;     // 1048576
 
 constexpr int64_t kAllRows = 20000000;  // logits up to which every row is summed in the first launch
 constexpr int kRejections = 4;          // launches for rejected drawn children
+constexpr int kDepth = 16;              // for rows behind the root's
+
+// A workgroup is one group of threads for a segment, or four of them side by side (verify_finish_kernel), of which each sums
+// a segment and all do the rest alike.
+__device__ __forceinline__ int thread_of() { return threadIdx.x % kEndThreads; }
+__device__ __forceinline__ int group_of() { return threadIdx.x / kEndThreads; }
 
 // Of a segment: the weights' sum by its maximum (by 0 where that is not finite; NaN if there is a logit that is NaN or
 // +inf), the maximum and its first index.
@@ -199,7 +204,7 @@ struct SegmentShared {
 
 // The workgroup's maximum; its first index too, if that is asked for.
 __device__ __forceinline__ void segment_top(SegmentShared& sh, float& top, int& first, bool index) {
-  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+  const int lane = thread_of() & 63, w = thread_of() >> 6;
   const float wave = wave_top(top);
   const int at = index ? first_of(top, wave, first) : 0;
   __syncthreads();  // the last use is over
@@ -220,7 +225,7 @@ __device__ __forceinline__ void segment_top(SegmentShared& sh, float& top, int& 
 __device__ __forceinline__ double segment_sum(SegmentShared& sh, double x) {
   x = wave_sum64(x);
   __syncthreads();  // the last use is over
-  if ((threadIdx.x & 63) == 0) sh.scan[threadIdx.x >> 6] = x;
+  if ((thread_of() & 63) == 0) sh.scan[thread_of() >> 6] = x;
   __syncthreads();
   double all = 0.0;
   for (int i = 0; i < kEndThreads / 64; ++i) all += sh.scan[i];
@@ -232,7 +237,7 @@ template <bool VEC, bool IN_ORDER>
 __device__ __forceinline__ void segment_load(const float* __restrict__ row, int begin, int vocab, float pad, float (&v)[kEndElems]) {
 #pragma unroll
   for (int j = 0; j < kEndElems / 4; ++j) {
-    const float4 x = quad_at<VEC>(row, begin + (IN_ORDER ? threadIdx.x * kEndElems + 4 * j : 4 * threadIdx.x + 4 * kEndThreads * j), vocab, pad);
+    const float4 x = quad_at<VEC>(row, begin + (IN_ORDER ? thread_of() * kEndElems + 4 * j : 4 * thread_of() + 4 * kEndThreads * j), vocab, pad);
     v[4 * j] = x.x;
     v[4 * j + 1] = x.y;
     v[4 * j + 2] = x.z;
@@ -240,13 +245,15 @@ __device__ __forceinline__ void segment_load(const float* __restrict__ row, int 
   }
 }
 // The place in the segment of a thread's element e, as they are loaded out of order.
-__device__ __forceinline__ int element_at(int e) { return 4 * threadIdx.x + 4 * kEndThreads * (e / 4) + e % 4; }
+__device__ __forceinline__ int element_at(int e) { return 4 * thread_of() + 4 * kEndThreads * (e / 4) + e % 4; }
 
 // ---------------------------------------------------------------- a launch's part
 
+constexpr int kGroups = 4;
+
 struct VerifyShared {
-  SegmentShared seg;
-  uint32_t out[kSegment / 32];            // tokens given and rejected
+  SegmentShared seg[kGroups];
+  uint32_t out[kGroups][kSegment / 32];   // tokens given and rejected
   uint64_t kids[fi::kMaxTreeNodes / 64];  // the node's children, as bits
   int tokens[fi::kMaxTreeNodes];
   float accept[fi::kMaxTreeNodes];
@@ -305,16 +312,16 @@ __device__ __forceinline__ void look_up(const VerifyArgs& a, const Sequence& s, 
 // Marks the tokens of a segment that were tried (tokens given, and rejected).
 __device__ __forceinline__ void mark_tried(const VerifyArgs& a, VerifyShared& sh, const Sequence& q, int node, int begin) {
   __syncthreads();
-  for (int i = threadIdx.x; i < kSegment / 32; i += kEndThreads) sh.out[i] = 0;
+  for (int i = thread_of(); i < kSegment / 32; i += kEndThreads) sh.out[group_of()][i] = 0;
   __syncthreads();
-  for (int j = node + 1 + threadIdx.x; j < q.n; j += kEndThreads) {
+  for (int j = node + 1 + thread_of(); j < q.n; j += kEndThreads) {
     const int x = a.tokens[q.first + j];
     if (a.parents[q.first + j] == node && x >= begin && x < min(begin + kSegment, a.vocab))
-      atomicOr(&sh.out[(x - begin) >> 5], 1u << ((x - begin) & 31));
+      atomicOr(&sh.out[group_of()][(x - begin) >> 5], 1u << ((x - begin) & 31));
   }
   __syncthreads();
 }
-__device__ __forceinline__ bool was_tried(const VerifyShared& sh, int e) { return ((sh.out[e >> 5] >> (e & 31)) & 1) != 0; }
+__device__ __forceinline__ bool was_tried(const VerifyShared& sh, int e) { return ((sh.out[group_of()][e >> 5] >> (e & 31)) & 1) != 0; }
 
 // The sums of a segment that the walk asks for; thread 0 stores them.  Meanwhile the thread's node is looked up, as a child of
 // node `from`: only the last workgroup needs it, but that then waits for nothing.
@@ -326,15 +333,15 @@ __device__ __forceinline__ void sum_segment(const VerifyArgs& a, VerifyShared& s
   float v[kEndElems], q[kEndElems];
   segment_load<VEC, false>(a.logits + (int64_t)(s.first + walk.node) * a.ld, begin, a.vocab, -INFINITY, v);
   if (less) segment_load<VEC, false>(a.probs + (int64_t)(s.first + walk.node) * a.ld_probs, begin, a.vocab, 0.0f, q);
-  mine = node_at(a, s, threadIdx.x);
-  look_up(a, s, from, threadIdx.x, mine);
+  mine = node_at(a, s, thread_of());
+  look_up(a, s, from, thread_of(), mine);
   double sum = 0.0;
   if (less) {
     const Weights by{s.k, s.k * walk.ref};
 #pragma unroll
     for (int e = 0; e < kEndElems; ++e) sum += __builtin_fmax(weight(v[e], by) - walk.off * q[e], 0.0);
-    sum = segment_sum(sh.seg, sum);
-    if (threadIdx.x == 0) put(&a.rests[(size_t)s.index * a.segments + segment], sum);
+    sum = segment_sum(sh.seg[group_of()], sum);
+    if (thread_of() == 0 && segment < a.segments) put(&a.rests[(size_t)s.index * a.segments + segment], sum);
     return;
   }
   float top = walk.ref;
@@ -356,13 +363,13 @@ __device__ __forceinline__ void sum_segment(const VerifyArgs& a, VerifyShared& s
       for (int e = kEndElems - 1; e >= 0; --e)  // (a thread's elements rise)
         if (v[e] == top) first = begin + element_at(e);
     }
-    segment_top(sh.seg, top, first, s.greedy);
+    segment_top(sh.seg[group_of()], top, first, s.greedy);
   }
   const Weights by{s.k, s.k * finite_or_zero(top)};
 #pragma unroll
   for (int e = 0; e < kEndElems; ++e) sum += weight(v[e], by);
-  sum = segment_sum(sh.seg, bad ? NAN : sum);
-  if (threadIdx.x != 0) return;
+  sum = segment_sum(sh.seg[group_of()], bad ? NAN : sum);
+  if (thread_of() != 0 || segment >= a.segments) return;
   if (walk.phase == kRest) {
     put(&a.rests[(size_t)s.index * a.segments + segment], sum);
   } else {
@@ -377,7 +384,7 @@ __device__ __forceinline__ void sum_segment(const VerifyArgs& a, VerifyShared& s
 __device__ __forceinline__ void find_children(const VerifyArgs& a, VerifyShared& sh, const Sequence& s, const Walk& walk, const Weights& by,
                                               const Node& mine) {
   __syncthreads();  // the last use is over
-  for (int j = threadIdx.x; j < (s.n + 63) / 64 * 64; j += kEndThreads) {  // whole waves
+  for (int j = thread_of(); j < (s.n + 63) / 64 * 64; j += kEndThreads) {  // whole waves
     Node x = mine;
     if (j >= kEndThreads) {
       x = node_at(a, s, j);
@@ -423,7 +430,7 @@ __device__ __forceinline__ double of_lane(double v, int lane) {
 template <bool VEC>
 __device__ __forceinline__ void pick_token(const VerifyArgs& a, VerifyShared& sh, const Sequence& s, const Walk& walk,
                                            const double (&part)[kPer], bool rest, float pick_u) {
-  const int tid = threadIdx.x, lane = tid & 63, per = (a.segments + 63) / 64;
+  const int tid = thread_of(), lane = tid & 63, per = (a.segments + 63) / 64;
   const float* row = a.logits + (int64_t)(s.first + walk.node) * a.ld;
   const bool less = rest && a.probs, without = rest && !a.probs;
   double share = 0.0;
@@ -437,7 +444,7 @@ __device__ __forceinline__ void pick_token(const VerifyArgs& a, VerifyShared& sh
   bool passed = false;
 #pragma unroll
   for (int i = 0; i < kPer; ++i) {
-    if (part[i] > kNothing && !passed) {
+    if (part[i] > kNothing / kPer && !passed) {
       segment = per * lane + i;
       before = at;
       passed = at + part[i] > target;
@@ -470,13 +477,13 @@ __device__ __forceinline__ void pick_token(const VerifyArgs& a, VerifyShared& sh
   }
   run = wave_scan64(here);
   __syncthreads();  // the last use is over
-  if (lane == 63) sh.seg.scan[tid >> 6] = run;
+  if (lane == 63) sh.seg[0].scan[tid >> 6] = run;
   __syncthreads();
   int wave = 0;
   passed = false;
 #pragma unroll
   for (int i = 0; i < kEndThreads / 64; ++i) {
-    const double all = sh.seg.scan[i];
+    const double all = sh.seg[0].scan[i];
     if (all > 0.0 && !passed) {
       wave = i;
       at = before;
@@ -510,7 +517,7 @@ __device__ __forceinline__ void pick_token(const VerifyArgs& a, VerifyShared& sh
 // need of each other is their lanes' nodes.
 template <bool VEC>
 __device__ __forceinline__ void advance(const VerifyArgs& a, VerifyShared& sh, const Sequence& s, Walk& walk, Node& mine, float pick_u) {
-  const int tid = threadIdx.x, lane = tid & 63, per = (a.segments + 63) / 64;
+  const int tid = thread_of(), lane = tid & 63, per = (a.segments + 63) / 64;
   while (true) {  // mine is looked up at the walk's node
     const bool rest = walk.phase == kRest;
     double part[kPer] = {}, total;
@@ -557,7 +564,6 @@ __device__ __forceinline__ void advance(const VerifyArgs& a, VerifyShared& sh, c
         walk.phase = kDone;
         return;
       }
-      walk.total = total;  // 1 at least: the largest logit's
     }
     // the children
     int accepted = -1;
@@ -604,7 +610,7 @@ __device__ __forceinline__ void advance(const VerifyArgs& a, VerifyShared& sh, c
         a.out_tokens[(size_t)s.index * (a.max_path + 1) + walk.count] = sh.tokens[accepted];
       }
       if (tid == 0) a.out_count[s.index] = walk.count + 1;
-      walk = Walk{accepted, walk.count + 1, kTotal, -1, 0.0f, 0.0, 0.0, 0.0};
+      walk = Walk{accepted, walk.count + 1, kTotal, -1, 0.0f, 0.0, 0.0};
       if (!a.all_rows) return;
       look_up(a, s, walk.node, tid, mine);
       continue;
@@ -629,7 +635,7 @@ __device__ __forceinline__ void advance(const VerifyArgs& a, VerifyShared& sh, c
 
 // What a sequence's first advance finds: nothing accepted yet.
 __device__ __forceinline__ void begin_outputs(const VerifyArgs& a, const Sequence& s, const Node& mine) {
-  const int tid = threadIdx.x;
+  const int tid = thread_of();
   for (int i = tid; i < a.max_path; i += kEndThreads) a.out_path[(size_t)s.index * a.max_path + i] = -1;
   for (int i = tid; i <= a.max_path; i += kEndThreads) a.out_tokens[(size_t)s.index * (a.max_path + 1) + i] = -1;
   if (tid == 0) {
@@ -654,7 +660,7 @@ __global__ __launch_bounds__(kEndThreads) void verify_pass_kernel(VerifyArgs a) 
   const bool rows = FIRST && a.all_rows;
   const int seq = rows ? blockIdx.y / a.max_query_len : blockIdx.y;
   const int node = rows ? blockIdx.y - seq * a.max_query_len : 0;
-  Walk walk{node, 0, kTotal, -1, 0.0f, 0.0, 0.0, 0.0};
+  Walk walk{node, 0, kTotal, -1, 0.0f, 0.0, 0.0};
   if (!FIRST) walk = a.walks[seq];
   const Sequence s = sequence_of(a, seq);
   const float pick_u = a.pick_u[seq];
@@ -670,7 +676,7 @@ __global__ __launch_bounds__(kEndThreads) void verify_pass_kernel(VerifyArgs a) 
   Node mine;
   sum_segment<VEC>(a, sh, s, walk, blockIdx.x, from, mine);
   if (threadIdx.x == 0) {
-    __builtin_amdgcn_s_waitcnt(0);  // the sums are there before the arrival
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // the sums are there before the arrival
     // (the last of `of` to arrive)
     auto last_of = [&](int counter, int of) {
       unsigned* at = a.counters + (size_t)counter * a.apart;
@@ -688,17 +694,17 @@ __global__ __launch_bounds__(kEndThreads) void verify_pass_kernel(VerifyArgs a) 
   if (threadIdx.x == 0) a.walks[seq] = walk;
 }
 
-// The walks that are left, a workgroup each.
+// The walks that are left, a workgroup each: 40 us a row of 128k logits (48 with two groups, 72 with one).
 template <bool VEC>
-__global__ __launch_bounds__(kEndThreads) void verify_finish_kernel(VerifyArgs a) {
+__global__ __launch_bounds__(kGroups * kEndThreads) void verify_finish_kernel(VerifyArgs a) {
   __shared__ VerifyShared sh;
   Walk walk = a.walks[blockIdx.x];
   if (walk.phase == kDone) return;
   const Sequence s = sequence_of(a, blockIdx.x);
   while (walk.phase != kDone) {  // each round tries a child, goes to one, or ends the walk
     Node mine;
-    for (int i = 0; i < a.segments; ++i) sum_segment<VEC>(a, sh, s, walk, i, walk.node, mine);
-    if (threadIdx.x == 0) __builtin_amdgcn_s_waitcnt(0);
+    for (int i = 0; i < a.segments; i += kGroups) sum_segment<VEC>(a, sh, s, walk, i + group_of(), walk.node, mine);
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     __syncthreads();
     advance<VEC>(a, sh, s, walk, mine, a.pick_u[blockIdx.x]);
     __syncthreads();
@@ -773,8 +779,9 @@ int32_t fi_verify_drafts(fi_context* ctx, const float* d_logits, int32_t ld, int
   const int needed = a.all_rows ? (d_draft_probs ? max_query_len - 1 : 1)
                                 : (d_draft_probs && depth > 0 ? max_query_len - 1 : depth);
   // Launches for four rejections, then one that takes what is left, a workgroup a walk: 16 trees of 32 nodes 96 us
-  // (109 with launches for eight, 280 with none).
-  const int passes = std::min(needed, (a.all_rows ? 0 : depth) + kRejections);
+  // (109 with launches for eight, 280 with none).  max_path may be a loose bound, and a launch that finds nothing to do costs
+  // 1 to 3 us: rows behind the first kDepth are left to that as well.
+  const int passes = std::min(needed, (a.all_rows ? 0 : std::min(depth, kDepth)) + kRejections);
   auto launch = [&](auto vec_rows) {
     constexpr bool VEC = decltype(vec_rows)::value;
     const unsigned segments = static_cast<unsigned>(a.segments);
@@ -782,7 +789,7 @@ int32_t fi_verify_drafts(fi_context* ctx, const float* d_logits, int32_t ld, int
                        dim3(kEndThreads), 0, ctx->stream, a);
     for (int i = 0; i < passes; ++i)
       hipLaunchKernelGGL((verify_pass_kernel<VEC, false>), dim3(segments, num_seqs), dim3(kEndThreads), 0, ctx->stream, a);
-    if (passes < needed) hipLaunchKernelGGL((verify_finish_kernel<VEC>), dim3(num_seqs), dim3(kEndThreads), 0, ctx->stream, a);
+    if (passes < needed) hipLaunchKernelGGL((verify_finish_kernel<VEC>), dim3(num_seqs), dim3(kGroups * kEndThreads), 0, ctx->stream, a);
   };
   if (vec)
     launch(std::true_type{});

@@ -653,9 +653,10 @@ int32_t fi_attn_tree_paged(fi_context* ctx, const float* d_q, const void* d_k_ca
  * gets -1, 0 and 0.  Where a sampled row that decides holds NaN or +inf, or a row nothing but -inf, the walk ends without a last
  * token (-1) and is reported as Runtime by fi_ctx_check_faults; so is a drafted token outside the vocabulary,
  * which is passed over, and a parent that is not before its node.  vocab at most 1048576 (Unsupported otherwise);
- * at most 65535 sequences.  A walk goes from launch to launch: 1 + min(max_path, max_query_len - 1) of them, with
- * d_draft_probs up to five more; at most two and six where num_seqs * max_query_len * vocab is up to 2 * 10^7.  Uses the context
- * workspace. */
+ * at most 65535 sequences.  A walk goes from launch to launch: 1 + min(max_path, max_query_len - 1) of them, 22 at most, with
+ * d_draft_probs up to five more; two and six where num_seqs * max_query_len * vocab is up to 2 * 10^7.  What they leave
+ * (a path of more than 20 tokens, more than four rejected drawn tokens) one workgroup a sequence finishes, at some 40 us
+ * a row.  Uses the context workspace. */
 int32_t fi_verify_drafts(fi_context* ctx, const float* d_logits, int32_t ld, int32_t vocab, const int32_t* d_tokens,
                          const int32_t* d_parents, const int32_t* d_cu_seqlens, int32_t num_seqs, int32_t max_query_len,
                          const float* d_temperature, const float* d_draft_probs, int32_t draft_ld, int32_t distinct,

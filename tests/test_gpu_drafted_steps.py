@@ -219,6 +219,31 @@ def test_verify_of_many_rows(gpu_ctx, mode):
         assert all(bool((x[b] == y[0]).all()) for x, y in zip(out, alone)), b
 
 
+@pytest.mark.parametrize("mode", ["given", "drawn", "distinct"])
+def test_verify_of_long_paths(gpu_ctx, mode):
+    """Paths of more tokens than have a launch each: sequences that end before, there, and behind."""
+    rng = np.random.default_rng(51)
+    nodes, vocab = [40, 40, 23, 40], 130000
+    assert len(nodes) * max(nodes) * vocab > 20000000
+    temperature = np.array([1.0, 0.0, 0.8, 0.7])
+    s = inputs(rng, nodes, vocab, mode, temperature)
+    at = 0
+    for b, n in enumerate(nodes):  # chains of the likeliest tokens, accepted whatever u
+        for i in range(1, n):
+            s["parents"][at + i] = i - 1
+            s["tokens"][at + i] = s["logits"][at + i - 1].argmax()
+        s["accept"][at:at + n] = 0.0
+        at += n
+    s["tokens"][80 + 23 + 9] = (s["tokens"][80 + 23 + 9] + 1) % vocab  # the last one's ninth is not, mostly
+    s["accept"][80 + 23 + 9] = 0.999
+    for longest in (39, 18, 3):
+        out = run(gpu_ctx, s, nodes, temperature, mode == "distinct", max_path=longest)
+        gpu_ctx.sync()
+        gpu_ctx.check_faults()
+        assert out[2].tolist()[:2] == [longest] * 2
+        check(out, s, nodes, temperature, mode == "distinct", max_path=longest, what=longest)
+
+
 @pytest.mark.parametrize("mode", ["given", "drawn"])
 @pytest.mark.parametrize("vocab", [262144, 262145, 600004, 1048576])
 def test_verify_of_wide_vocabularies(gpu_ctx, mode, vocab):
