@@ -778,8 +778,8 @@ int32_t fi_verify_drafts(fi_context* ctx, const float* d_logits, int32_t ld, int
   const int depth = std::min(max_path, std::max(max_query_len - 1, 0));
   const int needed = a.all_rows ? (d_draft_probs ? max_query_len - 1 : 1)
                                 : (d_draft_probs && depth > 0 ? max_query_len - 1 : depth);
-  // Launches for four rejections, then one that takes what is left, a workgroup a walk: 16 trees of 32 nodes 96 us
-  // (109 with launches for eight, 280 with none).  max_path may be a loose bound, and a launch that finds nothing to do costs
+  // Launches for four rejections, then one that takes what is left, a workgroup a walk: 16 trees of up to 32 nodes, drawn, 97 us
+  // in the mean of twelve (110 with launches for two, 98 for six, 103 for eight), 64 of them 169 (193, 166, 169).  max_path may be a loose bound, and a launch that finds nothing to do costs
   // 1 to 3 us: rows behind the first kDepth are left to that as well.
   const int passes = std::min(needed, (a.all_rows ? 0 : std::min(depth, kDepth)) + kRejections);
   auto launch = [&](auto vec_rows) {
