@@ -6,7 +6,8 @@
 // Rows are packed: row r of a (sequence, kv head) is head r % G of node r / G, so that any group size fills
 // 64-row tiles (four waves of 16 rows).  One workgroup a (sequence, kv head, tile), or, where those leave CUs
 // idle, a part of its keys: the lengths are on the device, so each workgroup works out the cut from them
-// (find_unit), and a tile's unnormalised partials are joined by its last workgroup or by tree_join_kernel.  The products are the prefill kernels': S^T = K Q^T leaves a lane the scores of
+// (find_unit), and a tile's unnormalised partials are joined by its last workgroup, or by a launch of their own
+// (tree_join_rows_kernel, tree_join_kernel).  The products are the prefill kernels': S^T = K Q^T leaves a lane the scores of
 // one row, O^T = V^T P^T takes them as its B operand from registers, the f32 operands go as three bf16
 // pieces (x = hi + mid + lo exactly), and the exponents' reference point moves only when a chunk's maximum
 // passes it by 2^8.  K and V of bf16 pools are exact in bf16 (three products a product), f32 pools' are split as well
@@ -215,6 +216,7 @@ struct Unit {
   int nodes, kend, c_lo, c_hi;
 };
 
+constexpr int kRowJoins = 128;      // tiles up to which the join is a workgroup a row
 constexpr int kPlanned = kThreads;  // sequences of a planned launch, at most: a thread each
 
 struct PlanShared {
@@ -1018,7 +1020,7 @@ __global__ __launch_bounds__(kThreads, D == 128 && POOL == FI_DTYPE_F32 ? 2 : 3)
   attend_piece<D, POOL, false>(a, u, sh);
 }
 
-// The join in a launch of its own: 256 quads of a (sequence, tile, kv head) at a time.
+// The join in a launch of its own, of many tiles: 256 quads of a (sequence, tile, kv head) at a time.
 template <int D>
 __global__ __launch_bounds__(kThreads) void tree_join_kernel(TreeArgs a, int units) {
   constexpr int BLOCKS = kRows * (D / 4) / kThreads;
@@ -1031,6 +1033,63 @@ __global__ __launch_bounds__(kThreads) void tree_join_kernel(TreeArgs a, int uni
     const int tiles = (min(t.nodes, a.max_query_len) * a.group + kRows - 1) / kRows;
     if (tile >= tiles) continue;
     join_parts<D, 1, false>(a, t, kvh, tile, (plan.x + tile) * a.hkv + kvh, tiles * a.hkv, plan.y, share * kThreads + threadIdx.x, 0);
+  }
+}
+
+// The same where few tiles have many parts: a workgroup a row, whose threads share the parts (strands of every S-th, each in
+// order, then joined in pairs), so that the partials' way is not one part behind the other: one sequence of 100000
+// tokens, 2 kv heads of 64, 320 parts: 7 us, 52 with 256 quads a workgroup.
+template <int D>
+__global__ __launch_bounds__(kThreads) void tree_join_rows_kernel(TreeArgs a, int rows) {
+  constexpr int DQ = D / 4, S = kThreads / DQ, N = 4;
+  __shared__ float4 s_acc[S][DQ];
+  __shared__ float2 s_ml[S];
+  const int q = threadIdx.x % DQ, strand = threadIdx.x / DQ;
+  for (int i = blockIdx.x; i < rows; i += gridDim.x) {  // what is skipped is so for the workgroup
+    const int kvh = i / kRows % a.hkv, tile = i / kRows / a.hkv % a.ntiles, seq = i / kRows / a.hkv / a.ntiles;
+    const int2 plan = a.plan[seq];
+    if (plan.y <= 1) continue;
+    const fi::TreeSpan t = fi::tree_span(a.cu_seqlens, a.context_lens, seq);
+    const int nodes = min(t.nodes, a.max_query_len), tiles = (nodes * a.group + kRows - 1) / kRows;
+    const int r = tile * kRows + i % kRows, node = static_cast<int>(a.by_group.div(r));
+    if (node >= nodes) continue;
+    const size_t first = (size_t)((plan.x + tile) * a.hkv + kvh) * kRows + i % kRows, step = (size_t)tiles * a.hkv * kRows;
+    float mx = -INFINITY, l = 0.0f;
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+    auto add = [&](float2 ml, float4 x) {
+      if (ml.x == -INFINITY) return;
+      const float to = fmaxf(mx, ml.x), old = __builtin_amdgcn_exp2f(mx - to), now = __builtin_amdgcn_exp2f(ml.x - to);
+      mx = to;
+      l = l * old + now * ml.y;
+      acc = make_float4(acc.x * old + now * x.x, acc.y * old + now * x.y, acc.z * old + now * x.z, acc.w * old + now * x.w);
+    };
+    for (int p0 = strand; p0 < plan.y; p0 += N * S) {
+      float2 ml[N];
+      float4 x[N];
+#pragma unroll
+      for (int n = 0; n < N; ++n) {
+        const size_t row = first + step * min(p0 + n * S, plan.y - 1);
+        ml[n] = get2<false>(a.part_ml + row * 2);
+        x[n] = *reinterpret_cast<const float4*>(a.part_acc + row * D + 4 * q);
+      }
+#pragma unroll
+      for (int n = 0; n < N; ++n)
+        if (p0 + n * S < plan.y) add(ml[n], x[n]);
+    }
+    for (int half = S / 2; half >= 1; half /= 2) {
+      __syncthreads();  // the last step's (row's) readers are done
+      if (strand >= half && strand < 2 * half) {
+        s_acc[strand][q] = acc;
+        if (q == 0) s_ml[strand] = make_float2(mx, l);
+      }
+      __syncthreads();
+      if (strand < half) add(s_ml[strand + half], s_acc[strand + half][q]);
+    }
+    if (strand != 0) continue;
+    const int head = kvh * a.group + (r - node * a.group);
+    const float inv = l == 0.0f && sees_nothing(a, t, key_end(a, t), a.mask + (size_t)(t.first + node) * a.words) ? 0.0f : 1.0f / l;
+    *reinterpret_cast<float4*>(a.out + ((size_t)(t.first + node) * a.hq + head) * D + 4 * q) =
+        make_float4(acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv);
   }
 }
 
@@ -1060,9 +1119,11 @@ int32_t launch_tree(fi_context* ctx, TreeArgs& a) {
     FI_TRY(fi::ensure_workspace(ctx, acc + ml + kPlanned * sizeof(int2)));
     a.part_acc = static_cast<float*>(ctx->workspace);
     a.part_ml = reinterpret_cast<float*>(static_cast<char*>(ctx->workspace) + acc);
-    // The last workgroup of a tile joins up to eight parts by itself; more take it longer than a launch of its own
-    // (one sequence of 4000 tokens, 16 parts: 38.3 us against 27.2; of 700, six parts: 18.6 against 20.1).
-    join = chunks > 8 * a.least;
+    // The last workgroup of a tile joins its parts by itself where they are few and tiles many; otherwise a launch does
+    // (one sequence of 700 tokens over 14/2 heads of 64, f32, six parts: 19.1 us by itself, 16.6 by a launch; 32
+    // sequences of 200 to 1900 over 32/8 heads of 128, 256 tiles of up to eight: 64.5 and 59.6; 60 of them, 480 tiles: 75.4
+    // and 80.1).
+    join = chunks > (tiles <= cus ? 4 : 8) * a.least;
     if (join)
       a.plan = reinterpret_cast<int2*>(static_cast<char*>(ctx->workspace) + acc + ml);
     else
@@ -1073,7 +1134,12 @@ int32_t launch_tree(fi_context* ctx, TreeArgs& a) {
   else
     hipLaunchKernelGGL((attn_tree_kernel<D, POOL>), dim3(static_cast<unsigned>(grid)), dim3(kThreads), 0, ctx->stream, a);
   FI_CHECK_LAUNCH("attn_tree_kernel");
-  if (join) {
+  if (join && tiles <= kRowJoins) {
+    const int64_t rows = tiles * kRows;
+    hipLaunchKernelGGL((tree_join_rows_kernel<D>), dim3(static_cast<unsigned>(std::min<int64_t>(rows, 8 * cus))), dim3(kThreads), 0,
+                       ctx->stream, a, static_cast<int>(rows));
+    FI_CHECK_LAUNCH("tree_join_rows_kernel");
+  } else if (join) {
     const int64_t blocks = std::min<int64_t>(tiles * (kRows * (D / 4) / kThreads), 8 * cus);
     hipLaunchKernelGGL((tree_join_kernel<D>), dim3(static_cast<unsigned>(blocks)), dim3(kThreads), 0, ctx->stream, a,
                        static_cast<int>(tiles));

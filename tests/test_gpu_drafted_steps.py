@@ -344,6 +344,8 @@ LAYOUTS = {
     "nothing but empty ones": ([(0, 0)] * 3, 4, 2, 32),
     "joined in the launch": ([(1900, 3), (1800, 70), (0, 2)], 8, 2, 64),
     "joined by a launch": ([(2100, 3), (1800, 70), (0, 2)], 8, 2, 64),
+    "joined by a launch of many tiles": ([(6000, 4)] + [(20, 3)] * 40, 8, 4, 32),
+    "joined in a launch of many tiles": ([(1900, 9)] + [(20, 3)] * 70, 8, 4, 32),
     "several tiles a sequence": ([(1000, 200), (30, 140)], 8, 2, 32),
 }
 
