@@ -553,7 +553,7 @@ struct Row {
       top = fmaxf(top, fi::lane_xor32(top, lane));
       const int by = min(14 - __builtin_amdgcn_frexp_expf(top), 126);
       up = __builtin_ldexpf(1.0f, by);
-      c2 = __builtin_ldexpf(c2 / UP, -by);
+      c2 = fmaxf(__builtin_ldexpf(c2 / UP, -by), 1.17549435e-38f);  // 0 would make NaN of what is hidden; scores are below 2^40
     }
 #pragma unroll
     for (int s = 0; s < DS; ++s) {

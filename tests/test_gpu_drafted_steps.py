@@ -393,6 +393,24 @@ SCALES = {
 }
 
 
+@pytest.mark.parametrize("kind", ["f32", "bf16", "mxfp4"])
+@pytest.mark.parametrize("scale,size", [(1e-8, 1e-36), (1e-12, 1e-30), (1e20, 1e-20), (1e-20, 1e20), (1e-30, 1e-38), (0.125, 1e-42)])
+def test_small_and_large_scales_and_queries(gpu_ctx, kind, scale, size):
+    """The scale and Q's sizes make up for each other, or leave scores of nothing: every key that is seen weighs the same."""
+    rng = np.random.default_rng(61)
+    hq, hkv, d, prefix, n = 4, 2, 64, 90, 21
+    keys, nb = prefix + n, 9
+    (kd, kv), (vd, vv) = pool_of(rng, kind, nb, hkv, BS, d), pool_of(rng, kind, nb, hkv, BS, d)
+    tables = tables_of(rng, [keys], BS, nb)
+    trees, mask = trees_of(rng, [n])
+    q = (rng.standard_normal((n, hq, d)) * size).astype(np.float32)
+    q[4] = 0.0
+    got = checked(gpu_ctx, attend(gpu_ctx, kind, q, (kd, vd), tables, [n], [keys], mask, hkv, BS, nb, scale))
+    k, v = (fp4.rows_of(x, tables[0], keys, BS) for x in (kv, vv))
+    shown = ref.visible(ref.ancestors(trees[0]), prefix, keys)
+    ref.check_attention(got, q, k, v, shown, float(np.float32(scale)), PIECES[kind], (scale, size))
+
+
 @pytest.mark.parametrize("d,prefix", [(32, 500), (64, 490), (128, 497), (128, 5000)])
 @pytest.mark.parametrize("scales", list(SCALES))
 def test_scales_of_four_bit_groups(gpu_ctx, scales, d, prefix):
