@@ -244,6 +244,52 @@ def test_verify_of_long_paths(gpu_ctx, mode):
         check(out, s, nodes, temperature, mode == "distinct", max_path=longest, what=longest)
 
 
+def test_verify_of_many_rows_captured(gpu_ctx):
+    """All of the launches in a graph: rows, rejections, what is left; replayed with other random numbers."""
+    import torch
+
+    from ferrisinfer_amd import Context
+
+    rng = np.random.default_rng(54)
+    nodes, vocab, temperature = [40, 12, 33, 25], 130000, np.array([1.0, 0.7, 0.0, 1.3])
+    assert len(nodes) * max(nodes) * vocab > 20000000
+    s = inputs(rng, nodes, vocab, "drawn", temperature)
+    s["parents"][1:40] = 0  # a root of many children
+    s["tokens"][1:40] = rng.choice(vocab, 39, replace=False)
+    stream = torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(stream):
+        ctx = Context(0)
+        held = {k: dev(v) for k, v in s.items()}
+        cu, heat = dev(np.concatenate([[0], np.cumsum(nodes)]).astype(np.int32)), dev(temperature.astype(np.float32))
+        i = lambda *n: torch.zeros(n, dtype=torch.int32, device="cuda")  # noqa: E731
+
+        def call(out):
+            ctx.verify_drafts(held["logits"], held["tokens"], held["parents"], cu, 40, heat, held["accept"], held["pick"], held["probs"],
+                              False, *out)
+
+        out, eager = ([i(4, 21), i(4, 20), i(4), torch.zeros(4, device="cuda")] for _ in range(2))
+        call(out)
+        graph = torch.cuda.CUDAGraph()
+        stream.synchronize()
+        with torch.cuda.graph(graph, stream=stream):
+            call(out)
+        for k in range(4):
+            new = rng.random(sum(nodes)).astype(np.float32), rng.random(4).astype(np.float32)
+            if k == 1:
+                new[0][:] = 0.0  # the longest paths
+            held["accept"].copy_(dev(new[0]))
+            held["pick"].copy_(dev(new[1]))
+            call(eager)
+            stream.synchronize()
+            graph.replay()
+            stream.synchronize()
+            assert all(torch.equal(x, y) for x, y in zip(out, eager)), k
+            check(out, dict(s, accept=new[0], pick=new[1]), nodes, temperature, max_path=20, what=k)
+        ctx.check_faults()
+        ctx.close()
+
+
 @pytest.mark.parametrize("mode", ["given", "drawn"])
 @pytest.mark.parametrize("vocab", [262144, 262145, 600004, 1048576])
 def test_verify_of_wide_vocabularies(gpu_ctx, mode, vocab):
