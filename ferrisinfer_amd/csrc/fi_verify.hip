@@ -173,11 +173,13 @@ __device__ __forceinline__ float4 quad_at(const float* __restrict__ row, int at,
 
 // ---------------------------------------------------------------- segments of a row
 
+// 16 elements a thread: 64 sequences of five rows of 128k logits 88 us (8: 97, 32: 109), 16 trees 96 (93, 119), one
+// sequence of 152k 21 (22, 23).
 constexpr int kEndThreads = 256;
-constexpr int kEndElems = 16;                          // consecutive elements a thread
-constexpr int kSegment = kEndThreads * kEndElems;      // 4096
-constexpr int kMaxSegments = 256;                      // a thread each when they are joined
-constexpr int kMaxVocab = kSegment * kMaxSegments;     // 1048576
+constexpr int kEndElems = 16;
+constexpr int kSegment = kEndThreads * kEndElems;   // 4096
+constexpr int kMaxSegments = 256;                   // four a lane when they are joined
+constexpr int kMaxVocab = kSegment * kMaxSegments;  // 1048576
 
 constexpr int64_t kAllRows = 20000000;  // logits up to which every row is summed in the first launch
 constexpr int kRejections = 4;          // launches for rejected drawn children
