@@ -70,8 +70,8 @@ struct Walk {
   double off, taken;  // a and s
 };
 
-// A row's weights are 2^(k l - c): k = log2(e) / temperature, l the logit, c = k times the reference point.  (c is one
-// rounded number for the whole row, so that its rounding is a common factor of them.)
+// Weights by a reference point are 2^(k l - c): k = log2(e) / temperature, l the logit, c = k times the point.  c is one
+// rounded number, so that its rounding is a common factor of them.
 struct Weights {
   double k, c;
 };
@@ -81,6 +81,18 @@ constexpr float kMinTemperature = 1.1920929e-7f;  // as sampling has it (f32::EP
 
 __device__ __forceinline__ double row_scale(float temperature) {
   return kLog2E / static_cast<double>(fmaxf(temperature, kMinTemperature));
+}
+
+// That factor must stay near 1: where a segment is all masked by a finite number, c of 2^128 is off by up to 2^75, which is
+// no exponent.  From |c| = 2^40 on (it is within 2^-13 there) the next lower logit is 2^-24 of the point below it at least,
+// 2^16 in k l, and weighs nothing by the largest one.  So a k of half that does as well, and a power of two makes k l and c exact.
+__device__ __forceinline__ Weights weights_by(double k, float point) {
+  Weights w{k, k * point};
+  if (__builtin_fabs(w.c) >= 1099511627776.0) {  // the same for all threads that sum together
+    w.k = __builtin_ldexp(0.5, __builtin_amdgcn_frexp_exp(k));
+    w.c = w.k * point;
+  }
+  return w;
 }
 
 // 2^x for x in [-1100, 1000]: 2^n times a polynomial in f, |f| <= 1/2, through 2^f at the eleven Chebyshev
@@ -339,7 +351,7 @@ __device__ __forceinline__ void sum_segment(const VerifyArgs& a, VerifyShared& s
   look_up(a, s, from, thread_of(), mine);
   double sum = 0.0;
   if (less) {
-    const Weights by{s.k, s.k * walk.ref};
+    const Weights by = weights_by(s.k, walk.ref);
 #pragma unroll
     for (int e = 0; e < kEndElems; ++e) sum += __builtin_fmax(weight(v[e], by) - walk.off * q[e], 0.0);
     sum = segment_sum(sh.seg[group_of()], sum);
@@ -367,7 +379,7 @@ __device__ __forceinline__ void sum_segment(const VerifyArgs& a, VerifyShared& s
     }
     segment_top(sh.seg[group_of()], top, first, s.greedy);
   }
-  const Weights by{s.k, s.k * finite_or_zero(top)};
+  const Weights by = weights_by(s.k, finite_or_zero(top));
 #pragma unroll
   for (int e = 0; e < kEndElems; ++e) sum += weight(v[e], by);
   sum = segment_sum(sh.seg[group_of()], bad ? NAN : sum);
@@ -469,7 +481,7 @@ __device__ __forceinline__ void pick_token(const VerifyArgs& a, VerifyShared& sh
 #pragma unroll
     for (int e = 0; e < kEndElems; ++e) v[e] = was_tried(sh, tid * kEndElems + e) ? -INFINITY : v[e];
   }
-  const Weights by{s.k, s.k * walk.ref};
+  const Weights by = weights_by(s.k, walk.ref);
   const double off = less ? walk.off : 0.0;
   double left[kEndElems], here = 0.0;
 #pragma unroll
@@ -571,7 +583,7 @@ __device__ __forceinline__ void advance(const VerifyArgs& a, VerifyShared& sh, c
     int accepted = -1;
     bool rejected = false;
     if (walk.count < a.max_path && (!rest || a.probs)) {
-      find_children(a, sh, s, walk, Weights{s.k, s.k * walk.ref}, mine);
+      find_children(a, sh, s, walk, weights_by(s.k, walk.ref), mine);
       if (s.greedy) {
         int best = 0x7fffffff;
         for (int j = lane; j < s.n; j += 64)

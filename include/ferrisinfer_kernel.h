@@ -646,7 +646,7 @@ int32_t fi_attn_tree_paged(fi_context* ctx, const float* d_q, const void* d_k_ca
  * nothing is left; the last index with any for a pick_u of 1 or more).  d_accept_u f32 [T] (of the drafted nodes) and d_pick_u
  * f32 [B] are uniform in [0, 1), and do not count where temperature[b] <= 0 (a child is accepted when it is the first of the
  * largest).  Comparisons are decided in 64-bit accuracy.  Logits of -inf have no
- * probability: mask them to sample from a top-k or top-p set.
+ * probability: mask them (or with a finite number far below the others) to sample from a top-k or top-p set.
  * Outputs: d_out_tokens int32 [B, max_path + 1], the accepted tokens, then the last one, then -1; d_out_path
  * int32 [B, max_path], the accepted nodes, then -1; d_out_count int32 [B], how many; d_out_prob f32 [B], the last
  * token's probability under rho / sum(rho) (greedy: p's softmax at temperature 1).  A sequence without rows

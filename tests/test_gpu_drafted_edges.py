@@ -1,0 +1,57 @@
+"""Steps over drafted tokens where a draft, a mask or a length is at the end of what is allowed."""
+import numpy as np
+import pytest
+
+from test_gpu_verify_drafts import check, inputs, run
+
+pytestmark = pytest.mark.gpu
+
+
+FAR = [np.finfo(np.float32).min, np.float32(-1e30), np.float32(-1e20), np.float32(-1e9)]
+
+
+@pytest.mark.parametrize("mode", ["given", "drawn", "distinct"])
+@pytest.mark.parametrize("far", FAR, ids=lambda x: f"{x:.0e}")
+@pytest.mark.parametrize("seqs,vocab", [(16, 20000), (16, 128256)])
+def test_finite_masks(gpu_ctx, mode, far, seqs, vocab):
+    """Tokens that are masked by a finite number: most segments of a row hold nothing else, and some rows.  The
+    temperatures are those at which such a number's product with 1 / temperature is rounded, up and down."""
+    rng = np.random.default_rng(31)
+    nodes = [11] * seqs  # 23 million logits are summed a row a launch, 3.5 million all at once
+    temperature = np.resize([0.0, 0.3, 0.6, 0.7, 0.8, 1.0, 1.3, 1e-9], seqs)
+    s = inputs(rng, nodes, vocab, mode, temperature)
+    x = s["logits"].reshape(seqs, 11, vocab)
+    kept = np.argsort(-x, -1)[..., :50]
+    masked = np.full_like(x, far)
+    np.put_along_axis(masked, kept, np.take_along_axis(x, kept, -1), -1)
+    x[:] = masked
+    x[3, :, 5000:] = far                # all but the first tokens, some of them masked as well
+    x[4] = far                          # rows of nothing else: all alike
+    x[6, :, :vocab - 40] = far
+    x[6, :, vocab - 40:] = -7.5
+    x[7, :, :9000] = np.float32(-np.inf)  # both kinds
+    x[9, 0] = -far                      # and the other end
+    x[10, :, 17] = -far
+    out = run(gpu_ctx, s, nodes, temperature, mode == "distinct")
+    gpu_ctx.sync()
+    gpu_ctx.check_faults()
+    check(out, s, nodes, temperature, mode == "distinct")
+
+
+@pytest.mark.parametrize("mode", ["given", "drawn"])
+def test_large_logits(gpu_ctx, mode):
+    """Logits of any size that f32 has: only the largest ones weigh anything where f32's steps are wide."""
+    rng = np.random.default_rng(32)
+    sizes = [1e4, 1e7, 1e9, 1e11, 1e13, 1e15, 1e20, 1e30, 3e38]
+    seqs, vocab = 2 * len(sizes), 9000
+    nodes, temperature = [4] * seqs, np.resize([1.0, 0.37], seqs)
+    s = inputs(rng, nodes, vocab, mode, temperature, liked=False)
+    x = s["logits"].reshape(seqs, 4, vocab)
+    for b in range(seqs):
+        x[b] = (rng.integers(-40, 1, (4, vocab)) * 2.0 ** -6 + rng.choice([-1, 1])) * sizes[b // 2]
+        s["tokens"].reshape(seqs, 4)[b, 1:] = x[b].argmax(-1)[s["parents"].reshape(seqs, 4)[b, 1:]]
+    x[np.isinf(x)] = np.finfo(np.float32).max
+    out = run(gpu_ctx, s, nodes, temperature)
+    gpu_ctx.sync()
+    gpu_ctx.check_faults()
+    check(out, s, nodes, temperature)
