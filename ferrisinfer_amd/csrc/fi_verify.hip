@@ -230,7 +230,7 @@ __device__ __forceinline__ void segment_top(SegmentShared& sh, float& top, int& 
   top = -INFINITY;
   first = 0x7fffffff;
   for (int i = 0; i < kEndThreads / 64; ++i)
-    if (sh.tops[i] > top) {
+    if (sh.tops[i] > top || (sh.tops[i] == top && sh.firsts[i] < first)) {  // (a wave's elements are not all before the next one's)
       top = sh.tops[i];
       first = sh.firsts[i];
     }

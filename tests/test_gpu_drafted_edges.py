@@ -55,3 +55,28 @@ def test_large_logits(gpu_ctx, mode):
     gpu_ctx.sync()
     gpu_ctx.check_faults()
     check(out, s, nodes, temperature)
+
+
+@pytest.mark.parametrize("vocab", [4096, 20000, 128256])
+def test_greedy_rows_take_the_first_of_the_largest(gpu_ctx, vocab):
+    """Equal maxima in a segment's waves and quads, in other segments, many of them; drafts on the first and on a later one."""
+    rng = np.random.default_rng(vocab)
+    places = [(300, 1030), (1030, 300, 4000), (255, 256), (256, 1024), (0, 4095), (4095, 1279, 1280), (1535, 1024, 770), (3, 1027, 2051, 3075),
+              (vocab - 1, 512), (vocab - 1, vocab - 2), (511, 1023, 2047), (1100, 900)]
+    nodes, temperature = [3] * (len(places) + 4), np.zeros(len(places) + 4)
+    s = inputs(rng, nodes, vocab, "given", temperature, liked=False)
+    x = s["logits"].reshape(-1, 3, vocab)
+    s["parents"][:] = [-1, 0, 0] * len(nodes)
+    tokens = s["tokens"].reshape(-1, 3)
+    for b, at in enumerate(places):
+        x[b, :, list(at)] = 40.0
+        tokens[b, 1:] = (at[0], min(at)) if b % 2 else (max(at), at[0])
+    for b in range(len(places), len(nodes)):  # logits of eight bits: hundreds of equal maxima
+        x[b] = np.round(np.clip(x[b], -4, 4) * 2) / 2
+        tokens[b, 1:] = rng.choice(np.nonzero(x[b, 0] == x[b, 0].max())[0], 2)
+    x[-1] = 0.0
+    tokens[-1, 1:] = 1, 0
+    out = run(gpu_ctx, s, nodes, temperature)
+    gpu_ctx.sync()
+    gpu_ctx.check_faults()
+    check(out, s, nodes, temperature)
