@@ -66,7 +66,7 @@ __device__ __forceinline__ int key_end(const TreeArgs& a, const fi::TreeSpan& t)
 __device__ __forceinline__ bool sees_nothing(const TreeArgs& a, const fi::TreeSpan& t, int kend, const uint64_t* mask) {
   if (t.prefix > 0) return false;
   for (int k0 = 0; k0 < kend; k0 += 64)
-    if (fi::mask_window(mask, a.words, k0 - t.prefix) & (kend - k0 < 64 ? (1ull << (kend - k0)) - 1 : ~0ull)) return false;
+    if (fi::mask_window(mask, a.words, k0 - t.prefix) & fi::keys_before(kend, k0)) return false;
   return true;
 }
 
@@ -579,8 +579,7 @@ struct Row {
   // 16 jt + 4 lk + v.
   template <int JT>
   __device__ __forceinline__ uint64_t hide(const TreeArgs& a, const Unit& u, int k0, v4f (&s)[JT]) const {
-    uint64_t seen = fi::mask_window(a.mask + place(a, u).row * a.words, a.words, k0 - u.t.prefix);
-    if (u.kend - k0 < 64) seen &= (1ull << (u.kend - k0)) - 1;
+    const uint64_t seen = fi::mask_window(a.mask + place(a, u).row * a.words, a.words, k0 - u.t.prefix) & fi::keys_before(u.kend, k0);
     const uint64_t mine = seen >> (4 * lk);
 #pragma unroll
     for (int jt = 0; jt < JT; ++jt)
@@ -631,13 +630,15 @@ struct Row {
     split2(pf, pp);
   }
 
-  // What is not finite in V, for the rows that see it: `keys` of the chunk at k0.
+  // What is not finite in V, for the rows that see it: `keys` of the chunk at k0, all before u.kend (their blocks are
+  // looked up again).
   template <typename P>
   __device__ __forceinline__ void add_special(const TreeArgs& a, const Unit& u, int k0, uint64_t keys, uint64_t seen) {
     for (; keys != 0; keys &= keys - 1) {  // workgroup-uniform
       const int key = __builtin_ctzll(keys), lb = static_cast<int>(a.by_block.div(k0 + key));
+      if (!((seen >> key) & 1)) continue;
       const int id = a.block_tables[(size_t)u.seq * a.max_blocks + lb];
-      if (id < 0 || id >= a.num_blocks || !((seen >> key) & 1)) continue;
+      if (id < 0 || id >= a.num_blocks) continue;
       const size_t at = ((size_t)id * a.hkv + u.kvh) * a.block_size + (k0 + key - lb * a.block_size);
 #pragma unroll
       for (int dt = 0; dt < DT; ++dt) {
@@ -797,7 +798,7 @@ __global__ __launch_bounds__(kThreads, 3) void attn_tree_bf16_kernel(TreeArgs a)
       wait_loads<0>();
     __syncthreads();
     uint16_t* vs = slots[v_slot];
-    if (past) {  // what is not finite in V is noted and cleared
+    if (past) {  // what is not finite in V is noted and cleared; the copies of the last key that lie past the end are cleared alone
 #pragma unroll 1
       for (int x = 0; x < PT; ++x) {
         uint4* at = reinterpret_cast<uint4*>(&vs[(PT * w + x) * 512 + 8 * lane]);
@@ -808,7 +809,7 @@ __global__ __launch_bounds__(kThreads, 3) void attn_tree_bf16_kernel(TreeArgs a)
         any |= Bf16::clear(v.w);
         if (any) {
           *at = v;
-          atomicOr(&s_special, 1ull << key_of(x));
+          atomicOr(&s_special, (1ull << key_of(x)) & fi::keys_before(u.kend, k0));
         }
       }
       __syncthreads();

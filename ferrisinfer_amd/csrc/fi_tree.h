@@ -34,4 +34,9 @@ __device__ __forceinline__ uint64_t mask_window(const uint64_t* __restrict__ row
   return bits;
 }
 
+// Which of the 64 keys k0 .. k0 + 63 lie before kend, as bits.
+__host__ __device__ inline uint64_t keys_before(int kend, int k0) {
+  return kend - k0 >= 64 ? ~0ull : kend <= k0 ? 0 : (1ull << (kend - k0)) - 1;
+}
+
 }  // namespace fi

@@ -2,6 +2,9 @@
 import numpy as np
 import pytest
 
+import draft_reference as ref
+from test_gpu_fp4_cache import tables_of
+from test_gpu_tree_attention import attend, checked, pool_of
 from test_gpu_verify_drafts import check, inputs, run
 
 pytestmark = pytest.mark.gpu
@@ -80,3 +83,35 @@ def test_greedy_rows_take_the_first_of_the_largest(gpu_ctx, vocab):
     gpu_ctx.sync()
     gpu_ctx.check_faults()
     check(out, s, nodes, temperature)
+
+
+@pytest.mark.parametrize("kind", ["f32", "bf16", "mxfp4"])
+@pytest.mark.parametrize("bs", [1, 5, 16])
+@pytest.mark.parametrize("keys", [65, 64, 129, 3, 160])
+def test_a_last_node_that_holds_no_numbers(gpu_ctx, kind, bs, keys):
+    """The last node's V, which fills the rest of a chunk, in block tables just as wide as the keys: the rows that see the node
+    get it, the others are as without."""
+    rng = np.random.default_rng(keys + bs)
+    hq, hkv, d, n = 4, 2, 64, 3
+    tables = tables_of(rng, [keys, keys], bs, 2 * keys + 2)
+    assert tables.shape == (2, -(-keys // bs))
+    nb = 2 * keys + 2
+    (kd, _), (vd, _) = pool_of(rng, kind, nb, hkv, bs, d), pool_of(rng, kind, nb, hkv, bs, d)
+    seen = ref.ancestors([-1, 0, 0])  # the last node is seen by itself alone
+    mask = np.concatenate([ref.words_of(seen, 1)] * 2)
+    q = rng.standard_normal((2 * n, hq, d)).astype(np.float32)
+    args = (gpu_ctx, kind, q, (kd, vd), tables, [n, n], [keys, keys], mask, hkv, bs, nb, d ** -0.5)
+    before = checked(gpu_ctx, attend(*args))
+    assert np.isfinite(before).all()
+    for b in range(2):
+        block, row = tables[b][(keys - 1) // bs], (keys - 1) % bs
+        if kind == "mxfp4":
+            vd[nb * hkv * bs * (d // 2):].view(nb, hkv, bs, d // 32)[block, 1, row, 0] = 255
+        else:
+            vd[block, 1, row, 3] = float("nan")
+    got = checked(gpu_ctx, attend(*args))
+    blind = np.tile([True, True, False], 2)
+    assert np.array_equal(got[blind], before[blind])
+    assert np.isnan(got[~blind][:, 2:, 3]).all() and np.array_equal(got[~blind][:, :2], before[~blind][:, :2])
+    # (four bits: of the group's columns; the others have theirs)
+    assert np.array_equal(got[~blind][:, :, 32:], before[~blind][:, :, 32:])
