@@ -10,16 +10,13 @@
 // (tree_join_rows_kernel, tree_join_kernel).  The products are the prefill kernels': S^T = K Q^T leaves a lane the scores of
 // one row, O^T = V^T P^T takes them as its B operand from registers, the f32 operands go as three bf16
 // pieces (x = hi + mid + lo exactly), and the exponents' reference point moves only when a chunk's maximum
-// passes it by 2^8.  K and V of bf16 pools are exact in bf16 (three products a product), f32 pools' are split as well
-// (the six cross products above 2^-24).  4-bit pools' are exact in f16 for any scale from 2^-18 to 2^8, and two f16 pieces
-// hold Q and the weights to 2^-23, which is less than what the third product's roundings cost: two products a
-// product.  A workgroup that meets another scale starts over in bf16.
+// passes it by 2^8.  K and V of bf16 and 4-bit pools are exact in bf16 (three products a product), f32 pools'
+// are split as well (the six cross products above 2^-24).
 //
 // Only chunks that reach past the prefix (one or two a tile of up to 64 nodes) look at masks.  There an element of V that is
 // not finite must reach only the rows that see its key, though the product multiplies every key by every row
 // (0 * NaN is NaN): it is staged as zero, its key noted, and added afterwards to the rows that see it.
 #include <algorithm>
-#include <type_traits>
 
 #include "fi_common.h"
 #include "fi_device.h"
@@ -110,7 +107,7 @@ struct Pool<FI_DTYPE_F32, D> {
     const bool x = special(v[r].x), y = special(v[r].y), z = special(v[r].z), w = special(v[r].w);
     return x || y || z || w;
   }
-  template <bool HALF, int KP, int VP, int K>
+  template <int KP, int VP, int K>
   __device__ __forceinline__ void store(int r, int key, int col, uint16_t (&ks)[PLANES][K][KP], uint16_t (&vs)[PLANES][K][VP]) {
     uint2 pk[3], pv[3];
     fi::split3_pk(k[r].x, k[r].y, pk[0].x, pk[1].x, pk[2].x);
@@ -157,32 +154,14 @@ struct Pool<FI_DTYPE_MXFP4, D> {
     vs8 = 127u;
     return true;
   }
-  // A group that f16 does not hold (NaN it does) when it is 2^5 as large: its least step, 2^(scale - 128), as a normal
-  // number, 2^-14 at least (the matrix instructions lose bits of others: 4.6e-6 where all were), its largest value,
-  // 6 * 2^(scale - 127), below 2^16.
-  static constexpr float UP_LOG2 = 5.0f, UP = 32.0f;
-  static __device__ __forceinline__ bool beyond_f16(const fi::Codes<SEG / 2>& x, uint32_t scale) {
-    uint32_t any = 0;
-#pragma unroll
-    for (int j = 0; j < SEG / 8; ++j) any |= x.w[j] & 0x77777777u;
-    return (scale > 135u && scale <= fi::kFp4MaxScale) || (scale < 109u && any != 0);
-  }
-  __device__ __forceinline__ bool beyond_f16() const { return beyond_f16(k, ks8) || beyond_f16(v, vs8); }
-  template <bool HALF, int KP, int VP, int K>
+  template <int KP, int VP, int K>
   __device__ __forceinline__ void store(int, int key, int col, uint16_t (&ks)[PLANES][K][KP], uint16_t (&vs)[PLANES][K][VP]) {
-    const float k2 = fi::fp4_scale_f32(ks8) * (HALF ? UP : 1.0f), v2 = fi::fp4_scale_f32(vs8) * (HALF ? UP : 1.0f);
+    const float k2 = fi::fp4_scale_f32(ks8), v2 = fi::fp4_scale_f32(vs8);
 #pragma unroll
     for (int j = 0; j < SEG / 8; ++j) {
-      *reinterpret_cast<uint4*>(&ks[0][key][col * SEG + 8 * j]) = HALF ? widen8_f16(k.w[j], k2) : fi::fp4_widen8(k.w[j], k2);
-      *reinterpret_cast<uint4*>(&vs[0][key][col * SEG + 8 * j]) = HALF ? widen8_f16(v.w[j], v2) : fi::fp4_widen8(v.w[j], v2);
+      *reinterpret_cast<uint4*>(&ks[0][key][col * SEG + 8 * j]) = fi::fp4_widen8(k.w[j], k2);
+      *reinterpret_cast<uint4*>(&vs[0][key][col * SEG + 8 * j]) = fi::fp4_widen8(v.w[j], v2);
     }
-  }
-  template <int kByte>
-  static __device__ __forceinline__ uint32_t widen2_f16(uint32_t codes, float scale) {
-    return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(codes, scale, kByte));
-  }
-  static __device__ __forceinline__ uint4 widen8_f16(uint32_t codes, float scale) {
-    return make_uint4(widen2_f16<0>(codes, scale), widen2_f16<1>(codes, scale), widen2_f16<2>(codes, scale), widen2_f16<3>(codes, scale));
   }
   // NaN, whatever the code, for the scales that clean() takes out (253 and 254 are not for a host to write)
   static __device__ __forceinline__ float4 values(const TreeArgs& a, size_t row, int d) {
@@ -486,33 +465,13 @@ __device__ __forceinline__ void join_last(const TreeArgs& a, const Unit& u) {
   join_parts<D, kRows * (D / 4) / kThreads, true>(a, u.t, u.kvh, u.tile, u.piece - u.part * step, step, u.nparts, threadIdx.x, kThreads);
 }
 
-// the same where one operand is exact in f16 and the other two pieces of it
-__device__ __forceinline__ v4f product(const f16x8 (&x)[1], const f16x8 (&f)[2], v4f acc) {
-  acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(x[0], f[1], acc, 0, 0, 0);
-  return __builtin_amdgcn_mfma_f32_16x16x32_f16(x[0], f[0], acc, 0, 0, 0);
-}
-// x = hi + lo to 2^-23 of itself, or 2^-25 where that is more
-__device__ __forceinline__ void split2(const f32x8& x, f16x8 (&p)[2]) {
-  p[0] = __builtin_convertvector(x, f16x8);
-  p[1] = __builtin_convertvector(x - __builtin_convertvector(p[0], f32x8), f16x8);
-}
-
 // A lane's row: row li of its wave's sixteen, shared by four lanes (lk).
-//
-// HALF: the pieces of Q and of the weights are two of f16 rather than three of bf16, beside K and V that f16 holds exactly.
-// f16 has a bottom (2^-24), so the row of Q is scaled to [2^13, 2^14) at its largest, which c2 takes back, and weights are
-// up to 2^15: what is below 2^-24 then is 2^-38 of the row's largest element and 2^-39 of the largest weight.
-template <int D, bool HALF>
+template <int D>
 struct Row {
-  static constexpr float LIFT = HALF ? 14.0f : 0.0f;  // of the weights, in log2 units
-  static constexpr float SLACK = HALF ? 1.0f : 8.0f;  // how far one may pass the reference point
-  static constexpr float UP_LOG2 = HALF ? Pool<FI_DTYPE_MXFP4, D>::UP_LOG2 : 0.0f;  // of K and V
-  static constexpr float UP = HALF ? Pool<FI_DTYPE_MXFP4, D>::UP : 1.0f;
   static constexpr int DS = D / 32;  // 32-wide d steps of Q K^T
   static constexpr int DT = D / 16;  // 16-wide output d tiles of P V
   int lane, li, lk;
-  using Pieces = std::conditional_t<HALF, f16x8[2], bf16x8[3]>;
-  Pieces qf[DS];     // Q pieces: B operand row li, d = 32 s + 8 lk .. + 7
+  bf16x8 qf[DS][3];  // Q pieces: B operand row li, d = 32 s + 8 lk .. + 7
   v4f o[DT];         // O^T tile dt: d = 16 dt + 4 lk + v, row li
   float m, l;        // the exponents' reference point (log2 units), this lane's share of the weights' sum
   float c2;          // scores -> log2 units
@@ -540,28 +499,8 @@ struct Row {
     lk = lane >> 4;
     const Place at = place(a, u);
     c2 = a.scale * 1.4426950408889634f;
-    float up = 1.0f;
-    if constexpr (HALF) {
-      float top = 0.0f;
 #pragma unroll
-      for (int s = 0; s < DS; ++s) {
-        const f32x8 v = query(a, at, s);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) top = fmaxf(top, fabsf(v[e]));
-      }
-      top = fmaxf(top, fi::lane_xor16(top, lane));
-      top = fmaxf(top, fi::lane_xor32(top, lane));
-      const int by = min(14 - __builtin_amdgcn_frexp_expf(top), 126);
-      up = __builtin_ldexpf(1.0f, by);
-      c2 = fmaxf(__builtin_ldexpf(c2 / UP, -by), 1.17549435e-38f);  // 0 would make NaN of what is hidden; scores are below 2^40
-    }
-#pragma unroll
-    for (int s = 0; s < DS; ++s) {
-      if constexpr (HALF)
-        split2(query(a, at, s) * up, qf[s]);
-      else
-        split3(query(a, at, s), qf[s]);
-    }
+    for (int s = 0; s < DS; ++s) split3(query(a, at, s), qf[s]);
 #pragma unroll
     for (int dt = 0; dt < DT; ++dt) o[dt] = v4f{0.f, 0.f, 0.f, 0.f};
     m = -INFINITY;
@@ -588,7 +527,7 @@ struct Row {
     return seen;
   }
 
-  // The scores' weights in their place, by a reference point that moves when a chunk's maximum passes it by 2^SLACK.
+  // The scores' weights in their place, by a reference point that moves when a chunk's maximum passes it by 2^8.
   template <int JT>
   __device__ __forceinline__ void weigh(v4f (&s)[JT]) {
     float mx = -INFINITY;
@@ -599,7 +538,7 @@ struct Row {
     mx = fmaxf(mx, fi::lane_xor16(mx, lane));
     mx = fmaxf(mx, fi::lane_xor32(mx, lane));
     const float m_chunk = mx * c2;
-    const float m_new = m_chunk > m + SLACK ? m_chunk : m;
+    const float m_new = m_chunk > m + 8.0f ? m_chunk : m;
     // no key seen yet: the point stays -inf, and scores of -inf weigh 0 against any finite one
     const float point = m_new == -INFINITY ? 0.0f : m_new;
     if (__builtin_amdgcn_ballot_w64(m_new != m) != 0) {  // after the first chunks, hardly ever
@@ -614,7 +553,7 @@ struct Row {
     for (int jt = 0; jt < JT; ++jt)
 #pragma unroll
       for (int v = 0; v < 4; ++v) {
-        s[jt][v] = __builtin_amdgcn_exp2f(fmaf(s[jt][v], c2, LIFT - point));
+        s[jt][v] = __builtin_amdgcn_exp2f(fmaf(s[jt][v], c2, -point));
         sum += s[jt][v];
       }
     l += sum;
@@ -624,10 +563,6 @@ struct Row {
   static __device__ __forceinline__ void pieces(const v4f& lo, const v4f& hi, bf16x8 (&pp)[3]) {
     const f32x8 pf = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
     split3(pf, pp);
-  }
-  static __device__ __forceinline__ void pieces(const v4f& lo, const v4f& hi, f16x8 (&pp)[2]) {
-    const f32x8 pf = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
-    split2(pf, pp);
   }
 
   // What is not finite in V, for the rows that see it: `keys` of the chunk at k0, all before u.kend (their blocks are
@@ -655,9 +590,8 @@ struct Row {
   __device__ __forceinline__ void finish(const TreeArgs& a, const Unit& u) {
     float sum = l + fi::lane_xor16(l, lane);
     sum += fi::lane_xor32(sum, lane);
-    sum *= UP;  // as o is
-    if (u.nparts > 1) {  // by a point that takes the lifts back: another part may be without
-      store_part<D>(a, u, 16 * (threadIdx.x >> 6) + li, lk, o, sum != sum ? 0.f : m - LIFT - UP_LOG2, sum);
+    if (u.nparts > 1) {
+      store_part<D>(a, u, 16 * (threadIdx.x >> 6) + li, lk, o, sum != sum ? 0.f : m, sum);
       return;
     }
     const Place p = place(a, u);
@@ -695,7 +629,7 @@ __device__ __forceinline__ void wait_loads() {
 template <int D>
 __global__ __launch_bounds__(kThreads, 3) void attn_tree_bf16_kernel(TreeArgs a) {
   constexpr int KB = 64, JT = KB / 16, KS = KB / 32;
-  constexpr int DS = Row<D, false>::DS, DT = Row<D, false>::DT;
+  constexpr int DS = Row<D>::DS, DT = Row<D>::DT;
   constexpr int JB = 2;                // score tiles whose K fragments are held at once, twice
   constexpr int DB = DT < 4 ? DT : 2;  // d tiles whose V fragments are
   constexpr int PIECES = D / 8;        // 16-byte pieces of a row
@@ -707,7 +641,7 @@ __global__ __launch_bounds__(kThreads, 3) void attn_tree_bf16_kernel(TreeArgs a)
   Unit u;
   if (!find_unit<KB>(a, u)) return;
   const int tid = threadIdx.x, w = __builtin_amdgcn_readfirstlane(tid >> 6);
-  Row<D, false> row;
+  Row<D> row;
   row.init(a, u);
   const int lane = row.lane, li = row.li, lk = row.lk;
 
@@ -861,37 +795,21 @@ __global__ __launch_bounds__(kThreads, 3) void attn_tree_bf16_kernel(TreeArgs a)
 // ---- f32 and 4-bit pools: through registers, which convert them ----
 
 template <int D, int POOL>
-struct TreeShared {
+__global__ __launch_bounds__(kThreads, D == 128 && POOL == FI_DTYPE_F32 ? 2 : 3) void attn_tree_kernel(TreeArgs a) {
   using P = Pool<POOL, D>;
-  __align__(16) uint16_t Ks[P::PLANES][P::KB][D == 128 && P::PLANES == 1 ? D + 16 : D + 8];  // padded rows (see prefill_bf16_kernel)
-  __align__(16) uint16_t Vs[P::PLANES][P::KB][D + 8];                                       // (transposing reads)
-  unsigned long long special[2];  // by the chunk's parity: keys whose V is not finite throughout
-  int beyond;                     // a group that f16 does not hold
-};
-
-// A workgroup's piece.  HALF: K and V as f16, two products a product; false where f16 does not hold a group of them exactly,
-// and the piece is taken again as bf16, with three (2 sequences of 60000 to 100000 tokens, 32/8 heads of 128, 4-bit: 251 us
-// with three products, 207 with two; 64 sequences of 2000 to 4000 175 and 141).  Both in one loop, by the chunk, took
-// 235: the registers of either are the kernel's.
-template <int D, int POOL, bool HALF>
-__device__ __forceinline__ bool attend_piece(const TreeArgs& a, const Unit& u, TreeShared<D, POOL>& sh) {
-  using P = Pool<POOL, D>;
-  using R = Row<D, HALF>;
-  using X8 = std::conditional_t<HALF, f16x8, bf16x8>;
-  constexpr bool AGAIN = POOL == FI_DTYPE_MXFP4 && !HALF;  // hardly ever: Q's pieces are made a chunk, so that its registers are few
   constexpr int KB = P::KB, PLANES = P::PLANES, PT = P::PT, LANES = P::LANES;
-  constexpr int JT = KB / 16, KS = KB / 32, DS = R::DS, DT = R::DT;
-  auto& Ks = sh.Ks;
-  auto& Vs = sh.Vs;
-  int tid = threadIdx.x;
-  if constexpr (AGAIN) asm volatile("" : "+v"(tid));  // nothing of the two runs is kept for both
-  R row;
+  constexpr int JT = KB / 16, KS = KB / 32, DS = Row<D>::DS, DT = Row<D>::DT;
+  constexpr int KPK = D == 128 && PLANES == 1 ? D + 16 : D + 8;  // padded LDS rows of K (see prefill_bf16_kernel)
+  constexpr int KPV = D + 8;                                     // of V (transposing reads)
+  __shared__ __align__(16) uint16_t Ks[PLANES][KB][KPK];
+  __shared__ __align__(16) uint16_t Vs[PLANES][KB][KPV];
+  __shared__ unsigned long long s_special[2];  // by the chunk's parity: keys whose V is not finite throughout
+
+  Unit u;
+  if (!find_unit<KB>(a, u)) return;
+  const int tid = threadIdx.x;
+  Row<D> row;
   row.init(a, u);
-  if constexpr (AGAIN) {
-    row.lane = tid & 63;
-    row.li = tid & 15;
-    row.lk = (tid & 63) >> 4;
-  }
   const int lane = row.lane, li = row.li, lk = row.lk;
 
   // Staging: a wave's lanes look up the blocks of a chunk's keys, a chunk ahead of its loads; a thread takes
@@ -921,30 +839,25 @@ __device__ __forceinline__ bool attend_piece(const TreeArgs& a, const Unit& u, T
         if (c * KB + key >= u.kend)
           in.zero(x);
         else if (in.clean(x))
-          atomicOr(&sh.special[c & 1], 1ull << key);
+          atomicOr(&s_special[c & 1], 1ull << key);
       }
     }
-    if constexpr (HALF) {
-      if (in.beyond_f16()) sh.beyond = 1;
-    }
 #pragma unroll
-    for (int x = 0; x < PT; ++x) in.template store<HALF>(x, tid / LANES + x * (kThreads / LANES), tid % LANES, Ks, Vs);
+    for (int x = 0; x < PT; ++x) in.store(x, tid / LANES + x * (kThreads / LANES), tid % LANES, Ks, Vs);
     __syncthreads();
-    return !HALF || sh.beyond == 0;  // workgroup-uniform: only a stage writes it
   };
 
-  if (tid < 2) sh.special[tid] = 0;
-  if (HALF && tid == 0) sh.beyond = 0;
+  if (tid < 2) s_special[tid] = 0;
   if (u.c_lo < u.c_hi) {  // workgroup-uniform
     lookup(u.c_lo);
     fetch();
     lookup(u.c_lo + 1);
     __syncthreads();
-    if (!stage(u.c_lo)) return false;
+    stage(u.c_lo);
   }
   for (int c = u.c_lo; c < u.c_hi; ++c) {
     const int k0 = c * KB;
-    if (tid == 0) sh.special[(c + 1) & 1] = 0;  // last read in chunk c - 1
+    if (tid == 0) s_special[(c + 1) & 1] = 0;  // last read in chunk c - 1
     fetch();
     lookup(c + 2);
     __builtin_amdgcn_sched_barrier(0);
@@ -953,27 +866,15 @@ __device__ __forceinline__ bool attend_piece(const TreeArgs& a, const Unit& u, T
     v4f s[JT];
 #pragma unroll
     for (int jt = 0; jt < JT; ++jt) s[jt] = v4f{0.f, 0.f, 0.f, 0.f};
-    auto k_times = [&](int x, const typename R::Pieces& qf) {
+#pragma unroll
+    for (int x = 0; x < DS; ++x)
 #pragma unroll
       for (int jt = 0; jt < JT; ++jt) {
-        X8 kf[PLANES];
+        bf16x8 kf[PLANES];
 #pragma unroll
-        for (int p = 0; p < PLANES; ++p) kf[p] = *reinterpret_cast<const X8*>(&Ks[p][16 * jt + li][32 * x + 8 * lk]);
-        s[jt] = product(kf, qf, s[jt]);
+        for (int p = 0; p < PLANES; ++p) kf[p] = *reinterpret_cast<const bf16x8*>(&Ks[p][16 * jt + li][32 * x + 8 * lk]);
+        s[jt] = product<PLANES>(kf, row.qf[x], s[jt]);
       }
-    };
-    if constexpr (AGAIN) {
-      const typename R::Place at = row.place(a, u);
-#pragma unroll 1
-      for (int x = 0; x < DS; ++x) {
-        typename R::Pieces qf;
-        split3(row.query(a, at, x), qf);
-        k_times(x, qf);
-      }
-    } else {
-#pragma unroll
-      for (int x = 0; x < DS; ++x) k_times(x, row.qf[x]);
-    }
     const bool past = reaches<KB>(u, c);
     uint64_t seen = ~0ull;
     if (past) seen = row.hide(a, u, k0, s);
@@ -982,43 +883,28 @@ __device__ __forceinline__ bool attend_piece(const TreeArgs& a, const Unit& u, T
     // ---- O^T += V^T P^T ----
 #pragma unroll
     for (int t = 0; t < KS; ++t) {
-      typename R::Pieces pp;
+      bf16x8 pp[3];
       row.pieces(s[2 * t], s[2 * t + 1], pp);
       const int vrow = 32 * t + 4 * lk + (li >> 2), vcol = 4 * (li & 3);  // as in prefill_bf16_kernel
 #pragma unroll
       for (int dt = 0; dt < DT; ++dt) {
-        X8 vf[PLANES];
+        bf16x8 vf[PLANES];
 #pragma unroll
         for (int p = 0; p < PLANES; ++p) {
           const v4s lo = lds_read_tr16(&Vs[p][vrow][16 * dt + vcol]);
           const v4s hi = lds_read_tr16(&Vs[p][vrow + 16][16 * dt + vcol]);
-          vf[p] = __builtin_bit_cast(X8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+          vf[p] = __builtin_bit_cast(bf16x8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
         }
-        row.o[dt] = product(vf, pp, row.o[dt]);
+        row.o[dt] = product<PLANES>(vf, pp, row.o[dt]);
       }
     }
-    if (past) row.template add_special<P>(a, u, k0, sh.special[c & 1], seen);
+    if (past) row.template add_special<P>(a, u, k0, s_special[c & 1], seen);
     __syncthreads();  // every wave is done with this chunk's K and V
-    if (c + 1 < u.c_hi) {  // workgroup-uniform
-      if (!stage(c + 1)) return false;
-    }
+    if (c + 1 < u.c_hi) stage(c + 1);  // workgroup-uniform
   }
   if (bad_block) atomicOr(a.faults, FI_FAULT_BLOCK_RANGE);
   row.finish(a, u);
   join_last<D>(a, u);
-  return true;
-}
-
-template <int D, int POOL>
-__global__ __launch_bounds__(kThreads, D == 128 && POOL == FI_DTYPE_F32 ? 2 : 3) void attn_tree_kernel(TreeArgs a) {
-  __shared__ TreeShared<D, POOL> sh;
-  Unit u;
-  if (!find_unit<Pool<POOL, D>::KB>(a, u)) return;
-  if constexpr (POOL == FI_DTYPE_MXFP4) {
-    if (attend_piece<D, POOL, true>(a, u, sh)) return;
-    __syncthreads();  // every wave has seen that
-  }
-  attend_piece<D, POOL, false>(a, u, sh);
 }
 
 // The join in a launch of its own, of many tiles: 256 quads of a (sequence, tile, kv head) at a time.

@@ -617,8 +617,7 @@ int32_t fi_tree_plan(fi_context* ctx, const int32_t* d_parents, const int32_t* d
  * context_lens[b] - nodes and those of the nodes whose bits d_tree_mask[t] has set (any mask, not only
  * fi_tree_plan's; bits past the tree are ignored).  q/out f32 [T, Hq, D]; scores, softmax and sums are
  * f32, and f32, bf16 and mxfp4 pools are attended in f32 accuracy; any number of query heads per KV head.  A row that
- * sees no key is zero; K and V of a node that a row does not see do not reach it, whatever they hold (over an mxfp4
- * pool a scale outside [2^-18, 2^8], seen or not, changes the roundings of the rows of its 64-row tile).
+ * sees no key is zero; K and V of a node that a row does not see do not reach it, whatever they hold.
  * max_context_len must bound every context_lens entry (it sizes the grid); positions of a longer one past it
  * are not attended, and it is reported as Runtime by fi_ctx_check_faults.  Keys are cut into parts by the launch's
  * sizes and joined in order, so equal calls give equal bits.  head_dim 32, 64 or 128 and max_context_len up to

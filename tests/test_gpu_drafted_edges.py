@@ -3,8 +3,9 @@ import numpy as np
 import pytest
 
 import draft_reference as ref
-from test_gpu_fp4_cache import tables_of
-from test_gpu_tree_attention import attend, checked, pool_of
+import fp4_reference as fp4
+from test_gpu_fp4_cache import dev, tables_of
+from test_gpu_tree_attention import PIECES, attend, checked, pool_of, trees_of
 from test_gpu_verify_drafts import check, inputs, run
 
 pytestmark = pytest.mark.gpu
@@ -115,3 +116,57 @@ def test_a_last_node_that_holds_no_numbers(gpu_ctx, kind, bs, keys):
     assert np.isnan(got[~blind][:, 2:, 3]).all() and np.array_equal(got[~blind][:, :2], before[~blind][:, :2])
     # (four bits: of the group's columns; the others have theirs)
     assert np.array_equal(got[~blind][:, :, 32:], before[~blind][:, :, 32:])
+
+
+@pytest.mark.parametrize("kind", ["f32", "bf16", "mxfp4"])
+@pytest.mark.parametrize("d,prefix", [(64, 490), (128, 497), (128, 5000)])
+def test_channels_of_very_different_sizes(gpu_ctx, kind, d, prefix):
+    """K's channels are 2^20 apart in size and Q's the other way round, by powers of two: the scores, and what an f32 product
+    of them rounds, are as without."""
+    rng = np.random.default_rng(d + prefix)
+    hq, hkv, n, bs = 8, 2, 11, 16
+    keys = prefix + n
+    nb = -(-keys // bs) + 1
+    tables = tables_of(rng, [keys], bs, nb)
+    (kd, kv), (vd, vv) = pool_of(rng, kind, nb, hkv, bs, d), pool_of(rng, kind, nb, hkv, bs, d)
+    by = np.where(np.arange(d // 32) % 2, -12, 8)
+    each = np.repeat(np.exp2(by), 32)
+    if kind == "mxfp4":
+        scales = kd[nb * hkv * bs * (d // 2):].view(-1, d // 32)
+        scales.copy_(dev((scales.cpu().numpy().astype(np.int64) + by).astype(np.uint8)))
+    else:
+        kd *= dev(each.astype(np.float32)).to(kd.dtype)
+    kv = kv * each
+    trees, mask = trees_of(rng, [n])
+    q = (rng.standard_normal((n, hq, d)) / each).astype(np.float32)
+    got = checked(gpu_ctx, attend(gpu_ctx, kind, q, (kd, vd), tables, [n], [keys], mask, hkv, bs, nb, d ** -0.5))
+    k, v = (fp4.rows_of(x, tables[0], keys, bs) for x in (kv, vv))
+    ref.check_attention(got, q, k, v, ref.visible(ref.ancestors(trees[0]), prefix, keys), d ** -0.5, PIECES[kind])
+
+
+@pytest.mark.parametrize("kind", ["f32", "bf16", "mxfp4"])
+@pytest.mark.parametrize("prefix", [400, 3000])
+@pytest.mark.parametrize("ahead", [8.0, 14.0, 20.0, 30.0, 45.0])
+def test_a_key_that_takes_the_weight_and_gives_nothing(gpu_ctx, kind, prefix, ahead):
+    """The first key's score is far above the others' and its V is zero: what is left are weights of 2^-12 to 2^-65."""
+    rng = np.random.default_rng(prefix)
+    hq, hkv, d, n, bs = 8, 2, 64, 9, 16
+    keys = prefix + n
+    nb = -(-keys // bs) + 1
+    tables = tables_of(rng, [keys], bs, nb)
+    (kd, kv), (vd, vv) = pool_of(rng, kind, nb, hkv, bs, d), pool_of(rng, kind, nb, hkv, bs, d)
+    first = tables[0, 0]
+    if kind == "mxfp4":
+        for pool, code in ((kd, 0x22), (vd, 0)):  # codes of 1, of 0; scales of 1
+            pool[:nb * hkv * bs * (d // 2)].view(nb, hkv, bs, d // 2)[first, :, 0] = code
+            pool[nb * hkv * bs * (d // 2):].view(nb, hkv, bs, d // 32)[first, :, 0] = 127
+    else:
+        kd[first, :, 0] = 1.0
+        vd[first, :, 0] = 0.0
+    kv[first, :, 0], vv[first, :, 0] = 1.0, 0.0
+    trees, mask = trees_of(rng, [n])
+    q = rng.standard_normal((n, hq, d)).astype(np.float32) * np.float32(0.1)
+    q += np.float32(ahead / np.sqrt(d))  # the first key's score: `ahead` and a little
+    got = checked(gpu_ctx, attend(gpu_ctx, kind, q, (kd, vd), tables, [n], [keys], mask, hkv, bs, nb, d ** -0.5))
+    k, v = (fp4.rows_of(x, tables[0], keys, bs) for x in (kv, vv))
+    ref.check_attention(got, q, k, v, ref.visible(ref.ancestors(trees[0]), prefix, keys), d ** -0.5, PIECES[kind])
