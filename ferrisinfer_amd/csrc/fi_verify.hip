@@ -70,10 +70,11 @@ struct Walk {
   double off, taken;  // a and s
 };
 
-// Weights by a reference point are 2^(k l - c): k = log2(e) / temperature, l the logit, c = k times the point.  c is one
-// rounded number, so that its rounding is a common factor of them.
+// Weights by a reference point are 2^(k (l - point)): k = log2(e) / temperature, l the logit.  (The difference comes first:
+// k l and k point are 2^128 where a row is masked by finite numbers, and their roundings 2^75.  As one fused operation with k point
+// rounded beforehand it was no faster.)
 struct Weights {
-  double k, c;
+  double k, point;
 };
 
 constexpr double kLog2E = 1.4426950408889634;
@@ -83,19 +84,7 @@ __device__ __forceinline__ double row_scale(float temperature) {
   return kLog2E / static_cast<double>(fmaxf(temperature, kMinTemperature));
 }
 
-// That factor must stay near 1: where a segment is all masked by a finite number, c of 2^128 is off by up to 2^75, which is
-// no exponent.  From |c| = 2^40 on (it is within 2^-13 there) the next lower logit is 2^-24 of the point below it at least,
-// 2^16 in k l, and weighs nothing by the largest one.  So a k of half that does as well, and a power of two makes k l and c exact.
-__device__ __forceinline__ Weights weights_by(double k, float point) {
-  Weights w{k, k * point};
-  if (__builtin_fabs(w.c) >= 1099511627776.0) {  // the same for all threads that sum together
-    w.k = __builtin_ldexp(0.5, __builtin_amdgcn_frexp_exp(k));
-    w.c = w.k * point;
-  }
-  return w;
-}
-
-// 2^x for x in [-1100, 1000]: 2^n times a polynomial in f, |f| <= 1/2, through 2^f at the eleven Chebyshev
+// 2^x for x in [-1100, 0]: 2^n times a polynomial in f, |f| <= 1/2, through 2^f at the eleven Chebyshev
 // points; it is within 3.2e-16 of 2^f.
 __device__ __forceinline__ double exp2_64(double x) {
   const double n = __builtin_rint(x), f = x - n;
@@ -113,17 +102,15 @@ __device__ __forceinline__ double exp2_64(double x) {
   return __builtin_ldexp(s, static_cast<int>(n));
 }
 
-// A logit's weight, by a reference point that no logit of the row passes; one of -inf (and, where k is 0, NaN from
-// it) weighs nothing.
+// A logit's weight, by a reference point that none of those summed passes; one of -inf (and, where k is 0, NaN from it) weighs
+// nothing.
 __device__ __forceinline__ double weight(double l, const Weights& w) {
-  return exp2_64(__builtin_fmax(__builtin_fma(l, w.k, -w.c), -1100.0));
+  return exp2_64(__builtin_fmax((l - w.point) * w.k, -1100.0));
 }
 
 // What weights by `from` are multiplied with to be weights by `to`, which is no less.
 __device__ __forceinline__ double change_of_ref(double k, float from, float to) {
-#pragma clang fp contract(off)  // the difference of the two c, as they are
-  const double c_from = k * from, c_to = k * to;
-  return exp2_64(__builtin_fmax(c_from - c_to, -1100.0));
+  return weight(from, Weights{k, to});
 }
 
 __device__ __forceinline__ float finite_or_zero(float x) { return fabsf(x) <= 3.402823466e38f ? x : 0.0f; }
@@ -351,7 +338,7 @@ __device__ __forceinline__ void sum_segment(const VerifyArgs& a, VerifyShared& s
   look_up(a, s, from, thread_of(), mine);
   double sum = 0.0;
   if (less) {
-    const Weights by = weights_by(s.k, walk.ref);
+    const Weights by{s.k, walk.ref};
 #pragma unroll
     for (int e = 0; e < kEndElems; ++e) sum += __builtin_fmax(weight(v[e], by) - walk.off * q[e], 0.0);
     sum = segment_sum(sh.seg[group_of()], sum);
@@ -379,7 +366,7 @@ __device__ __forceinline__ void sum_segment(const VerifyArgs& a, VerifyShared& s
     }
     segment_top(sh.seg[group_of()], top, first, s.greedy);
   }
-  const Weights by = weights_by(s.k, finite_or_zero(top));
+  const Weights by{s.k, finite_or_zero(top)};
 #pragma unroll
   for (int e = 0; e < kEndElems; ++e) sum += weight(v[e], by);
   sum = segment_sum(sh.seg[group_of()], bad ? NAN : sum);
@@ -481,7 +468,7 @@ __device__ __forceinline__ void pick_token(const VerifyArgs& a, VerifyShared& sh
 #pragma unroll
     for (int e = 0; e < kEndElems; ++e) v[e] = was_tried(sh, tid * kEndElems + e) ? -INFINITY : v[e];
   }
-  const Weights by = weights_by(s.k, walk.ref);
+  const Weights by{s.k, walk.ref};
   const double off = less ? walk.off : 0.0;
   double left[kEndElems], here = 0.0;
 #pragma unroll
@@ -583,7 +570,7 @@ __device__ __forceinline__ void advance(const VerifyArgs& a, VerifyShared& sh, c
     int accepted = -1;
     bool rejected = false;
     if (walk.count < a.max_path && (!rest || a.probs)) {
-      find_children(a, sh, s, walk, weights_by(s.k, walk.ref), mine);
+      find_children(a, sh, s, walk, Weights{s.k, walk.ref}, mine);
       if (s.greedy) {
         int best = 0x7fffffff;
         for (int j = lane; j < s.n; j += 64)
