@@ -61,7 +61,7 @@ __device__ __forceinline__ int key_end(const TreeArgs& a, const fi::TreeSpan& t)
 }
 // Whether a row sees no key at all: then it is zero, where a row whose scores are all -inf is NaN.
 __device__ __forceinline__ bool sees_nothing(const TreeArgs& a, const fi::TreeSpan& t, int kend, const uint64_t* mask) {
-  if (t.prefix > 0) return false;
+  if (t.prefix > 0 && kend > 0) return false;
   for (int k0 = 0; k0 < kend; k0 += 64)
     if (fi::mask_window(mask, a.words, k0 - t.prefix) & fi::keys_before(kend, k0)) return false;
   return true;

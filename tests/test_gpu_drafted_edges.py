@@ -170,3 +170,20 @@ def test_a_key_that_takes_the_weight_and_gives_nothing(gpu_ctx, kind, prefix, ah
     got = checked(gpu_ctx, attend(gpu_ctx, kind, q, (kd, vd), tables, [n], [keys], mask, hkv, bs, nb, d ** -0.5))
     k, v = (fp4.rows_of(x, tables[0], keys, bs) for x in (kv, vv))
     ref.check_attention(got, q, k, v, ref.visible(ref.ancestors(trees[0]), prefix, keys), d ** -0.5, PIECES[kind])
+
+
+@pytest.mark.parametrize("kind", ["f32", "bf16", "mxfp4"])
+def test_lengths_past_a_bound_of_nothing(gpu_ctx, kind):
+    """max_context_len 0: no row sees a key, whatever the lengths are, and those are reported."""
+    from ferrisinfer_amd import FerrisError
+
+    rng = np.random.default_rng(34)
+    hkv, d, bs, nb, nodes = 2, 64, 16, 8, [3, 5, 2]
+    pools = [pool_of(rng, kind, nb, hkv, bs, d)[0] for _ in range(2)]
+    _, mask = trees_of(rng, nodes)
+    q = rng.standard_normal((10, 4, d)).astype(np.float32)
+    for lens in ([20, 30, 2], [20, 0, 2]):
+        out = attend(gpu_ctx, kind, q, pools, tables_of(rng, lens, bs, nb), nodes, lens, mask, hkv, bs, nb, 0.1, longest=0)
+        with pytest.raises(FerrisError) as e:
+            gpu_ctx.check_faults()
+        assert "context" in e.value.message and bool((out == 0).all())
