@@ -608,9 +608,9 @@ struct Row {
 
 // One load of a wave from the pool to LDS: lane i's 16 bytes to lds + 16 i.  In assembly, because the
 // compiler would wait for every such load before the next read of the same LDS array; what waits for them is
-// wait_loads and a barrier.
+// wait_loads and a barrier.  m0, the LDS address, needs a wait state between its write and the load.
 __device__ __forceinline__ void load_to_lds(const uint8_t* src, uint32_t lds) {
-  asm volatile("s_mov_b32 m0, %1\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(src), "s"(__builtin_amdgcn_readfirstlane(lds))
+  asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(src), "s"(__builtin_amdgcn_readfirstlane(lds))
                : "m0", "memory");
 }
 // Until at most N of this wave's loads are on their way (they end in the order of their issue).
