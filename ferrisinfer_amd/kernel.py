@@ -223,6 +223,8 @@ def check_logit_rows(name, what, t, rows, vocab) -> None:
         raise FerrisError(3, f"{name}: {what} must be of shape {[rows, vocab]}, not {list(t.shape)}")
     if vocab > 1 and int(t.stride(1)) != 1:
         raise FerrisError(4, f"{name}: the rows of {what} must be contiguous")
+    if row_stride(t) > 0x7fffffff:
+        raise FerrisError(8, f"{name}: rows of {what} of 2^31 elements and more apart")
 
 
 def row_stride(t) -> int:
