@@ -732,8 +732,8 @@ int32_t fi_verify_drafts(fi_context* ctx, const float* d_logits, int32_t ld, int
   FI_REQUIRE(max_path < fi::kMaxTreeNodes, FI_ERR_INVALID_SHAPE, "fi_verify_drafts: max_path is more than a tree can be deep");
   FI_REQUIRE(num_seqs <= 65535, FI_ERR_INVALID_SHAPE, "fi_verify_drafts: at most 65535 sequences per call");
   if (num_seqs == 0) return FI_OK;
-  FI_REQUIRE(d_logits && d_tokens && d_parents && d_cu_seqlens && d_temperature && d_accept_u && d_pick_u && d_out_tokens &&
-                 (d_out_path || max_path == 0) && d_out_count && d_out_prob,
+  FI_REQUIRE(((d_logits && d_tokens && d_parents && d_accept_u) || max_query_len == 0) && d_cu_seqlens && d_temperature && d_pick_u &&
+                 d_out_tokens && (d_out_path || max_path == 0) && d_out_count && d_out_prob,
              FI_ERR_INVALID_CONFIG, "fi_verify_drafts: null pointer");
   VerifyArgs a{};
   a.logits = d_logits;

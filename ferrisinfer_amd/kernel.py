@@ -227,6 +227,11 @@ def check_logit_rows(name, what, t, rows, vocab) -> None:
         raise FerrisError(8, f"{name}: rows of {what} of 2^31 elements and more apart")
 
 
+def bound_of(max_query_len, rows) -> int:
+    """max_query_len of a drafted step; none where there are no rows, whose arrays have no address."""
+    return int(max_query_len) if rows > 0 else min(int(max_query_len), 0)
+
+
 def row_stride(t) -> int:
     """Elements from a row to the next (a tensor of one row may give any number for it)."""
     return int(t.stride(0)) if int(t.shape[0]) > 1 else int(t.shape[1])
@@ -599,7 +604,7 @@ class Context:
                      context_lens=(context_lens, (seqs,)), positions_out=(positions_out, (rows,)))
         check_arrays("tree_plan", "int64", mask_out=(mask_out, (rows, words)))
         check(self.lib.fi_tree_plan(self.handle, ptr(parents), ptr(cu_seqlens), ptr(context_lens), seqs,
-                                    int(max_query_len), words, ptr(mask_out), ptr(positions_out)))
+                                    bound_of(max_query_len, rows), words, ptr(mask_out), ptr(positions_out)))
 
     def attn_tree_paged(self, q, k_cache, v_cache, kv_dtype, block_tables, cu_seqlens, context_lens, tree_mask,
                         max_query_len, max_context_len, num_kv_heads, block_size, num_blocks, scale, out):
@@ -613,7 +618,7 @@ class Context:
         check_arrays("attn_tree_paged", "int64", tree_mask=(tree_mask, (t, words)))
         check(self.lib.fi_attn_tree_paged(self.handle, ptr(q), ptr(k_cache), ptr(v_cache), int(kv_dtype),
                                           ptr(block_tables), blocks, ptr(cu_seqlens), ptr(context_lens), ptr(tree_mask),
-                                          words, seqs, int(max_query_len), int(max_context_len), num_q_heads,
+                                          words, seqs, bound_of(max_query_len, t), int(max_context_len), num_q_heads,
                                           int(num_kv_heads), head_dim, int(block_size), int(num_blocks), float(scale),
                                           ptr(out)))
 
@@ -633,7 +638,7 @@ class Context:
         check_arrays(name, "float32", temperature=(temperature, (seqs,)), accept_u=(accept_u, (rows,)),
                      pick_u=(pick_u, (seqs,)), prob_out=(prob_out, (seqs,)))
         check(self.lib.fi_verify_drafts(self.handle, ptr(logits), row_stride(logits), vocab, ptr(tokens), ptr(parents),
-                                        ptr(cu_seqlens), seqs, int(max_query_len), ptr(temperature), ptr(draft_probs),
+                                        ptr(cu_seqlens), seqs, bound_of(max_query_len, rows), ptr(temperature), ptr(draft_probs),
                                         0 if draft_probs is None else row_stride(draft_probs), 1 if distinct else 0,
                                         ptr(accept_u), ptr(pick_u), longest, ptr(tokens_out), ptr(path_out),
                                         ptr(count_out), ptr(prob_out)))

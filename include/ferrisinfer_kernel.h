@@ -602,7 +602,8 @@ int32_t fi_sample_reserve(fi_context* ctx, int32_t rows, int32_t vocab);
  * the sequence then has context_lens[b] - nodes + 1 + count[b] cached positions, and the last token of
  * out_tokens is the next step's node 0.
  * max_query_len (at most 1024, Unsupported otherwise) must bound every tree's nodes; rows of a longer tree
- * past it are left as they were and reported as Runtime by fi_ctx_check_faults. */
+ * past it are left as they were and reported as Runtime by fi_ctx_check_faults.  With max_query_len 0 there are no rows,
+ * and the arrays of rows may be null. */
 
 /* d_tree_mask[t] = the nodes that row t may attend, its ancestors and itself, as bits of its sequence's
  * nodes (uint64 [T, mask_words], node j bit j % 64 of word j / 64); d_positions[t] = context_lens[b] - nodes +

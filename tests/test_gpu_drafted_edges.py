@@ -187,3 +187,31 @@ def test_lengths_past_a_bound_of_nothing(gpu_ctx, kind):
         with pytest.raises(FerrisError) as e:
             gpu_ctx.check_faults()
         assert "context" in e.value.message and bool((out == 0).all())
+
+
+@pytest.mark.parametrize("seqs", [1, 3])
+def test_steps_without_rows(gpu_ctx, seqs):
+    """No sequence has a node, and the arrays of rows none: an empty tensor has no address."""
+    import torch
+
+    i = lambda *n: torch.full(n, 5, dtype=torch.int32, device="cuda")  # noqa: E731
+    f = lambda *n: torch.full(n, 5.0, device="cuda")  # noqa: E731
+    mask, cu, lens = torch.zeros((0, 1), dtype=torch.int64, device="cuda"), i(seqs + 1) * 0, i(seqs)
+    gpu_ctx.tree_plan(i(0), cu, lens, 4, mask, i(0))
+    pools = [torch.zeros(4, 2, 16, 64, device="cuda") for _ in range(2)]
+    gpu_ctx.attn_tree_paged(f(0, 4, 64), *pools, 0, i(seqs, 1) * 0, cu, lens, mask, 4, 16, 2, 16, 4, 0.1, f(0, 4, 64))
+    for probs in (None, f(0, 50)):
+        tokens, path, count, prob = i(seqs, 4), i(seqs, 3), i(seqs), f(seqs)
+        gpu_ctx.verify_drafts(f(0, 50), i(0), i(0), cu, 4, f(seqs), f(0), f(seqs), probs, False, tokens, path, count, prob)
+        gpu_ctx.sync()
+        assert bool((tokens == -1).all()) and bool((path == -1).all()) and bool((count == 0).all()) and bool((prob == 0).all())
+    gpu_ctx.kv_keep_path([pools[0]], [pools[1]], 0, i(seqs, 1) * 0, cu, lens, path, 4, 16, 2, 64)
+    gpu_ctx.check_faults()
+    # lengths that say otherwise are reported: rows that are not there are not read
+    cu[-1] = 2
+    gpu_ctx.verify_drafts(f(0, 50), i(0), i(0), cu, 4, f(seqs), f(0), f(seqs), None, False, tokens, path, count, prob)
+    from ferrisinfer_amd import FerrisError
+
+    with pytest.raises(FerrisError) as e:
+        gpu_ctx.check_faults()
+    assert "query" in e.value.message and bool((tokens == -1).all())
