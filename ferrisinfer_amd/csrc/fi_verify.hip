@@ -578,6 +578,8 @@ __device__ __forceinline__ void advance(const VerifyArgs& a, VerifyShared& sh, c
         best = first_of(0.0f, 0.0f, best);
         accepted = best == 0x7fffffff ? -1 : best;
       } else if (!a.probs) {
+        // (a difference: within 1e-14 of the row's sum.  Summing the row again where little is left costs registers, a wave a SIMD
+        // less: 96 us for 90 where 64 drafts of four tokens are verified.)
         double left = total;
         for (int j = next_child(sh, s.n, walk.node); j >= 0; j = next_child(sh, s.n, j)) {
           bool out = false;  // an earlier child of the same token has been taken out

@@ -621,7 +621,8 @@ int32_t fi_tree_plan(fi_context* ctx, const int32_t* d_parents, const int32_t* d
  * sees no key is zero; K and V of a node that a row does not see do not reach it, whatever they hold.
  * max_context_len must bound every context_lens entry (it sizes the grid); positions of a longer one past it
  * are not attended, and it is reported as Runtime by fi_ctx_check_faults.  Keys are cut into parts by the launch's
- * sizes and joined in order, so equal calls give equal bits.  head_dim 32, 64 or 128 and max_context_len up to
+ * sizes and the lengths of all its sequences, on the device, and joined in order: calls that are equal in all of these give equal
+ * bits, and a sequence in another batch may be rounded otherwise.  head_dim 32, 64 or 128 and max_context_len up to
  * 2^30, pools of up to 2^32 head rows (Unsupported otherwise); q, out and the pools 16-byte aligned
  * (InvalidLayout); scale positive and finite (InvalidConfig).  Uses the context workspace. */
 int32_t fi_attn_tree_paged(fi_context* ctx, const float* d_q, const void* d_k_cache, const void* d_v_cache, int32_t kv_dtype,
@@ -645,7 +646,8 @@ int32_t fi_attn_tree_paged(fi_context* ctx, const float* d_q, const void* d_k_ca
  * of the last are not tried then), the last token is the first index whose running sum of rho passes pick_u * sum(rho) (rho = p where
  * nothing is left; the last index with any for a pick_u of 1 or more).  d_accept_u f32 [T] (of the drafted nodes) and d_pick_u
  * f32 [B] are uniform in [0, 1), and do not count where temperature[b] <= 0 (a child is accepted when it is the first of the
- * largest).  Comparisons are decided in 64-bit accuracy.  Logits of -inf have no
+ * largest).  Comparisons are decided in 64-bit accuracy; of given drafts' comparisons sum(rho) is the row's
+ * sum less the rejected tokens', within 2^-46 of that (a draft that held all but 2^-24 and was rejected leaves 22 bits).  Logits of -inf have no
  * probability: mask them (or with a finite number far below the others) to sample from a top-k or top-p set.
  * Outputs: d_out_tokens int32 [B, max_path + 1], the accepted tokens, then the last one, then -1; d_out_path
  * int32 [B, max_path], the accepted nodes, then -1; d_out_count int32 [B], how many; d_out_prob f32 [B], the last

@@ -86,6 +86,32 @@ def test_greedy_rows_take_the_first_of_the_largest(gpu_ctx, vocab):
     check(out, s, nodes, temperature)
 
 
+@pytest.mark.parametrize("seqs,ahead,vocab", [(24, 0, 5000), (16, 0, 140000), (8, 22, 100000)], ids=["rows at once", "a row a launch", "far down"])
+def test_given_drafts_that_leave_little(gpu_ctx, seqs, ahead, vocab):
+    """A draft that the model all but wants, rejected by a random number next to 1: it leaves 1e-7 of the row, and the next
+    ones are held against that, which is within 2^-46 of the row."""
+    rng = np.random.default_rng(33)
+    size, n = 8, 8 + ahead
+    nodes, temperature = [n] * seqs, np.ones(seqs)
+    parents = list(range(-1, ahead)) + [ahead] * (size - 1)  # (`ahead` accepted ones in front)
+    s = dict(logits=np.full((seqs * n, vocab), -200.0, np.float32), tokens=np.zeros(seqs * n, np.int32),
+             parents=np.tile(parents, seqs).astype(np.int32), accept=rng.random(seqs * n).astype(np.float32),
+             pick=rng.random(seqs).astype(np.float32), probs=None)
+    x, tokens, u = s["logits"].reshape(seqs, n, vocab), s["tokens"].reshape(seqs, n), s["accept"].reshape(seqs, n)
+    for b in range(seqs):
+        liked = rng.choice(vocab, 9, replace=False)
+        x[b, :, liked[0]] = 30.0
+        tokens[b, :ahead + 1] = liked[0]
+        u[b, :ahead + 1] = 0.0
+        x[b, ahead, liked[1:]] = 30.0 - 15.9 - 2.08 + rng.random(8).astype(np.float32) / 64  # eight that have 1.2e-7 in all
+        tokens[b, ahead + 1:] = [liked[0], liked[1], liked[0], liked[2], liked[1], liked[3], int(rng.integers(vocab))]
+        u[b, ahead + 1] = 1 - 2.0 ** -24
+    out = run(gpu_ctx, s, nodes, temperature)
+    gpu_ctx.sync()
+    gpu_ctx.check_faults()
+    check(out, s, nodes, temperature)
+
+
 @pytest.mark.parametrize("kind", ["f32", "bf16", "mxfp4"])
 @pytest.mark.parametrize("bs", [1, 5, 16])
 @pytest.mark.parametrize("keys", [65, 64, 129, 3, 160])
