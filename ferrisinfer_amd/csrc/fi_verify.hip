@@ -172,8 +172,8 @@ __device__ __forceinline__ float4 quad_at(const float* __restrict__ row, int at,
 
 // ---------------------------------------------------------------- segments of a row
 
-// 16 elements a thread: 64 sequences of five rows of 128k logits 88 us (8: 97, 32: 109), 16 trees 96 (93, 119), one
-// sequence of 152k 21 (22, 23).
+// 16 elements a thread: 64 sequences of five rows of 128k logits 90 us (8: 92, 32: 111), 16 trees 98 (92, 121), one
+// sequence of 152k 22 (22, 25).
 constexpr int kEndThreads = 256;
 constexpr int kEndElems = 16;
 constexpr int kSegment = kEndThreads * kEndElems;   // 4096
@@ -654,7 +654,7 @@ __device__ __forceinline__ void begin_outputs(const VerifyArgs& a, const Sequenc
 }
 
 // One launch of the walks: a workgroup a (segment, sequence), or, the first launch where all rows are summed,
-// a (segment, row).  What bounds it: the rows of 64 sequences of 128k logits, 33 MB, take 16 us.  8 us of that are the
+// a (segment, row).  What bounds it: the rows of 64 sequences of 128k logits, 33 MB, take 16 to 18 us.  8 us of that are the
 // exponentials, 1.05e12 a second in 64 bits (as many bytes of logits as 4.2 TB/s); the rest is the arrival and the
 // last workgroup's way, one memory latency after the other.  16 sequences take 9 us, one 8.
 template <bool VEC, bool FIRST>
@@ -760,8 +760,8 @@ int32_t fi_verify_drafts(fi_context* ctx, const float* d_logits, int32_t ld, int
   a.segments = (vocab + kSegment - 1) / kSegment;
   const int64_t rows = static_cast<int64_t>(num_seqs) * max_query_len;
   // Few rows are all summed in the first launch, so that a walk goes through accepted tokens without further ones: one
-  // sequence of 8 rows of 152k logits 22 us, 37 with a launch a row; 24 sequences of 5 rows of 128k 51 and 57; 32 of
-  // them 61 and 63; 24 of 8 rows of 152k 62 and 59; 64 of 5 rows of 128k 93 and 88.
+  // sequence of 8 rows of 152k logits 22 us, 38 with a launch a row; 24 sequences of 5 rows of 128k, drawn, 51 and 58; 32 of
+  // them 62 and 64; 24 of 8 rows of 152k, given, 61 and 56, drawn 77 and 91; 64 of 5 rows of 128k 98 and 89.
   a.all_rows = max_path > 0 && max_query_len > 1 && rows <= 65535 && rows + num_seqs <= FI_MERGE_COUNTERS && rows * vocab <= kAllRows;
   // Arrivals at one line follow each other at 11 ns: counters a line each, as far as there are lines (64 sequences of five rows,
   // all rows summed: 63 us, 117 with the counters side by side).
@@ -781,8 +781,8 @@ int32_t fi_verify_drafts(fi_context* ctx, const float* d_logits, int32_t ld, int
   const int depth = std::min(max_path, std::max(max_query_len - 1, 0));
   const int needed = a.all_rows ? (d_draft_probs ? max_query_len - 1 : 1)
                                 : (d_draft_probs && depth > 0 ? max_query_len - 1 : depth);
-  // Launches for four rejections, then one that takes what is left, a workgroup a walk: 16 trees of up to 32 nodes, drawn, 97 us
-  // in the mean of twelve (110 with launches for two, 98 for six, 103 for eight), 64 of them 169 (193, 166, 169).  max_path may be a loose bound, and a launch that finds nothing to do costs
+  // Launches for four rejections, then one that takes what is left, a workgroup a walk: 16 trees of up to 32 nodes, drawn, 99 us
+  // in the mean of twelve (112 with launches for two, 99 for six, 103 for eight), 64 of them 173 (198, 170, 172).  max_path may be a loose bound, and a launch that finds nothing to do costs
   // 1 to 3 us: rows behind the first kDepth are left to that as well.
   const int passes = std::min(needed, (a.all_rows ? 0 : std::min(depth, kDepth)) + kRejections);
   auto launch = [&](auto vec_rows) {
