@@ -2,7 +2,9 @@
 // moved to their places behind the prefix.  No counterpart in the reference, whose sessions feed one sampled
 // token a step (crates/ferrisinfer-runtime/src/session.rs:246-262).
 #include <algorithm>
+#include <exception>
 #include <type_traits>
+#include <vector>
 
 #include "fi_common.h"
 #include "fi_device.h"
@@ -61,7 +63,7 @@ constexpr int kLayersPerLaunch = 64;
 constexpr int kBatch = 8;  // rows of a path that are loaded before any of them is stored
 
 struct KeepArgs {
-  void* pools[2 * kLayersPerLaunch];  // K and V of each layer
+  void* pools[2 * kLayersPerLaunch];  // K and V arrays, each once
   const int* block_tables;
   const int* cu_seqlens;
   const int* context_lens;
@@ -185,10 +187,19 @@ int32_t fi_kv_keep_path(fi_context* ctx, void* const* k_caches, void* const* v_c
   FI_REQUIRE(k_caches && v_caches && d_block_tables && d_cu_seqlens && d_context_lens && d_path, FI_ERR_INVALID_CONFIG,
              "fi_kv_keep_path: null pointer");
   uintptr_t bits = 0;  // every layer is checked before any layer's rows move
-  for (int32_t l = 0; l < num_layers; ++l) {
-    FI_REQUIRE(k_caches[l] && v_caches[l], FI_ERR_INVALID_CONFIG, "fi_kv_keep_path: null pointer");
-    if (kv_dtype == FI_DTYPE_MXFP4) FI_TRY(fi::check_fp4_pool("fi_kv_keep_path", k_caches[l], v_caches[l], head_dim));
-    bits |= reinterpret_cast<uintptr_t>(k_caches[l]) | reinterpret_cast<uintptr_t>(v_caches[l]);
+  std::vector<void*> pools;  // each array once: rows that have moved must not move again, nor two workgroups move the same
+  try {
+    for (int32_t l = 0; l < num_layers; ++l) {
+      FI_REQUIRE(k_caches[l] && v_caches[l], FI_ERR_INVALID_CONFIG, "fi_kv_keep_path: null pointer");
+      if (kv_dtype == FI_DTYPE_MXFP4) FI_TRY(fi::check_fp4_pool("fi_kv_keep_path", k_caches[l], v_caches[l], head_dim));
+      bits |= reinterpret_cast<uintptr_t>(k_caches[l]) | reinterpret_cast<uintptr_t>(v_caches[l]);
+      pools.push_back(k_caches[l]);
+      pools.push_back(v_caches[l]);
+    }
+    std::sort(pools.begin(), pools.end());
+    pools.erase(std::unique(pools.begin(), pools.end()), pools.end());
+  } catch (const std::exception& e) {
+    return fi::set_error(FI_ERR_RUNTIME, std::string("fi_kv_keep_path: ") + e.what());
   }
   KeepArgs a{};
   a.block_tables = d_block_tables;
@@ -204,13 +215,9 @@ int32_t fi_kv_keep_path(fi_context* ctx, void* const* k_caches, void* const* v_c
   a.second = kv_dtype == FI_DTYPE_MXFP4 ? fi::fp4_code_bytes(num_blocks, num_kv_heads, block_size, head_dim) : 0;
   a.blocks = fi::FastDiv(static_cast<uint32_t>(block_size));
   const int cell = kv_dtype == FI_DTYPE_F32 ? 4 : 2;
-  for (int32_t l0 = 0; l0 < num_layers; l0 += kLayersPerLaunch) {
-    const int layers = std::min(num_layers - l0, kLayersPerLaunch);
-    a.pools_in_launch = 2 * layers;
-    for (int l = 0; l < layers; ++l) {
-      a.pools[2 * l] = k_caches[l0 + l];
-      a.pools[2 * l + 1] = v_caches[l0 + l];
-    }
+  for (size_t at = 0; at < pools.size(); at += 2 * kLayersPerLaunch) {
+    a.pools_in_launch = static_cast<int>(std::min<size_t>(pools.size() - at, 2 * kLayersPerLaunch));
+    std::copy_n(pools.begin() + at, a.pools_in_launch, a.pools);
     if (kv_dtype == FI_DTYPE_MXFP4) {
       if (head_dim == 32)
         launch_keep<quad, uint8_t>(ctx, a, num_seqs, 1);

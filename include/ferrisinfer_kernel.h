@@ -666,12 +666,13 @@ int32_t fi_verify_drafts(fi_context* ctx, const float* d_logits, int32_t ld, int
                          int32_t* d_out_path, int32_t* d_out_count, float* d_out_prob);
 
 /* Moves the K/V rows of each sequence's accepted path to the positions behind its node 0, in num_layers pools of
- * one shape in one launch (64 layers each): the row of node path[b][i] to position context_lens[b] - nodes + 1 + i.
+ * one shape in one launch (128 arrays each): the row of node path[b][i] to position context_lens[b] - nodes + 1 + i.
  * k_caches and v_caches are HOST arrays of device pointers, read during the call.  d_path int32 [B, max_path] as
  * fi_verify_drafts writes it: nodes in rising order, ended by a negative entry or max_path; an entry that does
  * not rise or is no node of the tree ends the path and is reported as Runtime by fi_ctx_check_faults, as is a block id
  * outside the pool, whose rows stay.  Rows move as if all were read before any is written; other rows are left
- * as they were.  The blocks of these positions must be the sequence's own (fi_kv_copy_blocks first where a
+ * as they were.  An array that is listed more than once (layers that share a cache, K and V in one) is moved once, and arrays
+ * must not overlap otherwise.  The blocks of these positions must be the sequence's own (fi_kv_copy_blocks first where a
  * block is shared). */
 int32_t fi_kv_keep_path(fi_context* ctx, void* const* k_caches, void* const* v_caches, int32_t num_layers, int32_t kv_dtype,
                         const int32_t* d_block_tables, int32_t max_blocks_per_seq, const int32_t* d_cu_seqlens,

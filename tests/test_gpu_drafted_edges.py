@@ -6,6 +6,7 @@ import draft_reference as ref
 import fp4_reference as fp4
 from test_gpu_fp4_cache import dev, tables_of
 from test_gpu_tree_attention import PIECES, attend, checked, pool_of, trees_of
+from test_gpu_tree_rows import moved, rows
 from test_gpu_verify_drafts import check, inputs, run
 
 pytestmark = pytest.mark.gpu
@@ -241,3 +242,23 @@ def test_steps_without_rows(gpu_ctx, seqs):
     with pytest.raises(FerrisError) as e:
         gpu_ctx.check_faults()
     assert "query" in e.value.message and bool((tokens == -1).all())
+
+
+@pytest.mark.parametrize("layers", [1, 3, 70])
+def test_pools_that_are_listed_more_than_once(gpu_ctx, layers):
+    """Layers that share a cache, and K and V in one array: the rows move once."""
+    rng = np.random.default_rng(35)
+    nb, hkv, bs, d, paths = 6, 2, 16, 32, [[2, 3, 5, 8], [1, 4, 5, 9]]
+    pools = [pool_of(rng, "bf16", nb, hkv, bs, d)[0] for _ in range(2)]
+    table = np.array([[2, 0, 4], [1, 5, 3]], np.int32)
+    for k, v in [([pools[0]], [pools[0]]), ([pools[0]] * 2, [pools[1]] * 2), ([pools[0], pools[1]], [pools[1], pools[0]])]:
+        before = [rows(x, "bf16", nb, hkv, bs, d) for x in pools]
+        gpu_ctx.kv_keep_path(k * layers, v * layers, 1, dev(table), dev(np.array([0, 10, 20], np.int32)), dev(np.array([40, 33], np.int32)),
+                             dev(np.array(paths, np.int32)), nb, bs, hkv, d)
+        gpu_ctx.sync()
+        gpu_ctx.check_faults()
+        for x, old in zip(pools, before):
+            if x is pools[0] or len(k) > 1:
+                for b, prefix in enumerate((30, 23)):
+                    old = moved(old, table[b], prefix, paths[b], bs)
+            assert np.array_equal(rows(x, "bf16", nb, hkv, bs, d), old)
