@@ -658,7 +658,7 @@ int32_t fi_attn_tree_paged(fi_context* ctx, const float* d_q, const void* d_k_ca
  * at most 65535 sequences.  A walk goes from launch to launch: 1 + min(max_path, max_query_len - 1) of them, 22 at most, with
  * d_draft_probs up to five more; two and six where num_seqs * max_query_len * vocab is up to 2 * 10^7.  What they leave
  * (a path of more than 20 tokens, more than four rejected drawn tokens) one workgroup a sequence finishes, at some 40 us
- * a row.  Uses the context workspace. */
+ * a row.  Given siblings are compared with each other: a call with 31 of them that are all rejected takes 88 us, 127 0.9 ms, 1023 57 ms.  Uses the context workspace. */
 int32_t fi_verify_drafts(fi_context* ctx, const float* d_logits, int32_t ld, int32_t vocab, const int32_t* d_tokens,
                          const int32_t* d_parents, const int32_t* d_cu_seqlens, int32_t num_seqs, int32_t max_query_len,
                          const float* d_temperature, const float* d_draft_probs, int32_t draft_ld, int32_t distinct,
